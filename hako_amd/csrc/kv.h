@@ -1,0 +1,16 @@
+// kv.h — the quantised cache as the kernels see it (include/hako_attn.h).
+#pragma once
+#include "../../include/hako_attn.h"
+#include "hako_dev.h"
+#include "hako_rt.h"
+
+namespace hako {
+
+// Bytes of a code.
+inline int kv_elt(int type) { return type == HAKO_KV_Q8 ? 1 : 2; }
+// The checks every call makes of its cache; 0 or an error code.
+int kv_check(const hako_gpu_kv *kv);
+// ... and of a row pointer and stride (floats): 16-byte rows of at least `width`.
+int rows_check(const char *what, const void *p, int64_t stride, int64_t width);
+
+}  // namespace hako

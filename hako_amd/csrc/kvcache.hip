@@ -1,0 +1,324 @@
+// kvcache.hip — the quantised key/value cache: tokens appended (their queries
+// and keys rotated in the same pass) and rows read back.
+#include "kv.h"
+
+namespace hako {
+
+int kv_check(const hako_gpu_kv *kv) {
+	if (!kv) return set_error(HAKO_GPU_EINVAL, "null cache");
+	if (kv->type != HAKO_KV_F16 && kv->type != HAKO_KV_Q8)
+		return set_error(HAKO_GPU_ETYPE, "cache type %d", kv->type);
+	if (kv->n_slots < 1 || kv->max_seq < 1 || kv->n_kv_heads < 1 || kv->n_kv_heads > 65535 ||
+	    (kv->head_dim != 64 && kv->head_dim != 128))
+		return set_error(HAKO_GPU_EINVAL, "unsupported cache shape: %d slots of %d positions, %d heads of %d",
+		                 kv->n_slots, kv->max_seq, kv->n_kv_heads, kv->head_dim);
+	// one slot and head is read through 32-bit buffer offsets
+	if ((size_t)kv->max_seq * kv->head_dim * kv_elt(kv->type) >= kBufNone)
+		return set_error(HAKO_GPU_EINVAL, "max_seq %d x head_dim %d: one head's rows exceed 2 GiB", kv->max_seq,
+		                 kv->head_dim);
+	if (!kv->k || !kv->v || !kv->k_scale || !kv->v_scale) return set_error(HAKO_GPU_EINVAL, "null cache array");
+	if ((((uintptr_t)kv->k | (uintptr_t)kv->v) & 15) || (((uintptr_t)kv->k_scale | (uintptr_t)kv->v_scale) & 3))
+		return set_error(HAKO_GPU_EINVAL, "cache arrays need 16-byte (codes) and 4-byte (scales) alignment");
+	return HAKO_GPU_OK;
+}
+
+int rows_check(const char *what, const void *p, int64_t stride, int64_t width) {
+	if (!p) return set_error(HAKO_GPU_EINVAL, "null %s", what);
+	if ((uintptr_t)p & 15) return set_error(HAKO_GPU_EINVAL, "%s is not 16-byte aligned", what);
+	if (stride < width || (stride & 3))
+		return set_error(HAKO_GPU_EINVAL, "%s stride %lld: a multiple of 4 of at least %lld floats is wanted", what,
+		                 (long long)stride, (long long)width);
+	return HAKO_GPU_OK;
+}
+
+namespace {
+
+struct KvDev {
+	uint8_t *k, *v;
+	float *ks, *vs;
+	int n_slots, max_seq, kvh;
+};
+
+KvDev kv_dev(const hako_gpu_kv *kv) {
+	return {(uint8_t *)kv->k, (uint8_t *)kv->v, kv->k_scale, kv->v_scale, kv->n_slots, kv->max_seq, kv->n_kv_heads};
+}
+
+struct RopeDev {
+	const float *table;
+	int n_pos, rot, interleaved;
+};
+
+// Largest of the L lanes (8 or 16) of a row, as unsigned bits.
+template <int L>
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+	v = max(v, (uint32_t)dpp_i<kDppQuadSwap1>((int)v));
+	v = max(v, (uint32_t)dpp_i<kDppQuadSwap2>((int)v));
+	v = max(v, (uint32_t)dpp_i<kDppHalfMirror>((int)v));
+	if (L == 16) v = max(v, (uint32_t)dpp_i<kDppMirror>((int)v));
+	return v;
+}
+
+// a*c - b*s and a*s + b*c, each product and sum rounded (no fused form): the
+// codes of a key then follow from its definition alone.
+__device__ __forceinline__ void turn(float &a, float &b, float c, float s) {
+#pragma clang fp contract(off)
+	const float ac = a * c, bs = b * s, as = a * s, bc = b * c;
+	a = ac - bs;
+	b = as + bc;
+}
+
+// One lane's 8 values of a head row as codes at dims 4*u0.. and 4*u1.. of
+// `codes`, and (one lane) the row's scale.
+template <int L, bool Q8>
+__device__ __forceinline__ void put_row(const float v[8], int u0, int u1, uint8_t *codes, float *scale, bool first) {
+	uint32_t m = 0;
+#pragma unroll
+	for (int i = 0; i < 8; i++) m = max(m, __builtin_bit_cast(uint32_t, v[i]) & 0x7FFFFFFFu);
+	m = row_max<L>(m);
+	const bool finite = m < 0x7F800000u;
+	float sc;
+	if (Q8) {
+		const float amax = m < 0x00800000u ? 0.0f : __builtin_bit_cast(float, m);
+		sc = q8_xs(amax);
+		const float inv = finite ? q8_inv(amax, sc) : 0.0f;
+		uint32_t w[2];
+#pragma unroll
+		for (int h = 0; h < 2; h++) {
+			w[h] = 0;
+#pragma unroll
+			for (int i = 0; i < 4; i++) w[h] |= q8_code(ftz(v[4 * h + i]), inv) << (8 * i);
+		}
+		*(uint32_t *)(codes + 4 * u0) = w[0];
+		*(uint32_t *)(codes + 4 * u1) = w[1];
+	} else {
+		const int e = finite ? f16_split_exp(m < 0x00800000u ? 0.0f : __builtin_bit_cast(float, m)) : 0;
+		sc = __builtin_ldexpf(1.0f, e);
+		uint2 w[2];
+#pragma unroll
+		for (int h = 0; h < 2; h++) {
+			uint16_t c[4];
+#pragma unroll
+			for (int i = 0; i < 4; i++)
+				c[i] = finite ? __builtin_bit_cast(uint16_t, (_Float16)__builtin_ldexpf(v[4 * h + i], -e)) : 0;
+			w[h] = make_uint2(c[0] | ((uint32_t)c[1] << 16), c[2] | ((uint32_t)c[3] << 16));
+		}
+		*(uint2 *)(codes + 8 * u0) = w[0];
+		*(uint2 *)(codes + 8 * u1) = w[1];
+	}
+	if (first) *scale = finite ? sc : __builtin_nanf("");
+}
+
+// A head row (token, one of its query, key or value heads) is L = head_dim/8
+// lanes of two float4 each. The two of a lane hold whole pairs: unit u (dims
+// 4u..4u+3) with unit u + rot/8 in the half layout, any two in the
+// interleaved one; units past the rotated part are paired as they come.
+template <int HD, bool Q8>
+__global__ __launch_bounds__(256) void append_kernel(KvDev kv, const int *__restrict__ slot, const int *__restrict__ posv,
+                                                     int n_tok, const float *__restrict__ k,
+                                                     const float *__restrict__ v, int64_t kv_stride, RopeDev rope,
+                                                     const float *q, float *q_out, int H, int64_t q_stride,
+                                                     int64_t q_out_stride) {
+	constexpr int L = HD / 8;
+	const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+	const int per = H + 2 * kv.kvh, t = threadIdx.x % L;
+	const int64_t tok = row / per;
+	const int h = (int)(row - tok * per);
+	if (tok >= n_tok) return;
+	const int sl = slot ? slot[tok] : (int)tok, pos = posv[tok];
+	if (sl < 0 || sl >= kv.n_slots || pos < 0 || pos >= kv.max_seq || (rope.table && pos >= rope.n_pos)) return;
+	const bool is_q = h < H, is_v = h >= H + kv.kvh;
+	const float *src = is_q ? q + tok * q_stride + (int64_t)h * HD
+	                        : (is_v ? v + tok * kv_stride + (int64_t)(h - H - kv.kvh) * HD
+	                                : k + tok * kv_stride + (int64_t)(h - H) * HD);
+	const int ru = rope.table && !is_v ? rope.rot / 8 : 0;   // rotated units: 2 ru
+	int u0, u1;
+	if (t < ru) {
+		u0 = t;
+		u1 = t + ru;
+	} else {
+		u0 = 2 * t;
+		u1 = u0 + 1;
+	}
+	const float4 a = *(const float4 *)(src + 4 * u0), b = *(const float4 *)(src + 4 * u1);
+	float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+	if (t < ru) {
+		const float *tb = rope.table + (size_t)pos * rope.rot;
+		if (rope.interleaved) {
+			const float4 c0 = *(const float4 *)(tb + 4 * u0), c1 = *(const float4 *)(tb + 4 * u1);
+			turn(x[0], x[1], c0.x, c0.y);
+			turn(x[2], x[3], c0.z, c0.w);
+			turn(x[4], x[5], c1.x, c1.y);
+			turn(x[6], x[7], c1.z, c1.w);
+		} else {
+			const float4 c0 = *(const float4 *)(tb + 8 * t), c1 = *(const float4 *)(tb + 8 * t + 4);
+			turn(x[0], x[4], c0.x, c0.y);
+			turn(x[1], x[5], c0.z, c0.w);
+			turn(x[2], x[6], c1.x, c1.y);
+			turn(x[3], x[7], c1.z, c1.w);
+		}
+	}
+	if (is_q) {
+		float *dst = q_out + tok * q_out_stride + (int64_t)h * HD;
+		*(float4 *)(dst + 4 * u0) = make_float4(x[0], x[1], x[2], x[3]);
+		*(float4 *)(dst + 4 * u1) = make_float4(x[4], x[5], x[6], x[7]);
+		return;
+	}
+	const int hh = is_v ? h - H - kv.kvh : h - H;
+	const size_t r = ((size_t)sl * kv.kvh + hh) * kv.max_seq + pos;
+	put_row<L, Q8>(x, u0, u1, (is_v ? kv.v : kv.k) + r * HD * (Q8 ? 1 : 2), (is_v ? kv.vs : kv.ks) + r, t == 0);
+}
+
+// 8 codes of a row per lane.
+template <int HD, bool Q8>
+__global__ __launch_bounds__(256) void read_kernel(KvDev kv, const int *__restrict__ slot, const int *__restrict__ posv,
+                                                   int n_tok, float *__restrict__ k, float *__restrict__ v,
+                                                   int64_t kv_stride) {
+	constexpr int L = HD / 8;
+	const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+	const int per = 2 * kv.kvh, t = threadIdx.x % L;
+	const int64_t tok = row / per;
+	const int h = (int)(row - tok * per);
+	if (tok >= n_tok) return;
+	const int sl = slot ? slot[tok] : (int)tok, pos = posv[tok];
+	if (sl < 0 || sl >= kv.n_slots || pos < 0 || pos >= kv.max_seq) return;
+	const bool is_v = h >= kv.kvh;
+	const int hh = is_v ? h - kv.kvh : h;
+	float *dst = is_v ? v : k;
+	if (!dst) return;
+	dst += tok * kv_stride + (int64_t)hh * HD + 8 * t;
+	const size_t r = ((size_t)sl * kv.kvh + hh) * kv.max_seq + pos;
+	const uint8_t *src = (is_v ? kv.v : kv.k) + (r * HD + 8 * t) * (Q8 ? 1 : 2);
+	const float sc = (is_v ? kv.vs : kv.ks)[r];
+	float x[8];
+	if (Q8) {
+		const uint2 w = *(const uint2 *)src;
+#pragma unroll
+		for (int i = 0; i < 4; i++) {
+			x[i] = (float)(int8_t)(w.x >> (8 * i)) * sc;
+			x[4 + i] = (float)(int8_t)(w.y >> (8 * i)) * sc;
+		}
+	} else {
+		const uint4 w = *(const uint4 *)src;
+		const uint32_t d[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+		for (int i = 0; i < 4; i++) {
+			x[2 * i] = f16_to_f32(d[i] & 0xFFFFu) * sc;
+			x[2 * i + 1] = f16_to_f32(d[i] >> 16) * sc;
+		}
+	}
+	*(float4 *)dst = make_float4(x[0], x[1], x[2], x[3]);
+	*(float4 *)(dst + 4) = make_float4(x[4], x[5], x[6], x[7]);
+}
+
+int tokens_check(const hako_gpu_kv *kv, const int *slot, const int *pos, int n_tok) {
+	if (n_tok < 0) return set_error(HAKO_GPU_EINVAL, "%d tokens", n_tok);
+	if (!pos && n_tok) return set_error(HAKO_GPU_EINVAL, "null positions");
+	if (!slot && n_tok > kv->n_slots)
+		return set_error(HAKO_GPU_EINVAL, "%d tokens without slots in a cache of %d", n_tok, kv->n_slots);
+	return HAKO_GPU_OK;
+}
+
+// workgroups of 256/L rows each
+int row_blocks(int64_t rows, int HD, dim3 *grid) {
+	const int64_t n = (rows * (HD / 8) + 255) / 256;
+	if (n > 0x7FFFFFFF) return set_error(HAKO_GPU_EINVAL, "%lld head rows in one call", (long long)rows);
+	*grid = dim3((unsigned)n);
+	return HAKO_GPU_OK;
+}
+
+}  // namespace
+}  // namespace hako
+
+using namespace hako;
+
+extern "C" {
+
+int hako_gpu_kv_bytes(const hako_gpu_kv *kv, size_t *codes, size_t *scales) {
+	if (!kv || !codes || !scales) return set_error(HAKO_GPU_EINVAL, "null argument");
+	if (kv->type != HAKO_KV_F16 && kv->type != HAKO_KV_Q8)
+		return set_error(HAKO_GPU_ETYPE, "cache type %d", kv->type);
+	if (kv->n_slots < 1 || kv->max_seq < 1 || kv->n_kv_heads < 1 || (kv->head_dim != 64 && kv->head_dim != 128))
+		return set_error(HAKO_GPU_EINVAL, "unsupported cache shape: %d slots of %d positions, %d heads of %d",
+		                 kv->n_slots, kv->max_seq, kv->n_kv_heads, kv->head_dim);
+	const size_t rows = (size_t)kv->n_slots * kv->n_kv_heads * kv->max_seq;
+	*codes = rows * kv->head_dim * kv_elt(kv->type);
+	*scales = rows * sizeof(float);
+	return ok();
+}
+
+int hako_gpu_kv_append(const hako_gpu_kv *kv, const int *slot, const int *pos, int n_tok, const float *k,
+                       const float *v, int64_t kv_stride, const hako_gpu_rope *rope, const float *q, float *q_out,
+                       int n_heads, int64_t q_stride, int64_t q_out_stride) {
+	if (int rc = kv_check(kv)) return rc;
+	if (int rc = tokens_check(kv, slot, pos, n_tok)) return rc;
+	const int64_t kvw = (int64_t)kv->n_kv_heads * kv->head_dim;
+	if (int rc = rows_check("k", k, kv_stride, kvw)) return rc;
+	if (int rc = rows_check("v", v, kv_stride, kvw)) return rc;
+	RopeDev r{nullptr, 0, 0, 0};
+	if (rope) {
+		if (!rope->table || ((uintptr_t)rope->table & 15) || rope->n_pos < 1 || rope->rot_dim < 8 ||
+		    rope->rot_dim % 8 || rope->rot_dim > kv->head_dim || (rope->interleaved != 0 && rope->interleaved != 1))
+			return set_error(HAKO_GPU_EINVAL,
+			                 "rope: table %p (16-byte aligned), %d positions, rot_dim %d (a multiple of 8 up to %d), "
+			                 "interleaved %d",
+			                 (const void *)rope->table, rope->n_pos, rope->rot_dim, kv->head_dim, rope->interleaved);
+		r = {rope->table, rope->n_pos, rope->rot_dim, rope->interleaved};
+	}
+	int H = 0;
+	if (q || q_out) {
+		if (!rope) return set_error(HAKO_GPU_EINVAL, "queries without a rotation");
+		if (n_heads < 1 || n_heads > 65535) return set_error(HAKO_GPU_EINVAL, "%d query heads", n_heads);
+		if (int rc = rows_check("q", q, q_stride, (int64_t)n_heads * kv->head_dim)) return rc;
+		if (int rc = rows_check("q_out", q_out, q_out_stride, (int64_t)n_heads * kv->head_dim)) return rc;
+		if (q == q_out && q_stride != q_out_stride)
+			return set_error(HAKO_GPU_EINVAL, "queries rotated in place with two strides");
+		H = n_heads;
+	}
+	if (int rc = require_device()) return rc;
+	if (n_tok == 0) return ok();
+	dim3 grid;
+	if (int rc = row_blocks((int64_t)n_tok * (H + 2 * kv->n_kv_heads), kv->head_dim, &grid)) return rc;
+#define HK_APPEND(HD, Q8)                                                                                          \
+	hipLaunchKernelGGL((append_kernel<HD, Q8>), grid, dim3(256), 0, stream(), kv_dev(kv), slot, pos, n_tok, k, v,    \
+	                   kv_stride, r, q, q_out, H, q_stride, q_out_stride)
+	if (kv->head_dim == 128) {
+		if (kv->type == HAKO_KV_Q8) HK_APPEND(128, true);
+		else HK_APPEND(128, false);
+	} else {
+		if (kv->type == HAKO_KV_Q8) HK_APPEND(64, true);
+		else HK_APPEND(64, false);
+	}
+#undef HK_APPEND
+	HK_LAUNCHED("kv append");
+	return ok();
+}
+
+int hako_gpu_kv_read(const hako_gpu_kv *kv, const int *slot, const int *pos, int n_tok, float *k, float *v,
+                     int64_t kv_stride) {
+	if (int rc = kv_check(kv)) return rc;
+	if (int rc = tokens_check(kv, slot, pos, n_tok)) return rc;
+	if (!k && !v) return set_error(HAKO_GPU_EINVAL, "neither keys nor values wanted");
+	const int64_t kvw = (int64_t)kv->n_kv_heads * kv->head_dim;
+	if (k)
+		if (int rc = rows_check("k", k, kv_stride, kvw)) return rc;
+	if (v)
+		if (int rc = rows_check("v", v, kv_stride, kvw)) return rc;
+	if (int rc = require_device()) return rc;
+	if (n_tok == 0) return ok();
+	dim3 grid;
+	if (int rc = row_blocks((int64_t)n_tok * 2 * kv->n_kv_heads, kv->head_dim, &grid)) return rc;
+#define HK_READ(HD, Q8) \
+	hipLaunchKernelGGL((read_kernel<HD, Q8>), grid, dim3(256), 0, stream(), kv_dev(kv), slot, pos, n_tok, k, v, kv_stride)
+	if (kv->head_dim == 128) {
+		if (kv->type == HAKO_KV_Q8) HK_READ(128, true);
+		else HK_READ(128, false);
+	} else {
+		if (kv->type == HAKO_KV_Q8) HK_READ(64, true);
+		else HK_READ(64, false);
+	}
+#undef HK_READ
+	HK_LAUNCHED("kv read");
+	return ok();
+}
+
+}  // extern "C"

@@ -1,4 +1,4 @@
-"""ctypes view of the hako_gpu C ABI (include/hako_gpu.h) for tests and the bench.
+"""ctypes view of the hako_gpu C ABI (include/hako_gpu.h, include/hako_attn.h) for tests and the bench.
 
 Python never computes here: every call below is a C-ABI call into
 ``lib/libhako_gpu.so``. Loading fails loudly if the library has not been
@@ -17,10 +17,11 @@ GPU_LIB = os.path.join(LIB_DIR, "libhako_gpu.so")
 HOST_LIB = os.path.join(LIB_DIR, "libhako.so")
 
 TYPE_F32, TYPE_F16, TYPE_Q4_K, TYPE_Q6_K = 0, 1, 12, 14
+KV_F16, KV_Q8 = 1, 2
 
 _vp, _i, _i64, _sz = C.c_void_p, C.c_int, C.c_int64, C.c_size_t
 
-# name -> (restype, argtypes); mirrors include/hako_gpu.h one to one.
+# name -> (restype, argtypes); mirrors include/hako_gpu.h, hako_attn.h and hako_decode.h one to one.
 SIGNATURES = {
     "hako_gpu_init": (_i, [_i]),
     "hako_gpu_shutdown": (_i, []),
@@ -59,6 +60,11 @@ SIGNATURES = {
     "hako_gpu_q6k_gemm": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i]),
     "hako_gpu_matmul_batch": (_i, [_vp, _vp, _i, _vp, _vp, _i, _i, _i]),
     "hako_gpu_matmul_batch_noalloc": (_i, [_vp, _vp, _i, _vp, _vp, _i, _i, _i]),
+    "hako_gpu_kv_bytes": (_i, [_vp, C.POINTER(_sz), C.POINTER(_sz)]),
+    "hako_gpu_kv_append": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _i64, _vp, _vp, _vp, _i, _i64, _i64]),
+    "hako_gpu_kv_read": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _i64]),
+    "hako_gpu_attn_decode": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i, _i, C.c_float, _i, _i]),
+    "hako_gpu_attn_prompt": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i, _i, C.c_float, _i, _i]),
     "hako_gpu_decoder_create": (_i, [_vp, _i, _i, C.POINTER(_vp)]),
     "hako_gpu_decoder_destroy": (_i, [_vp]),
     "hako_gpu_decoder_kv": (_i, [_vp, C.POINTER(_vp), C.POINTER(_vp)]),
@@ -78,6 +84,17 @@ class HakoGpuError(RuntimeError):
 class DeviceInfo(C.Structure):
     _fields_ = [("name", C.c_char * 64), ("compute_units", C.c_int), ("clock_khz", C.c_int),
                 ("hbm_bytes", C.c_size_t), ("l2_bytes", C.c_int), ("lds_bytes_per_cu", C.c_int)]
+
+
+class Kv(C.Structure):
+    """hako_gpu_kv (include/hako_attn.h): a quantised key/value cache."""
+    _fields_ = [("type", _i), ("n_slots", _i), ("max_seq", _i), ("n_kv_heads", _i), ("head_dim", _i), ("k", _vp),
+                ("v", _vp), ("k_scale", _vp), ("v_scale", _vp)]
+
+
+class Rope(C.Structure):
+    """hako_gpu_rope (include/hako_attn.h): the angles of a rotation."""
+    _fields_ = [("table", _vp), ("n_pos", _i), ("rot_dim", _i), ("interleaved", _i)]
 
 
 _lib = None
@@ -239,6 +256,36 @@ class Gpu:
     def matmul_batch(self, y, x, qtype: int, w, bias, m: int, n_out: int, n_in: int):
         self.check(self.lib.hako_gpu_matmul_batch(_ptr(y), _ptr(x), qtype, _ptr(w), _ptr(bias), m, n_out, n_in),
                    "matmul_batch")
+
+    # the quantised cache and its attention
+    def kv_bytes(self, kv: Kv):
+        """Bytes of one code array and of one scale array."""
+        codes, scales = _sz(), _sz()
+        self.check(self.lib.hako_gpu_kv_bytes(C.byref(kv), C.byref(codes), C.byref(scales)), "kv_bytes")
+        return codes.value, scales.value
+
+    def kv_append(self, kv: Kv, slot, pos, n_tok: int, k, v, kv_stride: int, rope: Rope | None = None, q=None,
+                  q_out=None, n_heads: int = 0, q_stride: int = 0, q_out_stride: int = 0):
+        self.check(self.lib.hako_gpu_kv_append(C.byref(kv), _ptr(slot), _ptr(pos), n_tok, _ptr(k), _ptr(v), kv_stride,
+                                               None if rope is None else C.byref(rope), _ptr(q), _ptr(q_out), n_heads,
+                                               q_stride, q_out_stride), "kv_append")
+
+    def kv_read(self, kv: Kv, slot, pos, n_tok: int, k, v, kv_stride: int):
+        self.check(self.lib.hako_gpu_kv_read(C.byref(kv), _ptr(slot), _ptr(pos), n_tok, _ptr(k), _ptr(v), kv_stride),
+                   "kv_read")
+
+    def attn_decode(self, out, out_stride: int, q, q_stride: int, kv: Kv, slot, length, n_seq: int, n_heads: int,
+                    scale: float, prefix_slot: int = 0, prefix_len: int = 0):
+        self.check(self.lib.hako_gpu_attn_decode(_ptr(out), out_stride, _ptr(q), q_stride, C.byref(kv), _ptr(slot),
+                                                 _ptr(length), n_seq, n_heads, scale, prefix_slot, prefix_len),
+                   "attn_decode")
+
+    def attn_prompt(self, out, out_stride: int, q, q_stride: int, kv: Kv, slot, start, length, n_seq: int,
+                    n_heads: int, scale: float, prefix_slot: int = 0, prefix_len: int = 0):
+        """slot, start, length: host int32 arrays (slot may be None)."""
+        self.check(self.lib.hako_gpu_attn_prompt(_ptr(out), out_stride, _ptr(q), q_stride, C.byref(kv), _ptr(slot),
+                                                 _ptr(start), _ptr(length), n_seq, n_heads, scale, prefix_slot,
+                                                 prefix_len), "attn_prompt")
 
     def matmul_host(self, out: np.ndarray, x: np.ndarray, qtype: int, w_host: np.ndarray,
                     bias: np.ndarray | None, n_out: int, n_in: int):
