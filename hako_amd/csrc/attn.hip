@@ -1,12 +1,45 @@
 // attn.hip — attention over the quantised cache (include/hako_attn.h): single
 // tokens of many sequences, and whole packed prompts.
+//
+// One pass over the keys with a running maximum and sum (log2 units):
+//   u_p = scale log2(e) q.k_p,  M = max u_p,  l = sum 2^(u_p - M),
+//   o = sum 2^(u_p - M) v_p / l.
+// Both products run on the fp16 matrix cores with fp32 sums and keep fp32
+// accuracy: cache codes (int8 or half) are exact in fp16, and the fp32 factor
+// (the query; the weight times the value row's scale) goes in as two halves,
+// hi = its fp16 and lo = fp16 of the rest, 22 bits together. A query row is
+// first scaled by a power of two that puts its maximum into [2^14, 2^15), the
+// weights by one that puts them below 2^14, so that lo stays clear of the
+// half's subnormals over 2^-14 of the maximum.
+//
+// Scores are formed transposed (S^T = K Q^T: lanes hold queries, registers
+// keys), because then a lane's scores are, in its own registers, the operand
+// of the second product (O^T = V^T P^T) and the running maximum, sum and
+// rescaling belong to the lane; keys are dealt to the tile's rows so that a
+// lane's registers are consecutive keys.
 #include "kv.h"
+
+#include <algorithm>
+#include <float.h>
+#include <vector>
 
 namespace hako {
 namespace {
 
 constexpr int kMaxGroup = 16;    // query heads per key/value head
-constexpr int kSeqs = 128;       // sequences of one prompt launch (by value in the kernel arguments)
+constexpr int kSeqs = 96;        // sequences of one prompt launch (by value in the kernel arguments)
+constexpr int kWsAttn = 7;       // library workspace slot of the records
+constexpr int kKeys = 64;        // keys per chunk of the tiled kernel
+constexpr int kWaves = 4;        // waves per workgroup
+constexpr int kTileRows = 32 * kWaves;
+constexpr float kNone = -FLT_MAX;   // running maximum of a row that has seen no key
+constexpr float kUp = 6.0f;         // weights are 2^(u - M + 6): at most 2^14 while u <= M + kSlack
+constexpr float kSlack = 8.0f;      // M follows the maximum only when it is passed by this
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
 
 struct AttnKv {
 	const uint8_t *k, *v;
@@ -15,67 +48,806 @@ struct AttnKv {
 	int prefix_slot, prefix_len;
 };
 
+// A prompt launch: sequence s has len[s] tokens from row row[s] of q and
+// out, at positions start[s].. of slot[s]; items item[s].. of the grid are
+// its tiles, the last tile first, each in nsplit[s] parts of its keys.
 struct SeqTab {
-	int n;
-	int row[kSeqs + 1], slot[kSeqs], start[kSeqs];
+	int n, tile_tokens, unit;   // tokens per tile, chunks per part
+	int row[kSeqs], len[kSeqs], slot[kSeqs], start[kSeqs], item[kSeqs + 1], nsplit[kSeqs];
+	uint32_t rec[kSeqs];        // first record of a sequence whose tiles are split
 };
 
-template <bool Q8>
-__device__ __forceinline__ float code(const uint8_t *p, size_t i) {
-	return Q8 ? (float)((const int8_t *)p)[i] : (float)((const _Float16 *)p)[i];
+// The same value, made anew where this stands: addresses and masks that
+// follow from it are computed there rather than held in registers across a
+// loop.
+__device__ __forceinline__ int fresh(int v) {
+	asm volatile("" : "+v"(v));
+	return v;
 }
 
-// One wave per query row and head: positions one after the other, a running
-// maximum and sum.
-template <int HD, bool Q8>
-__device__ __forceinline__ void attend(const AttnKv &c, int slot, int end, const float *q, float *out, int kvh,
-                                       float scale) {
-	constexpr int N = HD / 64;
-	const int lane = threadIdx.x;
-	float qv[N], o[N];
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Four int8 codes as halves: byte + 128 under the exponent byte 0x64 is the
+// half 1024 + (code + 128).
+__device__ __forceinline__ h2 bytes_h2(uint32_t biased, uint32_t sel) {
+	const h2 t = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, biased, sel));
+	return t - (h2){(_Float16)1152.0f, (_Float16)1152.0f};
+}
+constexpr uint32_t kLo2 = 0x04010400u, kHi2 = 0x04030402u;
+constexpr uint32_t kFlip = 0x80808080u;
+
+// fp32 pair -> hi halves (toward zero; the rest is exact) and lo halves.
+__device__ __forceinline__ void split2(float a, float b, h2 &hi, h2 &lo) {
+	hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(a, b));
+	lo = (h2){(_Float16)(a - (float)hi.x), (_Float16)(b - (float)hi.y)};
+}
+
+// A power of two that brings a row of queries with maximum a to [2^14, 2^15).
+__device__ __forceinline__ int row_exp(float a) { return f16_split_exp(a) - 14; }
+
+// Eight queries scaled by 2^-e as hi and lo halves (each rounded to nearest).
+__device__ __forceinline__ void split_q(const float *x, int e, h8 &hi, h8 &lo) {
 #pragma unroll
-	for (int i = 0; i < N; i++) {
-		qv[i] = q[lane + 64 * i] * scale;
-		o[i] = 0.0f;
+	for (int j = 0; j < 8; j++) {
+		const float f = __builtin_ldexpf(x[j], -e);
+		hi[j] = (_Float16)f;
+		lo[j] = (_Float16)(f - (float)hi[j]);
 	}
-	float m = -INFINITY, l = 0.0f;
-	for (int p = 0; p < end; p++) {
-		const size_t r = ((size_t)(p < c.prefix_len ? c.prefix_slot : slot) * c.kvh + kvh) * c.max_seq + p;
-		float s = 0.0f;
+}
+
+// The exponent that value scales are divided by: that of their largest.
+__device__ __forceinline__ int scale_exp(float vmax) { return f16_split_exp(vmax); }
+__device__ __forceinline__ float finite_or0(float v) { return __builtin_isfinite(v) ? v : 0.0f; }
+
+// ── tiled kernel: up to 128 query rows against chunks of 64 keys ──
+//
+// Rows are (token, head of the group) pairs, token-major, so that one staged
+// chunk serves every query head of a key/value head. Four waves of 32 rows
+// (v_mfma_f32_32x32x16_f16); per chunk the workgroup converts the codes to
+// halves in LDS, keys as [key][dim] and values transposed as [dim][key], so
+// that every operand is one 16-byte LDS read. The next chunk's codes are in
+// registers while this one is computed; two LDS buffers, one barrier per chunk.
+
+// LDS places of a 16-byte unit, xored so that eight lanes in a row (and the
+// writers) meet different banks.
+template <int HD>
+__device__ __forceinline__ int k_unit(int key, int unit) {   // a key is HD/8 units
+	return unit ^ (((key & 3) | ((key >> 1) & 4) | ((key << 1) & 8)) & (HD / 8 - 1));
+}
+__device__ __forceinline__ int v_unit(int dim, int unit) { return unit ^ ((dim ^ (dim >> 2)) & 7); }
+
+template <int HD, bool Q8>
+struct Stage {
+	static constexpr int EB = Q8 ? 1 : 2;
+	static constexpr int KL = kKeys * HD * EB / 16 / 256;   // 16-byte key loads per thread
+	static constexpr int VQ = HD / 4;                       // dim quads; a thread takes 8 keys x 4 dims
+	static constexpr int VT = kKeys / 8 * VQ;               // threads that stage values (256 or 128)
+	uint4 k[KL];
+	uint32_t v[8][EB];
+	float ks, vs;
+
+	__device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t kr, __amdgpu_buffer_rsrc_t vr, __amdgpu_buffer_rsrc_t ksr,
+	                                     __amdgpu_buffer_rsrc_t vsr, int key0, int tid) {
 #pragma unroll
-		for (int i = 0; i < N; i++) s = __builtin_fmaf(qv[i], code<Q8>(c.k, r * HD + lane + 64 * i), s);
-		s = wave_sum(s) * c.ks[r];
-		const float mn = s > m ? s : m;
-		const float a = m == -INFINITY ? 0.0f : expf(m - mn);
-		const float w = expf(s - mn), wv = w * c.vs[r];
-		l = l * a + w;
+		for (int i = 0; i < KL; i++) {
+			const int u = tid + 256 * i;   // 16-byte unit of the chunk
+			k[i] = ld_b128(kr, (uint32_t)key0 * (HD * EB) + 16u * u);
+		}
+		if (VT == 256 || tid < VT) {
+			const int d = tid % VQ, kg = tid / VQ;
+			const uint32_t off = ((uint32_t)(key0 + 8 * kg) * HD + 4 * d) * EB;
 #pragma unroll
-		for (int i = 0; i < N; i++) o[i] = __builtin_fmaf(wv, code<Q8>(c.v, r * HD + lane + 64 * i), o[i] * a);
-		m = mn;
+			for (int j = 0; j < 8; j++) {
+				if (Q8) v[j][0] = __builtin_amdgcn_raw_buffer_load_b32(vr, (int)(off + j * HD), 0, 0);
+				else {
+					const uint2 t = ld_b64(vr, off + j * HD * 2);
+					v[j][0] = t.x;
+					v[j][EB - 1] = t.y;
+				}
+			}
+		}
+		if (tid < kKeys) {
+			ks = ld_f32(ksr, 4u * (uint32_t)(key0 + tid));
+			vs = ld_f32(vsr, 4u * (uint32_t)(key0 + tid));
+		}
+	}
+
+	// Converted into LDS: keys k_s [64][HD], values v_s [HD][64] halves, the
+	// scales; E follows the largest value scale (wave 0 keeps it).
+	__device__ __forceinline__ void store(uint8_t *k_s, uint8_t *v_s, float *ks_s, float *vs_s, int *e_s, int &E, int tid) {
+#pragma unroll
+		for (int i = 0; i < KL; i++) {
+			const int u = tid + 256 * i;
+			if (Q8) {
+				const int key = u / (HD / 16), c = u % (HD / 16);
+				const uint32_t w[4] = {k[i].x ^ kFlip, k[i].y ^ kFlip, k[i].z ^ kFlip, k[i].w ^ kFlip};
+#pragma unroll
+				for (int h = 0; h < 2; h++) {
+					const h2 a = bytes_h2(w[2 * h], kLo2), b = bytes_h2(w[2 * h], kHi2);
+					const h2 c2 = bytes_h2(w[2 * h + 1], kLo2), d = bytes_h2(w[2 * h + 1], kHi2);
+					*(h8 *)(k_s + key * (2 * HD) + 16 * k_unit<HD>(key, 2 * c + h)) =
+					    (h8){a.x, a.y, b.x, b.y, c2.x, c2.y, d.x, d.y};
+				}
+			} else {
+				const int key = u / (HD / 8), c = u % (HD / 8);
+				*(uint4 *)(k_s + key * (2 * HD) + 16 * k_unit<HD>(key, c)) = k[i];
+			}
+		}
+		if (VT == 256 || tid < VT) {
+			const int d = tid % VQ, kg = tid / VQ;
+			h2 t[4][4];   // [dim][key pair]
+#pragma unroll
+			for (int p = 0; p < 4; p++) {
+				if (Q8) {
+					const uint32_t a = v[2 * p][0] ^ kFlip, b = v[2 * p + 1][0] ^ kFlip;
+					const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x05010400u), hi = __builtin_amdgcn_perm(b, a, 0x07030602u);
+					t[0][p] = bytes_h2(lo, kLo2);
+					t[1][p] = bytes_h2(lo, kHi2);
+					t[2][p] = bytes_h2(hi, kLo2);
+					t[3][p] = bytes_h2(hi, kHi2);
+				} else {
+#pragma unroll
+					for (int w = 0; w < 2; w++) {
+						const uint32_t a = v[2 * p][w * (EB - 1)], b = v[2 * p + 1][w * (EB - 1)];
+						t[2 * w][p] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(b, a, 0x05040100u));
+						t[2 * w + 1][p] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(b, a, 0x07060302u));
+					}
+				}
+			}
+#pragma unroll
+			for (int i = 0; i < 4; i++) {
+				const int dim = 4 * d + i;
+				*(h8 *)(v_s + dim * (2 * kKeys) + 16 * v_unit(dim, kg)) =
+				    (h8){t[i][0].x, t[i][0].y, t[i][1].x, t[i][1].y, t[i][2].x, t[i][2].y, t[i][3].x, t[i][3].y};
+			}
+		}
+		if (tid < kKeys) {
+			E = max(E, scale_exp(wave_max(finite_or0(vs))));
+			ks_s[tid] = ks;
+			vs_s[tid] = __builtin_ldexpf(vs, -E);
+			if (tid == 0) *e_s = E;
+		}
+	}
+};
+
+// One wave's 32 rows over the chunks of a part. lim: the lane's row sees keys
+// (positions) below it; out: O^T (value sums, times 2^E), M and l.
+template <int HD, bool Q8>
+struct Tile {
+	static constexpr int KS = HD / 16, DT = HD / 32;
+	static constexpr int kKB = kKeys * HD * 2, kVB = HD * kKeys * 2;
+	struct Lds {
+		uint8_t k[2][kKB], v[2][kVB];
+		float ks[2][kKeys], vs[2][kKeys];
+		int e[2];
+	};
+	h8 qh[KS], ql[KS];
+	float esc;      // 2^e of the row
+	f16v o[DT];
+	float M, l;
+	int E;
+
+	// The lane's row q (null: an idle row), times scale log2(e).
+	__device__ __forceinline__ void query(const float *q, float scale, int lane) {
+		const int h = lane >> 5;
+		float x[KS * 8], a = 0.0f;
+#pragma unroll
+		for (int s = 0; s < KS; s++) {
+			float4 u = make_float4(0, 0, 0, 0), w = u;
+			if (q) {
+				u = *(const float4 *)(q + 16 * s + 8 * h);
+				w = *(const float4 *)(q + 16 * s + 8 * h + 4);
+			}
+			const float y[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+#pragma unroll
+			for (int j = 0; j < 8; j++) {
+				x[8 * s + j] = y[j] * scale;
+				a = __builtin_fmaxf(a, __builtin_fabsf(x[8 * s + j]));
+			}
+		}
+		a = __builtin_fmaxf(a, __shfl_xor(a, 32));
+		const int e = row_exp(a);
+		esc = __builtin_ldexpf(1.0f, e);
+#pragma unroll
+		for (int s = 0; s < KS; s++) split_q(x + 8 * s, e, qh[s], ql[s]);
+#pragma unroll
+		for (int d = 0; d < DT; d++)
+#pragma unroll
+			for (int v = 0; v < 16; v++) o[d][v] = 0.0f;
+		M = kNone;
+		l = 0.0f;
+		E = -126;
+	}
+
+	// 32 keys (half `t` of the chunk in LDS buffer `b`) at positions key0..; MASK: some row of the wave does not see
+	// all of them.
+	template <bool MASK>
+	__device__ __forceinline__ void half(const Lds &s, int b, int t, int key0, int lim, int lane) {
+		lane = fresh(lane);
+		const int h = lane >> 5, i = lane & 31;
+		// tile row i is key 16 (i>>4) + 8 ((i>>2)&1) + 4 ((i>>3)&1) + (i&3): register v of a lane is then key
+		// 16 (v>>3) + 8 h + (v&7)
+		const int key = 32 * t + (i & 16) + ((i << 1) & 8) + ((i >> 1) & 4) + (i & 3);
+		const uint8_t *kr = s.k[b] + key * (2 * HD);
+		f16v sc;
+#pragma unroll
+		for (int v = 0; v < 16; v++) sc[v] = 0.0f;
+#pragma unroll
+		for (int k = 0; k < KS; k++) {
+			const h8 a = *(const h8 *)(kr + 16 * k_unit<HD>(key, 2 * k + h));
+			sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[k], sc, 0, 0, 0);
+			sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[k], sc, 0, 0, 0);
+		}
+		feed<KS>();
+		__builtin_amdgcn_sched_barrier(0);
+		float mx = -INFINITY;
+#pragma unroll
+		for (int g = 0; g < 4; g++) {
+			const float4 ks = *(const float4 *)(s.ks[b] + 32 * t + 16 * (g >> 1) + 8 * h + 4 * (g & 1));
+			const float kv[4] = {ks.x, ks.y, ks.z, ks.w};
+#pragma unroll
+			for (int j = 0; j < 4; j++) {
+				const int v = 4 * g + j;
+				float x = sc[v] * kv[j];
+				if (MASK) x = key0 + 32 * t + 16 * (v >> 3) + 8 * h + (v & 7) < lim ? x : -INFINITY;
+				sc[v] = x;
+				mx = __builtin_fmaxf(mx, x);
+			}
+		}
+		mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32)) * esc;
+		if (__any(mx > M + kSlack)) {
+			const float mn = mx > M + kSlack ? mx : M;
+			const float f = exp2_(M - mn);   // 0 from kNone
+			M = mn;
+			l *= f;
+#pragma unroll
+			for (int d = 0; d < DT; d++)
+#pragma unroll
+				for (int v = 0; v < 16; v++) o[d][v] *= f;
+		}
+		const float c = kUp - M;
+		h2 ph[8], pl[8];
+#pragma unroll
+		for (int g = 0; g < 4; g++) {
+			const float4 vs = *(const float4 *)(s.vs[b] + 32 * t + 16 * (g >> 1) + 8 * h + 4 * (g & 1));
+			const float vv[4] = {vs.x, vs.y, vs.z, vs.w};
+			float w[4];
+#pragma unroll
+			for (int j = 0; j < 4; j++) {
+				const int v = 4 * g + j;
+				const float p = exp2_(__builtin_fmaf(sc[v], esc, c));
+				l += p;
+				w[j] = p * vv[j];
+				if (MASK) w[j] = sc[v] == -INFINITY ? 0.0f : w[j];   // a scale that may not be seen may be NaN
+			}
+			split2(w[0], w[1], ph[2 * g], pl[2 * g]);
+			split2(w[2], w[3], ph[2 * g + 1], pl[2 * g + 1]);
+		}
+		__builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+		for (int k = 0; k < 2; k++) {
+			const h8 bh = (h8){ph[4 * k].x, ph[4 * k].y, ph[4 * k + 1].x, ph[4 * k + 1].y,
+			                   ph[4 * k + 2].x, ph[4 * k + 2].y, ph[4 * k + 3].x, ph[4 * k + 3].y};
+			const h8 bl = (h8){pl[4 * k].x, pl[4 * k].y, pl[4 * k + 1].x, pl[4 * k + 1].y,
+			                   pl[4 * k + 2].x, pl[4 * k + 2].y, pl[4 * k + 3].x, pl[4 * k + 3].y};
+#pragma unroll
+			for (int d = 0; d < DT; d++) {
+				const int dim = 32 * d + i;
+				const h8 a = *(const h8 *)(s.v[b] + dim * (2 * kKeys) + 16 * v_unit(dim, 4 * t + 2 * k + h));
+				o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, bh, o[d], 0, 0, 0);
+				o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, bl, o[d], 0, 0, 0);
+			}
+		}
+		feed<2 * DT>();
+		__builtin_amdgcn_sched_barrier(0);
+	}
+
+	// N operand reads from LDS, two products each: the reads three ahead of their products.
+	template <int N>
+	static __device__ __forceinline__ void feed() {
+		__builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+#pragma unroll
+		for (int i = 0; i < N; i++) {
+			__builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+			if (i + 3 < N) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+		}
+	}
+
+	// Chunks [c0, c1) of a tile that sees positions below `end`: first the prefix's, then the slot's own from
+	// prefix_len on. lo, hi: the least and greatest lim of the wave's rows.
+	__device__ __forceinline__ void chunks(const AttnKv &c, int kvh, int slot, int end, int c0, int c1, int lim, int lo,
+	                                       int hi, Lds &s, int tid) {
+		constexpr int EB = Q8 ? 1 : 2;
+		const int lane = tid & 63;
+		const int pend = min(c.prefix_len, end), nc1 = (pend + kKeys - 1) / kKeys;
+		auto base = [&](int sl) { return ((size_t)sl * c.kvh + kvh) * c.max_seq; };
+		const size_t b0 = base(c.prefix_len > 0 ? c.prefix_slot : slot), b1 = base(slot);
+		Stage<HD, Q8> st;
+		auto load = [&](int ch) {
+			const bool pre = ch < nc1;
+			const size_t r = pre ? b0 : b1;
+			const uint32_t n = (uint32_t)(pre ? pend : end);   // rows past it read as zeros
+			st.load(stream_rsrc(uniform_ptr(c.k + r * HD * EB), n * HD * EB), stream_rsrc(uniform_ptr(c.v + r * HD * EB), n * HD * EB),
+			        stream_rsrc(uniform_ptr(c.ks + r), n * 4), stream_rsrc(uniform_ptr(c.vs + r), n * 4),
+			        pre ? kKeys * ch : c.prefix_len + kKeys * (ch - nc1), fresh(tid));
+		};
+		int Es = -126;
+		if (c0 < c1) {
+			load(c0);
+			st.store(s.k[0], s.v[0], s.ks[0], s.vs[0], &s.e[0], Es, tid);
+		}
+		__syncthreads();
+		for (int ch = c0; ch < c1; ch++) {
+			const int b = (ch - c0) & 1;
+			const bool more = ch + 1 < c1;
+			if (more) load(ch + 1);
+			__builtin_amdgcn_sched_barrier(0);
+			const bool pre = ch < nc1;
+			const int key0 = pre ? kKeys * ch : c.prefix_len + kKeys * (ch - nc1);
+			// rows see keys below min(lim, what the chunk holds)
+			const int top = pre ? pend : end;
+			const int e = s.e[b];
+			if (e != E) {
+				const float f = __builtin_ldexpf(1.0f, E - e);
+#pragma unroll
+				for (int d = 0; d < DT; d++)
+#pragma unroll
+					for (int v = 0; v < 16; v++) o[d][v] *= f;
+				E = e;
+			}
+#pragma unroll 1
+			for (int t = 0; t < 2; t++) {
+				const int k0 = key0 + 32 * t;
+				if (k0 >= min(hi, top)) continue;   // no row of the wave sees any of these keys
+				if (k0 + 32 <= min(lo, top)) half<false>(s, b, t, key0, 0, lane);
+				else half<true>(s, b, t, key0, min(lim, top), lane);
+			}
+			__builtin_amdgcn_sched_barrier(0);
+			if (more) st.store(s.k[b ^ 1], s.v[b ^ 1], s.ks[b ^ 1], s.vs[b ^ 1], &s.e[b ^ 1], Es, fresh(tid));
+			__syncthreads();
+		}
+		l += __shfl_xor(l, 32);
+	}
+
+	// The row's value sums times f to dst.
+	__device__ __forceinline__ void put(float *dst, float f, int lane) const {
+		const int h = lane >> 5;
+#pragma unroll
+		for (int d = 0; d < DT; d++)
+#pragma unroll
+			for (int g = 0; g < 4; g++)
+				*(float4 *)(dst + 32 * d + 8 * g + 4 * h) = make_float4(o[d][4 * g] * f, o[d][4 * g + 1] * f,
+				                                                        o[d][4 * g + 2] * f, o[d][4 * g + 3] * f);
+	}
+};
+
+__device__ __forceinline__ int wave_min_i(int v) {
+#pragma unroll
+	for (int k = 1; k < 64; k <<= 1) v = min(v, __shfl_xor(v, k));
+	return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int wave_max_i(int v) {
+#pragma unroll
+	for (int k = 1; k < 64; k <<= 1) v = max(v, __shfl_xor(v, k));
+	return __builtin_amdgcn_readfirstlane(v);
+}
+
+// chunks of a tile that sees positions below `end`
+__host__ __device__ __forceinline__ int tile_chunks(int end, int prefix) {
+	const int p = prefix < end ? prefix : end;
+	return (p + kKeys - 1) / kKeys + (end - p + kKeys - 1) / kKeys;
+}
+
+// Records: value sums rec_o [record][HD] and (M, l) rec_ml [record].
+template <int HD, bool Q8>
+__global__ __launch_bounds__(256, 2) void prompt_kernel(AttnKv c, SeqTab t, float *out, int64_t ldo, const float *q,
+                                                        int64_t ldq, int G, float scale, float *__restrict__ rec_o,
+                                                        float2 *__restrict__ rec_ml) {
+	__shared__ typename Tile<HD, Q8>::Lds s;
+	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+	const int kvh = blockIdx.x % c.kvh, item = blockIdx.x / c.kvh;
+	int sq = 0;
+	while (item >= t.item[sq + 1]) sq++;
+	const int ns = t.nsplit[sq], it = item - t.item[sq];
+	const int ntile = (t.len[sq] + t.tile_tokens - 1) / t.tile_tokens;
+	const int tile = ntile - 1 - it / ns, part = it % ns;
+	const int tok0 = tile * t.tile_tokens, ntok = min(t.tile_tokens, t.len[sq] - tok0);
+	const int end = t.start[sq] + tok0 + ntok, nc = tile_chunks(end, c.prefix_len);
+	const int c0 = part * t.unit, c1 = min(nc, c0 + t.unit);
+	if (c0 >= nc) return;
+	const int r = 32 * wave + (lane & 31), tok = r / G, g = r - tok * G;
+	const bool on = tok < ntok;
+	const int lim = on ? t.start[sq] + tok0 + tok + 1 : 0;
+	const int lo = wave_min_i(on ? lim : 0x7FFFFFFF), hi = wave_max_i(lim);
+	const int64_t row = (int64_t)t.row[sq] + tok0 + tok;
+	const int head = kvh * G + g;
+	Tile<HD, Q8> w;
+	w.query(on ? q + row * ldq + head * HD : nullptr, scale, lane);
+	w.chunks(c, kvh, t.slot[sq], end, c0, c1, lim, lo, hi, s, tid);
+	if (!on) return;
+	if (nc <= t.unit) {
+		w.put(out + row * ldo + head * HD, __builtin_ldexpf(1.0f, w.E) / w.l, lane);
+		return;
+	}
+	const size_t rec = (size_t)t.rec[sq] + ((size_t)(tok0 + tok) * (c.kvh * G) + head) * ns + part;
+	w.put(rec_o + rec * HD, __builtin_ldexpf(1.0f, w.E), lane);
+	if (lane < 32) rec_ml[rec] = make_float2(w.M, w.l);
+}
+
+// The prefix of a batch: rows are (sequence, head of the group), every row
+// over the prefix's keys below its length; always to records.
+template <int HD, bool Q8>
+__global__ __launch_bounds__(256, 2) void prefix_kernel(AttnKv c, const float *q, int64_t ldq, const int *__restrict__ slot,
+                                                        const int *__restrict__ len, int n_seq, int G, float scale,
+                                                        int unit, int nrec, float *__restrict__ rec_o,
+                                                        float2 *__restrict__ rec_ml) {
+	__shared__ typename Tile<HD, Q8>::Lds s;
+	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+	const int kvh = blockIdx.x % c.kvh, part = blockIdx.x / c.kvh;
+	const int64_t r = (int64_t)blockIdx.y * kTileRows + 32 * wave + (lane & 31);
+	const int sq = (int)(r / G), g = (int)(r - (int64_t)sq * G);
+	const bool on = sq < n_seq;
+	int lim = 0;
+	if (on) {
+		const int sl = slot ? slot[sq] : sq;
+		lim = sl < 0 || sl >= c.n_slots ? 0 : min(max(len[sq], 0), c.prefix_len);
+	}
+	const int lo = wave_min_i(on ? lim : 0x7FFFFFFF), hi = wave_max_i(lim);
+	const int head = kvh * G + g, nc = (c.prefix_len + kKeys - 1) / kKeys;
+	Tile<HD, Q8> w;
+	w.query(on ? q + sq * ldq + head * HD : nullptr, scale, lane);
+	w.chunks(c, kvh, c.prefix_slot, c.prefix_len, part * unit, min(nc, part * unit + unit), lim, lo, hi, s, tid);
+	if (!on) return;
+	const size_t rec = ((size_t)sq * (c.kvh * G) + head) * nrec + part;
+	w.put(rec_o + rec * HD, __builtin_ldexpf(1.0f, w.E), lane);
+	if (lane < 32) rec_ml[rec] = make_float2(w.M, w.l);
+}
+
+// ── single tokens: the up to 16 query heads of a group over one sequence's own keys ──
+//
+// Workgroup (key/value head, part, sequence); each wave takes steps of 32
+// keys, codes straight from memory into the matrix-core operands
+// (v_mfma_f32_16x16x32_f16: keys need no transposition, values are paired by
+// byte permutes), keys of the next step loaded while this one's weights form
+// and values while the next scores do; the waves meet once, in LDS.
+template <int HD, bool Q8>
+struct Row16 {
+	static constexpr int EB = Q8 ? 1 : 2;
+	static constexpr int KS = HD / 32;                // 32-dim steps of the score product
+	static constexpr int KL = HD * EB / 64;           // 16-byte loads of a key per lane (a key is four lanes)
+	static constexpr int VD = HD / 16;                // dims per lane of a value row (a row is 16 lanes)
+	static constexpr int VW = VD * EB / 4;            // dwords of them
+	h8 qh[KS], ql[KS];
+	float esc;
+	f4 o[VD];
+	float M, l;
+	int E;
+	uint4 k[2][KL];
+	uint32_t v[8][VW];
+	float ks[8], vs[8];
+
+	// dims of step s, lane group g, place j: KL loads of 16 bytes at 16 g + 64 i
+	static __device__ __forceinline__ int dim0(int s, int g) {
+		return Q8 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g;
+	}
+
+	__device__ __forceinline__ void query(const float *q, float scale, int lane) {
+		const int g = lane >> 4;
+		float x[KS * 8], a = 0.0f;
+#pragma unroll
+		for (int s = 0; s < KS; s++) {
+			float4 u = make_float4(0, 0, 0, 0), w = u;
+			if (q) {
+				u = *(const float4 *)(q + dim0(s, g));
+				w = *(const float4 *)(q + dim0(s, g) + 4);
+			}
+			const float y[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+#pragma unroll
+			for (int j = 0; j < 8; j++) {
+				x[8 * s + j] = y[j] * scale;
+				a = __builtin_fmaxf(a, __builtin_fabsf(x[8 * s + j]));
+			}
+		}
+		a = __builtin_fmaxf(a, __shfl_xor(a, 16));
+		a = __builtin_fmaxf(a, __shfl_xor(a, 32));
+		const int e = row_exp(a);
+		esc = __builtin_ldexpf(1.0f, e);
+#pragma unroll
+		for (int s = 0; s < KS; s++) split_q(x + 8 * s, e, qh[s], ql[s]);
+#pragma unroll
+		for (int d = 0; d < VD; d++) o[d] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+		M = kNone;
+		l = 0.0f;
+		E = -126;
+	}
+
+	// tile row i of key tile t is key 8 (i>>2) + 4 t + (i&3): a lane's eight scores are keys 8 g + 0..7
+	__device__ __forceinline__ void load_k(__amdgpu_buffer_rsrc_t kr, __amdgpu_buffer_rsrc_t ksr, int key0, int lane) {
+		const int i = lane & 15, g = lane >> 4;
+#pragma unroll
+		for (int t = 0; t < 2; t++) {
+			const uint32_t off = (uint32_t)(key0 + 8 * (i >> 2) + 4 * t + (i & 3)) * (HD * EB) + 16u * g;
+#pragma unroll
+			for (int n = 0; n < KL; n++) k[t][n] = ld_b128(kr, off + 64u * n);
+		}
+#pragma unroll
+		for (int t = 0; t < 2; t++) {
+			const float4 x = __builtin_bit_cast(float4, ld_b128(ksr, 4u * (uint32_t)(key0 + 8 * g + 4 * t)));
+			ks[4 * t] = x.x, ks[4 * t + 1] = x.y, ks[4 * t + 2] = x.z, ks[4 * t + 3] = x.w;
+		}
+	}
+	__device__ __forceinline__ void load_v(__amdgpu_buffer_rsrc_t vr, __amdgpu_buffer_rsrc_t vsr, int key0, int lane) {
+		const int i = lane & 15, g = lane >> 4;
+#pragma unroll
+		for (int j = 0; j < 8; j++) {
+			const uint32_t off = ((uint32_t)(key0 + 8 * g + j) * HD + VD * i) * EB;
+			if (VW == 1) v[j][0] = __builtin_amdgcn_raw_buffer_load_b32(vr, (int)off, 0, 0);
+			if (VW == 2) {
+				const uint2 x = ld_b64(vr, off);
+				v[j][0] = x.x;
+				v[j][VW - 1] = x.y;
+			}
+			if (VW == 4) {
+				const uint4 x = ld_b128(vr, off);
+				v[j][0] = x.x;
+				v[j][1 % VW] = x.y;
+				v[j][2 % VW] = x.z;
+				v[j][VW - 1] = x.w;
+			}
+		}
+#pragma unroll
+		for (int t = 0; t < 2; t++) {
+			const float4 x = __builtin_bit_cast(float4, ld_b128(vsr, 4u * (uint32_t)(key0 + 8 * g + 4 * t)));
+			vs[4 * t] = x.x, vs[4 * t + 1] = x.y, vs[4 * t + 2] = x.z, vs[4 * t + 3] = x.w;
+		}
+	}
+
+	__device__ __forceinline__ void scores(f4 sc[2]) {
+#pragma unroll
+		for (int t = 0; t < 2; t++) {
+			sc[t] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+			for (int s = 0; s < KS; s++) {
+				h8 a;
+				if (Q8) {
+					const uint32_t w[4] = {k[t][s >> 1].x, k[t][s >> 1].y, k[t][s >> 1].z, k[t][s >> 1].w};
+					const uint32_t x = w[2 * (s & 1)] ^ kFlip, y = w[2 * (s & 1) + 1] ^ kFlip;
+					const h2 p = bytes_h2(x, kLo2), q2 = bytes_h2(x, kHi2), r = bytes_h2(y, kLo2), u = bytes_h2(y, kHi2);
+					a = (h8){p.x, p.y, q2.x, q2.y, r.x, r.y, u.x, u.y};
+				} else {
+					a = __builtin_bit_cast(h8, k[t][s % KL]);
+				}
+				sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[s], sc[t], 0, 0, 0);
+				sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[s], sc[t], 0, 0, 0);
+			}
+		}
+	}
+
+	// Weights of the 32 keys from key0, those at end and past it left out.
+	__device__ __forceinline__ void weigh(f4 sc[2], int key0, int end, int lane, h8 &ph, h8 &pl) {
+		const int g = lane >> 4;
+		float x[8], mx = -INFINITY, vm = 0.0f;
+#pragma unroll
+		for (int j = 0; j < 8; j++) {
+			x[j] = key0 + 8 * g + j < end ? sc[j >> 2][j & 3] * ks[j] : -INFINITY;
+			mx = __builtin_fmaxf(mx, x[j]);
+			vm = __builtin_fmaxf(vm, finite_or0(vs[j]));
+		}
+		mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16));
+		vm = __builtin_fmaxf(vm, __shfl_xor(vm, 16));
+		mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32)) * esc;
+		vm = __builtin_fmaxf(vm, __shfl_xor(vm, 32));
+		const int e = max(E, scale_exp(vm));
+		if (__any(mx > M + kSlack || e != E)) {
+			const float mn = mx > M + kSlack ? mx : M;
+			const float f = exp2_(M - mn);
+			M = mn;
+			l *= f;
+			const float fo = __builtin_ldexpf(f, E - e);
+			E = e;
+#pragma unroll
+			for (int d = 0; d < VD; d++) o[d] *= fo;
+		}
+		const float c = kUp - M, vf = __builtin_ldexpf(1.0f, -E);
+#pragma unroll
+		for (int j = 0; j < 8; j += 2) {
+			float w[2];
+#pragma unroll
+			for (int n = 0; n < 2; n++) {
+				const float p = exp2_(__builtin_fmaf(x[j + n], esc, c));
+				l += p;
+				w[n] = key0 + 8 * g + j + n < end ? p * (vs[j + n] * vf) : 0.0f;
+			}
+			h2 a, b;
+			split2(w[0], w[1], a, b);
+			ph[j] = a.x, ph[j + 1] = a.y;
+			pl[j] = b.x, pl[j + 1] = b.y;
+		}
+	}
+
+	// tile row i of dim tile d is dim VD i + d
+	__device__ __forceinline__ void values(h8 ph, h8 pl) {
+#pragma unroll
+		for (int d = 0; d < VD; d += 2) {
+			h2 t[2][4];
+#pragma unroll
+			for (int p = 0; p < 4; p++) {
+				const uint32_t a = v[2 * p][d * EB / 4], b = v[2 * p + 1][d * EB / 4];
+				if (Q8) {
+					const uint32_t m = __builtin_amdgcn_perm(b ^ kFlip, a ^ kFlip, d & 2 ? 0x07030602u : 0x05010400u);
+					t[0][p] = bytes_h2(m, kLo2);
+					t[1][p] = bytes_h2(m, kHi2);
+				} else {
+					t[0][p] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(b, a, 0x05040100u));
+					t[1][p] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(b, a, 0x07060302u));
+				}
+			}
+#pragma unroll
+			for (int n = 0; n < 2; n++) {
+				const h8 a = (h8){t[n][0].x, t[n][0].y, t[n][1].x, t[n][1].y, t[n][2].x, t[n][2].y, t[n][3].x, t[n][3].y};
+				o[d + n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph, o[d + n], 0, 0, 0);
+				o[d + n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl, o[d + n], 0, 0, 0);
+			}
+		}
+	}
+};
+
+// Keys per part of a sequence with n own keys in at most `parts` parts.
+__device__ __forceinline__ int part_keys(int n, int parts) {
+	const int per = (n + parts - 1) / parts;
+	return (per + 32 * kWaves - 1) / (32 * kWaves) * (32 * kWaves);
+}
+// A sequence's own keys [prefix, end): end, 0 where it has no slot.
+__device__ __forceinline__ int own_end(const AttnKv &c, const int *slot, const int *len, int sq, int &sl) {
+	sl = slot ? slot[sq] : sq;
+	return sl < 0 || sl >= c.n_slots ? 0 : min(max(len[sq], 0), c.max_seq);
+}
+
+template <int HD, bool Q8>
+__global__ __launch_bounds__(256) void decode_kernel(AttnKv c, float *out, int64_t ldo, const float *q, int64_t ldq,
+                                                     const int *__restrict__ slot, const int *__restrict__ len, int G,
+                                                     float scale, int parts, int rec0, int nrec,
+                                                     float *__restrict__ rec_o, float2 *__restrict__ rec_ml) {
+	constexpr int EB = Q8 ? 1 : 2;
+	__shared__ float o_s[kWaves][kMaxGroup][HD + 4];
+	__shared__ float ml_s[kWaves][kMaxGroup][2];
+	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+	const int kvh = blockIdx.x, part = blockIdx.y, sq = blockIdx.z;
+	int sl;
+	const int end = own_end(c, slot, len, sq, sl), n = max(end - c.prefix_len, 0);
+	const int per = part_keys(n, parts);
+	const int first = c.prefix_len + part * per, last = min(end, first + per);   // this part's keys
+	if (first >= end && (part > 0 || nrec > 0)) return;   // a record that the merge does not read
+	const int i = lane & 15, g = lane >> 4;
+	const int head = kvh * G + i;
+	Row16<HD, Q8> w;
+	w.query(i < G ? q + sq * ldq + head * HD : nullptr, scale, lane);
+	const size_t r = ((size_t)(end > 0 ? sl : 0) * c.kvh + kvh) * c.max_seq;
+	const uint32_t rows = (uint32_t)max(last, 0);
+	const __amdgpu_buffer_rsrc_t kr = stream_rsrc(uniform_ptr(c.k + r * HD * EB), rows * HD * EB);
+	const __amdgpu_buffer_rsrc_t vr = stream_rsrc(uniform_ptr(c.v + r * HD * EB), rows * HD * EB);
+	const __amdgpu_buffer_rsrc_t ksr = stream_rsrc(uniform_ptr(c.ks + r), rows * 4);
+	const __amdgpu_buffer_rsrc_t vsr = stream_rsrc(uniform_ptr(c.vs + r), rows * 4);
+	int key0 = first + 32 * wave;
+	if (key0 < last) {
+		w.load_k(kr, ksr, key0, lane);
+		w.load_v(vr, vsr, key0, lane);
+		for (; key0 < last; key0 += 32 * kWaves) {
+			f4 sc[2];
+			h8 ph, pl;
+			w.scores(sc);
+			w.weigh(sc, key0, last, lane, ph, pl);
+			const int next = key0 + 32 * kWaves;
+			if (next < last) w.load_k(kr, ksr, next, lane);
+			w.values(ph, pl);
+			if (next < last) w.load_v(vr, vsr, next, lane);
+		}
+	}
+	w.l += __shfl_xor(w.l, 16);
+	w.l += __shfl_xor(w.l, 32);
+	// the waves' sums meet: rows i, dims VD (4 g + v) + d
+	const float f = __builtin_ldexpf(1.0f, w.E);
+#pragma unroll
+	for (int v = 0; v < 4; v++)
+#pragma unroll
+		for (int d = 0; d < w.VD; d += 4)
+			*(float4 *)&o_s[wave][i][w.VD * (4 * g + v) + d] =
+			    make_float4(w.o[d][v] * f, w.o[d + 1][v] * f, w.o[d + 2][v] * f, w.o[d + 3][v] * f);
+	if (g == 0) {
+		ml_s[wave][i][0] = w.M;
+		ml_s[wave][i][1] = w.l;
+	}
+	__syncthreads();
+	for (int t = tid; t < G * (HD / 4); t += 256) {
+		const int row = t / (HD / 4), d = t % (HD / 4) * 4;
+		float m = ml_s[0][row][0];
+#pragma unroll
+		for (int k = 1; k < kWaves; k++) m = __builtin_fmaxf(m, ml_s[k][row][0]);
+		float ls = 0.0f;
+		float4 a = make_float4(0, 0, 0, 0);
+#pragma unroll
+		for (int k = 0; k < kWaves; k++) {
+			const float x = exp2_(ml_s[k][row][0] - m);
+			const float4 b = *(const float4 *)&o_s[k][row][d];
+			ls = __builtin_fmaf(ml_s[k][row][1], x, ls);
+			a.x = __builtin_fmaf(b.x, x, a.x);
+			a.y = __builtin_fmaf(b.y, x, a.y);
+			a.z = __builtin_fmaf(b.z, x, a.z);
+			a.w = __builtin_fmaf(b.w, x, a.w);
+		}
+		const int hd = kvh * G + row;
+		if (nrec == 0) {
+			const float z = ls == 0.0f ? 0.0f : 1.0f / ls;
+			*(float4 *)(out + sq * ldo + hd * HD + d) = make_float4(a.x * z, a.y * z, a.z * z, a.w * z);
+		} else {
+			const size_t rec = ((size_t)sq * (c.kvh * G) + hd) * nrec + rec0 + part;
+			*(float4 *)(rec_o + rec * HD + d) = a;
+			if (d == 0) rec_ml[rec] = make_float2(m, ls);
+		}
+	}
+}
+
+// One head's n records joined by HD/4 lanes of a wave's 64 (four dims each,
+// 256/HD records at a time), in an order that their number alone sets.
+template <int HD>
+__device__ __forceinline__ void join(const float *__restrict__ ro, const float2 *__restrict__ ml, int n, float *dst, int lane) {
+	constexpr int L = HD / 4, W = 64 / L;
+	float m = kNone;
+	for (int k = lane; k < n; k += 64) m = __builtin_fmaxf(m, ml[k].x);
+	m = wave_max(m);
+	float ls = 0.0f;
+	float4 a = make_float4(0, 0, 0, 0);
+	const int d = lane % L * 4;
+#pragma unroll 4
+	for (int k = lane / L; k < n; k += W) {
+		const float2 x = ml[k];
+		const float f = exp2_(x.x - m);
+		const float4 b = *(const float4 *)(ro + (size_t)k * HD + d);
+		ls = __builtin_fmaf(x.y, f, ls);
+		a.x = __builtin_fmaf(b.x, f, a.x);
+		a.y = __builtin_fmaf(b.y, f, a.y);
+		a.z = __builtin_fmaf(b.z, f, a.z);
+		a.w = __builtin_fmaf(b.w, f, a.w);
 	}
 #pragma unroll
-	for (int i = 0; i < N; i++) out[lane + 64 * i] = end > 0 ? o[i] / l : 0.0f;
+	for (int k = L; k < 64; k <<= 1) {
+		ls += __shfl_xor(ls, k);
+		a.x += __shfl_xor(a.x, k);
+		a.y += __shfl_xor(a.y, k);
+		a.z += __shfl_xor(a.z, k);
+		a.w += __shfl_xor(a.w, k);
+	}
+	if (lane < L) {
+		const float z = ls == 0.0f ? 0.0f : 1.0f / ls;
+		*(float4 *)(dst + d) = make_float4(a.x * z, a.y * z, a.z * z, a.w * z);
+	}
 }
 
-template <int HD, bool Q8>
-__global__ __launch_bounds__(64) void decode_kernel(AttnKv c, float *out, int64_t ldo, const float *q, int64_t ldq,
-                                                    const int *__restrict__ slot, const int *__restrict__ len, int G,
-                                                    float scale) {
-	const int s = blockIdx.x, h = blockIdx.y;
-	const int sl = slot ? slot[s] : s;
-	int end = min(max(len[s], 0), c.max_seq);
-	if (sl < 0 || sl >= c.n_slots) end = 0;
-	attend<HD, Q8>(c, sl, end, q + s * ldq + h * HD, out + s * ldo + h * HD, h / G, scale);
+template <int HD>
+__global__ __launch_bounds__(64) void decode_join_kernel(AttnKv c, float *out, int64_t ldo, const int *__restrict__ slot,
+                                                         const int *__restrict__ len, int H, int parts, int rec0,
+                                                         int nrec, const float *__restrict__ rec_o,
+                                                         const float2 *__restrict__ rec_ml) {
+	const int h = blockIdx.x, sq = blockIdx.y;
+	int sl;
+	const int end = own_end(c, slot, len, sq, sl), n = max(end - c.prefix_len, 0);
+	const int per = part_keys(n, parts), used = n > 0 ? (n + per - 1) / per : 0;
+	const size_t rec = ((size_t)sq * H + h) * nrec;
+	join<HD>(rec_o + rec * HD, rec_ml + rec, rec0 + used, out + sq * ldo + h * HD, threadIdx.x);
 }
 
-template <int HD, bool Q8>
-__global__ __launch_bounds__(64) void prompt_kernel(AttnKv c, SeqTab t, float *out, int64_t ldo, const float *q,
-                                                    int64_t ldq, int G, float scale) {
-	const int row = blockIdx.x, h = blockIdx.y;
-	int s = 0;
-	while (row >= t.row[s + 1]) s++;
-	attend<HD, Q8>(c, t.slot[s], t.start[s] + row - t.row[s] + 1, q + row * ldq + h * HD, out + row * ldo + h * HD,
-	               h / G, scale);
+// Tokens of sequence sq of the launch whose tile was split.
+template <int HD>
+__global__ __launch_bounds__(64) void prompt_join_kernel(SeqTab t, int sq, int prefix_len, float *out, int64_t ldo, int H,
+                                                         const float *__restrict__ rec_o,
+                                                         const float2 *__restrict__ rec_ml) {
+	const int tok = blockIdx.x, h = blockIdx.y, ns = t.nsplit[sq];
+	const int tile = tok / t.tile_tokens;
+	const int nc = tile_chunks(t.start[sq] + min((tile + 1) * t.tile_tokens, t.len[sq]), prefix_len);
+	if (nc <= t.unit) return;
+	const size_t rec = (size_t)t.rec[sq] + ((size_t)tok * H + h) * ns;
+	join<HD>(rec_o + rec * HD, rec_ml + rec, (nc + t.unit - 1) / t.unit, out + ((int64_t)t.row[sq] + tok) * ldo + h * HD,
+	         threadIdx.x);
 }
 
 int attn_check(float *out, int64_t ldo, const float *q, int64_t ldq, const hako_gpu_kv *kv, int n_seq, int H,
@@ -100,21 +872,104 @@ AttnKv attn_kv(const hako_gpu_kv *kv, int prefix_slot, int prefix_len) {
 	        kv->n_kv_heads, prefix_slot, prefix_len};
 }
 
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// Room for n records of HD value sums and (M, l).
+int records(size_t n, int HD, float **o, float2 **ml) {
+	void *p = nullptr;
+	if (int rc = workspace(kWsAttn, n * (HD + 2) * sizeof(float), &p)) return rc;
+	*o = (float *)p;
+	*ml = (float2 *)(*o + n * HD);
+	return HAKO_GPU_OK;
+}
+
+template <int HD, bool Q8>
+int decode(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq, const int *slot, const int *len,
+           int n_seq, int H, float scale) {
+	const int G = H / c.kvh, own = c.max_seq - c.prefix_len;
+	const int slots = 2 * cu_count();   // workgroups that run at once
+	// own keys: parts of at least 32 keys a wave, until the workgroups fill the chip
+	int parts = (own + 32 * kWaves - 1) / (32 * kWaves);
+	const int64_t pairs = (int64_t)n_seq * c.kvh;
+	const int fill = (int)std::max<int64_t>(1, (slots + pairs - 1) / pairs);
+	parts = std::max(1, std::min(parts, fill));
+	// the prefix: parts of whole chunks, until its tiles fill the chip
+	const int64_t tiles = ((int64_t)n_seq * G + kTileRows - 1) / kTileRows;
+	const int nc = (c.prefix_len + kKeys - 1) / kKeys;
+	int unit = 1, pparts = 0;
+	if (nc) {
+		const int want = (int)std::max<int64_t>(1, slots / (tiles * c.kvh));
+		unit = std::max(1, (nc + want - 1) / want);
+		pparts = (nc + unit - 1) / unit;
+	}
+	const int nrec = pparts + parts > 1 ? pparts + parts : 0;
+	float *ro = nullptr;
+	float2 *ml = nullptr;
+	if (nrec)
+		if (int rc = records((size_t)n_seq * H * nrec, HD, &ro, &ml)) return rc;
+	if (pparts) {
+		hipLaunchKernelGGL((prefix_kernel<HD, Q8>), dim3(c.kvh * pparts, (unsigned)tiles), dim3(256), 0, stream(), c, q, ldq,
+		                   slot, len, n_seq, G, scale * kLog2e, unit, nrec, ro, ml);
+		HK_LAUNCHED("attention prefix");
+	}
+	hipLaunchKernelGGL((decode_kernel<HD, Q8>), dim3(c.kvh, parts, n_seq), dim3(256), 0, stream(), c, out, ldo, q, ldq, slot,
+	                   len, G, scale * kLog2e, parts, pparts, nrec, ro, ml);
+	HK_LAUNCHED("attention");
+	if (nrec) {
+		hipLaunchKernelGGL(decode_join_kernel<HD>, dim3(H, n_seq), dim3(64), 0, stream(), c, out, ldo, slot, len, H, parts,
+		                   pparts, nrec, ro, ml);
+		HK_LAUNCHED("attention join");
+	}
+	return HAKO_GPU_OK;
+}
+
+// One launch of up to kSeqs sequences, in the order given (the longest first).
+template <int HD, bool Q8>
+int prompt(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, const float *q, int64_t ldq, int H, float scale) {
+	const int G = H / c.kvh;
+	t.tile_tokens = kTileRows / G;
+	// chunks per part: what each of the workgroups that run at once would take if all were shared out evenly
+	int64_t total = 0;
+	for (int s = 0; s < t.n; s++)
+		for (int k = 0; k < t.len[s]; k += t.tile_tokens)
+			total += tile_chunks(t.start[s] + std::min(k + t.tile_tokens, t.len[s]), c.prefix_len);
+	const int64_t slots = 2 * cu_count();
+	t.unit = (int)std::max<int64_t>(4, (total * c.kvh + slots - 1) / slots);
+	int64_t items = 0, recs = 0;
+	for (int s = 0; s < t.n; s++) {
+		t.nsplit[s] = (tile_chunks(t.start[s] + t.len[s], c.prefix_len) + t.unit - 1) / t.unit;
+		t.item[s] = (int)items;
+		items += (int64_t)((t.len[s] + t.tile_tokens - 1) / t.tile_tokens) * t.nsplit[s];
+		t.rec[s] = (uint32_t)recs;
+		if (t.nsplit[s] > 1) recs += (int64_t)t.len[s] * H * t.nsplit[s];
+	}
+	t.item[t.n] = (int)items;
+	if (items * c.kvh > 0x7FFFFFFF || recs > 0xFFFFFFFFll)
+		return set_error(HAKO_GPU_EINVAL, "%lld tiles and %lld records in one call", (long long)(items * c.kvh), (long long)recs);
+	float *ro = nullptr;
+	float2 *ml = nullptr;
+	if (recs)
+		if (int rc = records((size_t)recs, HD, &ro, &ml)) return rc;
+	hipLaunchKernelGGL((prompt_kernel<HD, Q8>), dim3((unsigned)(items * c.kvh)), dim3(256), 0, stream(), c, t, out, ldo, q,
+	                   ldq, G, scale * kLog2e, ro, ml);
+	HK_LAUNCHED("attention");
+	for (int s = 0; s < t.n; s++)
+		if (t.nsplit[s] > 1) {
+			hipLaunchKernelGGL(prompt_join_kernel<HD>, dim3(t.len[s], H), dim3(64), 0, stream(), t, s, c.prefix_len, out, ldo, H,
+			                   ro, ml);
+			HK_LAUNCHED("attention join");
+		}
+	return HAKO_GPU_OK;
+}
+
 }  // namespace
 }  // namespace hako
 
 using namespace hako;
 
-#define HK_KV_SWITCH(kv, CALL)                             \
-	do {                                                   \
-		if ((kv)->head_dim == 128) {                       \
-			if ((kv)->type == HAKO_KV_Q8) CALL(128, true); \
-			else CALL(128, false);                         \
-		} else {                                           \
-			if ((kv)->type == HAKO_KV_Q8) CALL(64, true);  \
-			else CALL(64, false);                          \
-		}                                                  \
-	} while (0)
+#define HK_KV_SWITCH(kv, CALL)                                     \
+	((kv)->head_dim == 128 ? ((kv)->type == HAKO_KV_Q8 ? CALL(128, true) : CALL(128, false)) \
+	                       : ((kv)->type == HAKO_KV_Q8 ? CALL(64, true) : CALL(64, false)))
 
 extern "C" {
 
@@ -125,15 +980,13 @@ int hako_gpu_attn_decode(float *out, int64_t out_stride, const float *q, int64_t
 	if (!len && n_seq) return set_error(HAKO_GPU_EINVAL, "null lengths");
 	if (!slot && n_seq > kv->n_slots)
 		return set_error(HAKO_GPU_EINVAL, "%d sequences without slots in a cache of %d", n_seq, kv->n_slots);
+	if (n_seq > 65535) return set_error(HAKO_GPU_EINVAL, "%d sequences in one call (at most 65535)", n_seq);
 	if (int rc = require_device()) return rc;
 	if (n_seq == 0) return ok();
 	const AttnKv c = attn_kv(kv, prefix_slot, prefix_len);
-#define HK_DECODE(HD, Q8)                                                                                          \
-	hipLaunchKernelGGL((decode_kernel<HD, Q8>), dim3(n_seq, n_heads), dim3(64), 0, stream(), c, out, out_stride, q, \
-	                   q_stride, slot, len, n_heads / kv->n_kv_heads, scale)
-	HK_KV_SWITCH(kv, HK_DECODE);
+#define HK_DECODE(HD, Q8) decode<HD, Q8>(c, out, out_stride, q, q_stride, slot, len, n_seq, n_heads, scale)
+	if (int rc = HK_KV_SWITCH(kv, HK_DECODE)) return rc;
 #undef HK_DECODE
-	HK_LAUNCHED("attention");
 	return ok();
 }
 
@@ -154,26 +1007,25 @@ int hako_gpu_attn_prompt(float *out, int64_t out_stride, const float *q, int64_t
 	if (rows > 0x7FFFFFFF) return set_error(HAKO_GPU_EINVAL, "%lld tokens in one call", (long long)rows);
 	if (int rc = require_device()) return rc;
 	const AttnKv c = attn_kv(kv, prefix_slot, prefix_len);
-	int64_t row = 0;
-	for (int s = 0; s < n_seq;) {
-		SeqTab t;
-		t.n = 0;
-		t.row[0] = 0;
-		const int64_t row0 = row;
-		for (; s < n_seq && t.n < kSeqs; s++) {
-			if (len[s] == 0) continue;
+	// the sequences with tokens, those that end last (the longest tiles) first
+	std::vector<int> order, row(n_seq);
+	for (int s = 0, r = 0; s < n_seq; r += len[s++]) {
+		row[s] = r;
+		if (len[s]) order.push_back(s);
+	}
+	std::stable_sort(order.begin(), order.end(), [&](int a, int b) { return start[a] + len[a] > start[b] + len[b]; });
+	for (size_t i = 0; i < order.size();) {
+		SeqTab t{};
+		for (; i < order.size() && t.n < kSeqs; i++, t.n++) {
+			const int s = order[i];
+			t.row[t.n] = row[s];
+			t.len[t.n] = len[s];
 			t.slot[t.n] = slot ? slot[s] : s;
 			t.start[t.n] = start[s];
-			row += len[s];
-			t.row[++t.n] = (int)(row - row0);
 		}
-		if (t.n == 0) break;
-#define HK_PROMPT(HD, Q8)                                                                                          \
-	hipLaunchKernelGGL((prompt_kernel<HD, Q8>), dim3((unsigned)(row - row0), n_heads), dim3(64), 0, stream(), c, t, \
-	                   out + row0 * out_stride, out_stride, q + row0 * q_stride, q_stride, n_heads / kv->n_kv_heads, scale)
-		HK_KV_SWITCH(kv, HK_PROMPT);
+#define HK_PROMPT(HD, Q8) prompt<HD, Q8>(c, t, out, out_stride, q, q_stride, n_heads, scale)
+		if (int rc = HK_KV_SWITCH(kv, HK_PROMPT)) return rc;
 #undef HK_PROMPT
-		HK_LAUNCHED("attention");
 	}
 	return ok();
 }
