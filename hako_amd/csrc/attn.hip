@@ -97,7 +97,6 @@ __device__ __forceinline__ void split_q(const float *x, int e, h8 &hi, h8 &lo) {
 
 // The exponent that value scales are divided by: that of their largest.
 __device__ __forceinline__ int scale_exp(float vmax) { return f16_split_exp(vmax); }
-__device__ __forceinline__ float finite_or0(float v) { return __builtin_isfinite(v) ? v : 0.0f; }
 
 // ── tiled kernel: up to 128 query rows against chunks of 64 keys ──
 //
@@ -202,9 +201,11 @@ struct Stage {
 			}
 		}
 		if (tid < kKeys) {
-			E = max(E, scale_exp(wave_max(finite_or0(vs))));
-			ks_s[tid] = ks;
-			vs_s[tid] = __builtin_ldexpf(vs, -E);
+			// a value row that is not finite makes its scores NaN, which a row that may not see it masks
+			const bool fin = __builtin_isfinite(vs);
+			E = max(E, scale_exp(wave_max(fin ? vs : 0.0f)));
+			ks_s[tid] = fin ? ks : __builtin_nanf("");
+			vs_s[tid] = fin ? __builtin_ldexpf(vs, -E) : 0.0f;
 			if (tid == 0) *e_s = E;
 		}
 	}
@@ -217,8 +218,10 @@ struct Tile {
 	static constexpr int KS = HD / 16, DT = HD / 32;
 	static constexpr int kKB = kKeys * HD * 2, kVB = HD * kKeys * 2;
 	struct Lds {
-		uint8_t k[2][kKB], v[2][kVB];
-		float ks[2][kKeys], vs[2][kKeys];
+		alignas(16) uint8_t k[2][kKB];
+		alignas(16) uint8_t v[2][kVB];
+		alignas(16) float ks[2][kKeys];
+		alignas(16) float vs[2][kKeys];
 		int e[2];
 	};
 	h8 qh[KS], ql[KS];
@@ -259,10 +262,10 @@ struct Tile {
 		E = -126;
 	}
 
-	// 32 keys (half `t` of the chunk in LDS buffer `b`) at positions key0..; MASK: some row of the wave does not see
-	// all of them.
-	template <bool MASK>
-	__device__ __forceinline__ void half(const Lds &s, int b, int t, int key0, int lim, int lane) {
+	// 32 keys (half `t` of the chunk in LDS buffer `b`, whose first is at position key0); mask: some row of the wave
+	// does not see all of them. (Two instances of this, with and without the mask, cost a second set of the value sums'
+	// registers.)
+	__device__ __forceinline__ void half(const Lds &s, int b, int t, int key0, bool mask, int lim, int lane) {
 		lane = fresh(lane);
 		const int h = lane >> 5, i = lane & 31;
 		// tile row i is key 16 (i>>4) + 8 ((i>>2)&1) + 4 ((i>>3)&1) + (i&3): register v of a lane is then key
@@ -287,13 +290,16 @@ struct Tile {
 			const float kv[4] = {ks.x, ks.y, ks.z, ks.w};
 #pragma unroll
 			for (int j = 0; j < 4; j++) {
-				const int v = 4 * g + j;
-				float x = sc[v] * kv[j];
-				if (MASK) x = key0 + 32 * t + 16 * (v >> 3) + 8 * h + (v & 7) < lim ? x : -INFINITY;
-				sc[v] = x;
-				mx = __builtin_fmaxf(mx, x);
+				sc[4 * g + j] *= kv[j];
 			}
 		}
+		if (mask) {
+			const int n = lim - key0 - 32 * t - 8 * h;
+#pragma unroll
+			for (int v = 0; v < 16; v++) sc[v] = 16 * (v >> 3) + (v & 7) < n ? sc[v] : -INFINITY;
+		}
+#pragma unroll
+		for (int v = 0; v < 16; v++) mx = __builtin_fmaxf(mx, sc[v]);
 		mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32)) * esc;
 		if (__any(mx > M + kSlack)) {
 			const float mn = mx > M + kSlack ? mx : M;
@@ -318,7 +324,6 @@ struct Tile {
 				const float p = exp2_(__builtin_fmaf(sc[v], esc, c));
 				l += p;
 				w[j] = p * vv[j];
-				if (MASK) w[j] = sc[v] == -INFINITY ? 0.0f : w[j];   // a scale that may not be seen may be NaN
 			}
 			split2(w[0], w[1], ph[2 * g], pl[2 * g]);
 			split2(w[2], w[3], ph[2 * g + 1], pl[2 * g + 1]);
@@ -399,8 +404,7 @@ struct Tile {
 			for (int t = 0; t < 2; t++) {
 				const int k0 = key0 + 32 * t;
 				if (k0 >= min(hi, top)) continue;   // no row of the wave sees any of these keys
-				if (k0 + 32 <= min(lo, top)) half<false>(s, b, t, key0, 0, lane);
-				else half<true>(s, b, t, key0, min(lim, top), lane);
+				half(s, b, t, key0, k0 + 32 > min(lo, top), min(lim, top), lane);
 			}
 			__builtin_amdgcn_sched_barrier(0);
 			if (more) st.store(s.k[b ^ 1], s.v[b ^ 1], s.ks[b ^ 1], s.vs[b ^ 1], &s.e[b ^ 1], Es, fresh(tid));
@@ -629,9 +633,12 @@ struct Row16 {
 		float x[8], mx = -INFINITY, vm = 0.0f;
 #pragma unroll
 		for (int j = 0; j < 8; j++) {
-			x[j] = key0 + 8 * g + j < end ? sc[j >> 2][j & 3] * ks[j] : -INFINITY;
+			// a value row that is not finite makes its score NaN
+			const bool fin = __builtin_isfinite(vs[j]);
+			x[j] = key0 + 8 * g + j < end ? (fin ? sc[j >> 2][j & 3] * ks[j] : __builtin_nanf("")) : -INFINITY;
+			vs[j] = fin ? vs[j] : 0.0f;
 			mx = __builtin_fmaxf(mx, x[j]);
-			vm = __builtin_fmaxf(vm, finite_or0(vs[j]));
+			vm = __builtin_fmaxf(vm, vs[j]);
 		}
 		mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16));
 		vm = __builtin_fmaxf(vm, __shfl_xor(vm, 16));
@@ -656,7 +663,7 @@ struct Row16 {
 			for (int n = 0; n < 2; n++) {
 				const float p = exp2_(__builtin_fmaf(x[j + n], esc, c));
 				l += p;
-				w[n] = key0 + 8 * g + j + n < end ? p * (vs[j + n] * vf) : 0.0f;
+				w[n] = p * (vs[j + n] * vf);
 			}
 			h2 a, b;
 			split2(w[0], w[1], a, b);
@@ -709,7 +716,7 @@ __global__ __launch_bounds__(256) void decode_kernel(AttnKv c, float *out, int64
                                                      float scale, int parts, int rec0, int nrec,
                                                      float *__restrict__ rec_o, float2 *__restrict__ rec_ml) {
 	constexpr int EB = Q8 ? 1 : 2;
-	__shared__ float o_s[kWaves][kMaxGroup][HD + 4];
+	__shared__ __align__(16) float o_s[kWaves][kMaxGroup][HD + 4];
 	__shared__ float ml_s[kWaves][kMaxGroup][2];
 	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
 	const int kvh = blockIdx.x, part = blockIdx.y, sq = blockIdx.z;
