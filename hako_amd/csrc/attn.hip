@@ -30,8 +30,7 @@ constexpr int kMaxGroup = 16;    // query heads per key/value head
 constexpr int kSeqs = 96;        // sequences of one prompt launch (by value in the kernel arguments)
 constexpr int kWsAttn = 7;       // library workspace slot of the records
 constexpr int kKeys = 64;        // keys per chunk of the tiled kernel
-constexpr int kWaves = 4;        // waves per workgroup
-constexpr int kTileRows = 32 * kWaves;
+constexpr int kWaves = 4;        // waves per workgroup of the single-token kernel
 constexpr float kNone = -FLT_MAX;   // running maximum of a row that has seen no key
 constexpr float kUp = 6.0f;         // weights are 2^(u - M + 6): at most 2^14 while u <= M + kSlack
 constexpr float kSlack = 8.0f;      // M follows the maximum only when it is passed by this
@@ -107,36 +106,42 @@ __device__ __forceinline__ int scale_exp(float vmax) { return f16_split_exp(vmax
 // that every operand is one 16-byte LDS read. The next chunk's codes are in
 // registers while this one is computed; two LDS buffers, one barrier per chunk.
 
-// LDS places of a 16-byte unit, xored so that eight lanes in a row (and the
-// writers) meet different banks.
+// Rows in LDS are padded by 16 bytes, so that lanes on consecutive rows meet
+// different banks. A chunk's keys lie in the order of the score tiles' rows
+// (key_row), its value dims with equal dim % 4 together (dim_row): both let
+// the lanes that write a chunk, and those that read it, go row by row.
 template <int HD>
-__device__ __forceinline__ int k_unit(int key, int unit) {   // a key is HD/8 units
-	return unit ^ (((key & 3) | ((key >> 1) & 4) | ((key << 1) & 8)) & (HD / 8 - 1));
-}
-__device__ __forceinline__ int v_unit(int dim, int unit) { return unit ^ ((dim ^ (dim >> 2)) & 7); }
+constexpr int kKeyRow = 2 * HD + 16;
+constexpr int kDimRow = 2 * kKeys + 16;
+// Row of a key: tile row 8 a + 4 h + b holds key 16 (a>>1) + 8 h + 4 (a&1) + b
+// (of its 32), so that register v of lane half h is key 16 (v>>3) + 8 h + (v&7).
+__device__ __forceinline__ int key_row(int key) { return (key & ~12) | ((key >> 1) & 4) | ((key << 1) & 8); }
+template <int HD>
+__device__ __forceinline__ int dim_row(int dim) { return (dim & 3) * (HD / 4) + (dim >> 2); }
 
-template <int HD, bool Q8>
+template <int HD, bool Q8, int NT>
 struct Stage {
 	static constexpr int EB = Q8 ? 1 : 2;
-	static constexpr int KL = kKeys * HD * EB / 16 / 256;   // 16-byte key loads per thread
-	static constexpr int VQ = HD / 4;                       // dim quads; a thread takes 8 keys x 4 dims
-	static constexpr int VT = kKeys / 8 * VQ;               // threads that stage values (256 or 128)
+	static constexpr int KU = kKeys * HD * EB / 16, KL = (KU + NT - 1) / NT;   // 16-byte key loads of a chunk, per thread
+	static constexpr int VQ = HD / 4;                                          // dim quads
+	static constexpr int VK = kKeys * VQ / NT < 8 ? 4 : 8;                     // a thread takes VK keys x 4 dims of the values
+	static constexpr int VT = kKeys / VK * VQ;                                 // threads that stage values
 	uint4 k[KL];
-	uint32_t v[8][EB];
+	uint32_t v[VK][EB];
 	float ks, vs;
 
 	__device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t kr, __amdgpu_buffer_rsrc_t vr, __amdgpu_buffer_rsrc_t ksr,
 	                                     __amdgpu_buffer_rsrc_t vsr, int key0, int tid) {
 #pragma unroll
 		for (int i = 0; i < KL; i++) {
-			const int u = tid + 256 * i;   // 16-byte unit of the chunk
-			k[i] = ld_b128(kr, (uint32_t)key0 * (HD * EB) + 16u * u);
+			const int u = tid + NT * i;   // 16-byte unit of the chunk
+			k[i] = ld_b128(kr, KU % NT && u >= KU ? kBufNone : (uint32_t)key0 * (HD * EB) + 16u * u);
 		}
-		if (VT == 256 || tid < VT) {
+		if (VT == NT || tid < VT) {
 			const int d = tid % VQ, kg = tid / VQ;
-			const uint32_t off = ((uint32_t)(key0 + 8 * kg) * HD + 4 * d) * EB;
+			const uint32_t off = ((uint32_t)(key0 + VK * kg) * HD + 4 * d) * EB;
 #pragma unroll
-			for (int j = 0; j < 8; j++) {
+			for (int j = 0; j < VK; j++) {
 				if (Q8) v[j][0] = __builtin_amdgcn_raw_buffer_load_b32(vr, (int)(off + j * HD), 0, 0);
 				else {
 					const uint2 t = ld_b64(vr, off + j * HD * 2);
@@ -156,7 +161,8 @@ struct Stage {
 	__device__ __forceinline__ void store(uint8_t *k_s, uint8_t *v_s, float *ks_s, float *vs_s, int *e_s, int &E, int tid) {
 #pragma unroll
 		for (int i = 0; i < KL; i++) {
-			const int u = tid + 256 * i;
+			const int u = tid + NT * i;
+			if (KU % NT && u >= KU) break;
 			if (Q8) {
 				const int key = u / (HD / 16), c = u % (HD / 16);
 				const uint32_t w[4] = {k[i].x ^ kFlip, k[i].y ^ kFlip, k[i].z ^ kFlip, k[i].w ^ kFlip};
@@ -164,19 +170,19 @@ struct Stage {
 				for (int h = 0; h < 2; h++) {
 					const h2 a = bytes_h2(w[2 * h], kLo2), b = bytes_h2(w[2 * h], kHi2);
 					const h2 c2 = bytes_h2(w[2 * h + 1], kLo2), d = bytes_h2(w[2 * h + 1], kHi2);
-					*(h8 *)(k_s + key * (2 * HD) + 16 * k_unit<HD>(key, 2 * c + h)) =
+					*(h8 *)(k_s + key_row(key) * kKeyRow<HD> + 32 * c + 16 * h) =
 					    (h8){a.x, a.y, b.x, b.y, c2.x, c2.y, d.x, d.y};
 				}
 			} else {
 				const int key = u / (HD / 8), c = u % (HD / 8);
-				*(uint4 *)(k_s + key * (2 * HD) + 16 * k_unit<HD>(key, c)) = k[i];
+				*(uint4 *)(k_s + key_row(key) * kKeyRow<HD> + 16 * c) = k[i];
 			}
 		}
-		if (VT == 256 || tid < VT) {
+		if (VT == NT || tid < VT) {
 			const int d = tid % VQ, kg = tid / VQ;
-			h2 t[4][4];   // [dim][key pair]
+			h2 t[4][VK / 2];   // [dim][key pair]
 #pragma unroll
-			for (int p = 0; p < 4; p++) {
+			for (int p = 0; p < VK / 2; p++) {
 				if (Q8) {
 					const uint32_t a = v[2 * p][0] ^ kFlip, b = v[2 * p + 1][0] ^ kFlip;
 					const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x05010400u), hi = __builtin_amdgcn_perm(b, a, 0x07030602u);
@@ -196,8 +202,12 @@ struct Stage {
 #pragma unroll
 			for (int i = 0; i < 4; i++) {
 				const int dim = 4 * d + i;
-				*(h8 *)(v_s + dim * (2 * kKeys) + 16 * v_unit(dim, kg)) =
-				    (h8){t[i][0].x, t[i][0].y, t[i][1].x, t[i][1].y, t[i][2].x, t[i][2].y, t[i][3].x, t[i][3].y};
+				uint8_t *at = v_s + dim_row<HD>(dim) * kDimRow + 2 * VK * kg;
+				if (VK == 8)
+					*(h8 *)at = (h8){t[i][0].x, t[i][0].y, t[i][1].x, t[i][1].y, t[i][VK / 2 - 2].x, t[i][VK / 2 - 2].y,
+					                 t[i][VK / 2 - 1].x, t[i][VK / 2 - 1].y};
+				else
+					*(uint2 *)at = make_uint2(__builtin_bit_cast(uint32_t, t[i][0]), __builtin_bit_cast(uint32_t, t[i][1]));
 			}
 		}
 		if (tid < kKeys) {
@@ -213,10 +223,10 @@ struct Stage {
 
 // One wave's 32 rows over the chunks of a part. lim: the lane's row sees keys
 // (positions) below it; out: O^T (value sums, times 2^E), M and l.
-template <int HD, bool Q8>
+template <int HD, bool Q8, int NW>
 struct Tile {
 	static constexpr int KS = HD / 16, DT = HD / 32;
-	static constexpr int kKB = kKeys * HD * 2, kVB = HD * kKeys * 2;
+	static constexpr int kKB = kKeys * kKeyRow<HD>, kVB = HD * kDimRow;
 	struct Lds {
 		alignas(16) uint8_t k[2][kKB];
 		alignas(16) uint8_t v[2][kVB];
@@ -262,44 +272,45 @@ struct Tile {
 		E = -126;
 	}
 
-	// 32 keys (half `t` of the chunk in LDS buffer `b`, whose first is at position key0); mask: some row of the wave
-	// does not see all of them. (Two instances of this, with and without the mask, cost a second set of the value sums'
-	// registers.)
-	__device__ __forceinline__ void half(const Lds &s, int b, int t, int key0, bool mask, int lim, int lane) {
+	// The 64 keys of the chunk in LDS buffer `b`, the first at position key0; mask: some row of the wave does not see
+	// all of them. (Two instances of this, with and without the mask, cost a second set of the value sums' registers.)
+	// The weights of the second 32 keys form while the matrix cores add up the values of the first.
+	__device__ __forceinline__ void chunk(const Lds &s, int b, int key0, bool mask, int lim, int lane) {
 		lane = fresh(lane);
 		const int h = lane >> 5, i = lane & 31;
-		// tile row i is key 16 (i>>4) + 8 ((i>>2)&1) + 4 ((i>>3)&1) + (i&3): register v of a lane is then key
-		// 16 (v>>3) + 8 h + (v&7)
-		const int key = 32 * t + (i & 16) + ((i << 1) & 8) + ((i >> 1) & 4) + (i & 3);
-		const uint8_t *kr = s.k[b] + key * (2 * HD);
-		f16v sc;
+		const uint8_t *kr = s.k[b] + i * kKeyRow<HD> + 16 * h;
+		f16v sc[2];
 #pragma unroll
-		for (int v = 0; v < 16; v++) sc[v] = 0.0f;
+		for (int v = 0; v < 16; v++) sc[0][v] = sc[1][v] = 0.0f;
 #pragma unroll
-		for (int k = 0; k < KS; k++) {
-			const h8 a = *(const h8 *)(kr + 16 * k_unit<HD>(key, 2 * k + h));
-			sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[k], sc, 0, 0, 0);
-			sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[k], sc, 0, 0, 0);
-		}
-		feed<KS>();
+		for (int k = 0; k < KS; k++)
+#pragma unroll
+			for (int t = 0; t < 2; t++) {
+				const h8 a = *(const h8 *)(kr + 32 * t * kKeyRow<HD> + 32 * k);
+				sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[k], sc[t], 0, 0, 0);
+				sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[k], sc[t], 0, 0, 0);
+			}
+		feed<2 * KS>();
 		__builtin_amdgcn_sched_barrier(0);
 		float mx = -INFINITY;
 #pragma unroll
-		for (int g = 0; g < 4; g++) {
-			const float4 ks = *(const float4 *)(s.ks[b] + 32 * t + 16 * (g >> 1) + 8 * h + 4 * (g & 1));
-			const float kv[4] = {ks.x, ks.y, ks.z, ks.w};
+		for (int t = 0; t < 2; t++)
 #pragma unroll
-			for (int j = 0; j < 4; j++) {
-				sc[4 * g + j] *= kv[j];
+			for (int g = 0; g < 4; g++) {
+				const float4 ks = *(const float4 *)(s.ks[b] + 32 * t + 16 * (g >> 1) + 8 * h + 4 * (g & 1));
+				const float kv[4] = {ks.x, ks.y, ks.z, ks.w};
+#pragma unroll
+				for (int j = 0; j < 4; j++) sc[t][4 * g + j] *= kv[j];
 			}
-		}
 		if (mask) {
-			const int n = lim - key0 - 32 * t - 8 * h;
+			const int n = lim - key0 - 8 * h;
 #pragma unroll
-			for (int v = 0; v < 16; v++) sc[v] = 16 * (v >> 3) + (v & 7) < n ? sc[v] : -INFINITY;
+			for (int t = 0; t < 2; t++)
+#pragma unroll
+				for (int v = 0; v < 16; v++) sc[t][v] = 32 * t + 16 * (v >> 3) + (v & 7) < n ? sc[t][v] : -INFINITY;
 		}
 #pragma unroll
-		for (int v = 0; v < 16; v++) mx = __builtin_fmaxf(mx, sc[v]);
+		for (int v = 0; v < 16; v++) mx = __builtin_fmaxf(__builtin_fmaxf(sc[0][v], sc[1][v]), mx);
 		mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32)) * esc;
 		if (__any(mx > M + kSlack)) {
 			const float mn = mx > M + kSlack ? mx : M;
@@ -311,40 +322,47 @@ struct Tile {
 #pragma unroll
 				for (int v = 0; v < 16; v++) o[d][v] *= f;
 		}
+		h8 ph[2], pl[2];
+		weigh(s, b, 0, sc[0], h, ph, pl);
+		h8 qh2[2] = {ph[0], ph[1]}, ql2[2] = {pl[0], pl[1]};
+		weigh(s, b, 1, sc[1], h, ph, pl);
+		add(s, b, 0, i, h, qh2, ql2);
+		add(s, b, 1, i, h, ph, pl);
+		__builtin_amdgcn_sched_barrier(0);
+	}
+
+	// Scores -> weights times the value scales, as halves, and their sum.
+	__device__ __forceinline__ void weigh(const Lds &s, int b, int t, const f16v &sc, int h, h8 ph[2], h8 pl[2]) {
 		const float c = kUp - M;
-		h2 ph[8], pl[8];
 #pragma unroll
 		for (int g = 0; g < 4; g++) {
 			const float4 vs = *(const float4 *)(s.vs[b] + 32 * t + 16 * (g >> 1) + 8 * h + 4 * (g & 1));
 			const float vv[4] = {vs.x, vs.y, vs.z, vs.w};
-			float w[4];
 #pragma unroll
-			for (int j = 0; j < 4; j++) {
-				const int v = 4 * g + j;
-				const float p = exp2_(__builtin_fmaf(sc[v], esc, c));
-				l += p;
-				w[j] = p * vv[j];
+			for (int j = 0; j < 4; j += 2) {
+				const float p0 = exp2_(__builtin_fmaf(sc[4 * g + j], esc, c)), p1 = exp2_(__builtin_fmaf(sc[4 * g + j + 1], esc, c));
+				l += p0;
+				l += p1;
+				h2 a, d;
+				split2(p0 * vv[j], p1 * vv[j + 1], a, d);
+				ph[g >> 1][4 * (g & 1) + j] = a.x;
+				ph[g >> 1][4 * (g & 1) + j + 1] = a.y;
+				pl[g >> 1][4 * (g & 1) + j] = d.x;
+				pl[g >> 1][4 * (g & 1) + j + 1] = d.y;
 			}
-			split2(w[0], w[1], ph[2 * g], pl[2 * g]);
-			split2(w[2], w[3], ph[2 * g + 1], pl[2 * g + 1]);
 		}
-		__builtin_amdgcn_sched_barrier(0);
+	}
+
+	// o += the values of 32 keys times their weights.
+	__device__ __forceinline__ void add(const Lds &s, int b, int t, int i, int h, const h8 ph[2], const h8 pl[2]) {
 #pragma unroll
-		for (int k = 0; k < 2; k++) {
-			const h8 bh = (h8){ph[4 * k].x, ph[4 * k].y, ph[4 * k + 1].x, ph[4 * k + 1].y,
-			                   ph[4 * k + 2].x, ph[4 * k + 2].y, ph[4 * k + 3].x, ph[4 * k + 3].y};
-			const h8 bl = (h8){pl[4 * k].x, pl[4 * k].y, pl[4 * k + 1].x, pl[4 * k + 1].y,
-			                   pl[4 * k + 2].x, pl[4 * k + 2].y, pl[4 * k + 3].x, pl[4 * k + 3].y};
+		for (int k = 0; k < 2; k++)
 #pragma unroll
 			for (int d = 0; d < DT; d++) {
-				const int dim = 32 * d + i;
-				const h8 a = *(const h8 *)(s.v[b] + dim * (2 * kKeys) + 16 * v_unit(dim, 4 * t + 2 * k + h));
-				o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, bh, o[d], 0, 0, 0);
-				o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, bl, o[d], 0, 0, 0);
+				const h8 a = *(const h8 *)(s.v[b] + (32 * d + i) * kDimRow + 64 * t + 32 * k + 16 * h);
+				o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[k], o[d], 0, 0, 0);
+				o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[k], o[d], 0, 0, 0);
 			}
-		}
-		feed<2 * DT>();
-		__builtin_amdgcn_sched_barrier(0);
 	}
 
 	// N operand reads from LDS, two products each: the reads three ahead of their products.
@@ -367,7 +385,7 @@ struct Tile {
 		const int pend = min(c.prefix_len, end), nc1 = (pend + kKeys - 1) / kKeys;
 		auto base = [&](int sl) { return ((size_t)sl * c.kvh + kvh) * c.max_seq; };
 		const size_t b0 = base(c.prefix_len > 0 ? c.prefix_slot : slot), b1 = base(slot);
-		Stage<HD, Q8> st;
+		Stage<HD, Q8, 64 * NW> st;
 		auto load = [&](int ch) {
 			const bool pre = ch < nc1;
 			const size_t r = pre ? b0 : b1;
@@ -376,17 +394,24 @@ struct Tile {
 			        stream_rsrc(uniform_ptr(c.ks + r), n * 4), stream_rsrc(uniform_ptr(c.vs + r), n * 4),
 			        pre ? kKeys * ch : c.prefix_len + kKeys * (ch - nc1), fresh(tid));
 		};
+		// A wave's registers hold the codes two chunks on from the buffer that is read. The waves of a SIMD (w, w + 4)
+		// put them into LDS at opposite ends of a chunk, so that one has vector work while the other has matrix work.
 		int Es = -126;
 		if (c0 < c1) {
 			load(c0);
 			st.store(s.k[0], s.v[0], s.ks[0], s.vs[0], &s.e[0], Es, tid);
+			if (c0 + 1 < c1) load(c0 + 1);
 		}
+		const bool early = __builtin_amdgcn_readfirstlane(tid >> 6) >= 4;
 		__syncthreads();
 		for (int ch = c0; ch < c1; ch++) {
 			const int b = (ch - c0) & 1;
-			const bool more = ch + 1 < c1;
-			if (more) load(ch + 1);
-			__builtin_amdgcn_sched_barrier(0);
+			auto stage = [&] {
+				if (ch + 1 < c1) st.store(s.k[b ^ 1], s.v[b ^ 1], s.ks[b ^ 1], s.vs[b ^ 1], &s.e[b ^ 1], Es, fresh(tid));
+				if (ch + 2 < c1) load(ch + 2);
+				__builtin_amdgcn_sched_barrier(0);
+			};
+			if (early) stage();
 			const bool pre = ch < nc1;
 			const int key0 = pre ? kKeys * ch : c.prefix_len + kKeys * (ch - nc1);
 			// rows see keys below min(lim, what the chunk holds)
@@ -400,28 +425,23 @@ struct Tile {
 					for (int v = 0; v < 16; v++) o[d][v] *= f;
 				E = e;
 			}
-#pragma unroll 1
-			for (int t = 0; t < 2; t++) {
-				const int k0 = key0 + 32 * t;
-				if (k0 >= min(hi, top)) continue;   // no row of the wave sees any of these keys
-				half(s, b, t, key0, k0 + 32 > min(lo, top), min(lim, top), lane);
-			}
-			__builtin_amdgcn_sched_barrier(0);
-			if (more) st.store(s.k[b ^ 1], s.v[b ^ 1], s.ks[b ^ 1], s.vs[b ^ 1], &s.e[b ^ 1], Es, fresh(tid));
+			if (key0 < min(hi, top))   // some row of the wave sees some of these keys
+				chunk(s, b, key0, key0 + kKeys > min(lo, top), min(lim, top), lane);
+			if (!early) stage();
 			__syncthreads();
 		}
 		l += __shfl_xor(l, 32);
 	}
 
-	// The row's value sums times f to dst.
+	// The row's value sums times f to dst: row 8 a + 4 h + b of tile d is dim_row 32 d + ..
 	__device__ __forceinline__ void put(float *dst, float f, int lane) const {
 		const int h = lane >> 5;
 #pragma unroll
-		for (int d = 0; d < DT; d++)
-#pragma unroll
-			for (int g = 0; g < 4; g++)
-				*(float4 *)(dst + 32 * d + 8 * g + 4 * h) = make_float4(o[d][4 * g] * f, o[d][4 * g + 1] * f,
-				                                                        o[d][4 * g + 2] * f, o[d][4 * g + 3] * f);
+		for (int v = 0; v < 4 * DT; v++) {
+			const int r = 8 * (v >> 2) + 4 * h + (v & 3);   // quad of dims
+			*(float4 *)(dst + 4 * r) = DT == 4 ? make_float4(o[0][v] * f, o[1][v] * f, o[2 % DT][v] * f, o[3 % DT][v] * f)
+			                                   : make_float4(o[0][v] * f, o[0][v + 8] * f, o[1][v] * f, o[1][v + 8] * f);
+		}
 	}
 };
 
@@ -443,11 +463,11 @@ __host__ __device__ __forceinline__ int tile_chunks(int end, int prefix) {
 }
 
 // Records: value sums rec_o [record][HD] and (M, l) rec_ml [record].
-template <int HD, bool Q8>
-__global__ __launch_bounds__(256, 2) void prompt_kernel(AttnKv c, SeqTab t, float *out, int64_t ldo, const float *q,
+template <int HD, bool Q8, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void prompt_kernel(AttnKv c, SeqTab t, float *out, int64_t ldo, const float *q,
                                                         int64_t ldq, int G, float scale, float *__restrict__ rec_o,
                                                         float2 *__restrict__ rec_ml) {
-	__shared__ typename Tile<HD, Q8>::Lds s;
+	__shared__ typename Tile<HD, Q8, NW>::Lds s;
 	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
 	const int kvh = blockIdx.x % c.kvh, item = blockIdx.x / c.kvh;
 	int sq = 0;
@@ -465,7 +485,7 @@ __global__ __launch_bounds__(256, 2) void prompt_kernel(AttnKv c, SeqTab t, floa
 	const int lo = wave_min_i(on ? lim : 0x7FFFFFFF), hi = wave_max_i(lim);
 	const int64_t row = (int64_t)t.row[sq] + tok0 + tok;
 	const int head = kvh * G + g;
-	Tile<HD, Q8> w;
+	Tile<HD, Q8, NW> w;
 	w.query(on ? q + row * ldq + head * HD : nullptr, scale, lane);
 	w.chunks(c, kvh, t.slot[sq], end, c0, c1, lim, lo, hi, s, tid);
 	if (!on) return;
@@ -480,15 +500,15 @@ __global__ __launch_bounds__(256, 2) void prompt_kernel(AttnKv c, SeqTab t, floa
 
 // The prefix of a batch: rows are (sequence, head of the group), every row
 // over the prefix's keys below its length; always to records.
-template <int HD, bool Q8>
-__global__ __launch_bounds__(256, 2) void prefix_kernel(AttnKv c, const float *q, int64_t ldq, const int *__restrict__ slot,
+template <int HD, bool Q8, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void prefix_kernel(AttnKv c, const float *q, int64_t ldq, const int *__restrict__ slot,
                                                         const int *__restrict__ len, int n_seq, int G, float scale,
                                                         int unit, int nrec, float *__restrict__ rec_o,
                                                         float2 *__restrict__ rec_ml) {
-	__shared__ typename Tile<HD, Q8>::Lds s;
+	__shared__ typename Tile<HD, Q8, NW>::Lds s;
 	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
 	const int kvh = blockIdx.x % c.kvh, part = blockIdx.x / c.kvh;
-	const int64_t r = (int64_t)blockIdx.y * kTileRows + 32 * wave + (lane & 31);
+	const int64_t r = (int64_t)blockIdx.y * (32 * NW) + 32 * wave + (lane & 31);
 	const int sq = (int)(r / G), g = (int)(r - (int64_t)sq * G);
 	const bool on = sq < n_seq;
 	int lim = 0;
@@ -498,7 +518,7 @@ __global__ __launch_bounds__(256, 2) void prefix_kernel(AttnKv c, const float *q
 	}
 	const int lo = wave_min_i(on ? lim : 0x7FFFFFFF), hi = wave_max_i(lim);
 	const int head = kvh * G + g, nc = (c.prefix_len + kKeys - 1) / kKeys;
-	Tile<HD, Q8> w;
+	Tile<HD, Q8, NW> w;
 	w.query(on ? q + sq * ldq + head * HD : nullptr, scale, lane);
 	w.chunks(c, kvh, c.prefix_slot, c.prefix_len, part * unit, min(nc, part * unit + unit), lim, lo, hi, s, tid);
 	if (!on) return;
@@ -901,11 +921,12 @@ int decode(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq
 	const int fill = (int)std::max<int64_t>(1, (slots + pairs - 1) / pairs);
 	parts = std::max(1, std::min(parts, fill));
 	// the prefix: parts of whole chunks, until its tiles fill the chip
-	const int64_t tiles = ((int64_t)n_seq * G + kTileRows - 1) / kTileRows;
+	constexpr int NW = 8;
+	const int64_t tiles = ((int64_t)n_seq * G + 32 * NW - 1) / (32 * NW);
 	const int nc = (c.prefix_len + kKeys - 1) / kKeys;
 	int unit = 1, pparts = 0;
 	if (nc) {
-		const int want = (int)std::max<int64_t>(1, slots / (tiles * c.kvh));
+		const int want = (int)std::max<int64_t>(1, cu_count() * (8 / NW) / (tiles * c.kvh));
 		unit = std::max(1, (nc + want - 1) / want);
 		pparts = (nc + unit - 1) / unit;
 	}
@@ -915,7 +936,7 @@ int decode(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq
 	if (nrec)
 		if (int rc = records((size_t)n_seq * H * nrec, HD, &ro, &ml)) return rc;
 	if (pparts) {
-		hipLaunchKernelGGL((prefix_kernel<HD, Q8>), dim3(c.kvh * pparts, (unsigned)tiles), dim3(256), 0, stream(), c, q, ldq,
+		hipLaunchKernelGGL((prefix_kernel<HD, Q8, NW>), dim3(c.kvh * pparts, (unsigned)tiles), dim3(64 * NW), 0, stream(), c, q, ldq,
 		                   slot, len, n_seq, G, scale * kLog2e, unit, nrec, ro, ml);
 		HK_LAUNCHED("attention prefix");
 	}
@@ -933,14 +954,15 @@ int decode(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq
 // One launch of up to kSeqs sequences, in the order given (the longest first).
 template <int HD, bool Q8>
 int prompt(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, const float *q, int64_t ldq, int H, float scale) {
+	constexpr int NW = 8;
 	const int G = H / c.kvh;
-	t.tile_tokens = kTileRows / G;
+	t.tile_tokens = 32 * NW / G;
 	// chunks per part: what each of the workgroups that run at once would take if all were shared out evenly
 	int64_t total = 0;
 	for (int s = 0; s < t.n; s++)
 		for (int k = 0; k < t.len[s]; k += t.tile_tokens)
 			total += tile_chunks(t.start[s] + std::min(k + t.tile_tokens, t.len[s]), c.prefix_len);
-	const int64_t slots = 2 * cu_count();
+	const int64_t slots = cu_count() * (8 / NW);
 	t.unit = (int)std::max<int64_t>(4, (total * c.kvh + slots - 1) / slots);
 	int64_t items = 0, recs = 0;
 	for (int s = 0; s < t.n; s++) {
@@ -957,7 +979,7 @@ int prompt(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, const float *q, 
 	float2 *ml = nullptr;
 	if (recs)
 		if (int rc = records((size_t)recs, HD, &ro, &ml)) return rc;
-	hipLaunchKernelGGL((prompt_kernel<HD, Q8>), dim3((unsigned)(items * c.kvh)), dim3(256), 0, stream(), c, t, out, ldo, q,
+	hipLaunchKernelGGL((prompt_kernel<HD, Q8, NW>), dim3((unsigned)(items * c.kvh)), dim3(64 * NW), 0, stream(), c, t, out, ldo, q,
 	                   ldq, G, scale * kLog2e, ro, ml);
 	HK_LAUNCHED("attention");
 	for (int s = 0; s < t.n; s++)
