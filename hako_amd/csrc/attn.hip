@@ -27,7 +27,7 @@ namespace hako {
 namespace {
 
 constexpr int kMaxGroup = 16;    // query heads per key/value head
-constexpr int kSeqs = 96;        // sequences of one prompt launch (by value in the kernel arguments)
+constexpr int kSeqs = 64;        // sequences of one prompt launch (by value in the kernel arguments)
 constexpr int kWsAttn = 7;       // library workspace slot of the records
 constexpr int kKeys = 64;        // keys per chunk of the tiled kernel
 constexpr int kWaves = 4;        // waves per workgroup of the single-token kernel
@@ -49,11 +49,14 @@ struct AttnKv {
 
 // A prompt launch: sequence s has len[s] tokens from row row[s] of q and
 // out, at positions start[s].. of slot[s]; items item[s].. of the grid are
-// its tiles, the last tile first, each in nsplit[s] parts of its keys.
+// its tiles, the last tile first, each in nsplit[s] parts of its keys. The
+// tiles of more than `unit` chunks, whose parts are joined, hold the last
+// join[s + 1] - join[s] tokens.
 struct SeqTab {
 	int n, tile_tokens, unit;   // tokens per tile, chunks per part
 	int row[kSeqs], len[kSeqs], slot[kSeqs], start[kSeqs], item[kSeqs + 1], nsplit[kSeqs];
-	uint32_t rec[kSeqs];        // first record of a sequence whose tiles are split
+	int join[kSeqs + 1];
+	uint32_t rec[kSeqs];        // first record of a sequence's split tokens
 };
 
 // The same value, made anew where this stands: addresses and masks that
@@ -493,7 +496,8 @@ __global__ __launch_bounds__(64 * NW, 2) void prompt_kernel(AttnKv c, SeqTab t, 
 		w.put(out + row * ldo + head * HD, __builtin_ldexpf(1.0f, w.E) / w.l, lane);
 		return;
 	}
-	const size_t rec = (size_t)t.rec[sq] + ((size_t)(tok0 + tok) * (c.kvh * G) + head) * ns + part;
+	const int split = t.len[sq] - (t.join[sq + 1] - t.join[sq]);   // the first split token
+	const size_t rec = (size_t)t.rec[sq] + ((size_t)(tok0 + tok - split) * (c.kvh * G) + head) * ns + part;
 	w.put(rec_o + rec * HD, __builtin_ldexpf(1.0f, w.E), lane);
 	if (lane < 32) rec_ml[rec] = make_float2(w.M, w.l);
 }
@@ -747,8 +751,8 @@ __global__ __launch_bounds__(256) void decode_kernel(AttnKv c, float *out, int64
 	if (first >= end && (part > 0 || nrec > 0)) return;   // a record that the merge does not read
 	const int i = lane & 15, g = lane >> 4;
 	const int head = kvh * G + i;
+	// the first step's codes are on their way before the queries are asked for
 	Row16<HD, Q8> w;
-	w.query(i < G ? q + sq * ldq + head * HD : nullptr, scale, lane);
 	const size_t r = ((size_t)(end > 0 ? sl : 0) * c.kvh + kvh) * c.max_seq;
 	const uint32_t rows = (uint32_t)max(last, 0);
 	const __amdgpu_buffer_rsrc_t kr = stream_rsrc(uniform_ptr(c.k + r * HD * EB), rows * HD * EB);
@@ -756,9 +760,12 @@ __global__ __launch_bounds__(256) void decode_kernel(AttnKv c, float *out, int64
 	const __amdgpu_buffer_rsrc_t ksr = stream_rsrc(uniform_ptr(c.ks + r), rows * 4);
 	const __amdgpu_buffer_rsrc_t vsr = stream_rsrc(uniform_ptr(c.vs + r), rows * 4);
 	int key0 = first + 32 * wave;
-	if (key0 < last) {
-		w.load_k(kr, ksr, key0, lane);
-		w.load_v(vr, vsr, key0, lane);
+	const bool any = key0 < last;   // (keys past the last read as zeros)
+	w.load_k(kr, ksr, any ? key0 : 0, lane);
+	w.load_v(vr, vsr, any ? key0 : 0, lane);
+	__builtin_amdgcn_sched_barrier(0);
+	w.query(i < G ? q + sq * ldq + head * HD : nullptr, scale, lane);
+	if (any) {
 		for (; key0 < last; key0 += 32 * kWaves) {
 			f4 sc[2];
 			h8 ph, pl;
@@ -814,19 +821,37 @@ __global__ __launch_bounds__(256) void decode_kernel(AttnKv c, float *out, int64
 	}
 }
 
-// One head's n records joined by HD/4 lanes of a wave's 64 (four dims each,
-// 256/HD records at a time), in an order that their number alone sets.
+// One head's n records joined by a workgroup of kJoin waves: HD/4 lanes to a
+// record (four dims each), so that 64 kJoin / (HD/4) of them are under way at
+// a time; the lanes' sums meet by shuffles and then in LDS, in an order that n
+// alone sets.
+constexpr int kJoin = 4;
 template <int HD>
-__device__ __forceinline__ void join(const float *__restrict__ ro, const float2 *__restrict__ ml, int n, float *dst, int lane) {
-	constexpr int L = HD / 4, W = 64 / L;
+__device__ __forceinline__ void join(const float *__restrict__ ro, const float2 *__restrict__ ml, int n, float *dst) {
+	constexpr int L = HD / 4, W = 64 * kJoin / L;
+	__shared__ float m_s[kJoin];
+	__shared__ float a_s[kJoin][HD + 4];
+	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+	const int d = tid % L * 4, k0 = tid / L;
+	// the first round's records and every thread's share of the maxima at once
+	float4 b0 = make_float4(0, 0, 0, 0);
+	float2 x0 = make_float2(kNone, 0.0f);
+	if (k0 < n) {
+		b0 = *(const float4 *)(ro + (size_t)k0 * HD + d);
+		x0 = ml[k0];
+	}
 	float m = kNone;
-	for (int k = lane; k < n; k += 64) m = __builtin_fmaxf(m, ml[k].x);
+	for (int k = tid; k < n; k += 64 * kJoin) m = __builtin_fmaxf(m, ml[k].x);
 	m = wave_max(m);
-	float ls = 0.0f;
-	float4 a = make_float4(0, 0, 0, 0);
-	const int d = lane % L * 4;
+	if (lane == 0) m_s[wave] = m;
+	__syncthreads();
+#pragma unroll
+	for (int k = 0; k < kJoin; k++) m = __builtin_fmaxf(m, m_s[k]);
+	const float f0 = exp2_(x0.x - m);
+	float ls = x0.y * f0;
+	float4 a = make_float4(b0.x * f0, b0.y * f0, b0.z * f0, b0.w * f0);
 #pragma unroll 4
-	for (int k = lane / L; k < n; k += W) {
+	for (int k = k0 + W; k < n; k += W) {
 		const float2 x = ml[k];
 		const float f = exp2_(x.x - m);
 		const float4 b = *(const float4 *)(ro + (size_t)k * HD + d);
@@ -845,13 +870,23 @@ __device__ __forceinline__ void join(const float *__restrict__ ro, const float2 
 		a.w += __shfl_xor(a.w, k);
 	}
 	if (lane < L) {
-		const float z = ls == 0.0f ? 0.0f : 1.0f / ls;
-		*(float4 *)(dst + d) = make_float4(a.x * z, a.y * z, a.z * z, a.w * z);
+		*(float4 *)&a_s[wave][d] = a;
+		if (d == 0) a_s[wave][HD] = ls;
+	}
+	__syncthreads();
+	if (tid < HD) {
+		float o = a_s[0][tid], l = a_s[0][HD];
+#pragma unroll
+		for (int k = 1; k < kJoin; k++) {
+			o += a_s[k][tid];
+			l += a_s[k][HD];
+		}
+		dst[tid] = l == 0.0f ? 0.0f : o / l;
 	}
 }
 
 template <int HD>
-__global__ __launch_bounds__(64) void decode_join_kernel(AttnKv c, float *out, int64_t ldo, const int *__restrict__ slot,
+__global__ __launch_bounds__(64 * kJoin) void decode_join_kernel(AttnKv c, float *out, int64_t ldo, const int *__restrict__ slot,
                                                          const int *__restrict__ len, int H, int parts, int rec0,
                                                          int nrec, const float *__restrict__ rec_o,
                                                          const float2 *__restrict__ rec_ml) {
@@ -860,21 +895,23 @@ __global__ __launch_bounds__(64) void decode_join_kernel(AttnKv c, float *out, i
 	const int end = own_end(c, slot, len, sq, sl), n = max(end - c.prefix_len, 0);
 	const int per = part_keys(n, parts), used = n > 0 ? (n + per - 1) / per : 0;
 	const size_t rec = ((size_t)sq * H + h) * nrec;
-	join<HD>(rec_o + rec * HD, rec_ml + rec, rec0 + used, out + sq * ldo + h * HD, threadIdx.x);
+	join<HD>(rec_o + rec * HD, rec_ml + rec, rec0 + used, out + sq * ldo + h * HD);
 }
 
-// Tokens of sequence sq of the launch whose tile was split.
+// The tokens whose tiles were split: the last ones of each sequence.
 template <int HD>
-__global__ __launch_bounds__(64) void prompt_join_kernel(SeqTab t, int sq, int prefix_len, float *out, int64_t ldo, int H,
+__global__ __launch_bounds__(64 * kJoin) void prompt_join_kernel(SeqTab t, int prefix_len, float *out, int64_t ldo, int H,
                                                          const float *__restrict__ rec_o,
                                                          const float2 *__restrict__ rec_ml) {
-	const int tok = blockIdx.x, h = blockIdx.y, ns = t.nsplit[sq];
-	const int tile = tok / t.tile_tokens;
+	const int h = blockIdx.y;
+	int sq = 0;
+	while ((int)blockIdx.x >= t.join[sq + 1]) sq++;
+	const int split = t.join[sq + 1] - t.join[sq];   // split tokens of the sequence
+	const int j = blockIdx.x - t.join[sq], tok = t.len[sq] - split + j;
+	const int tile = tok / t.tile_tokens, ns = t.nsplit[sq];
 	const int nc = tile_chunks(t.start[sq] + min((tile + 1) * t.tile_tokens, t.len[sq]), prefix_len);
-	if (nc <= t.unit) return;
-	const size_t rec = (size_t)t.rec[sq] + ((size_t)tok * H + h) * ns;
-	join<HD>(rec_o + rec * HD, rec_ml + rec, (nc + t.unit - 1) / t.unit, out + ((int64_t)t.row[sq] + tok) * ldo + h * HD,
-	         threadIdx.x);
+	const size_t rec = (size_t)t.rec[sq] + ((size_t)j * H + h) * ns;
+	join<HD>(rec_o + rec * HD, rec_ml + rec, (nc + t.unit - 1) / t.unit, out + ((int64_t)t.row[sq] + tok) * ldo + h * HD);
 }
 
 int attn_check(float *out, int64_t ldo, const float *q, int64_t ldq, const hako_gpu_kv *kv, int n_seq, int H,
@@ -921,7 +958,7 @@ int decode(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq
 	const int fill = (int)std::max<int64_t>(1, (slots + pairs - 1) / pairs);
 	parts = std::max(1, std::min(parts, fill));
 	// the prefix: parts of whole chunks, until its tiles fill the chip
-	constexpr int NW = 8;
+	constexpr int NW = 4;
 	const int64_t tiles = ((int64_t)n_seq * G + 32 * NW - 1) / (32 * NW);
 	const int nc = (c.prefix_len + kKeys - 1) / kKeys;
 	int unit = 1, pparts = 0;
@@ -944,7 +981,7 @@ int decode(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq
 	                   len, G, scale * kLog2e, parts, pparts, nrec, ro, ml);
 	HK_LAUNCHED("attention");
 	if (nrec) {
-		hipLaunchKernelGGL(decode_join_kernel<HD>, dim3(H, n_seq), dim3(64), 0, stream(), c, out, ldo, slot, len, H, parts,
+		hipLaunchKernelGGL(decode_join_kernel<HD>, dim3(H, n_seq), dim3(64 * kJoin), 0, stream(), c, out, ldo, slot, len, H, parts,
 		                   pparts, nrec, ro, ml);
 		HK_LAUNCHED("attention join");
 	}
@@ -952,9 +989,8 @@ int decode(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq
 }
 
 // One launch of up to kSeqs sequences, in the order given (the longest first).
-template <int HD, bool Q8>
-int prompt(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, const float *q, int64_t ldq, int H, float scale) {
-	constexpr int NW = 8;
+template <int HD, bool Q8, int NW>
+int prompt_tiles(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, const float *q, int64_t ldq, int H, float scale) {
 	const int G = H / c.kvh;
 	t.tile_tokens = 32 * NW / G;
 	// chunks per part: what each of the workgroups that run at once would take if all were shared out evenly
@@ -970,7 +1006,14 @@ int prompt(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, const float *q, 
 		t.item[s] = (int)items;
 		items += (int64_t)((t.len[s] + t.tile_tokens - 1) / t.tile_tokens) * t.nsplit[s];
 		t.rec[s] = (uint32_t)recs;
-		if (t.nsplit[s] > 1) recs += (int64_t)t.len[s] * H * t.nsplit[s];
+		// (a tile sees more chunks than those before it)
+		int first = 0;
+		while (first < t.len[s] &&
+		       tile_chunks(t.start[s] + std::min(first + t.tile_tokens, t.len[s]), c.prefix_len) <= t.unit)
+			first += t.tile_tokens;
+		first = std::min(first, t.len[s]);
+		t.join[s + 1] = t.join[s] + t.len[s] - first;
+		recs += (int64_t)(t.len[s] - first) * H * t.nsplit[s];
 	}
 	t.item[t.n] = (int)items;
 	if (items * c.kvh > 0x7FFFFFFF || recs > 0xFFFFFFFFll)
@@ -982,13 +1025,21 @@ int prompt(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, const float *q, 
 	hipLaunchKernelGGL((prompt_kernel<HD, Q8, NW>), dim3((unsigned)(items * c.kvh)), dim3(64 * NW), 0, stream(), c, t, out, ldo, q,
 	                   ldq, G, scale * kLog2e, ro, ml);
 	HK_LAUNCHED("attention");
-	for (int s = 0; s < t.n; s++)
-		if (t.nsplit[s] > 1) {
-			hipLaunchKernelGGL(prompt_join_kernel<HD>, dim3(t.len[s], H), dim3(64), 0, stream(), t, s, c.prefix_len, out, ldo, H,
-			                   ro, ml);
-			HK_LAUNCHED("attention join");
-		}
+	if (t.join[t.n]) {
+		hipLaunchKernelGGL(prompt_join_kernel<HD>, dim3(t.join[t.n], H), dim3(64 * kJoin), 0, stream(), t, c.prefix_len, out, ldo,
+		                   H, ro, ml);
+		HK_LAUNCHED("attention join");
+	}
 	return HAKO_GPU_OK;
+}
+
+// Eight waves to a staged chunk, or four where the tiles of eight would not give every CU two to do.
+template <int HD, bool Q8>
+int prompt(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, const float *q, int64_t ldq, int H, float scale) {
+	int64_t tiles = 0;
+	for (int s = 0; s < t.n; s++) tiles += (t.len[s] + 256 / (H / c.kvh) - 1) / (256 / (H / c.kvh));
+	return tiles * c.kvh >= 2 * cu_count() ? prompt_tiles<HD, Q8, 8>(c, t, out, ldo, q, ldq, H, scale)
+	                                       : prompt_tiles<HD, Q8, 4>(c, t, out, ldo, q, ldq, H, scale);
 }
 
 }  // namespace
