@@ -31,6 +31,9 @@ constexpr int kSeqs = 64;        // sequences of one prompt launch (by value in 
 constexpr int kWsAttn = 7;       // library workspace slot of the records
 constexpr int kKeys = 64;        // keys per chunk of the tiled kernel
 constexpr int kWaves = 4;        // waves per workgroup of the single-token kernel
+constexpr int kTileWaves = 8;    // waves per workgroup of the tiled kernel, 32 rows each
+constexpr int64_t kBigSteps = 32;
+constexpr int kMinUnit = 16;
 constexpr float kNone = -FLT_MAX;   // running maximum of a row that has seen no key
 constexpr float kUp = 6.0f;         // weights are 2^(u - M + 6): at most 2^14 while u <= M + kSlack
 constexpr float kSlack = 8.0f;      // M follows the maximum only when it is passed by this
@@ -39,6 +42,9 @@ typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));
+
+// prompts: 1 = direct kernel, 2 = tiled kernel, 0 = by shape (tuning knob)
+int g_attn_prompt = 0;
 
 struct AttnKv {
 	const uint8_t *k, *v;
@@ -459,10 +465,344 @@ __device__ __forceinline__ int wave_max_i(int v) {
 	return __builtin_amdgcn_readfirstlane(v);
 }
 
-// chunks of a tile that sees positions below `end`
-__host__ __device__ __forceinline__ int tile_chunks(int end, int prefix) {
+// Steps of K keys of a tile that sees positions below `end`: the prefix's, then its own.
+template <int K>
+__host__ __device__ __forceinline__ int tile_steps(int end, int prefix) {
 	const int p = prefix < end ? prefix : end;
-	return (p + kKeys - 1) / kKeys + (end - p + kKeys - 1) / kKeys;
+	return (p + K - 1) / K + (end - p + K - 1) / K;
+}
+
+// What a workgroup of a prompt launch works on. A tile of nc steps is
+// ceil(nc / unit) parts of equal length.
+struct Item {
+	int sq, slot, tok0, ntok, end, part, parts, c0, c1;
+};
+template <int K>
+__device__ __forceinline__ bool item_of(const SeqTab &t, int item, int prefix_len, Item &x) {
+	int sq = 0;
+	while (item >= t.item[sq + 1]) sq++;
+	const int ns = t.nsplit[sq], it = item - t.item[sq];
+	const int ntile = (t.len[sq] + t.tile_tokens - 1) / t.tile_tokens;
+	x.sq = sq;
+	x.slot = t.slot[sq];
+	x.tok0 = (ntile - 1 - it / ns) * t.tile_tokens;
+	x.ntok = min(t.tile_tokens, t.len[sq] - x.tok0);
+	x.end = t.start[sq] + x.tok0 + x.ntok;
+	x.part = it % ns;
+	const int nc = tile_steps<K>(x.end, prefix_len);
+	x.parts = (nc + t.unit - 1) / t.unit;
+	const int per = (nc + x.parts - 1) / x.parts;
+	x.c0 = x.part * per;
+	x.c1 = min(nc, x.c0 + per);
+	return x.part < x.parts;
+}
+// Record of a split token's query head and part.
+__device__ __forceinline__ size_t record_of(const SeqTab &t, const Item &x, int tok, int H, int head) {
+	const int first = t.len[x.sq] - (t.join[x.sq + 1] - t.join[x.sq]);   // the first split token
+	return (size_t)t.rec[x.sq] + ((size_t)(x.tok0 + tok - first) * H + head) * t.nsplit[x.sq] + x.part;
+}
+
+// ── direct kernel: 32 query rows, the keys dealt to the waves ──
+//
+// The same products on 32 rows, but each wave takes its own steps of 32 keys
+// with the codes straight from memory in the operands' registers (keys as they
+// lie; values paired by byte permutes), and the waves meet once, in LDS. It
+// converts every chunk once per 32 rows where the tiled kernel does once per
+// 256, and needs neither barriers nor long runs of keys: a call too small to
+// give every CU several of those tiles ends sooner with it.
+template <int HD, bool Q8>
+struct Direct {
+	static constexpr int EB = Q8 ? 1 : 2;
+	static constexpr int KS = HD / 16, DT = HD / 32;
+	static constexpr int KL = HD * EB / 32;   // 16-byte loads of a key per lane (a key is two lanes)
+	static constexpr int VW = DT * EB / 4 > 0 ? DT * EB / 4 : 1;   // dwords of a value row per lane (DT dims; a row is 32 lanes)
+	h8 qh[KS], ql[KS];
+	float esc;
+	f16v o[DT];
+	float M, l;
+	int E;
+	uint4 k[KL];
+	uint32_t v[16][VW];
+	float sc1;   // lanes 0..31: the keys' scales, 32..63: the values'
+
+	// dims of step s, lane half h, place j
+	static __device__ __forceinline__ int dim0(int s, int h) { return Q8 ? 32 * (s >> 1) + 16 * h + 8 * (s & 1) : 16 * s + 8 * h; }
+
+	__device__ __forceinline__ void query(const float *q, float scale, int lane) {
+		const int h = lane >> 5;
+		float x[KS * 8], a = 0.0f;
+#pragma unroll
+		for (int s = 0; s < KS; s++) {
+			float4 u = make_float4(0, 0, 0, 0), w = u;
+			if (q) {
+				u = *(const float4 *)(q + dim0(s, h));
+				w = *(const float4 *)(q + dim0(s, h) + 4);
+			}
+			const float y[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+#pragma unroll
+			for (int j = 0; j < 8; j++) {
+				x[8 * s + j] = y[j] * scale;
+				a = __builtin_fmaxf(a, __builtin_fabsf(x[8 * s + j]));
+			}
+		}
+		a = __builtin_fmaxf(a, __shfl_xor(a, 32));
+		const int e = row_exp(a);
+		esc = __builtin_ldexpf(1.0f, e);
+#pragma unroll
+		for (int s = 0; s < KS; s++) split_q(x + 8 * s, e, qh[s], ql[s]);
+#pragma unroll
+		for (int d = 0; d < DT; d++)
+#pragma unroll
+			for (int v = 0; v < 16; v++) o[d][v] = 0.0f;
+		M = kNone;
+		l = 0.0f;
+		E = -126;
+	}
+
+	// Tile row i is the key of row i in key_row's order (an involution): register v of a lane's scores is key
+	// 16 (v>>3) + 8 h + (v&7).
+	__device__ __forceinline__ void load_k(__amdgpu_buffer_rsrc_t kr, __amdgpu_buffer_rsrc_t ksr, __amdgpu_buffer_rsrc_t vsr,
+	                                       int key0, int lane) {
+		const int i = lane & 31, h = lane >> 5;
+		const uint32_t off = (uint32_t)(key0 + key_row(i)) * (HD * EB) + 16u * h;
+#pragma unroll
+		for (int n = 0; n < KL; n++) k[n] = ld_b128(kr, off + 32u * n);
+		const uint32_t so = 4u * (uint32_t)(key0 + i);
+		sc1 = h ? ld_f32(vsr, so) : ld_f32(ksr, so);
+	}
+	// dims DT i..; keys 16 s + 8 h + j
+	__device__ __forceinline__ void load_v(__amdgpu_buffer_rsrc_t vr, int key0, int lane) {
+		const int i = lane & 31, h = lane >> 5;
+#pragma unroll
+		for (int n = 0; n < 16; n++) {
+			const uint32_t off = ((uint32_t)(key0 + 16 * (n >> 3) + 8 * h + (n & 7)) * HD + DT * i) * EB;
+			if (DT * EB == 2) v[n][0] = ld_b16(vr, off);
+			if (DT * EB == 4) v[n][0] = __builtin_amdgcn_raw_buffer_load_b32(vr, (int)off, 0, 0);
+			if (DT * EB == 8) {
+				const uint2 x = ld_b64(vr, off);
+				v[n][0] = x.x;
+				v[n][VW - 1] = x.y;
+			}
+		}
+	}
+
+	// The step's 32 keys from key0; mask: some row does not see all of them. sx: 64 floats of the wave's own in LDS.
+	__device__ __forceinline__ void scores(f16v &sc) {
+#pragma unroll
+		for (int v = 0; v < 16; v++) sc[v] = 0.0f;
+#pragma unroll
+		for (int s = 0; s < KS; s++) {
+			h8 a;
+			if (Q8) {
+				const uint32_t w[4] = {k[(s >> 1) % KL].x, k[(s >> 1) % KL].y, k[(s >> 1) % KL].z, k[(s >> 1) % KL].w};
+				const uint32_t x = w[2 * (s & 1)] ^ kFlip, y = w[2 * (s & 1) + 1] ^ kFlip;
+				const h2 p = bytes_h2(x, kLo2), q2 = bytes_h2(x, kHi2), r = bytes_h2(y, kLo2), u = bytes_h2(y, kHi2);
+				a = (h8){p.x, p.y, q2.x, q2.y, r.x, r.y, u.x, u.y};
+			} else {
+				a = __builtin_bit_cast(h8, k[s % KL]);
+			}
+			sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[s], sc, 0, 0, 0);
+			sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[s], sc, 0, 0, 0);
+		}
+	}
+
+	// The step's scales into the wave's own 64 floats of LDS, the values' divided by 2^E; 2^-(change of E).
+	__device__ __forceinline__ float scales(float *sx, int lane) {
+		const float other = __shfl_xor(sc1, 32);
+		const bool fin = __builtin_isfinite(lane < 32 ? other : sc1);   // the value row's scale
+		const int e = max(E, scale_exp(wave_max(lane >= 32 && fin ? sc1 : 0.0f)));
+		// a value row that is not finite makes its score NaN
+		sx[lane] = lane < 32 ? (fin ? sc1 : __builtin_nanf("")) : (fin ? __builtin_ldexpf(sc1, -e) : 0.0f);
+		const float f = __builtin_ldexpf(1.0f, E - e);
+		E = e;
+		__builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+		__builtin_amdgcn_wave_barrier();
+		__builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+		return f;
+	}
+
+	__device__ __forceinline__ void weigh(f16v &sc, const float *sx, float fe, int key0, bool mask, int lim, int lane, h8 ph[2],
+	                                      h8 pl[2]) {
+		const int h = lane >> 5;
+		float mx = -INFINITY;
+#pragma unroll
+		for (int g = 0; g < 4; g++) {
+			const float4 ks = *(const float4 *)(sx + 16 * (g >> 1) + 8 * h + 4 * (g & 1));
+			const float kv[4] = {ks.x, ks.y, ks.z, ks.w};
+#pragma unroll
+			for (int j = 0; j < 4; j++) sc[4 * g + j] *= kv[j];
+		}
+		if (mask) {
+			const int n = lim - key0 - 8 * h;
+#pragma unroll
+			for (int v = 0; v < 16; v++) sc[v] = 16 * (v >> 3) + (v & 7) < n ? sc[v] : -INFINITY;
+		}
+#pragma unroll
+		for (int v = 0; v < 16; v++) mx = __builtin_fmaxf(mx, sc[v]);
+		mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32)) * esc;
+		if (__any(mx > M + kSlack || fe != 1.0f)) {
+			const float mn = mx > M + kSlack ? mx : M;
+			const float f = exp2_(M - mn);   // 0 from kNone
+			M = mn;
+			l *= f;
+			const float fo = f * fe;
+#pragma unroll
+			for (int d = 0; d < DT; d++)
+#pragma unroll
+				for (int v = 0; v < 16; v++) o[d][v] *= fo;
+		}
+		const float c = kUp - M;
+#pragma unroll
+		for (int g = 0; g < 4; g++) {
+			const float4 vs = *(const float4 *)(sx + 32 + 16 * (g >> 1) + 8 * h + 4 * (g & 1));
+			const float vv[4] = {vs.x, vs.y, vs.z, vs.w};
+#pragma unroll
+			for (int j = 0; j < 4; j += 2) {
+				const float p0 = exp2_(__builtin_fmaf(sc[4 * g + j], esc, c)), p1 = exp2_(__builtin_fmaf(sc[4 * g + j + 1], esc, c));
+				l += p0;
+				l += p1;
+				h2 a, d;
+				split2(p0 * vv[j], p1 * vv[j + 1], a, d);
+				ph[g >> 1][4 * (g & 1) + j] = a.x;
+				ph[g >> 1][4 * (g & 1) + j + 1] = a.y;
+				pl[g >> 1][4 * (g & 1) + j] = d.x;
+				pl[g >> 1][4 * (g & 1) + j + 1] = d.y;
+			}
+		}
+	}
+
+	// tile row i of dim tile d is dim DT i + d
+	__device__ __forceinline__ void values(const h8 ph[2], const h8 pl[2]) {
+#pragma unroll
+		for (int s = 0; s < 2; s++)
+#pragma unroll
+			for (int d = 0; d < DT; d += 2) {
+				h2 t[2][4];
+#pragma unroll
+				for (int p = 0; p < 4; p++) {
+					const uint32_t a = v[8 * s + 2 * p][d * EB / 4], b = v[8 * s + 2 * p + 1][d * EB / 4];
+					if (Q8) {
+						const uint32_t m = __builtin_amdgcn_perm(b ^ kFlip, a ^ kFlip, d & 2 ? 0x07030602u : 0x05010400u);
+						t[0][p] = bytes_h2(m, kLo2);
+						t[1][p] = bytes_h2(m, kHi2);
+					} else {
+						t[0][p] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(b, a, 0x05040100u));
+						t[1][p] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(b, a, 0x07060302u));
+					}
+				}
+#pragma unroll
+				for (int n = 0; n < 2; n++) {
+					const h8 a = (h8){t[n][0].x, t[n][0].y, t[n][1].x, t[n][1].y, t[n][2].x, t[n][2].y, t[n][3].x, t[n][3].y};
+					o[d + n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[s], o[d + n], 0, 0, 0);
+					o[d + n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[s], o[d + n], 0, 0, 0);
+				}
+			}
+	}
+};
+
+template <int HD>
+struct DirectLds {
+	alignas(16) float o[kWaves][32][HD + 4];
+	float ml[kWaves][32][2];
+	alignas(16) float sx[kWaves][64];
+};
+
+// 32 rows over steps [c0, c1) of their tile's keys. row: out row (null: idle row), or rec: its record.
+template <int HD, bool Q8>
+__device__ __forceinline__ void direct_rows(const AttnKv &c, DirectLds<HD> &s, int kvh, int slot, int end, int c0, int c1,
+                                            const float *q, float scale, int lim, float *out, float *rec_o, float2 *rec_ml) {
+	constexpr int EB = Q8 ? 1 : 2;
+	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+	const int pend = min(c.prefix_len, end), nc1 = (pend + 31) / 32;
+	auto base = [&](int sl) { return ((size_t)sl * c.kvh + kvh) * c.max_seq; };
+	const size_t b0 = base(c.prefix_len > 0 ? c.prefix_slot : slot), b1 = base(slot);
+	Direct<HD, Q8> w;
+	auto first_key = [&](int ch) { return ch < nc1 ? 32 * ch : c.prefix_len + 32 * (ch - nc1); };
+	auto load_k = [&](int ch) {
+		const size_t r = ch < nc1 ? b0 : b1;
+		const uint32_t n = (uint32_t)(ch < nc1 ? pend : end);   // rows past it read as zeros
+		w.load_k(stream_rsrc(uniform_ptr(c.k + r * HD * EB), n * HD * EB), stream_rsrc(uniform_ptr(c.ks + r), n * 4),
+		         stream_rsrc(uniform_ptr(c.vs + r), n * 4), first_key(ch), fresh(lane));
+	};
+	auto load_v = [&](int ch) {
+		const size_t r = ch < nc1 ? b0 : b1;
+		const uint32_t n = (uint32_t)(ch < nc1 ? pend : end);
+		w.load_v(stream_rsrc(uniform_ptr(c.v + r * HD * EB), n * HD * EB), first_key(ch), fresh(lane));
+	};
+	int ch = c0 + wave;
+	if (ch < c1) {
+		load_k(ch);
+		load_v(ch);
+	}
+	__builtin_amdgcn_sched_barrier(0);
+	w.query(q, scale, lane);
+	const int lo = wave_min_i(q ? lim : 0x7FFFFFFF);
+	float *sx = s.sx[wave];
+	for (; ch < c1; ch += kWaves) {
+		const int key0 = first_key(ch), top = ch < nc1 ? pend : end;
+		f16v sc;
+		h8 ph[2], pl[2];
+		w.scores(sc);
+		const float fe = w.scales(sx, lane);
+		if (ch + kWaves < c1) load_k(ch + kWaves);
+		__builtin_amdgcn_sched_barrier(0);
+		w.weigh(sc, sx, fe, key0, key0 + 32 > min(lo, top), min(lim, top), fresh(lane), ph, pl);
+		w.values(ph, pl);
+		if (ch + kWaves < c1) load_v(ch + kWaves);
+		__builtin_amdgcn_sched_barrier(0);
+	}
+	w.l += __shfl_xor(w.l, 32);
+	// the waves' sums meet: row i, dims DT (8 (v>>2) + 4 h + (v&3)) + d
+	const int i = lane & 31, h = lane >> 5;
+	const float f = __builtin_ldexpf(1.0f, w.E);
+#pragma unroll
+	for (int v = 0; v < 16; v++) {
+		float *at = &s.o[wave][i][w.DT * (8 * (v >> 2) + 4 * h + (v & 3))];
+		if (w.DT == 4)
+			*(float4 *)at = make_float4(w.o[0][v] * f, w.o[1][v] * f, w.o[2 % w.DT][v] * f, w.o[3 % w.DT][v] * f);
+		else
+			*(float2 *)at = make_float2(w.o[0][v] * f, w.o[1][v] * f);
+	}
+	if (h == 0) {
+		s.ml[wave][i][0] = w.M;
+		s.ml[wave][i][1] = w.l;
+	}
+	__syncthreads();
+	// eight threads to a row, every eighth quad of its dims each
+	const int row = tid >> 3;
+	// (the row's pointers are in lane `row` of every wave)
+	const uint64_t po = (uint64_t)(uintptr_t)out, pr = (uint64_t)(uintptr_t)rec_o, pm = (uint64_t)(uintptr_t)rec_ml;
+	auto from = [&](uint64_t x) {
+		return (uint64_t)(uint32_t)__shfl((int)(uint32_t)x, row) | ((uint64_t)(uint32_t)__shfl((int)(x >> 32), row) << 32);
+	};
+	float *dst = (float *)(uintptr_t)from(po), *ro = (float *)(uintptr_t)from(pr);
+	float2 *rm = (float2 *)(uintptr_t)from(pm);
+	if (!dst && !ro) return;
+	float m = s.ml[0][row][0];
+#pragma unroll
+	for (int k = 1; k < kWaves; k++) m = __builtin_fmaxf(m, s.ml[k][row][0]);
+	float x[kWaves], ls = 0.0f;
+#pragma unroll
+	for (int k = 0; k < kWaves; k++) {
+		x[k] = exp2_(s.ml[k][row][0] - m);
+		ls = __builtin_fmaf(s.ml[k][row][1], x[k], ls);
+	}
+	const float z = ro ? 1.0f : (ls == 0.0f ? 0.0f : 1.0f / ls);
+	float *to = ro ? ro : dst;
+#pragma unroll
+	for (int d = 4 * (tid & 7); d < HD; d += 32) {
+		float4 a = make_float4(0, 0, 0, 0);
+#pragma unroll
+		for (int k = 0; k < kWaves; k++) {
+			const float4 b = *(const float4 *)&s.o[k][row][d];
+			a.x = __builtin_fmaf(b.x, x[k], a.x);
+			a.y = __builtin_fmaf(b.y, x[k], a.y);
+			a.z = __builtin_fmaf(b.z, x[k], a.z);
+			a.w = __builtin_fmaf(b.w, x[k], a.w);
+		}
+		*(float4 *)(to + d) = make_float4(a.x * z, a.y * z, a.z * z, a.w * z);
+	}
+	if (ro && (tid & 7) == 0) *rm = make_float2(m, ls);
 }
 
 // Records: value sums rec_o [record][HD] and (M, l) rec_ml [record].
@@ -472,63 +812,69 @@ __global__ __launch_bounds__(64 * NW, 2) void prompt_kernel(AttnKv c, SeqTab t, 
                                                         float2 *__restrict__ rec_ml) {
 	__shared__ typename Tile<HD, Q8, NW>::Lds s;
 	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-	const int kvh = blockIdx.x % c.kvh, item = blockIdx.x / c.kvh;
-	int sq = 0;
-	while (item >= t.item[sq + 1]) sq++;
-	const int ns = t.nsplit[sq], it = item - t.item[sq];
-	const int ntile = (t.len[sq] + t.tile_tokens - 1) / t.tile_tokens;
-	const int tile = ntile - 1 - it / ns, part = it % ns;
-	const int tok0 = tile * t.tile_tokens, ntok = min(t.tile_tokens, t.len[sq] - tok0);
-	const int end = t.start[sq] + tok0 + ntok, nc = tile_chunks(end, c.prefix_len);
-	const int c0 = part * t.unit, c1 = min(nc, c0 + t.unit);
-	if (c0 >= nc) return;
-	const int r = 32 * wave + (lane & 31), tok = r / G, g = r - tok * G;
-	const bool on = tok < ntok;
-	const int lim = on ? t.start[sq] + tok0 + tok + 1 : 0;
+	const int kvh = blockIdx.x % c.kvh;
+	Item x;
+	if (!item_of<kKeys>(t, blockIdx.x / c.kvh, c.prefix_len, x)) return;
+	const int r = 32 * wave + (lane & 31), tok = r / G, head = kvh * G + r - tok * G;
+	const bool on = tok < x.ntok;
+	const int lim = on ? t.start[x.sq] + x.tok0 + tok + 1 : 0;
 	const int lo = wave_min_i(on ? lim : 0x7FFFFFFF), hi = wave_max_i(lim);
-	const int64_t row = (int64_t)t.row[sq] + tok0 + tok;
-	const int head = kvh * G + g;
+	const int64_t row = (int64_t)t.row[x.sq] + x.tok0 + tok;
 	Tile<HD, Q8, NW> w;
 	w.query(on ? q + row * ldq + head * HD : nullptr, scale, lane);
-	w.chunks(c, kvh, t.slot[sq], end, c0, c1, lim, lo, hi, s, tid);
+	w.chunks(c, kvh, x.slot, x.end, x.c0, x.c1, lim, lo, hi, s, tid);
 	if (!on) return;
-	if (nc <= t.unit) {
+	if (x.parts == 1) {
 		w.put(out + row * ldo + head * HD, __builtin_ldexpf(1.0f, w.E) / w.l, lane);
 		return;
 	}
-	const int split = t.len[sq] - (t.join[sq + 1] - t.join[sq]);   // the first split token
-	const size_t rec = (size_t)t.rec[sq] + ((size_t)(tok0 + tok - split) * (c.kvh * G) + head) * ns + part;
+	const size_t rec = record_of(t, x, tok, c.kvh * G, head);
 	w.put(rec_o + rec * HD, __builtin_ldexpf(1.0f, w.E), lane);
 	if (lane < 32) rec_ml[rec] = make_float2(w.M, w.l);
 }
 
+// The direct kernel's items: tiles of 32 rows, parts of `unit` steps of 32 keys.
+template <int HD, bool Q8>
+__global__ __launch_bounds__(64 * kWaves, 2) void prompt_direct_kernel(AttnKv c, SeqTab t, float *out, int64_t ldo, const float *q,
+                                                               int64_t ldq, int G, float scale, float *__restrict__ rec_o,
+                                                               float2 *__restrict__ rec_ml) {
+	__shared__ DirectLds<HD> s;
+	const int lane = threadIdx.x & 63;
+	const int kvh = blockIdx.x % c.kvh;
+	Item x;
+	if (!item_of<32>(t, blockIdx.x / c.kvh, c.prefix_len, x)) return;
+	const int r = lane & 31, tok = r / G, head = kvh * G + r - tok * G;
+	const bool on = tok < x.ntok, whole = x.parts == 1;
+	const int64_t row = (int64_t)t.row[x.sq] + x.tok0 + tok;
+	const size_t rec = on && !whole ? record_of(t, x, tok, c.kvh * G, head) : 0;
+	direct_rows<HD, Q8>(c, s, kvh, x.slot, x.end, x.c0, x.c1, on ? q + row * ldq + head * HD : nullptr, scale,
+	                    on ? t.start[x.sq] + x.tok0 + tok + 1 : 0, on && whole ? out + row * ldo + head * HD : nullptr,
+	                    on && !whole ? rec_o + rec * HD : nullptr, rec_ml + rec);
+}
+
 // The prefix of a batch: rows are (sequence, head of the group), every row
 // over the prefix's keys below its length; always to records.
-template <int HD, bool Q8, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void prefix_kernel(AttnKv c, const float *q, int64_t ldq, const int *__restrict__ slot,
+template <int HD, bool Q8>
+__global__ __launch_bounds__(64 * kWaves, 2) void prefix_kernel(AttnKv c, const float *q, int64_t ldq, const int *__restrict__ slot,
                                                         const int *__restrict__ len, int n_seq, int G, float scale,
                                                         int unit, int nrec, float *__restrict__ rec_o,
                                                         float2 *__restrict__ rec_ml) {
-	__shared__ typename Tile<HD, Q8, NW>::Lds s;
-	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+	__shared__ DirectLds<HD> s;
+	const int lane = threadIdx.x & 63;
 	const int kvh = blockIdx.x % c.kvh, part = blockIdx.x / c.kvh;
-	const int64_t r = (int64_t)blockIdx.y * (32 * NW) + 32 * wave + (lane & 31);
-	const int sq = (int)(r / G), g = (int)(r - (int64_t)sq * G);
+	const int64_t r = (int64_t)blockIdx.y * 32 + (lane & 31);
+	const int sq = (int)(r / G), head = kvh * G + (int)(r - (int64_t)sq * G);
 	const bool on = sq < n_seq;
 	int lim = 0;
 	if (on) {
 		const int sl = slot ? slot[sq] : sq;
 		lim = sl < 0 || sl >= c.n_slots ? 0 : min(max(len[sq], 0), c.prefix_len);
 	}
-	const int lo = wave_min_i(on ? lim : 0x7FFFFFFF), hi = wave_max_i(lim);
-	const int head = kvh * G + g, nc = (c.prefix_len + kKeys - 1) / kKeys;
-	Tile<HD, Q8, NW> w;
-	w.query(on ? q + sq * ldq + head * HD : nullptr, scale, lane);
-	w.chunks(c, kvh, c.prefix_slot, c.prefix_len, part * unit, min(nc, part * unit + unit), lim, lo, hi, s, tid);
-	if (!on) return;
-	const size_t rec = ((size_t)sq * (c.kvh * G) + head) * nrec + part;
-	w.put(rec_o + rec * HD, __builtin_ldexpf(1.0f, w.E), lane);
-	if (lane < 32) rec_ml[rec] = make_float2(w.M, w.l);
+	const size_t rec = on ? ((size_t)sq * (c.kvh * G) + head) * nrec + part : 0;
+	const int nc = (c.prefix_len + 31) / 32;
+	direct_rows<HD, Q8>(c, s, kvh, c.prefix_slot, c.prefix_len, part * unit, min(nc, part * unit + unit),
+	                    on ? q + (int64_t)sq * ldq + head * HD : nullptr, scale, lim, nullptr, on ? rec_o + rec * HD : nullptr,
+	                    rec_ml + rec);
 }
 
 // ── single tokens: the up to 16 query heads of a group over one sequence's own keys ──
@@ -899,7 +1245,7 @@ __global__ __launch_bounds__(64 * kJoin) void decode_join_kernel(AttnKv c, float
 }
 
 // The tokens whose tiles were split: the last ones of each sequence.
-template <int HD>
+template <int HD, int K>
 __global__ __launch_bounds__(64 * kJoin) void prompt_join_kernel(SeqTab t, int prefix_len, float *out, int64_t ldo, int H,
                                                          const float *__restrict__ rec_o,
                                                          const float2 *__restrict__ rec_ml) {
@@ -909,7 +1255,7 @@ __global__ __launch_bounds__(64 * kJoin) void prompt_join_kernel(SeqTab t, int p
 	const int split = t.join[sq + 1] - t.join[sq];   // split tokens of the sequence
 	const int j = blockIdx.x - t.join[sq], tok = t.len[sq] - split + j;
 	const int tile = tok / t.tile_tokens, ns = t.nsplit[sq];
-	const int nc = tile_chunks(t.start[sq] + min((tile + 1) * t.tile_tokens, t.len[sq]), prefix_len);
+	const int nc = tile_steps<K>(t.start[sq] + min((tile + 1) * t.tile_tokens, t.len[sq]), prefix_len);
 	const size_t rec = (size_t)t.rec[sq] + ((size_t)j * H + h) * ns;
 	join<HD>(rec_o + rec * HD, rec_ml + rec, (nc + t.unit - 1) / t.unit, out + ((int64_t)t.row[sq] + tok) * ldo + h * HD);
 }
@@ -957,14 +1303,13 @@ int decode(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq
 	const int64_t pairs = (int64_t)n_seq * c.kvh;
 	const int fill = (int)std::max<int64_t>(1, (slots + pairs - 1) / pairs);
 	parts = std::max(1, std::min(parts, fill));
-	// the prefix: parts of whole chunks, until its tiles fill the chip
-	constexpr int NW = 4;
-	const int64_t tiles = ((int64_t)n_seq * G + 32 * NW - 1) / (32 * NW);
-	const int nc = (c.prefix_len + kKeys - 1) / kKeys;
+	// the prefix: parts of at least a step for each wave, until its tiles fill the chip
+	const int64_t tiles = ((int64_t)n_seq * G + 31) / 32;
+	const int nc = (c.prefix_len + 31) / 32;
 	int unit = 1, pparts = 0;
 	if (nc) {
-		const int want = (int)std::max<int64_t>(1, cu_count() * (8 / NW) / (tiles * c.kvh));
-		unit = std::max(1, (nc + want - 1) / want);
+		const int want = (int)std::max<int64_t>(1, slots / (tiles * c.kvh));
+		unit = std::max(kWaves, ((nc + want - 1) / want + kWaves - 1) / kWaves * kWaves);
 		pparts = (nc + unit - 1) / unit;
 	}
 	const int nrec = pparts + parts > 1 ? pparts + parts : 0;
@@ -973,7 +1318,7 @@ int decode(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq
 	if (nrec)
 		if (int rc = records((size_t)n_seq * H * nrec, HD, &ro, &ml)) return rc;
 	if (pparts) {
-		hipLaunchKernelGGL((prefix_kernel<HD, Q8, NW>), dim3(c.kvh * pparts, (unsigned)tiles), dim3(64 * NW), 0, stream(), c, q, ldq,
+		hipLaunchKernelGGL((prefix_kernel<HD, Q8>), dim3(c.kvh * pparts, (unsigned)tiles), dim3(64 * kWaves), 0, stream(), c, q, ldq,
 		                   slot, len, n_seq, G, scale * kLog2e, unit, nrec, ro, ml);
 		HK_LAUNCHED("attention prefix");
 	}
@@ -988,28 +1333,22 @@ int decode(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq
 	return HAKO_GPU_OK;
 }
 
-// One launch of up to kSeqs sequences, in the order given (the longest first).
-template <int HD, bool Q8, int NW>
-int prompt_tiles(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, const float *q, int64_t ldq, int H, float scale) {
-	const int G = H / c.kvh;
-	t.tile_tokens = 32 * NW / G;
-	// chunks per part: what each of the workgroups that run at once would take if all were shared out evenly
-	int64_t total = 0;
-	for (int s = 0; s < t.n; s++)
-		for (int k = 0; k < t.len[s]; k += t.tile_tokens)
-			total += tile_chunks(t.start[s] + std::min(k + t.tile_tokens, t.len[s]), c.prefix_len);
-	const int64_t slots = cu_count() * (8 / NW);
-	t.unit = (int)std::max<int64_t>(4, (total * c.kvh + slots - 1) / slots);
+// One launch of up to kSeqs sequences, in the order given (the longest
+// first): tiles of `rows` query rows, steps of K keys, parts of `unit` steps.
+template <int HD, bool Q8, int K, class Launch>
+int prompt_launch(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, int H, int rows, int64_t unit, Launch launch) {
+	t.tile_tokens = rows / (H / c.kvh);
+	t.unit = (int)std::min<int64_t>(unit, 0x7FFFFFFF);
 	int64_t items = 0, recs = 0;
 	for (int s = 0; s < t.n; s++) {
-		t.nsplit[s] = (tile_chunks(t.start[s] + t.len[s], c.prefix_len) + t.unit - 1) / t.unit;
+		t.nsplit[s] = (tile_steps<K>(t.start[s] + t.len[s], c.prefix_len) + t.unit - 1) / t.unit;
 		t.item[s] = (int)items;
 		items += (int64_t)((t.len[s] + t.tile_tokens - 1) / t.tile_tokens) * t.nsplit[s];
 		t.rec[s] = (uint32_t)recs;
-		// (a tile sees more chunks than those before it)
+		// (a tile sees no fewer steps than those before it)
 		int first = 0;
 		while (first < t.len[s] &&
-		       tile_chunks(t.start[s] + std::min(first + t.tile_tokens, t.len[s]), c.prefix_len) <= t.unit)
+		       tile_steps<K>(t.start[s] + std::min(first + t.tile_tokens, t.len[s]), c.prefix_len) <= t.unit)
 			first += t.tile_tokens;
 		first = std::min(first, t.len[s]);
 		t.join[s + 1] = t.join[s] + t.len[s] - first;
@@ -1022,27 +1361,48 @@ int prompt_tiles(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, const floa
 	float2 *ml = nullptr;
 	if (recs)
 		if (int rc = records((size_t)recs, HD, &ro, &ml)) return rc;
-	hipLaunchKernelGGL((prompt_kernel<HD, Q8, NW>), dim3((unsigned)(items * c.kvh)), dim3(64 * NW), 0, stream(), c, t, out, ldo, q,
-	                   ldq, G, scale * kLog2e, ro, ml);
+	launch(dim3((unsigned)(items * c.kvh)), ro, ml);
 	HK_LAUNCHED("attention");
-	if (t.join[t.n]) {
-		hipLaunchKernelGGL(prompt_join_kernel<HD>, dim3(t.join[t.n], H), dim3(64 * kJoin), 0, stream(), t, c.prefix_len, out, ldo,
-		                   H, ro, ml);
+	if (recs) {
+		hipLaunchKernelGGL((prompt_join_kernel<HD, K>), dim3(t.join[t.n], H), dim3(64 * kJoin), 0, stream(), t, c.prefix_len, out,
+		                   ldo, H, ro, ml);
 		HK_LAUNCHED("attention join");
 	}
 	return HAKO_GPU_OK;
 }
 
-// Eight waves to a staged chunk, or four where the tiles of eight would not give every CU two to do.
+// Steps of K keys over all tiles of `rows` rows.
+template <int K>
+int64_t all_steps(const AttnKv &c, const SeqTab &t, int tokens) {
+	int64_t n = 0;
+	for (int s = 0; s < t.n; s++)
+		for (int k = 0; k < t.len[s]; k += tokens)
+			n += tile_steps<K>(t.start[s] + std::min(k + tokens, t.len[s]), c.prefix_len);
+	return n * c.kvh;
+}
+
 template <int HD, bool Q8>
 int prompt(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, const float *q, int64_t ldq, int H, float scale) {
-	int64_t tiles = 0;
-	for (int s = 0; s < t.n; s++) tiles += (t.len[s] + 256 / (H / c.kvh) - 1) / (256 / (H / c.kvh));
-	return tiles * c.kvh >= 2 * cu_count() ? prompt_tiles<HD, Q8, 8>(c, t, out, ldo, q, ldq, H, scale)
-	                                       : prompt_tiles<HD, Q8, 4>(c, t, out, ldo, q, ldq, H, scale);
+	const int G = H / c.kvh;
+	const int64_t big = all_steps<kKeys>(c, t, 32 * kTileWaves / G);
+	if (g_attn_prompt ? g_attn_prompt == 2 : big >= kBigSteps * cu_count())
+		return prompt_launch<HD, Q8, kKeys>(
+		    c, t, out, ldo, H, 32 * kTileWaves, std::max<int64_t>(4, 2 * (big / cu_count())), [&](dim3 grid, float *ro, float2 *ml) {
+			    hipLaunchKernelGGL((prompt_kernel<HD, Q8, kTileWaves>), grid, dim3(64 * kTileWaves), 0, stream(), c, t, out, ldo, q,
+			                       ldq, G, scale * kLog2e, ro, ml);
+		    });
+	const int64_t steps = all_steps<32>(c, t, 32 / G), slots = 2 * cu_count();
+	const int64_t unit = std::max<int64_t>(kMinUnit, 2 * ((steps + slots - 1) / slots));
+	return prompt_launch<HD, Q8, 32>(c, t, out, ldo, H, 32, unit, [&](dim3 grid, float *ro, float2 *ml) {
+		hipLaunchKernelGGL((prompt_direct_kernel<HD, Q8>), grid, dim3(64 * kWaves), 0, stream(), c, t, out, ldo, q, ldq, G,
+		                   scale * kLog2e, ro, ml);
+	});
 }
 
 }  // namespace
+
+void attn_set_prompt(int v) { g_attn_prompt = v == 1 || v == 2 ? v : 0; }
+
 }  // namespace hako
 
 using namespace hako;

@@ -21,6 +21,8 @@ from hako_amd.gpu import KV_F16, KV_Q8, HakoGpuError, Rope
 
 pytestmark = pytest.mark.gpu
 
+TUNE_ATTN_PROMPT = 21
+
 TOL = 1e-5
 KINDS = [KV_Q8, KV_F16]
 
@@ -299,6 +301,13 @@ def test_decode_past_4_gib(gpu):
 
 # ── attention of whole prompts ──
 
+@pytest.fixture(params=[0, 1, 2], ids=["by shape", "direct", "tiled"])
+def prompt_kernel(gpu, request):
+    gpu.tune(TUNE_ATTN_PROMPT, request.param)
+    yield request.param
+    gpu.tune(TUNE_ATTN_PROMPT, 0)
+
+
 def run_prompt(gpu, c, q, slot, start, lens, scale, ps=0, pl=0, pad=0, in_place=False):
     n, H, hd = q.shape
     ld = H * hd + pad
@@ -332,7 +341,7 @@ def want_prompt(c, q, slot, start, lens, scale, ps=0, pl=0):
     (64, 2, 7, 300, [0, 31], [257, 129]), (64, 1, 1, 200, [0, 100, 199], [200, 33, 1]), (128, 1, 16, 100, [1], [99]),
     (128, 3, 5, 520, [511, 0], [9, 1]), (64, 8, 2, 128, [0, 0, 0], [128, 127, 1]), (128, 1, 3, 1500, [0], [700]),
     (128, 2, 1, 3000, [2900, 0], [64, 40]), (64, 1, 16, 4200, [4096, 0], [100, 3])])
-def test_prompt(gpu, kind, hd, kvh, G, max_seq, start, lens):
+def test_prompt(gpu, prompt_kernel, kind, hd, kvh, G, max_seq, start, lens):
     rng = np.random.default_rng(max_seq + hd)
     c = ref.Cache(gpu, kind, len(lens), max_seq, kvh, hd, rng)
     q = rng.standard_normal((sum(lens), kvh * G, hd)).astype(np.float32)
@@ -343,7 +352,7 @@ def test_prompt(gpu, kind, hd, kvh, G, max_seq, start, lens):
 
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("pl", [1, 63, 64, 100, 190])
-def test_prompt_prefix_slots_strides(gpu, kind, pl):
+def test_prompt_prefix_slots_strides(gpu, prompt_kernel, kind, pl):
     """A prefix in common of any length, a slot named twice, prompts that begin inside the prefix."""
     rng = np.random.default_rng(pl)
     c = ref.Cache(gpu, kind, 4, 400, 2, 128, rng)
@@ -356,7 +365,7 @@ def test_prompt_prefix_slots_strides(gpu, kind, pl):
 
 
 @pytest.mark.parametrize("kind", KINDS)
-def test_prompt_masked_rows(gpu, kind):
+def test_prompt_masked_rows(gpu, prompt_kernel, kind):
     """What a token may not see may hold anything: rows past the prompt's end NaN, and a later token's row not finite."""
     rng = np.random.default_rng(5)
     c = ref.Cache(gpu, kind, 2, 200, 1, 128, rng)
@@ -375,7 +384,7 @@ def test_prompt_masked_rows(gpu, kind):
     c.free()
 
 
-def test_prompt_many_sequences(gpu):
+def test_prompt_many_sequences(gpu, prompt_kernel):
     """More sequences than one launch takes, most of them short or empty."""
     rng = np.random.default_rng(9)
     n = 300
