@@ -27,13 +27,12 @@ namespace hako {
 namespace {
 
 constexpr int kMaxGroup = 16;    // query heads per key/value head
-constexpr int kSeqs = 64;        // sequences of one prompt launch (by value in the kernel arguments)
+constexpr int kSeqs = 48;        // sequences of one prompt launch (by value in the kernel arguments)
+constexpr int kItems = 480;      // items of a launch whose order the host sets (likewise)
 constexpr int kWsAttn = 7;       // library workspace slot of the records
 constexpr int kKeys = 64;        // keys per chunk of the tiled kernel
 constexpr int kWaves = 4;        // waves per workgroup of the single-token kernel
 constexpr int kTileWaves = 8;    // waves per workgroup of the tiled kernel, 32 rows each
-constexpr int64_t kBigSteps = 32;
-constexpr int kMinUnit = 16;
 constexpr float kNone = -FLT_MAX;   // running maximum of a row that has seen no key
 constexpr float kUp = 6.0f;         // weights are 2^(u - M + 6): at most 2^14 while u <= M + kSlack
 constexpr float kSlack = 8.0f;      // M follows the maximum only when it is passed by this
@@ -472,23 +471,37 @@ __host__ __device__ __forceinline__ int tile_steps(int end, int prefix) {
 	return (p + K - 1) / K + (end - p + K - 1) / K;
 }
 
+// The items of a launch, the longest first: sequence << 26 | tile << 8 | part.
+// Without (n 0) they go by sequence, tile and part.
+struct ItemTab {
+	int n;
+	uint32_t item[kItems];
+};
+
 // What a workgroup of a prompt launch works on. A tile of nc steps is
 // ceil(nc / unit) parts of equal length.
 struct Item {
 	int sq, slot, tok0, ntok, end, part, parts, c0, c1;
 };
 template <int K>
-__device__ __forceinline__ bool item_of(const SeqTab &t, int item, int prefix_len, Item &x) {
-	int sq = 0;
-	while (item >= t.item[sq + 1]) sq++;
-	const int ns = t.nsplit[sq], it = item - t.item[sq];
-	const int ntile = (t.len[sq] + t.tile_tokens - 1) / t.tile_tokens;
-	x.sq = sq;
-	x.slot = t.slot[sq];
-	x.tok0 = (ntile - 1 - it / ns) * t.tile_tokens;
-	x.ntok = min(t.tile_tokens, t.len[sq] - x.tok0);
-	x.end = t.start[sq] + x.tok0 + x.ntok;
-	x.part = it % ns;
+__device__ __forceinline__ bool item_of(const SeqTab &t, const ItemTab &order, int item, int prefix_len, Item &x) {
+	int tile;
+	if (order.n) {
+		const uint32_t v = order.item[item];
+		x.sq = (int)(v >> 26);
+		tile = (int)((v >> 8) & 0x3FFFFu);
+		x.part = (int)(v & 0xFFu);
+	} else {
+		x.sq = 0;
+		while (item >= t.item[x.sq + 1]) x.sq++;
+		const int ns = t.nsplit[x.sq], it = item - t.item[x.sq];
+		tile = (t.len[x.sq] + t.tile_tokens - 1) / t.tile_tokens - 1 - it / ns;
+		x.part = it % ns;
+	}
+	x.slot = t.slot[x.sq];
+	x.tok0 = tile * t.tile_tokens;
+	x.ntok = min(t.tile_tokens, t.len[x.sq] - x.tok0);
+	x.end = t.start[x.sq] + x.tok0 + x.ntok;
 	const int nc = tile_steps<K>(x.end, prefix_len);
 	x.parts = (nc + t.unit - 1) / t.unit;
 	const int per = (nc + x.parts - 1) / x.parts;
@@ -568,7 +581,9 @@ struct Direct {
 #pragma unroll
 		for (int n = 0; n < KL; n++) k[n] = ld_b128(kr, off + 32u * n);
 		const uint32_t so = 4u * (uint32_t)(key0 + i);
-		sc1 = h ? ld_f32(vsr, so) : ld_f32(ksr, so);
+		// (out of range loads are zeros: one of the two is)
+		sc1 = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, ld_f32(ksr, h ? kBufNone : so)) |
+		                                    __builtin_bit_cast(uint32_t, ld_f32(vsr, h ? so : kBufNone)));
 	}
 	// dims DT i..; keys 16 s + 8 h + j
 	__device__ __forceinline__ void load_v(__amdgpu_buffer_rsrc_t vr, int key0, int lane) {
@@ -807,14 +822,14 @@ __device__ __forceinline__ void direct_rows(const AttnKv &c, DirectLds<HD> &s, i
 
 // Records: value sums rec_o [record][HD] and (M, l) rec_ml [record].
 template <int HD, bool Q8, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void prompt_kernel(AttnKv c, SeqTab t, float *out, int64_t ldo, const float *q,
+__global__ __launch_bounds__(64 * NW, 2) void prompt_kernel(AttnKv c, SeqTab t, ItemTab order, float *out, int64_t ldo, const float *q,
                                                         int64_t ldq, int G, float scale, float *__restrict__ rec_o,
                                                         float2 *__restrict__ rec_ml) {
 	__shared__ typename Tile<HD, Q8, NW>::Lds s;
 	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
 	const int kvh = blockIdx.x % c.kvh;
 	Item x;
-	if (!item_of<kKeys>(t, blockIdx.x / c.kvh, c.prefix_len, x)) return;
+	if (!item_of<kKeys>(t, order, blockIdx.x / c.kvh, c.prefix_len, x)) return;
 	const int r = 32 * wave + (lane & 31), tok = r / G, head = kvh * G + r - tok * G;
 	const bool on = tok < x.ntok;
 	const int lim = on ? t.start[x.sq] + x.tok0 + tok + 1 : 0;
@@ -835,14 +850,14 @@ __global__ __launch_bounds__(64 * NW, 2) void prompt_kernel(AttnKv c, SeqTab t, 
 
 // The direct kernel's items: tiles of 32 rows, parts of `unit` steps of 32 keys.
 template <int HD, bool Q8>
-__global__ __launch_bounds__(64 * kWaves, 2) void prompt_direct_kernel(AttnKv c, SeqTab t, float *out, int64_t ldo, const float *q,
+__global__ __launch_bounds__(64 * kWaves, 2) void prompt_direct_kernel(AttnKv c, SeqTab t, ItemTab order, float *out, int64_t ldo, const float *q,
                                                                int64_t ldq, int G, float scale, float *__restrict__ rec_o,
                                                                float2 *__restrict__ rec_ml) {
 	__shared__ DirectLds<HD> s;
 	const int lane = threadIdx.x & 63;
 	const int kvh = blockIdx.x % c.kvh;
 	Item x;
-	if (!item_of<32>(t, blockIdx.x / c.kvh, c.prefix_len, x)) return;
+	if (!item_of<32>(t, order, blockIdx.x / c.kvh, c.prefix_len, x)) return;
 	const int r = lane & 31, tok = r / G, head = kvh * G + r - tok * G;
 	const bool on = tok < x.ntok, whole = x.parts == 1;
 	const int64_t row = (int64_t)t.row[x.sq] + x.tok0 + tok;
@@ -1244,20 +1259,42 @@ __global__ __launch_bounds__(64 * kJoin) void decode_join_kernel(AttnKv c, float
 	join<HD>(rec_o + rec * HD, rec_ml + rec, rec0 + used, out + sq * ldo + h * HD);
 }
 
-// The tokens whose tiles were split: the last ones of each sequence.
+// The tokens whose tiles were split (the last ones of each sequence), few
+// records each: HD/4 lanes to a query head, 1024/HD heads to a workgroup.
 template <int HD, int K>
-__global__ __launch_bounds__(64 * kJoin) void prompt_join_kernel(SeqTab t, int prefix_len, float *out, int64_t ldo, int H,
-                                                         const float *__restrict__ rec_o,
-                                                         const float2 *__restrict__ rec_ml) {
-	const int h = blockIdx.y;
+__global__ __launch_bounds__(256) void prompt_join_kernel(SeqTab t, int prefix_len, float *out, int64_t ldo, int H,
+                                                          const float *__restrict__ rec_o,
+                                                          const float2 *__restrict__ rec_ml) {
+	constexpr int L = HD / 4;
+	const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+	const int js = (int)(row / H), h = (int)(row - (int64_t)js * H), d = threadIdx.x % L * 4;
+	if (js >= t.join[t.n]) return;
 	int sq = 0;
-	while ((int)blockIdx.x >= t.join[sq + 1]) sq++;
+	while (js >= t.join[sq + 1]) sq++;
 	const int split = t.join[sq + 1] - t.join[sq];   // split tokens of the sequence
-	const int j = blockIdx.x - t.join[sq], tok = t.len[sq] - split + j;
+	const int j = js - t.join[sq], tok = t.len[sq] - split + j;
 	const int tile = tok / t.tile_tokens, ns = t.nsplit[sq];
 	const int nc = tile_steps<K>(t.start[sq] + min((tile + 1) * t.tile_tokens, t.len[sq]), prefix_len);
+	const int n = (nc + t.unit - 1) / t.unit;
 	const size_t rec = (size_t)t.rec[sq] + ((size_t)j * H + h) * ns;
-	join<HD>(rec_o + rec * HD, rec_ml + rec, (nc + t.unit - 1) / t.unit, out + ((int64_t)t.row[sq] + tok) * ldo + h * HD);
+	const float2 *ml = rec_ml + rec;
+	const float *ro = rec_o + rec * HD + d;
+	float m = kNone, ls = 0.0f;
+	for (int k = 0; k < n; k++) m = __builtin_fmaxf(m, ml[k].x);
+	float4 a = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+	for (int k = 0; k < n; k++) {
+		const float4 b = *(const float4 *)(ro + (size_t)k * HD);
+		const float2 x = ml[k];
+		const float f = exp2_(x.x - m);
+		ls = __builtin_fmaf(x.y, f, ls);
+		a.x = __builtin_fmaf(b.x, f, a.x);
+		a.y = __builtin_fmaf(b.y, f, a.y);
+		a.z = __builtin_fmaf(b.z, f, a.z);
+		a.w = __builtin_fmaf(b.w, f, a.w);
+	}
+	const float z = 1.0f / ls;
+	*(float4 *)(out + ((int64_t)t.row[sq] + tok) * ldo + (int64_t)h * HD + d) = make_float4(a.x * z, a.y * z, a.z * z, a.w * z);
 }
 
 int attn_check(float *out, int64_t ldo, const float *q, int64_t ldq, const hako_gpu_kv *kv, int n_seq, int H,
@@ -1355,17 +1392,42 @@ int prompt_launch(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, int H, in
 		recs += (int64_t)(t.len[s] - first) * H * t.nsplit[s];
 	}
 	t.item[t.n] = (int)items;
+	// few items: in order of their length, so that the last ones to start are the shortest
+	ItemTab order;
+	order.n = 0;
+	struct Len {
+		int steps;
+		uint32_t item;
+	} len[kItems];
+	int n = 0;
+	for (int s = 0; s < t.n && n <= kItems; s++) {
+		const int tiles = (t.len[s] + t.tile_tokens - 1) / t.tile_tokens;
+		if (tiles > kItems || t.nsplit[s] > 256) n = kItems + 1;
+		for (int i = tiles - 1; i >= 0 && n <= kItems; i--) {
+			const int nc = tile_steps<K>(t.start[s] + std::min((i + 1) * t.tile_tokens, t.len[s]), c.prefix_len);
+			const int parts = (nc + t.unit - 1) / t.unit, per = (nc + parts - 1) / parts;
+			if (n + parts > kItems) n = kItems + 1;
+			for (int k = 0; k < parts && n <= kItems; k++) len[n++] = {std::min(per, nc - k * per), (uint32_t)(s << 26 | i << 8 | k)};
+		}
+	}
+	if (n <= kItems) {
+		std::stable_sort(len, len + n, [](const Len &a, const Len &b) { return a.steps > b.steps; });
+		for (int i = 0; i < n; i++) order.item[i] = len[i].item;
+		order.n = n;
+		items = n;
+	}
 	if (items * c.kvh > 0x7FFFFFFF || recs > 0xFFFFFFFFll)
 		return set_error(HAKO_GPU_EINVAL, "%lld tiles and %lld records in one call", (long long)(items * c.kvh), (long long)recs);
 	float *ro = nullptr;
 	float2 *ml = nullptr;
 	if (recs)
 		if (int rc = records((size_t)recs, HD, &ro, &ml)) return rc;
-	launch(dim3((unsigned)(items * c.kvh)), ro, ml);
+	launch(dim3((unsigned)(items * c.kvh)), order, ro, ml);
 	HK_LAUNCHED("attention");
 	if (recs) {
-		hipLaunchKernelGGL((prompt_join_kernel<HD, K>), dim3(t.join[t.n], H), dim3(64 * kJoin), 0, stream(), t, c.prefix_len, out,
-		                   ldo, H, ro, ml);
+		const int64_t blocks = ((int64_t)t.join[t.n] * H * (HD / 4) + 255) / 256;
+		hipLaunchKernelGGL((prompt_join_kernel<HD, K>), dim3((unsigned)blocks), dim3(256), 0, stream(), t, c.prefix_len, out, ldo, H,
+		                   ro, ml);
 		HK_LAUNCHED("attention join");
 	}
 	return HAKO_GPU_OK;
@@ -1381,22 +1443,39 @@ int64_t all_steps(const AttnKv &c, const SeqTab &t, int tokens) {
 	return n * c.kvh;
 }
 
+// Which kernel (7B heads, one MI355X, direct / tiled): 200 tokens 10 / 20 us,
+// 512 16 / 31, 512 at position 3000 (52 thousand wave-steps of 32 rows x 32
+// keys) 73 / 73, 2000 tokens (63 thousand) 98 / 86, 8192 tokens 1601 / 880.
+// So the direct one up to 55 wave-steps for each SIMD.
+//
+// Parts: the tiled kernel splits tiles of more than 1.5 times an equal share
+// of the work (1, 1.5, 2 times: packed prompts of 4096 tokens 104 / 98 / 109
+// us, 2 x 1500 tokens 99 / 84 / 85: a part costs its record's way to memory and
+// back); the direct one tiles of more than a share where they are too few for
+// the chip (64 tokens at position 8000: 35 us, 40 at two shares), else of more
+// than two (512 at 3000: 73, 90 at one).
 template <int HD, bool Q8>
 int prompt(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, const float *q, int64_t ldq, int H, float scale) {
 	const int G = H / c.kvh;
-	const int64_t big = all_steps<kKeys>(c, t, 32 * kTileWaves / G);
-	if (g_attn_prompt ? g_attn_prompt == 2 : big >= kBigSteps * cu_count())
+	const int64_t cu = cu_count(), slots = 2 * cu;   // workgroups of the direct kernel that run at once
+	const int64_t steps = all_steps<32>(c, t, 32 / G);
+	if (g_attn_prompt ? g_attn_prompt == 2 : steps > 55 * 4 * cu) {
+		const int64_t all = all_steps<kKeys>(c, t, 32 * kTileWaves / G);
 		return prompt_launch<HD, Q8, kKeys>(
-		    c, t, out, ldo, H, 32 * kTileWaves, std::max<int64_t>(4, 2 * (big / cu_count())), [&](dim3 grid, float *ro, float2 *ml) {
-			    hipLaunchKernelGGL((prompt_kernel<HD, Q8, kTileWaves>), grid, dim3(64 * kTileWaves), 0, stream(), c, t, out, ldo, q,
-			                       ldq, G, scale * kLog2e, ro, ml);
+		    c, t, out, ldo, H, 32 * kTileWaves, std::max<int64_t>(4, (3 * all + 2 * cu - 1) / (2 * cu)),
+		    [&](dim3 grid, const ItemTab &order, float *ro, float2 *ml) {
+			    hipLaunchKernelGGL((prompt_kernel<HD, Q8, kTileWaves>), grid, dim3(64 * kTileWaves), 0, stream(), c, t, order, out,
+			                       ldo, q, ldq, G, scale * kLog2e, ro, ml);
 		    });
-	const int64_t steps = all_steps<32>(c, t, 32 / G), slots = 2 * cu_count();
-	const int64_t unit = std::max<int64_t>(kMinUnit, 2 * ((steps + slots - 1) / slots));
-	return prompt_launch<HD, Q8, 32>(c, t, out, ldo, H, 32, unit, [&](dim3 grid, float *ro, float2 *ml) {
-		hipLaunchKernelGGL((prompt_direct_kernel<HD, Q8>), grid, dim3(64 * kWaves), 0, stream(), c, t, out, ldo, q, ldq, G,
-		                   scale * kLog2e, ro, ml);
-	});
+	}
+	int64_t tiles = 0;
+	for (int s = 0; s < t.n; s++) tiles += (t.len[s] + 32 / G - 1) / (32 / G);
+	const int64_t share = (steps + slots - 1) / slots;
+	return prompt_launch<HD, Q8, 32>(c, t, out, ldo, H, 32, std::max<int64_t>(4 * kWaves, 2 * tiles * c.kvh <= slots ? share : 2 * share),
+	                                 [&](dim3 grid, const ItemTab &order, float *ro, float2 *ml) {
+		                                 hipLaunchKernelGGL((prompt_direct_kernel<HD, Q8>), grid, dim3(64 * kWaves), 0, stream(), c, t,
+		                                                    order, out, ldo, q, ldq, G, scale * kLog2e, ro, ml);
+	                                 });
 }
 
 }  // namespace
