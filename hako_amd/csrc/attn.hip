@@ -867,31 +867,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_direct_kernel(AttnKv c,
 	                    on && !whole ? rec_o + rec * HD : nullptr, rec_ml + rec);
 }
 
-// The prefix of a batch: rows are (sequence, head of the group), every row
-// over the prefix's keys below its length; always to records.
-template <int HD, bool Q8>
-__global__ __launch_bounds__(64 * kWaves, 2) void prefix_kernel(AttnKv c, const float *q, int64_t ldq, const int *__restrict__ slot,
-                                                        const int *__restrict__ len, int n_seq, int G, float scale,
-                                                        int unit, int nrec, float *__restrict__ rec_o,
-                                                        float2 *__restrict__ rec_ml) {
-	__shared__ DirectLds<HD> s;
-	const int lane = threadIdx.x & 63;
-	const int kvh = blockIdx.x % c.kvh, part = blockIdx.x / c.kvh;
-	const int64_t r = (int64_t)blockIdx.y * 32 + (lane & 31);
-	const int sq = (int)(r / G), head = kvh * G + (int)(r - (int64_t)sq * G);
-	const bool on = sq < n_seq;
-	int lim = 0;
-	if (on) {
-		const int sl = slot ? slot[sq] : sq;
-		lim = sl < 0 || sl >= c.n_slots ? 0 : min(max(len[sq], 0), c.prefix_len);
-	}
-	const size_t rec = on ? ((size_t)sq * (c.kvh * G) + head) * nrec + part : 0;
-	const int nc = (c.prefix_len + 31) / 32;
-	direct_rows<HD, Q8>(c, s, kvh, c.prefix_slot, c.prefix_len, part * unit, min(nc, part * unit + unit),
-	                    on ? q + (int64_t)sq * ldq + head * HD : nullptr, scale, lim, nullptr, on ? rec_o + rec * HD : nullptr,
-	                    rec_ml + rec);
-}
-
 // ── single tokens: the up to 16 query heads of a group over one sequence's own keys ──
 //
 // Workgroup (key/value head, part, sequence); each wave takes steps of 32
@@ -1095,16 +1070,19 @@ __device__ __forceinline__ int own_end(const AttnKv &c, const int *slot, const i
 	return sl < 0 || sl >= c.n_slots ? 0 : min(max(len[sq], 0), c.max_seq);
 }
 
+template <int HD>
+struct DecodeLds {
+	alignas(16) float o[kWaves][kMaxGroup][HD + 4];
+	float ml[kWaves][kMaxGroup][2];
+};
+
 template <int HD, bool Q8>
-__global__ __launch_bounds__(256) void decode_kernel(AttnKv c, float *out, int64_t ldo, const float *q, int64_t ldq,
-                                                     const int *__restrict__ slot, const int *__restrict__ len, int G,
-                                                     float scale, int parts, int rec0, int nrec,
-                                                     float *__restrict__ rec_o, float2 *__restrict__ rec_ml) {
+__device__ __forceinline__ void decode_part(const AttnKv &c, DecodeLds<HD> &s, int kvh, int part, int sq, float *out, int64_t ldo,
+                                            const float *q, int64_t ldq, const int *__restrict__ slot,
+                                            const int *__restrict__ len, int G, float scale, int parts, int rec0, int nrec,
+                                            float *__restrict__ rec_o, float2 *__restrict__ rec_ml) {
 	constexpr int EB = Q8 ? 1 : 2;
-	__shared__ __align__(16) float o_s[kWaves][kMaxGroup][HD + 4];
-	__shared__ float ml_s[kWaves][kMaxGroup][2];
 	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-	const int kvh = blockIdx.x, part = blockIdx.y, sq = blockIdx.z;
 	int sl;
 	const int end = own_end(c, slot, len, sq, sl), n = max(end - c.prefix_len, 0);
 	const int per = part_keys(n, parts);
@@ -1146,25 +1124,25 @@ __global__ __launch_bounds__(256) void decode_kernel(AttnKv c, float *out, int64
 	for (int v = 0; v < 4; v++)
 #pragma unroll
 		for (int d = 0; d < w.VD; d += 4)
-			*(float4 *)&o_s[wave][i][w.VD * (4 * g + v) + d] =
+			*(float4 *)&s.o[wave][i][w.VD * (4 * g + v) + d] =
 			    make_float4(w.o[d][v] * f, w.o[d + 1][v] * f, w.o[d + 2][v] * f, w.o[d + 3][v] * f);
 	if (g == 0) {
-		ml_s[wave][i][0] = w.M;
-		ml_s[wave][i][1] = w.l;
+		s.ml[wave][i][0] = w.M;
+		s.ml[wave][i][1] = w.l;
 	}
 	__syncthreads();
 	for (int t = tid; t < G * (HD / 4); t += 256) {
 		const int row = t / (HD / 4), d = t % (HD / 4) * 4;
-		float m = ml_s[0][row][0];
+		float m = s.ml[0][row][0];
 #pragma unroll
-		for (int k = 1; k < kWaves; k++) m = __builtin_fmaxf(m, ml_s[k][row][0]);
+		for (int k = 1; k < kWaves; k++) m = __builtin_fmaxf(m, s.ml[k][row][0]);
 		float ls = 0.0f;
 		float4 a = make_float4(0, 0, 0, 0);
 #pragma unroll
 		for (int k = 0; k < kWaves; k++) {
-			const float x = exp2_(ml_s[k][row][0] - m);
-			const float4 b = *(const float4 *)&o_s[k][row][d];
-			ls = __builtin_fmaf(ml_s[k][row][1], x, ls);
+			const float x = exp2_(s.ml[k][row][0] - m);
+			const float4 b = *(const float4 *)&s.o[k][row][d];
+			ls = __builtin_fmaf(s.ml[k][row][1], x, ls);
 			a.x = __builtin_fmaf(b.x, x, a.x);
 			a.y = __builtin_fmaf(b.y, x, a.y);
 			a.z = __builtin_fmaf(b.z, x, a.z);
@@ -1180,6 +1158,54 @@ __global__ __launch_bounds__(256) void decode_kernel(AttnKv c, float *out, int64
 			if (d == 0) rec_ml[rec] = make_float2(m, ls);
 		}
 	}
+}
+
+template <int HD, bool Q8>
+__global__ __launch_bounds__(256) void decode_kernel(AttnKv c, float *out, int64_t ldo, const float *q, int64_t ldq,
+                                                     const int *__restrict__ slot, const int *__restrict__ len, int G,
+                                                     float scale, int parts, int nrec, float *__restrict__ rec_o,
+                                                     float2 *__restrict__ rec_ml) {
+	__shared__ DecodeLds<HD> s;
+	decode_part<HD, Q8>(c, s, blockIdx.x, blockIdx.y, blockIdx.z, out, ldo, q, ldq, slot, len, G, scale, parts, 0, nrec, rec_o,
+	                    rec_ml);
+}
+
+// A batch with a prefix in one launch, so that the two kinds of work fill each
+// other's gaps: first the prefix's workgroups (rows are (sequence, head of the
+// group), every row over the prefix's keys below its length), then the
+// sequences' own; always to records.
+template <int HD, bool Q8>
+__global__ __launch_bounds__(64 * kWaves, 2) void prefix_kernel(AttnKv c, const float *q, int64_t ldq, const int *__restrict__ slot,
+                                                        const int *__restrict__ len, int n_seq, int G, float scale,
+                                                        int tiles, int pparts, int unit, int parts, int nrec,
+                                                        float *__restrict__ rec_o, float2 *__restrict__ rec_ml) {
+	__shared__ union Lds {
+		DirectLds<HD> a;
+		DecodeLds<HD> b;
+		__device__ Lds() {}
+	} s;
+	const int kvh = blockIdx.x % c.kvh;
+	int b = blockIdx.x / c.kvh;
+	if (b >= tiles * pparts) {
+		b -= tiles * pparts;
+		decode_part<HD, Q8>(c, s.b, kvh, b % parts, b / parts, nullptr, 0, q, ldq, slot, len, G, scale, parts, pparts, nrec, rec_o,
+		                    rec_ml);
+		return;
+	}
+	const int lane = threadIdx.x & 63, part = b / tiles;
+	const int64_t r = (int64_t)(b % tiles) * 32 + (lane & 31);
+	const int sq = (int)(r / G), head = kvh * G + (int)(r - (int64_t)sq * G);
+	const bool on = sq < n_seq;
+	int lim = 0;
+	if (on) {
+		const int sl = slot ? slot[sq] : sq;
+		lim = sl < 0 || sl >= c.n_slots ? 0 : min(max(len[sq], 0), c.prefix_len);
+	}
+	const size_t rec = on ? ((size_t)sq * (c.kvh * G) + head) * nrec + part : 0;
+	const int nc = (c.prefix_len + 31) / 32;
+	direct_rows<HD, Q8>(c, s.a, kvh, c.prefix_slot, c.prefix_len, part * unit, min(nc, part * unit + unit),
+	                    on ? q + (int64_t)sq * ldq + head * HD : nullptr, scale, lim, nullptr, on ? rec_o + rec * HD : nullptr,
+	                    rec_ml + rec);
 }
 
 // One head's n records joined by a workgroup of kJoin waves: HD/4 lanes to a
@@ -1338,7 +1364,9 @@ int decode(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq
 	// own keys: parts of at least 32 keys a wave, until the workgroups fill the chip
 	int parts = (own + 32 * kWaves - 1) / (32 * kWaves);
 	const int64_t pairs = (int64_t)n_seq * c.kvh;
-	const int fill = (int)std::max<int64_t>(1, (slots + pairs - 1) / pairs);
+	// (one part from a workgroup per CU on: 64 sequences of 1000 positions, 256 pairs, 16.5 us against 19.1 with two parts
+	// and their join; 16 of 4096, 64 pairs: 18.4 us with 8 parts, 20.0 with 4, 23.5 with 12)
+	const int fill = pairs >= cu_count() ? 1 : (int)((slots + pairs - 1) / pairs);
 	parts = std::max(1, std::min(parts, fill));
 	// the prefix: parts of at least a step for each wave, until its tiles fill the chip
 	const int64_t tiles = ((int64_t)n_seq * G + 31) / 32;
@@ -1355,12 +1383,14 @@ int decode(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq
 	if (nrec)
 		if (int rc = records((size_t)n_seq * H * nrec, HD, &ro, &ml)) return rc;
 	if (pparts) {
-		hipLaunchKernelGGL((prefix_kernel<HD, Q8>), dim3(c.kvh * pparts, (unsigned)tiles), dim3(64 * kWaves), 0, stream(), c, q, ldq,
-		                   slot, len, n_seq, G, scale * kLog2e, unit, nrec, ro, ml);
-		HK_LAUNCHED("attention prefix");
+		const int64_t blocks = (tiles * pparts + (int64_t)n_seq * parts) * c.kvh;
+		if (blocks > 0x7FFFFFFF) return set_error(HAKO_GPU_EINVAL, "%lld workgroups in one call", (long long)blocks);
+		hipLaunchKernelGGL((prefix_kernel<HD, Q8>), dim3((unsigned)blocks), dim3(64 * kWaves), 0, stream(), c, q, ldq, slot, len,
+		                   n_seq, G, scale * kLog2e, (int)tiles, pparts, unit, parts, nrec, ro, ml);
+	} else {
+		hipLaunchKernelGGL((decode_kernel<HD, Q8>), dim3(c.kvh, parts, n_seq), dim3(256), 0, stream(), c, out, ldo, q, ldq, slot,
+		                   len, G, scale * kLog2e, parts, nrec, ro, ml);
 	}
-	hipLaunchKernelGGL((decode_kernel<HD, Q8>), dim3(c.kvh, parts, n_seq), dim3(256), 0, stream(), c, out, ldo, q, ldq, slot,
-	                   len, G, scale * kLog2e, parts, pparts, nrec, ro, ml);
 	HK_LAUNCHED("attention");
 	if (nrec) {
 		hipLaunchKernelGGL(decode_join_kernel<HD>, dim3(H, n_seq), dim3(64 * kJoin), 0, stream(), c, out, ldo, slot, len, H, parts,
