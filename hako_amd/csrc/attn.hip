@@ -23,6 +23,11 @@
 #include <float.h>
 #include <vector>
 
+// CALL(HD, Q8) for a cache's head size and type.
+#define HK_KV_SWITCH(kv, CALL)                                     \
+	((kv)->head_dim == 128 ? ((kv)->type == HAKO_KV_Q8 ? CALL(128, true) : CALL(128, false)) \
+	                       : ((kv)->type == HAKO_KV_Q8 ? CALL(64, true) : CALL(64, false)))
+
 namespace hako {
 namespace {
 
@@ -50,6 +55,7 @@ struct AttnKv {
 	const float *ks, *vs;
 	int n_slots, max_seq, kvh;
 	int prefix_slot, prefix_len;
+	int len_add;   // added to every length (single tokens)
 };
 
 // A prompt launch: sequence s has len[s] tokens from row row[s] of q and
@@ -1067,7 +1073,7 @@ __device__ __forceinline__ int part_keys(int n, int parts) {
 // A sequence's own keys [prefix, end): end, 0 where it has no slot.
 __device__ __forceinline__ int own_end(const AttnKv &c, const int *slot, const int *len, int sq, int &sl) {
 	sl = slot ? slot[sq] : sq;
-	return sl < 0 || sl >= c.n_slots ? 0 : min(max(len[sq], 0), c.max_seq);
+	return sl < 0 || sl >= c.n_slots ? 0 : min(max(len[sq] + c.len_add, 0), c.max_seq);
 }
 
 template <int HD>
@@ -1198,8 +1204,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefix_kernel(AttnKv c, const 
 	const bool on = sq < n_seq;
 	int lim = 0;
 	if (on) {
-		const int sl = slot ? slot[sq] : sq;
-		lim = sl < 0 || sl >= c.n_slots ? 0 : min(max(len[sq], 0), c.prefix_len);
+		int sl;
+		lim = min(own_end(c, slot, len, sq, sl), c.prefix_len);
 	}
 	const size_t rec = on ? ((size_t)sq * (c.kvh * G) + head) * nrec + part : 0;
 	const int nc = (c.prefix_len + 31) / 32;
@@ -1340,9 +1346,9 @@ int attn_check(float *out, int64_t ldo, const float *q, int64_t ldq, const hako_
 	return HAKO_GPU_OK;
 }
 
-AttnKv attn_kv(const hako_gpu_kv *kv, int prefix_slot, int prefix_len) {
+AttnKv attn_kv(const hako_gpu_kv *kv, int prefix_slot, int prefix_len, int len_add) {
 	return {(const uint8_t *)kv->k, (const uint8_t *)kv->v, kv->k_scale, kv->v_scale, kv->n_slots, kv->max_seq,
-	        kv->n_kv_heads, prefix_slot, prefix_len};
+	        kv->n_kv_heads, prefix_slot, prefix_len, len_add};
 }
 
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -1356,28 +1362,44 @@ int records(size_t n, int HD, float **o, float2 **ml) {
 	return HAKO_GPU_OK;
 }
 
+// How the single tokens of a batch are shared out: own keys in `parts` parts,
+// the prefix (tiles of 32 rows) in pparts parts of `unit` steps, nrec records
+// to a query head (0: written at once).
+struct DecodePlan {
+	int64_t tiles;
+	int parts, pparts, unit, nrec;
+};
+DecodePlan decode_plan(int max_seq, int prefix_len, int kvh, int n_seq, int H) {
+	DecodePlan p{};
+	const int own = max_seq - prefix_len;
+	const int slots = 2 * cu_count();   // workgroups that run at once
+	// own keys: parts of at least 32 keys a wave, until the workgroups fill the chip (one part from a workgroup per CU on:
+	// 64 sequences of 1000 positions, 256 pairs, 16.5 us against 19.1 with two parts and their join; 16 of 4096, 64 pairs:
+	// 18.4 us with 8 parts, 20.0 with 4, 23.5 with 12)
+	p.parts = (own + 32 * kWaves - 1) / (32 * kWaves);
+	const int64_t pairs = (int64_t)n_seq * kvh;
+	const int fill = pairs >= cu_count() ? 1 : (int)((slots + pairs - 1) / pairs);
+	p.parts = std::max(1, std::min(p.parts, fill));
+	// the prefix: parts of at least a step for each wave, until its tiles fill the chip
+	p.tiles = ((int64_t)n_seq * (H / kvh) + 31) / 32;
+	const int nc = (prefix_len + 31) / 32;
+	p.unit = 1;
+	if (nc) {
+		const int want = (int)std::max<int64_t>(1, slots / (p.tiles * kvh));
+		p.unit = std::max(kWaves, ((nc + want - 1) / want + kWaves - 1) / kWaves * kWaves);
+		p.pparts = (nc + p.unit - 1) / p.unit;
+	}
+	p.nrec = p.pparts + p.parts > 1 ? p.pparts + p.parts : 0;
+	return p;
+}
+
 template <int HD, bool Q8>
 int decode(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq, const int *slot, const int *len,
            int n_seq, int H, float scale) {
-	const int G = H / c.kvh, own = c.max_seq - c.prefix_len;
-	const int slots = 2 * cu_count();   // workgroups that run at once
-	// own keys: parts of at least 32 keys a wave, until the workgroups fill the chip
-	int parts = (own + 32 * kWaves - 1) / (32 * kWaves);
-	const int64_t pairs = (int64_t)n_seq * c.kvh;
-	// (one part from a workgroup per CU on: 64 sequences of 1000 positions, 256 pairs, 16.5 us against 19.1 with two parts
-	// and their join; 16 of 4096, 64 pairs: 18.4 us with 8 parts, 20.0 with 4, 23.5 with 12)
-	const int fill = pairs >= cu_count() ? 1 : (int)((slots + pairs - 1) / pairs);
-	parts = std::max(1, std::min(parts, fill));
-	// the prefix: parts of at least a step for each wave, until its tiles fill the chip
-	const int64_t tiles = ((int64_t)n_seq * G + 31) / 32;
-	const int nc = (c.prefix_len + 31) / 32;
-	int unit = 1, pparts = 0;
-	if (nc) {
-		const int want = (int)std::max<int64_t>(1, slots / (tiles * c.kvh));
-		unit = std::max(kWaves, ((nc + want - 1) / want + kWaves - 1) / kWaves * kWaves);
-		pparts = (nc + unit - 1) / unit;
-	}
-	const int nrec = pparts + parts > 1 ? pparts + parts : 0;
+	const int G = H / c.kvh;
+	const DecodePlan p = decode_plan(c.max_seq, c.prefix_len, c.kvh, n_seq, H);
+	const int parts = p.parts, pparts = p.pparts, unit = p.unit, nrec = p.nrec;
+	const int64_t tiles = p.tiles;
 	float *ro = nullptr;
 	float2 *ml = nullptr;
 	if (nrec)
@@ -1510,15 +1532,26 @@ int prompt(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, const float *q, 
 
 }  // namespace
 
+int attn_decode(float *out, int64_t ldo, const float *q, int64_t ldq, const hako_gpu_kv *kv, const int *slot,
+                const int *len, int len_add, int n_seq, int H, float scale, int prefix_slot, int prefix_len) {
+	const AttnKv c = attn_kv(kv, prefix_slot, prefix_len, len_add);
+#define HK_DECODE(HD, Q8) decode<HD, Q8>(c, out, ldo, q, ldq, slot, len, n_seq, H, scale)
+	return HK_KV_SWITCH(kv, HK_DECODE);
+#undef HK_DECODE
+}
+
+int attn_decode_reserve(const hako_gpu_kv *kv, int n_seq, int H, int prefix_len) {
+	const DecodePlan p = decode_plan(kv->max_seq, prefix_len, kv->n_kv_heads, n_seq, H);
+	float *o;
+	float2 *ml;
+	return p.nrec ? records((size_t)n_seq * H * p.nrec, kv->head_dim, &o, &ml) : HAKO_GPU_OK;
+}
+
 void attn_set_prompt(int v) { g_attn_prompt = v == 1 || v == 2 ? v : 0; }
 
 }  // namespace hako
 
 using namespace hako;
-
-#define HK_KV_SWITCH(kv, CALL)                                     \
-	((kv)->head_dim == 128 ? ((kv)->type == HAKO_KV_Q8 ? CALL(128, true) : CALL(128, false)) \
-	                       : ((kv)->type == HAKO_KV_Q8 ? CALL(64, true) : CALL(64, false)))
 
 extern "C" {
 
@@ -1532,10 +1565,8 @@ int hako_gpu_attn_decode(float *out, int64_t out_stride, const float *q, int64_t
 	if (n_seq > 65535) return set_error(HAKO_GPU_EINVAL, "%d sequences in one call (at most 65535)", n_seq);
 	if (int rc = require_device()) return rc;
 	if (n_seq == 0) return ok();
-	const AttnKv c = attn_kv(kv, prefix_slot, prefix_len);
-#define HK_DECODE(HD, Q8) decode<HD, Q8>(c, out, out_stride, q, q_stride, slot, len, n_seq, n_heads, scale)
-	if (int rc = HK_KV_SWITCH(kv, HK_DECODE)) return rc;
-#undef HK_DECODE
+	if (int rc = attn_decode(out, out_stride, q, q_stride, kv, slot, len, 0, n_seq, n_heads, scale, prefix_slot, prefix_len))
+		return rc;
 	return ok();
 }
 
@@ -1555,7 +1586,7 @@ int hako_gpu_attn_prompt(float *out, int64_t out_stride, const float *q, int64_t
 	}
 	if (rows > 0x7FFFFFFF) return set_error(HAKO_GPU_EINVAL, "%lld tokens in one call", (long long)rows);
 	if (int rc = require_device()) return rc;
-	const AttnKv c = attn_kv(kv, prefix_slot, prefix_len);
+	const AttnKv c = attn_kv(kv, prefix_slot, prefix_len, 0);
 	// the sequences with tokens, those that end last (the longest tiles) first
 	std::vector<int> order, row(n_seq);
 	for (int s = 0, r = 0; s < n_seq; r += len[s++]) {

@@ -29,6 +29,7 @@
 #include "dequant_dev.h"
 #include "hako_dev.h"
 #include "hako_rt.h"
+#include "kv.h"
 #include "q4k_dev.h"
 #include "skinny.h"
 
@@ -1464,6 +1465,12 @@ struct hako_gpu_decoder {
 	float *x = nullptr, *xn = nullptr, *qkv = nullptr, *att = nullptr, *h = nullptr, *g = nullptr, *u = nullptr,
 	      *tmp = nullptr, *logits = nullptr, *part = nullptr, *kc = nullptr, *vc = nullptr;
 	float2 *rope = nullptr, *apart = nullptr;
+	// caches in 8 or 16 bits (HAKO_KV_*, in place of kc and vc), per layer,
+	// and the prefix that all sequences share (positions below prefix_len are
+	// sequence prefix_seq's)
+	int kv_type = 0, prefix_seq = 0, prefix_len = 0;
+	std::vector<hako_gpu_kv> kv;
+	int *pf_slot = nullptr;   // the sequence of a pass's tokens
 	int *tok = nullptr, *pos = nullptr, *ring = nullptr, *nout = nullptr;
 	// one sequence: the output projection's fixed-point residual accumulators
 	// (three: by layer parity, and the last layer of an odd count; then one
@@ -1696,6 +1703,19 @@ int attention(hako_gpu_decoder *d, int l, int8_t *mxq = nullptr, float *mxs = nu
 	const hako_gpu_model &m = d->m;
 	const int KV = d->kv_dim, HD = m.head_dim, G = m.n_heads / m.n_kv_heads;
 	const float scale = 1.0f / sqrtf((float)HD);
+	if (d->kv_type) {
+		// the cache calls: queries rotated in place and the new rows appended, then attention over pos + 1 positions
+		const hako_gpu_kv *kv = &d->kv[l];
+		const int D = m.d_model;
+		const hako_gpu_rope rope = {(const float *)d->rope, d->max_seq, HD, 0};
+		if (int rc = hako_gpu_kv_append(kv, nullptr, d->pos, d->n_seq, d->qkv + D, d->qkv + D + KV, d->qkv_dim, &rope, d->qkv,
+		                                d->qkv, m.n_heads, d->qkv_dim, d->qkv_dim))
+			return rc;
+		if (int rc = attn_decode(d->att, D, d->qkv, d->qkv_dim, kv, nullptr, d->pos, 1, d->n_seq, m.n_heads, scale,
+		                         d->prefix_seq, d->prefix_len))
+			return rc;
+		return mxq ? hako_gpu_quantize_q8_32(d->att, d->n_seq, D, mxq, mxs) : HAKO_GPU_OK;
+	}
 	const size_t kv_seq_stride = (size_t)m.n_layers * d->max_seq * KV;
 	float *kcl = d->kc + (size_t)l * d->max_seq * KV, *vcl = d->vc + (size_t)l * d->max_seq * KV;
 	// one sequence: a grid of chunks x KV heads leaves most CUs idle, so each
@@ -1927,7 +1947,7 @@ int enqueue_step(hako_gpu_decoder *d) {
 	if (d->n_seq > 1) return enqueue_batched_step(d);
 	const hako_gpu_model &m = d->m;
 	const int D = m.d_model, F = m.ffn_dim, KV = d->kv_dim;
-	const bool merge_o = merge_o_all(m, d->blocks);
+	const bool merge_o = !d->kv_type && merge_o_all(m, d->blocks);   // (its records are the fp32 caches')
 	hipLaunchKernelGGL(embed_kernel, dim3(d->n_seq), dim3(256), 0, stream(), (const uint8_t *)m.tok_embd, m.t_embd,
 	                   row_bytes(m.t_embd, D), d->tok, d->x, D, m.vocab);
 	HK_LAUNCHED("embed");
@@ -2096,6 +2116,9 @@ int check_room(hako_gpu_decoder *d, int n) {
 		if (pos[s] < 0 || pos[s] + n > d->max_seq)
 			return set_error(HAKO_GPU_EINVAL, "sequence %d at position %d has no room for %d steps (max_seq %d)", s,
 			                 pos[s], n, d->max_seq);
+		else if (pos[s] < d->prefix_len)
+			return set_error(HAKO_GPU_EINVAL, "sequence %d at position %d would write inside the prefix of %d positions", s,
+			                 pos[s], d->prefix_len);
 	return HAKO_GPU_OK;
 }
 
@@ -2129,8 +2152,7 @@ int prefill_alloc(hako_gpu_decoder *d) {
 	d->pf_part_bytes = rec < kPrefillRecordBytes ? rec : kPrefillRecordBytes;
 	const size_t D = m.d_model, F = m.ffn_dim, KV = d->kv_dim;
 	int rc = 0;
-#define HK_ALLOC(ptr, bytes) \
-	if (!rc) rc = dalloc(d, (bytes), (void **)&(ptr))
+#define HK_ALLOC(ptr, bytes) rc = rc ? rc : dalloc(d, (bytes), (void **)&(ptr))
 	HK_ALLOC(d->pf_x, 4 * C * D);
 	HK_ALLOC(d->pf_xn, 4 * C * D);
 	HK_ALLOC(d->pf_q, 4 * C * D);
@@ -2140,7 +2162,8 @@ int prefill_alloc(hako_gpu_decoder *d) {
 	HK_ALLOC(d->pf_tmp, 4 * C * D);
 	HK_ALLOC(d->pf_g, 4 * C * F);
 	HK_ALLOC(d->pf_u, 4 * C * F);
-	HK_ALLOC(d->pf_part, d->pf_part_bytes);
+	if (d->kv_type) HK_ALLOC(d->pf_slot, 4 * C);
+	else HK_ALLOC(d->pf_part, d->pf_part_bytes);
 	HK_ALLOC(d->pf_xq, C * (D > F ? D : F));
 	HK_ALLOC(d->pf_xs, 4 * C * (D > F ? D : F) / 32);
 	HK_ALLOC(d->pf_xh, 4 * C * F);
@@ -2164,7 +2187,12 @@ int prefill_chunk(hako_gpu_decoder *d, int seq, const int *tokens, int n, int po
 	for (int i = 0; i < n; i++) posv[i] = pos0 + i;
 	HK_HIP(hipMemcpyAsync(d->pf_tok, tokens, sizeof(int) * n, hipMemcpyHostToDevice, stream()));
 	HK_HIP(hipMemcpyAsync(d->pf_pos, posv.data(), sizeof(int) * n, hipMemcpyHostToDevice, stream()));
-	HK_HIP(hipStreamSynchronize(stream()));   // posv is this frame's
+	std::vector<int> slotv;
+	if (d->kv_type) {
+		slotv.assign(n, seq);
+		HK_HIP(hipMemcpyAsync(d->pf_slot, slotv.data(), sizeof(int) * n, hipMemcpyHostToDevice, stream()));
+	}
+	HK_HIP(hipStreamSynchronize(stream()));   // posv and slotv are this frame's
 	hipLaunchKernelGGL(embed_kernel, dim3(n), dim3(256), 0, stream(), (const uint8_t *)m.tok_embd, m.t_embd,
 	                   row_bytes(m.t_embd, D), d->pf_tok, d->pf_x, D, m.vocab);
 	HK_LAUNCHED("embed");
@@ -2172,8 +2200,8 @@ int prefill_chunk(hako_gpu_decoder *d, int seq, const int *tokens, int n, int po
 	const size_t seq_off = (size_t)seq * m.n_layers * d->max_seq * KV;
 	for (int l = 0; l < m.n_layers; l++) {
 		const hako_gpu_block &B = d->blocks[l];
-		float *kcl = d->kc + seq_off + (size_t)l * d->max_seq * KV;
-		float *vcl = d->vc + seq_off + (size_t)l * d->max_seq * KV;
+		float *kcl = d->kv_type ? nullptr : d->kc + seq_off + (size_t)l * d->max_seq * KV;
+		float *vcl = d->kv_type ? nullptr : d->vc + seq_off + (size_t)l * d->max_seq * KV;
 		// Q4_K matmuls of more than 16 tokens run fused: one rmsnorm+q8 launch
 		// per input, q/k/v as one launch over three row segments, gate/up as
 		// one launch writing silu(gate)*up, the residual added by the o and
@@ -2196,9 +2224,11 @@ int prefill_chunk(hako_gpu_decoder *d, int seq, const int *tokens, int n, int po
 			if (int rc = hako_gpu_matmul_batch(d->pf_k, d->pf_xn, B.t_k, B.wk, B.bk, n, KV, D)) return rc;
 			if (int rc = hako_gpu_matmul_batch(d->pf_v, d->pf_xn, B.t_v, B.wv, B.bv, n, KV, D)) return rc;
 		}
-		hipLaunchKernelGGL(rope_append_kernel, dim3(n), dim3(256), 0, stream(), d->pf_k, d->pf_v, d->rope, d->pf_pos,
-		                   kcl, vcl, KVH, HD, d->max_seq);
-		HK_LAUNCHED("rope_append");
+		if (!d->kv_type) {
+			hipLaunchKernelGGL(rope_append_kernel, dim3(n), dim3(256), 0, stream(), d->pf_k, d->pf_v, d->rope, d->pf_pos,
+			                   kcl, vcl, KVH, HD, d->max_seq);
+			HK_LAUNCHED("rope_append");
+		}
 		// token i attends over positions [0, pos0 + i] of the sequence's cache;
 		// the merge also writes the q8 rows of its output for a fused o
 		int8_t *mxq = f_o ? d->pf_xq : nullptr;
@@ -2207,7 +2237,18 @@ int prefill_chunk(hako_gpu_decoder *d, int seq, const int *tokens, int n, int po
 		// exit at once), also the record stride of the pass
 		const int pchunks = prefill_chunks(pos0 + n - 1);
 		const dim3 ag(pchunks, KVH, n), mg(G, KVH, n);
-		if (HD == 128 && pos0 + n <= kFlashPos) {
+		if (d->kv_type) {
+			const hako_gpu_kv *kv = &d->kv[l];
+			const hako_gpu_rope rope = {(const float *)d->rope, d->max_seq, HD, 0};
+			if (int rc = hako_gpu_kv_append(kv, d->pf_slot, d->pf_pos, n, d->pf_k, d->pf_v, KV, &rope, d->pf_q, d->pf_q, m.n_heads,
+			                                D, D))
+				return rc;
+			if (int rc = hako_gpu_attn_prompt(d->pf_att, D, d->pf_q, D, kv, &seq, &pos0, &n, 1, m.n_heads, scale, d->prefix_seq,
+			                                  d->prefix_len))
+				return rc;
+			if (mxq)
+				if (int rc = hako_gpu_quantize_q8_32(d->pf_att, n, D, mxq, mxs)) return rc;
+		} else if (HD == 128 && pos0 + n <= kFlashPos) {
 			// every token's keys in one workgroup: matrix cores, no merge pass
 			hipLaunchKernelGGL(attn_flash_kernel<kFlashQG>, dim3(m.n_heads, (n + 16 * kFlashQG - 1) / (16 * kFlashQG)),
 			                   dim3(128 * kFlashQG), 0, stream(), d->pf_q,
@@ -2272,11 +2313,40 @@ int prefill_chunk(hako_gpu_decoder *d, int seq, const int *tokens, int n, int po
 	return HAKO_GPU_OK;
 }
 
+// The caches of a decoder in 8 or 16 bits: one layer after the other, zeros.
+int typed_caches(hako_gpu_decoder *d) {
+	const hako_gpu_model &m = d->m;
+	hako_gpu_kv kv{d->kv_type, d->n_seq, d->max_seq, m.n_kv_heads, m.head_dim, nullptr, nullptr, nullptr, nullptr};
+	size_t codes, scales;
+	if (int rc = hako_gpu_kv_bytes(&kv, &codes, &scales)) return rc;
+	uint8_t *p[4];
+	for (int i = 0; i < 4; i++) {
+		const size_t bytes = (size_t)m.n_layers * (i < 2 ? codes : scales);
+		if (int rc = dalloc(d, bytes, (void **)&p[i])) return rc;
+		HK_HIP(hipMemset(p[i], 0, bytes));
+	}
+	for (int l = 0; l < m.n_layers; l++) {
+		kv.k = p[0] + l * codes;
+		kv.v = p[1] + l * codes;
+		kv.k_scale = (float *)(p[2] + l * scales);
+		kv.v_scale = (float *)(p[3] + l * scales);
+		if (int rc = kv_check(&kv)) return rc;
+		d->kv.push_back(kv);
+	}
+	return attn_decode_reserve(&kv, d->n_seq, m.n_heads, 0);
+}
+
 }  // namespace
 
 extern "C" {
 
 int hako_gpu_decoder_create(const hako_gpu_model *m, int n_seq, int max_seq, hako_gpu_decoder **out) {
+	return hako_gpu_decoder_create_kv(m, n_seq, max_seq, 0, out);
+}
+
+int hako_gpu_decoder_create_kv(const hako_gpu_model *m, int n_seq, int max_seq, int kv_type, hako_gpu_decoder **out) {
+	if (kv_type != 0 && kv_type != HAKO_KV_F16 && kv_type != HAKO_KV_Q8)
+		return set_error(HAKO_GPU_ETYPE, "cache type %d", kv_type);
 	if (int rc = require_device()) return rc;
 	if (!m || !out || !m->blocks) return set_error(HAKO_GPU_EINVAL, "null model or output");
 	*out = nullptr;
@@ -2292,7 +2362,7 @@ int hako_gpu_decoder_create(const hako_gpu_model *m, int n_seq, int max_seq, hak
 		                 m->n_layers, m->d_model, m->n_heads, m->n_kv_heads, m->head_dim, m->ffn_dim, m->vocab,
 		                 max_seq);
 	// one sequence's layer cache is read through 32-bit buffer offsets
-	if ((size_t)max_seq * m->n_kv_heads * m->head_dim * 4 >= kBufNone)
+	if (!kv_type && (size_t)max_seq * m->n_kv_heads * m->head_dim * 4 >= kBufNone)
 		return set_error(HAKO_GPU_EINVAL, "max_seq %d x kv_dim %d: a layer's cache of one sequence exceeds 2 GiB",
 		                 max_seq, m->n_kv_heads * m->head_dim);
 	if (!known_type(m->t_embd) || !known_type(m->t_out) || !m->tok_embd || !m->out_weight || !m->out_norm)
@@ -2312,6 +2382,7 @@ int hako_gpu_decoder_create(const hako_gpu_model *m, int n_seq, int max_seq, hak
 	d->n_seq = n_seq;
 	d->max_seq = max_seq;
 	d->max_chunks = (max_seq + kChunk - 1) / kChunk;
+	d->kv_type = kv_type;
 	d->kv_dim = m->n_kv_heads * m->head_dim;
 	d->qkv_dim = m->d_model + 2 * d->kv_dim;
 	const int D = m->d_model, F = m->ffn_dim, HD = m->head_dim;
@@ -2328,9 +2399,13 @@ int hako_gpu_decoder_create(const hako_gpu_model *m, int n_seq, int max_seq, hak
 	HK_ALLOC(d->u, sizeof(float) * n_seq * F);
 	HK_ALLOC(d->tmp, sizeof(float) * n_seq * D);
 	HK_ALLOC(d->logits, sizeof(float) * n_seq * m->vocab);
-	HK_ALLOC(d->part, sizeof(float) * n_seq * m->n_kv_heads * d->max_chunks * kMaxG * (HD + 2));
-	HK_ALLOC(d->kc, sizeof(float) * kvn);
-	HK_ALLOC(d->vc, sizeof(float) * kvn);
+	if (!kv_type) {
+		HK_ALLOC(d->part, sizeof(float) * n_seq * m->n_kv_heads * d->max_chunks * kMaxG * (HD + 2));
+		HK_ALLOC(d->kc, sizeof(float) * kvn);
+		HK_ALLOC(d->vc, sizeof(float) * kvn);
+	} else if (!rc) {
+		rc = typed_caches(d);
+	}
 	HK_ALLOC(d->rope, sizeof(float2) * (size_t)max_seq * (HD / 2));
 	HK_ALLOC(d->apart, sizeof(float2) * n_seq * kArgBlocks);
 	HK_ALLOC(d->tok, sizeof(int) * n_seq);
@@ -2367,8 +2442,8 @@ int hako_gpu_decoder_create(const hako_gpu_model *m, int n_seq, int max_seq, hak
 			rope[(size_t)p * (HD / 2) + i] = make_float2(cosf(ang), sinf(ang));
 		}
 	hipError_t e = hipMemcpy(d->rope, rope.data(), sizeof(float2) * rope.size(), hipMemcpyHostToDevice);
-	if (e == hipSuccess) e = hipMemset(d->kc, 0, sizeof(float) * kvn);
-	if (e == hipSuccess) e = hipMemset(d->vc, 0, sizeof(float) * kvn);
+	if (e == hipSuccess && !kv_type) e = hipMemset(d->kc, 0, sizeof(float) * kvn);
+	if (e == hipSuccess && !kv_type) e = hipMemset(d->vc, 0, sizeof(float) * kvn);
 	if (e == hipSuccess) e = hipMemset(d->pos, 0, sizeof(int) * n_seq);
 	if (e == hipSuccess) e = hipMemset(d->nout, 0, sizeof(int) * n_seq);
 	if (e == hipSuccess) e = hipMemset(d->oacc, 0, sizeof(long long) * 4 * acc_row(D));
@@ -2406,8 +2481,35 @@ int hako_gpu_decoder_on_destroy(hako_gpu_decoder *d, void (*fn)(void *), void *a
 
 int hako_gpu_decoder_kv(hako_gpu_decoder *d, float **k_cache, float **v_cache) {
 	if (!d) return set_error(HAKO_GPU_EINVAL, "null decoder");
+	if (d->kv_type) return set_error(HAKO_GPU_EINVAL, "the decoder's caches are not fp32: see hako_gpu_decoder_cache");
 	if (k_cache) *k_cache = d->kc;
 	if (v_cache) *v_cache = d->vc;
+	return ok();
+}
+
+int hako_gpu_decoder_cache(hako_gpu_decoder *d, int layer, hako_gpu_kv *kv) {
+	if (!d || !kv) return set_error(HAKO_GPU_EINVAL, "null decoder or cache");
+	if (!d->kv_type) return set_error(HAKO_GPU_EINVAL, "the decoder's caches are fp32: see hako_gpu_decoder_kv");
+	if (layer < 0 || layer >= d->m.n_layers) return set_error(HAKO_GPU_EINVAL, "layer %d of %d", layer, d->m.n_layers);
+	*kv = d->kv[layer];
+	return ok();
+}
+
+int hako_gpu_decoder_share_prefix(hako_gpu_decoder *d, int seq, int n) {
+	if (!d) return set_error(HAKO_GPU_EINVAL, "null decoder");
+	if (!d->kv_type) return set_error(HAKO_GPU_EINVAL, "a prefix is shared in a cache of 8 or 16 bits");
+	if (seq < 0 || seq >= d->n_seq || n < 0 || n > d->max_seq)
+		return set_error(HAKO_GPU_EINVAL, "prefix of %d positions of sequence %d: %d sequences of %d", n, seq, d->n_seq,
+		                 d->max_seq);
+	if (int rc = attn_decode_reserve(&d->kv[0], d->n_seq, d->m.n_heads, n)) return rc;
+	// the captured step holds the prefix it was captured with
+	HK_HIP(hipStreamSynchronize(stream()));
+	if (d->exec) HK_HIP(hipGraphExecDestroy(d->exec));
+	if (d->graph) HK_HIP(hipGraphDestroy(d->graph));
+	d->exec = nullptr;
+	d->graph = nullptr;
+	d->prefix_seq = seq;
+	d->prefix_len = n;
 	return ok();
 }
 
@@ -2461,15 +2563,18 @@ int hako_gpu_decoder_prefill(hako_gpu_decoder *d, int seq, const int *tokens, in
 	if (pos0 < 0 || pos0 + n > d->max_seq)
 		return set_error(HAKO_GPU_EINVAL, "sequence %d at position %d has no room for %d prompt tokens (max_seq %d)",
 		                 seq, pos0, n, d->max_seq);
+	if (pos0 < d->prefix_len)
+		return set_error(HAKO_GPU_EINVAL, "sequence %d at position %d would write inside the prefix of %d positions", seq, pos0,
+		                 d->prefix_len);
 	if (int rc = prefill_alloc(d)) return rc;
 	const int D = m.d_model;
 	int last = 0;
 	for (int c0 = 0; c0 < n; c0 += last) {
 		last = n - c0 < d->pf_chunk ? n - c0 : d->pf_chunk;
 		// halved while the pass's records exceed the buffer
-		while (last > 1 && prefill_rec_bytes(m, last, prefill_chunks(pos0 + c0 + last - 1)) > d->pf_part_bytes)
+		while (!d->kv_type && last > 1 && prefill_rec_bytes(m, last, prefill_chunks(pos0 + c0 + last - 1)) > d->pf_part_bytes)
 			last /= 2;
-		if (prefill_rec_bytes(m, last, prefill_chunks(pos0 + c0 + last - 1)) > d->pf_part_bytes)
+		if (!d->kv_type && prefill_rec_bytes(m, last, prefill_chunks(pos0 + c0 + last - 1)) > d->pf_part_bytes)
 			return set_error(HAKO_GPU_EINVAL, "attention records of one prompt token at position %d exceed %zu bytes",
 			                 pos0 + c0, d->pf_part_bytes);
 		if (int rc = prefill_chunk(d, seq, tokens + c0, last, pos0 + c0)) return rc;

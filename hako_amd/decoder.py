@@ -12,7 +12,7 @@ import ctypes as C
 import numpy as np
 
 from . import mlf2
-from .gpu import Gpu
+from .gpu import Gpu, Kv
 
 _vp, _i, _f = C.c_void_p, C.c_int, C.c_float
 
@@ -34,9 +34,9 @@ class Model(C.Structure):
 
 class Decoder:
     """A device decoder for the MLF2 file at `path` (n_seq sequences of up to
-    max_seq positions)."""
+    max_seq positions); kv_type: KV_Q8 or KV_F16 caches, or 0 for fp32."""
 
-    def __init__(self, gpu: Gpu, path: str, n_seq: int = 1, max_seq: int = 2048):
+    def __init__(self, gpu: Gpu, path: str, n_seq: int = 1, max_seq: int = 2048, kv_type: int = 0):
         self.gpu, self.lib = gpu, gpu.lib
         why = mlf2.check(path)
         if why:
@@ -86,7 +86,7 @@ class Decoder:
         m.blocks = blocks
         d = _vp()
         try:
-            gpu.check(self.lib.hako_gpu_decoder_create(C.byref(m), n_seq, max_seq, C.byref(d)), "decoder_create")
+            gpu.check(self.lib.hako_gpu_decoder_create_kv(C.byref(m), n_seq, max_seq, kv_type, C.byref(d)), "decoder_create")
         except Exception:
             gpu.mirror_release(self.data)
             raise
@@ -103,6 +103,16 @@ class Decoder:
         k, v = _vp(), _vp()
         self.gpu.check(self.lib.hako_gpu_decoder_kv(self.d, C.byref(k), C.byref(v)), "decoder_kv")
         return k.value, v.value
+
+    def cache(self, layer: int) -> Kv:
+        """The layer's cache of a decoder with KV_Q8 or KV_F16 caches."""
+        kv = Kv()
+        self.gpu.check(self.lib.hako_gpu_decoder_cache(self.d, layer, C.byref(kv)), "decoder_cache")
+        return kv
+
+    def share_prefix(self, seq: int, n: int):
+        """Positions below n of every sequence become those of sequence `seq`."""
+        self.gpu.check(self.lib.hako_gpu_decoder_share_prefix(self.d, seq, n), "decoder_share_prefix")
 
     def kv_offset(self, seq: int, layer: int, pos: int) -> int:
         """Byte offset of (seq, layer, pos) in either cache."""

@@ -21,7 +21,7 @@ KV_F16, KV_Q8 = 1, 2
 
 _vp, _i, _i64, _sz = C.c_void_p, C.c_int, C.c_int64, C.c_size_t
 
-# name -> (restype, argtypes); mirrors include/hako_gpu.h, hako_attn.h and hako_decode.h one to one.
+# name -> (restype, argtypes); mirrors include/hako_gpu.h and hako_decode.h one to one.
 SIGNATURES = {
     "hako_gpu_init": (_i, [_i]),
     "hako_gpu_shutdown": (_i, []),
@@ -60,12 +60,10 @@ SIGNATURES = {
     "hako_gpu_q6k_gemm": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i]),
     "hako_gpu_matmul_batch": (_i, [_vp, _vp, _i, _vp, _vp, _i, _i, _i]),
     "hako_gpu_matmul_batch_noalloc": (_i, [_vp, _vp, _i, _vp, _vp, _i, _i, _i]),
-    "hako_gpu_kv_bytes": (_i, [_vp, C.POINTER(_sz), C.POINTER(_sz)]),
-    "hako_gpu_kv_append": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _i64, _vp, _vp, _vp, _i, _i64, _i64]),
-    "hako_gpu_kv_read": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _i64]),
-    "hako_gpu_attn_decode": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i, _i, C.c_float, _i, _i]),
-    "hako_gpu_attn_prompt": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i, _i, C.c_float, _i, _i]),
     "hako_gpu_decoder_create": (_i, [_vp, _i, _i, C.POINTER(_vp)]),
+    "hako_gpu_decoder_create_kv": (_i, [_vp, _i, _i, _i, C.POINTER(_vp)]),
+    "hako_gpu_decoder_cache": (_i, [_vp, _i, _vp]),
+    "hako_gpu_decoder_share_prefix": (_i, [_vp, _i, _i]),
     "hako_gpu_decoder_destroy": (_i, [_vp]),
     "hako_gpu_decoder_kv": (_i, [_vp, C.POINTER(_vp), C.POINTER(_vp)]),
     "hako_gpu_decoder_set_pos": (_i, [_vp, _vp]),
@@ -74,6 +72,15 @@ SIGNATURES = {
     "hako_gpu_decoder_replay": (_i, [_vp, _i]),
     "hako_gpu_decoder_prefill": (_i, [_vp, _i, _vp, _i, _vp, _vp]),
     "hako_gpu_decoder_on_destroy": (_i, [_vp, _vp, _vp]),
+}
+
+# ... and include/hako_attn.h.
+ATTN_SIGNATURES = {
+    "hako_gpu_kv_bytes": (_i, [_vp, C.POINTER(_sz), C.POINTER(_sz)]),
+    "hako_gpu_kv_append": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _i64, _vp, _vp, _vp, _i, _i64, _i64]),
+    "hako_gpu_kv_read": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _i64]),
+    "hako_gpu_attn_decode": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i, _i, C.c_float, _i, _i]),
+    "hako_gpu_attn_prompt": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i, _i, C.c_float, _i, _i]),
 }
 
 
@@ -107,7 +114,7 @@ def load_library() -> C.CDLL:
         if not os.path.exists(GPU_LIB):
             raise HakoGpuError(f"{GPU_LIB} is not built; run __graft_entry__.build() (make -C hako_amd)")
         lib = C.CDLL(GPU_LIB)
-        for name, (res, args) in SIGNATURES.items():
+        for name, (res, args) in {**SIGNATURES, **ATTN_SIGNATURES}.items():
             fn = getattr(lib, name)
             fn.restype, fn.argtypes = res, args
         _lib = lib

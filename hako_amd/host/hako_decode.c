@@ -39,6 +39,10 @@ static const void *dev_tensor(const hakm_model *m, const char *name, int require
 }
 
 int hako_decoder_from_model(const hakm_model *m, int n_seq, int max_seq, hako_gpu_decoder **dec) {
+	return hako_decoder_from_model_kv(m, n_seq, max_seq, 0, dec);
+}
+
+int hako_decoder_from_model_kv(const hakm_model *m, int n_seq, int max_seq, int kv_type, hako_gpu_decoder **dec) {
 	if (!m || !dec || !m->map) return HAKO_GPU_EINVAL;
 	*dec = NULL;
 	char why[256];
@@ -96,7 +100,7 @@ int hako_decoder_from_model(const hakm_model *m, int n_seq, int max_seq, hako_gp
 		rc = hk_ensure_device();
 		hk_unlock();
 	}
-	if (!rc) rc = hako_gpu_decoder_create(&g, n_seq, max_seq, dec);
+	if (!rc) rc = hako_gpu_decoder_create_kv(&g, n_seq, max_seq, kv_type, dec);
 	free(blocks);
 	/* the decoder reads the mirror in place: pinned until it is destroyed */
 	if (!rc) rc = hk_model_pin(m, 1);

@@ -20,6 +20,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "hako_attn.h"
+
 #ifdef __cplusplus
 extern "C" {
 #endif
@@ -70,10 +72,29 @@ typedef struct hako_gpu_decoder hako_gpu_decoder;
 int hako_gpu_decoder_create(const hako_gpu_model *m, int n_seq, int max_seq, hako_gpu_decoder **dec);
 int hako_gpu_decoder_destroy(hako_gpu_decoder *dec);
 
+/* The same with KV caches of `kv_type`: HAKO_KV_Q8 or HAKO_KV_F16
+ * (hako_attn.h: a quarter or half of the fp32 caches' memory and reads; every
+ * key and value is rounded as that header says, so logits differ from the fp32
+ * caches' by what those roundings do), or 0 for fp32. The step and the prompt
+ * pass then run on the calls of hako_attn.h. */
+int hako_gpu_decoder_create_kv(const hako_gpu_model *m, int n_seq, int max_seq, int kv_type, hako_gpu_decoder **dec);
+
+/* Layer `layer`'s cache of such a decoder, for the calls of hako_attn.h: slot
+ * s is sequence s, positions below the next write position are filled. */
+int hako_gpu_decoder_cache(hako_gpu_decoder *dec, int layer, hako_gpu_kv *kv);
+
+/* From the next call on, positions [0, n) of every sequence are those of
+ * sequence seq (their keys and values are stored once, and a step reads them
+ * once for all); n 0 ends this. The caller fills them first (prefill of seq)
+ * and sets every sequence's position to n or past it: a call that would write
+ * below n is refused. Needs a cache of 8 or 16 bits. */
+int hako_gpu_decoder_share_prefix(hako_gpu_decoder *dec, int seq, int n);
+
 /* Device addresses of the fp32 KV caches, laid out as the reference's
  * (src/model.c:71-72, 117-118) once per sequence:
  * [n_seq][n_layers][max_seq][n_kv_heads*head_dim]. A caller may fill
- * positions below the next write position directly (a prefilled context). */
+ * positions below the next write position directly (a prefilled context).
+ * EINVAL for a decoder whose caches are not fp32. */
 int hako_gpu_decoder_kv(hako_gpu_decoder *dec, float **k_cache, float **v_cache);
 
 /* Set the next write position of every sequence (hakm_ctx.pos); pos[n_seq]. */

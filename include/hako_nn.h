@@ -57,6 +57,9 @@ int hako_model_release(const hakm_model *m);
  * hako_gpu_decoder_destroy(dec): release, eviction or replacement of it are
  * refused until then. */
 int hako_decoder_from_model(const hakm_model *m, int n_seq, int max_seq, hako_gpu_decoder **dec);
+/* The same with KV caches of 8 or 16 bits (kv_type as in
+ * hako_gpu_decoder_create_kv). */
+int hako_decoder_from_model_kv(const hakm_model *m, int n_seq, int max_seq, int kv_type, hako_gpu_decoder **dec);
 
 #ifdef __cplusplus
 }

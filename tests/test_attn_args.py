@@ -1,10 +1,12 @@
 """Refusals of the cache and attention calls: made from the arguments alone, so they need no device."""
 import ctypes as C
+import os
+import re
 
 import numpy as np
 import pytest
 
-from hako_amd.gpu import KV_F16, KV_Q8, Kv, Rope, load_library
+from hako_amd.gpu import ATTN_SIGNATURES, KV_F16, KV_Q8, Kv, Rope, load_library
 
 EINVAL, ENODEV, ETYPE = -1, -2, -6
 P = 0x10000   # an aligned address that no accepted call here reaches a device with
@@ -100,6 +102,20 @@ def test_decode_refuses(lib, bad):
     dict(slot=None, start=(0, 0, 0), length=(1, 1, 1), n=3)], ids=str)
 def test_prompt_refuses(lib, bad):
     assert prompt(lib, **bad) == EINVAL
+
+
+def test_binding_covers_the_header():
+    path = os.path.join(os.path.dirname(__file__), "..", "include", "hako_attn.h")
+    src = re.sub(r"/\*.*?\*/", "", open(path).read(), flags=re.S)
+    assert sorted(re.findall(r"^int (hako_gpu_\w+)\(", src, flags=re.M)) == sorted(ATTN_SIGNATURES)
+
+
+@pytest.mark.parametrize("call,args", [
+    ("hako_gpu_decoder_create_kv", (None, 1, 64, 3, None)), ("hako_gpu_decoder_create_kv", (None, 1, 64, -1, None)),
+    ("hako_gpu_decoder_cache", (None, 0, None)), ("hako_gpu_decoder_share_prefix", (None, 0, 0))])
+def test_decoder_calls_refuse(lib, call, args):
+    args = [C.byref(C.c_void_p()) if a is None and i == 4 else a for i, a in enumerate(args)]
+    assert getattr(lib, call)(*args) in (EINVAL, ETYPE)
 
 
 def test_kv_bytes(lib):
