@@ -21,6 +21,7 @@
 
 #include <algorithm>
 #include <float.h>
+#include <new>
 #include <vector>
 
 // CALL(HD, Q8) for a cache's head size and type.
@@ -36,11 +37,14 @@ constexpr int kSeqs = 48;        // sequences of one prompt launch (by value in 
 constexpr int kItems = 480;      // items of a launch whose order the host sets (likewise)
 constexpr int kWsAttn = 7;       // library workspace slot of the records
 constexpr int kKeys = 64;        // keys per chunk of the tiled kernel
-constexpr int kWaves = 4;        // waves per workgroup of the single-token kernel
-constexpr int kTileWaves = 8;    // waves per workgroup of the tiled kernel, 32 rows each
-constexpr float kNone = -FLT_MAX;   // running maximum of a row that has seen no key
+constexpr int kTileWaves = 8;    // its waves per workgroup, 32 rows each
+constexpr int kWaves = 4;        // waves per workgroup of the direct and the single-token kernel
+// M is a whole number not below the maximum it was taken from, so that what is
+// rescaled when it moves, and where sums meet, is so by exact powers of two;
+// it moves only when the maximum passes it by kSlack, which is rare.
+constexpr float kNone = -FLT_MAX;   // M of a row that has seen no key
 constexpr float kUp = 6.0f;         // weights are 2^(u - M + 6): at most 2^14 while u <= M + kSlack
-constexpr float kSlack = 8.0f;      // M follows the maximum only when it is passed by this
+constexpr float kSlack = 8.0f;
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
@@ -111,14 +115,26 @@ __device__ __forceinline__ void split_q(const float *x, int e, h8 &hi, h8 &lo) {
 // The exponent that value scales are divided by: that of their largest.
 __device__ __forceinline__ int scale_exp(float vmax) { return f16_split_exp(vmax); }
 
-// ── tiled kernel: up to 128 query rows against chunks of 64 keys ──
+// ── tiled kernel: 256 query rows against chunks of 64 keys ──
 //
 // Rows are (token, head of the group) pairs, token-major, so that one staged
-// chunk serves every query head of a key/value head. Four waves of 32 rows
+// chunk serves every query head of a key/value head. Eight waves of 32 rows
 // (v_mfma_f32_32x32x16_f16); per chunk the workgroup converts the codes to
 // halves in LDS, keys as [key][dim] and values transposed as [dim][key], so
-// that every operand is one 16-byte LDS read. The next chunk's codes are in
-// registers while this one is computed; two LDS buffers, one barrier per chunk.
+// that every operand is one 16-byte LDS read. Two LDS buffers, one barrier per
+// chunk.
+//
+// Bound: matrix work at the chip's power. 8192 tokens of 7B heads (28 / 4 of
+// 128, 481 GFLOP, each product twice: 962) take 0.84-0.90 ms, 1.1 PFLOP/s of
+// matrix operations; an 8192^3 fp16 product of the library runs at 1.09 here.
+// The matrix pipes are then busy 61% of the cycles, the vector pipes 57%, at
+// 1.8 GHz. On the way (the same call): 128-row tiles and one accumulator set
+// per masked and unmasked instance 1.51 ms; one instance, 16-byte LDS reads
+// 1.00; the weights of the second 32 keys formed under the values' products of
+// the first 0.95; 256 rows to a chunk 0.94; padded rows, no address arithmetic
+// in the loop 0.90 (868 against 907 us on one box); staging at opposite ends
+// of a chunk by a SIMD's two waves 0.84. No difference: wave priorities around
+// either product, reads left to the compiler's own order (871 against 869).
 
 // Rows in LDS are padded by 16 bytes, so that lanes on consecutive rows meet
 // different banks. A chunk's keys lie in the order of the score tiles' rows
@@ -133,13 +149,12 @@ __device__ __forceinline__ int key_row(int key) { return (key & ~12) | ((key >> 
 template <int HD>
 __device__ __forceinline__ int dim_row(int dim) { return (dim & 3) * (HD / 4) + (dim >> 2); }
 
-template <int HD, bool Q8, int NT>
+template <int HD, bool Q8>
 struct Stage {
-	static constexpr int EB = Q8 ? 1 : 2;
+	static constexpr int EB = Q8 ? 1 : 2, NT = 64 * kTileWaves;
 	static constexpr int KU = kKeys * HD * EB / 16, KL = (KU + NT - 1) / NT;   // 16-byte key loads of a chunk, per thread
-	static constexpr int VQ = HD / 4;                                          // dim quads
-	static constexpr int VK = kKeys * VQ / NT < 8 ? 4 : 8;                     // a thread takes VK keys x 4 dims of the values
-	static constexpr int VT = kKeys / VK * VQ;                                 // threads that stage values
+	static constexpr int VQ = HD / 4, VK = 4;                                  // dim quads; a thread takes 4 keys x 4 dims
+	static constexpr int VT = kKeys / VK * VQ;                                 // threads that stage values (512 or 256)
 	uint4 k[KL];
 	uint32_t v[VK][EB];
 	float ks, vs;
@@ -216,18 +231,14 @@ struct Stage {
 #pragma unroll
 			for (int i = 0; i < 4; i++) {
 				const int dim = 4 * d + i;
-				uint8_t *at = v_s + dim_row<HD>(dim) * kDimRow + 2 * VK * kg;
-				if (VK == 8)
-					*(h8 *)at = (h8){t[i][0].x, t[i][0].y, t[i][1].x, t[i][1].y, t[i][VK / 2 - 2].x, t[i][VK / 2 - 2].y,
-					                 t[i][VK / 2 - 1].x, t[i][VK / 2 - 1].y};
-				else
-					*(uint2 *)at = make_uint2(__builtin_bit_cast(uint32_t, t[i][0]), __builtin_bit_cast(uint32_t, t[i][1]));
+				*(uint2 *)(v_s + dim_row<HD>(dim) * kDimRow + 2 * VK * kg) =
+				    make_uint2(__builtin_bit_cast(uint32_t, t[i][0]), __builtin_bit_cast(uint32_t, t[i][1]));
 			}
 		}
 		if (tid < kKeys) {
 			// a value row that is not finite makes its scores NaN, which a row that may not see it masks
 			const bool fin = __builtin_isfinite(vs);
-			E = max(E, scale_exp(wave_max(fin ? vs : 0.0f)));
+			E = max(E, scale_exp(wave_max(fin ? __builtin_fabsf(vs) : 0.0f)));
 			ks_s[tid] = fin ? ks : __builtin_nanf("");
 			vs_s[tid] = fin ? __builtin_ldexpf(vs, -E) : 0.0f;
 			if (tid == 0) *e_s = E;
@@ -237,7 +248,7 @@ struct Stage {
 
 // One wave's 32 rows over the chunks of a part. lim: the lane's row sees keys
 // (positions) below it; out: O^T (value sums, times 2^E), M and l.
-template <int HD, bool Q8, int NW>
+template <int HD, bool Q8>
 struct Tile {
 	static constexpr int KS = HD / 16, DT = HD / 32;
 	static constexpr int kKB = kKeys * kKeyRow<HD>, kVB = HD * kDimRow;
@@ -327,7 +338,7 @@ struct Tile {
 		for (int v = 0; v < 16; v++) mx = __builtin_fmaxf(__builtin_fmaxf(sc[0][v], sc[1][v]), mx);
 		mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32)) * esc;
 		if (__any(mx > M + kSlack)) {
-			const float mn = mx > M + kSlack ? mx : M;
+			const float mn = mx > M + kSlack ? __builtin_ceilf(mx) : M;
 			const float f = exp2_(M - mn);   // 0 from kNone
 			M = mn;
 			l *= f;
@@ -336,12 +347,11 @@ struct Tile {
 #pragma unroll
 				for (int v = 0; v < 16; v++) o[d][v] *= f;
 		}
-		h8 ph[2], pl[2];
-		weigh(s, b, 0, sc[0], h, ph, pl);
-		h8 qh2[2] = {ph[0], ph[1]}, ql2[2] = {pl[0], pl[1]};
-		weigh(s, b, 1, sc[1], h, ph, pl);
-		add(s, b, 0, i, h, qh2, ql2);
-		add(s, b, 1, i, h, ph, pl);
+		h8 ph[2][2], pl[2][2];
+		weigh(s, b, 0, sc[0], h, ph[0], pl[0]);
+		weigh(s, b, 1, sc[1], h, ph[1], pl[1]);
+		add(s, b, 0, i, h, ph[0], pl[0]);
+		add(s, b, 1, i, h, ph[1], pl[1]);
 		__builtin_amdgcn_sched_barrier(0);
 	}
 
@@ -399,7 +409,7 @@ struct Tile {
 		const int pend = min(c.prefix_len, end), nc1 = (pend + kKeys - 1) / kKeys;
 		auto base = [&](int sl) { return ((size_t)sl * c.kvh + kvh) * c.max_seq; };
 		const size_t b0 = base(c.prefix_len > 0 ? c.prefix_slot : slot), b1 = base(slot);
-		Stage<HD, Q8, 64 * NW> st;
+		Stage<HD, Q8> st;
 		auto load = [&](int ch) {
 			const bool pre = ch < nc1;
 			const size_t r = pre ? b0 : b1;
@@ -631,7 +641,7 @@ struct Direct {
 	__device__ __forceinline__ float scales(float *sx, int lane) {
 		const float other = __shfl_xor(sc1, 32);
 		const bool fin = __builtin_isfinite(lane < 32 ? other : sc1);   // the value row's scale
-		const int e = max(E, scale_exp(wave_max(lane >= 32 && fin ? sc1 : 0.0f)));
+		const int e = max(E, scale_exp(wave_max(lane >= 32 && fin ? __builtin_fabsf(sc1) : 0.0f)));
 		// a value row that is not finite makes its score NaN
 		sx[lane] = lane < 32 ? (fin ? sc1 : __builtin_nanf("")) : (fin ? __builtin_ldexpf(sc1, -e) : 0.0f);
 		const float f = __builtin_ldexpf(1.0f, E - e);
@@ -662,7 +672,7 @@ struct Direct {
 		for (int v = 0; v < 16; v++) mx = __builtin_fmaxf(mx, sc[v]);
 		mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32)) * esc;
 		if (__any(mx > M + kSlack || fe != 1.0f)) {
-			const float mn = mx > M + kSlack ? mx : M;
+			const float mn = mx > M + kSlack ? __builtin_ceilf(mx) : M;
 			const float f = exp2_(M - mn);   // 0 from kNone
 			M = mn;
 			l *= f;
@@ -827,11 +837,11 @@ __device__ __forceinline__ void direct_rows(const AttnKv &c, DirectLds<HD> &s, i
 }
 
 // Records: value sums rec_o [record][HD] and (M, l) rec_ml [record].
-template <int HD, bool Q8, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void prompt_kernel(AttnKv c, SeqTab t, ItemTab order, float *out, int64_t ldo, const float *q,
+template <int HD, bool Q8>
+__global__ __launch_bounds__(64 * kTileWaves, 2) void prompt_kernel(AttnKv c, SeqTab t, ItemTab order, float *out, int64_t ldo, const float *q,
                                                         int64_t ldq, int G, float scale, float *__restrict__ rec_o,
                                                         float2 *__restrict__ rec_ml) {
-	__shared__ typename Tile<HD, Q8, NW>::Lds s;
+	__shared__ typename Tile<HD, Q8>::Lds s;
 	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
 	const int kvh = blockIdx.x % c.kvh;
 	Item x;
@@ -841,7 +851,7 @@ __global__ __launch_bounds__(64 * NW, 2) void prompt_kernel(AttnKv c, SeqTab t, 
 	const int lim = on ? t.start[x.sq] + x.tok0 + tok + 1 : 0;
 	const int lo = wave_min_i(on ? lim : 0x7FFFFFFF), hi = wave_max_i(lim);
 	const int64_t row = (int64_t)t.row[x.sq] + x.tok0 + tok;
-	Tile<HD, Q8, NW> w;
+	Tile<HD, Q8> w;
 	w.query(on ? q + row * ldq + head * HD : nullptr, scale, lane);
 	w.chunks(c, kvh, x.slot, x.end, x.c0, x.c1, lim, lo, hi, s, tid);
 	if (!on) return;
@@ -1004,7 +1014,7 @@ struct Row16 {
 			x[j] = key0 + 8 * g + j < end ? (fin ? sc[j >> 2][j & 3] * ks[j] : __builtin_nanf("")) : -INFINITY;
 			vs[j] = fin ? vs[j] : 0.0f;
 			mx = __builtin_fmaxf(mx, x[j]);
-			vm = __builtin_fmaxf(vm, vs[j]);
+			vm = __builtin_fmaxf(vm, __builtin_fabsf(vs[j]));
 		}
 		mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16));
 		vm = __builtin_fmaxf(vm, __shfl_xor(vm, 16));
@@ -1012,7 +1022,7 @@ struct Row16 {
 		vm = __builtin_fmaxf(vm, __shfl_xor(vm, 32));
 		const int e = max(E, scale_exp(vm));
 		if (__any(mx > M + kSlack || e != E)) {
-			const float mn = mx > M + kSlack ? mx : M;
+			const float mn = mx > M + kSlack ? __builtin_ceilf(mx) : M;
 			const float f = exp2_(M - mn);
 			M = mn;
 			l *= f;
@@ -1434,12 +1444,15 @@ int prompt_launch(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, int H, in
 		t.item[s] = (int)items;
 		items += (int64_t)((t.len[s] + t.tile_tokens - 1) / t.tile_tokens) * t.nsplit[s];
 		t.rec[s] = (uint32_t)recs;
-		// (a tile sees no fewer steps than those before it)
-		int first = 0;
-		while (first < t.len[s] &&
-		       tile_steps<K>(t.start[s] + std::min(first + t.tile_tokens, t.len[s]), c.prefix_len) <= t.unit)
-			first += t.tile_tokens;
-		first = std::min(first, t.len[s]);
+		// the first tile of more than `unit` steps (a tile sees no fewer than those before it)
+		int lo = 0, hi = (t.len[s] + t.tile_tokens - 1) / t.tile_tokens;
+		while (lo < hi) {
+			const int mid = (lo + hi) / 2;
+			const int64_t end = t.start[s] + std::min<int64_t>((int64_t)(mid + 1) * t.tile_tokens, t.len[s]);
+			if (tile_steps<K>((int)end, c.prefix_len) <= t.unit) lo = mid + 1;
+			else hi = mid;
+		}
+		const int first = (int)std::min<int64_t>((int64_t)lo * t.tile_tokens, t.len[s]);
 		t.join[s + 1] = t.join[s] + t.len[s] - first;
 		recs += (int64_t)(t.len[s] - first) * H * t.nsplit[s];
 	}
@@ -1463,12 +1476,12 @@ int prompt_launch(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, int H, in
 		}
 	}
 	if (n <= kItems) {
-		std::stable_sort(len, len + n, [](const Len &a, const Len &b) { return a.steps > b.steps; });
+		std::sort(len, len + n, [](const Len &a, const Len &b) { return a.steps != b.steps ? a.steps > b.steps : a.item < b.item; });
 		for (int i = 0; i < n; i++) order.item[i] = len[i].item;
 		order.n = n;
 		items = n;
 	}
-	if (items * c.kvh > 0x7FFFFFFF || recs > 0xFFFFFFFFll)
+	if (items * c.kvh > 0x7FFFFFFF || recs > 0xFFFFFFFFll || (int64_t)t.join[t.n] * H > 0x7FFFFFFF)
 		return set_error(HAKO_GPU_EINVAL, "%lld tiles and %lld records in one call", (long long)(items * c.kvh), (long long)recs);
 	float *ro = nullptr;
 	float2 *ml = nullptr;
@@ -1485,13 +1498,16 @@ int prompt_launch(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, int H, in
 	return HAKO_GPU_OK;
 }
 
-// Steps of K keys over all tiles of `rows` rows.
+// Steps of K keys over all tiles of `tokens` tokens: a sequence's tiles at the
+// mean of its first and last one's.
 template <int K>
 int64_t all_steps(const AttnKv &c, const SeqTab &t, int tokens) {
 	int64_t n = 0;
-	for (int s = 0; s < t.n; s++)
-		for (int k = 0; k < t.len[s]; k += tokens)
-			n += tile_steps<K>(t.start[s] + std::min(k + tokens, t.len[s]), c.prefix_len);
+	for (int s = 0; s < t.n; s++) {
+		const int64_t tiles = (t.len[s] + tokens - 1) / tokens;
+		n += (tiles * (tile_steps<K>(t.start[s] + std::min(tokens, t.len[s]), c.prefix_len) +
+		               tile_steps<K>(t.start[s] + t.len[s], c.prefix_len)) + 1) / 2;
+	}
 	return n * c.kvh;
 }
 
@@ -1516,7 +1532,7 @@ int prompt(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, const float *q, 
 		return prompt_launch<HD, Q8, kKeys>(
 		    c, t, out, ldo, H, 32 * kTileWaves, std::max<int64_t>(4, (3 * all + 2 * cu - 1) / (2 * cu)),
 		    [&](dim3 grid, const ItemTab &order, float *ro, float2 *ml) {
-			    hipLaunchKernelGGL((prompt_kernel<HD, Q8, kTileWaves>), grid, dim3(64 * kTileWaves), 0, stream(), c, t, order, out,
+			    hipLaunchKernelGGL((prompt_kernel<HD, Q8>), grid, dim3(64 * kTileWaves), 0, stream(), c, t, order, out,
 			                       ldo, q, ldq, G, scale * kLog2e, ro, ml);
 		    });
 	}
@@ -1588,12 +1604,21 @@ int hako_gpu_attn_prompt(float *out, int64_t out_stride, const float *q, int64_t
 	if (int rc = require_device()) return rc;
 	const AttnKv c = attn_kv(kv, prefix_slot, prefix_len, 0);
 	// the sequences with tokens, those that end last (the longest tiles) first
-	std::vector<int> order, row(n_seq);
+	std::vector<int> order, row;
+	try {
+		row.resize(n_seq);
+		order.reserve(n_seq);
+	} catch (const std::bad_alloc &) {
+		return set_error(HAKO_GPU_ENOMEM, "host memory for %d sequences", n_seq);
+	}
 	for (int s = 0, r = 0; s < n_seq; r += len[s++]) {
 		row[s] = r;
 		if (len[s]) order.push_back(s);
 	}
-	std::stable_sort(order.begin(), order.end(), [&](int a, int b) { return start[a] + len[a] > start[b] + len[b]; });
+	std::sort(order.begin(), order.end(), [&](int a, int b) {
+		const int ea = start[a] + len[a], eb = start[b] + len[b];
+		return ea != eb ? ea > eb : a < b;
+	});
 	for (size_t i = 0; i < order.size();) {
 		SeqTab t{};
 		for (; i < order.size() && t.n < kSeqs; i++, t.n++) {
