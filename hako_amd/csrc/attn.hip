@@ -500,10 +500,10 @@ struct Item {
 	int sq, slot, tok0, ntok, end, part, parts, c0, c1;
 };
 template <int K>
-__device__ __forceinline__ bool item_of(const SeqTab &t, const ItemTab &order, int item, int prefix_len, Item &x) {
+__device__ __forceinline__ bool item_of(const SeqTab &t, const ItemTab *order, int item, int prefix_len, Item &x) {
 	int tile;
-	if (order.n) {
-		const uint32_t v = order.item[item];
+	if (order && order->n) {
+		const uint32_t v = order->item[item];
 		x.sq = (int)(v >> 26);
 		tile = (int)((v >> 8) & 0x3FFFFu);
 		x.part = (int)(v & 0xFFu);
@@ -845,7 +845,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void prompt_kernel(AttnKv c, Se
 	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
 	const int kvh = blockIdx.x % c.kvh;
 	Item x;
-	if (!item_of<kKeys>(t, order, blockIdx.x / c.kvh, c.prefix_len, x)) return;
+	if (!item_of<kKeys>(t, &order, blockIdx.x / c.kvh, c.prefix_len, x)) return;
 	const int r = 32 * wave + (lane & 31), tok = r / G, head = kvh * G + r - tok * G;
 	const bool on = tok < x.ntok;
 	const int lim = on ? t.start[x.sq] + x.tok0 + tok + 1 : 0;
@@ -866,14 +866,14 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void prompt_kernel(AttnKv c, Se
 
 // The direct kernel's items: tiles of 32 rows, parts of `unit` steps of 32 keys.
 template <int HD, bool Q8>
-__global__ __launch_bounds__(64 * kWaves, 2) void prompt_direct_kernel(AttnKv c, SeqTab t, ItemTab order, float *out, int64_t ldo, const float *q,
+__global__ __launch_bounds__(64 * kWaves, 2) void prompt_direct_kernel(AttnKv c, SeqTab t, float *out, int64_t ldo, const float *q,
                                                                int64_t ldq, int G, float scale, float *__restrict__ rec_o,
                                                                float2 *__restrict__ rec_ml) {
 	__shared__ DirectLds<HD> s;
 	const int lane = threadIdx.x & 63;
 	const int kvh = blockIdx.x % c.kvh;
 	Item x;
-	if (!item_of<32>(t, order, blockIdx.x / c.kvh, c.prefix_len, x)) return;
+	if (!item_of<32>(t, nullptr, blockIdx.x / c.kvh, c.prefix_len, x)) return;
 	const int r = lane & 31, tok = r / G, head = kvh * G + r - tok * G;
 	const bool on = tok < x.ntok, whole = x.parts == 1;
 	const int64_t row = (int64_t)t.row[x.sq] + x.tok0 + tok;
@@ -1432,6 +1432,32 @@ int decode(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq
 	return HAKO_GPU_OK;
 }
 
+// A launch's items in order of their length, so that the last ones to start
+// are the shortest, where there are few enough for the table; their number,
+// or 0.
+template <int K>
+int sort_items(const SeqTab &t, int prefix_len, ItemTab &order) {
+	struct Len {
+		int steps;
+		uint32_t item;
+	} len[kItems];
+	int n = 0;
+	order.n = 0;
+	for (int s = 0; s < t.n; s++) {
+		const int tiles = (t.len[s] + t.tile_tokens - 1) / t.tile_tokens;
+		if (tiles > kItems || t.nsplit[s] > 256) return 0;
+		for (int i = tiles - 1; i >= 0; i--) {
+			const int nc = tile_steps<K>(t.start[s] + std::min((i + 1) * t.tile_tokens, t.len[s]), prefix_len);
+			const int parts = (nc + t.unit - 1) / t.unit, per = (nc + parts - 1) / parts;
+			if (n + parts > kItems) return 0;
+			for (int k = 0; k < parts; k++) len[n++] = {std::min(per, nc - k * per), (uint32_t)(s << 26 | i << 8 | k)};
+		}
+	}
+	std::sort(len, len + n, [](const Len &a, const Len &b) { return a.steps != b.steps ? a.steps > b.steps : a.item < b.item; });
+	for (int i = 0; i < n; i++) order.item[i] = len[i].item;
+	return order.n = n;
+}
+
 // One launch of up to kSeqs sequences, in the order given (the longest
 // first): tiles of `rows` query rows, steps of K keys, parts of `unit` steps.
 template <int HD, bool Q8, int K, class Launch>
@@ -1457,37 +1483,13 @@ int prompt_launch(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, int H, in
 		recs += (int64_t)(t.len[s] - first) * H * t.nsplit[s];
 	}
 	t.item[t.n] = (int)items;
-	// few items: in order of their length, so that the last ones to start are the shortest
-	ItemTab order;
-	order.n = 0;
-	struct Len {
-		int steps;
-		uint32_t item;
-	} len[kItems];
-	int n = 0;
-	for (int s = 0; s < t.n && n <= kItems; s++) {
-		const int tiles = (t.len[s] + t.tile_tokens - 1) / t.tile_tokens;
-		if (tiles > kItems || t.nsplit[s] > 256) n = kItems + 1;
-		for (int i = tiles - 1; i >= 0 && n <= kItems; i--) {
-			const int nc = tile_steps<K>(t.start[s] + std::min((i + 1) * t.tile_tokens, t.len[s]), c.prefix_len);
-			const int parts = (nc + t.unit - 1) / t.unit, per = (nc + parts - 1) / parts;
-			if (n + parts > kItems) n = kItems + 1;
-			for (int k = 0; k < parts && n <= kItems; k++) len[n++] = {std::min(per, nc - k * per), (uint32_t)(s << 26 | i << 8 | k)};
-		}
-	}
-	if (n <= kItems) {
-		std::sort(len, len + n, [](const Len &a, const Len &b) { return a.steps != b.steps ? a.steps > b.steps : a.item < b.item; });
-		for (int i = 0; i < n; i++) order.item[i] = len[i].item;
-		order.n = n;
-		items = n;
-	}
 	if (items * c.kvh > 0x7FFFFFFF || recs > 0xFFFFFFFFll || (int64_t)t.join[t.n] * H > 0x7FFFFFFF)
 		return set_error(HAKO_GPU_EINVAL, "%lld tiles and %lld records in one call", (long long)(items * c.kvh), (long long)recs);
 	float *ro = nullptr;
 	float2 *ml = nullptr;
 	if (recs)
 		if (int rc = records((size_t)recs, HD, &ro, &ml)) return rc;
-	launch(dim3((unsigned)(items * c.kvh)), order, ro, ml);
+	launch(items, ro, ml);
 	HK_LAUNCHED("attention");
 	if (recs) {
 		const int64_t blocks = ((int64_t)t.join[t.n] * H * (HD / 4) + 255) / 256;
@@ -1531,8 +1533,10 @@ int prompt(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, const float *q, 
 		const int64_t all = all_steps<kKeys>(c, t, 32 * kTileWaves / G);
 		return prompt_launch<HD, Q8, kKeys>(
 		    c, t, out, ldo, H, 32 * kTileWaves, std::max<int64_t>(4, (3 * all + 2 * cu - 1) / (2 * cu)),
-		    [&](dim3 grid, const ItemTab &order, float *ro, float2 *ml) {
-			    hipLaunchKernelGGL((prompt_kernel<HD, Q8>), grid, dim3(64 * kTileWaves), 0, stream(), c, t, order, out,
+		    [&](int64_t items, float *ro, float2 *ml) {
+			    ItemTab order;
+			    if (const int n = sort_items<kKeys>(t, c.prefix_len, order)) items = n;
+			    hipLaunchKernelGGL((prompt_kernel<HD, Q8>), dim3((unsigned)(items * c.kvh)), dim3(64 * kTileWaves), 0, stream(), c, t, order, out,
 			                       ldo, q, ldq, G, scale * kLog2e, ro, ml);
 		    });
 	}
@@ -1540,9 +1544,9 @@ int prompt(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, const float *q, 
 	for (int s = 0; s < t.n; s++) tiles += (t.len[s] + 32 / G - 1) / (32 / G);
 	const int64_t share = (steps + slots - 1) / slots;
 	return prompt_launch<HD, Q8, 32>(c, t, out, ldo, H, 32, std::max<int64_t>(4 * kWaves, 2 * tiles * c.kvh <= slots ? share : 2 * share),
-	                                 [&](dim3 grid, const ItemTab &order, float *ro, float2 *ml) {
-		                                 hipLaunchKernelGGL((prompt_direct_kernel<HD, Q8>), grid, dim3(64 * kWaves), 0, stream(), c, t,
-		                                                    order, out, ldo, q, ldq, G, scale * kLog2e, ro, ml);
+	                                 [&](int64_t items, float *ro, float2 *ml) {
+		                                 hipLaunchKernelGGL((prompt_direct_kernel<HD, Q8>), dim3((unsigned)(items * c.kvh)),
+		                                                    dim3(64 * kWaves), 0, stream(), c, t, out, ldo, q, ldq, G, scale * kLog2e, ro, ml);
 	                                 });
 }
 
