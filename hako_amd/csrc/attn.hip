@@ -554,31 +554,40 @@ struct Direct {
 	uint32_t v[16][VW];
 	float sc1;   // lanes 0..31: the keys' scales, 32..63: the values'
 
-	// dims of step s, lane half h, place j
-	static __device__ __forceinline__ int dim0(int s, int h) { return Q8 ? 32 * (s >> 1) + 16 * h + 8 * (s & 1) : 16 * s + 8 * h; }
-
-	__device__ __forceinline__ void query(const float *q, float scale, int lane) {
-		const int h = lane >> 5;
-		float x[KS * 8], a = 0.0f;
+	// The rows' queries, times scale log2(e): a thread converts HD/8 dims of row tid/8 (src), once for all waves, and the
+	// operands go through LDS (buf: HD * 128 bytes, es: 32 floats, both free again when this returns). Step s of the
+	// score product takes dims 16 s + 8 h.. (halves) or 32 (s>>1) + 16 h + 8 (s&1).. (8 bits, as a 16-byte load brings
+	// them) in lane half h.
+	__device__ __forceinline__ void query(const float *src, float scale, uint8_t *buf, float *es, int tid) {
+		constexpr int N = HD / 8;
+		const int t = tid & 7, row = tid >> 3, lane = tid & 63;
+		float x[N], a = 0.0f;
+#pragma unroll
+		for (int j = 0; j < N; j += 4) {
+			const float4 u = src ? *(const float4 *)(src + N * t + j) : make_float4(0, 0, 0, 0);
+			x[j] = u.x * scale, x[j + 1] = u.y * scale, x[j + 2] = u.z * scale, x[j + 3] = u.w * scale;
+		}
+#pragma unroll
+		for (int j = 0; j < N; j++) a = __builtin_fmaxf(a, __builtin_fabsf(x[j]));
+		const int e = row_exp(max8(a));
+		if (t == 0) es[row] = __builtin_ldexpf(1.0f, e);
+#pragma unroll
+		for (int j = 0; j < N / 8; j++) {
+			const int m = N / 8 * t + j;   // dims 8 m..
+			const int s = Q8 ? 2 * (m >> 2) + (m & 1) : m >> 1, h = Q8 ? (m >> 1) & 1 : m & 1;
+			h8 hi, lo;
+			split_q(x + 8 * j, e, hi, lo);
+			*(h8 *)(buf + 16 * (128 * s + 32 * h + row)) = hi;
+			*(h8 *)(buf + 16 * (128 * s + 64 + 32 * h + row)) = lo;
+		}
+		__syncthreads();
 #pragma unroll
 		for (int s = 0; s < KS; s++) {
-			float4 u = make_float4(0, 0, 0, 0), w = u;
-			if (q) {
-				u = *(const float4 *)(q + dim0(s, h));
-				w = *(const float4 *)(q + dim0(s, h) + 4);
-			}
-			const float y[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
-#pragma unroll
-			for (int j = 0; j < 8; j++) {
-				x[8 * s + j] = y[j] * scale;
-				a = __builtin_fmaxf(a, __builtin_fabsf(x[8 * s + j]));
-			}
+			qh[s] = *(const h8 *)(buf + 16 * (128 * s + lane));
+			ql[s] = *(const h8 *)(buf + 16 * (128 * s + 64 + lane));
 		}
-		a = __builtin_fmaxf(a, __shfl_xor(a, 32));
-		const int e = row_exp(a);
-		esc = __builtin_ldexpf(1.0f, e);
-#pragma unroll
-		for (int s = 0; s < KS; s++) split_q(x + 8 * s, e, qh[s], ql[s]);
+		esc = es[lane & 31];
+		__syncthreads();
 #pragma unroll
 		for (int d = 0; d < DT; d++)
 #pragma unroll
@@ -766,7 +775,13 @@ __device__ __forceinline__ void direct_rows(const AttnKv &c, DirectLds<HD> &s, i
 		load_v(ch);
 	}
 	__builtin_amdgcn_sched_barrier(0);
-	w.query(q, scale, lane);
+	// eight threads to a row, before the steps and after them (the row's pointers are in lane `row` of every wave)
+	const int row = tid >> 3;
+	auto from = [&](const void *p) {
+		const uint64_t x = (uint64_t)(uintptr_t)p;
+		return (uint64_t)(uint32_t)__shfl((int)(uint32_t)x, row) | ((uint64_t)(uint32_t)__shfl((int)(x >> 32), row) << 32);
+	};
+	w.query((const float *)(uintptr_t)from(q), scale, (uint8_t *)s.o, s.sx[0], tid);
 	const int lo = wave_min_i(q ? lim : 0x7FFFFFFF);
 	float *sx = s.sx[wave];
 	for (; ch < c1; ch += kWaves) {
@@ -799,15 +814,8 @@ __device__ __forceinline__ void direct_rows(const AttnKv &c, DirectLds<HD> &s, i
 		s.ml[wave][i][1] = w.l;
 	}
 	__syncthreads();
-	// eight threads to a row, every eighth quad of its dims each
-	const int row = tid >> 3;
-	// (the row's pointers are in lane `row` of every wave)
-	const uint64_t po = (uint64_t)(uintptr_t)out, pr = (uint64_t)(uintptr_t)rec_o, pm = (uint64_t)(uintptr_t)rec_ml;
-	auto from = [&](uint64_t x) {
-		return (uint64_t)(uint32_t)__shfl((int)(uint32_t)x, row) | ((uint64_t)(uint32_t)__shfl((int)(x >> 32), row) << 32);
-	};
-	float *dst = (float *)(uintptr_t)from(po), *ro = (float *)(uintptr_t)from(pr);
-	float2 *rm = (float2 *)(uintptr_t)from(pm);
+	float *dst = (float *)(uintptr_t)from(out), *ro = (float *)(uintptr_t)from(rec_o);
+	float2 *rm = (float2 *)(uintptr_t)from(rec_ml);
 	if (!dst && !ro) return;
 	float m = s.ml[0][row][0];
 #pragma unroll
