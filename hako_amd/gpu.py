@@ -122,8 +122,8 @@ def load_library() -> C.CDLL:
 
 
 def _ptr(a) -> int | None:
-    if a is None:
-        return None
+    if a is None or type(a) is int:
+        return a
     if isinstance(a, DevBuf):
         return a.ptr
     if isinstance(a, np.ndarray):
