@@ -910,9 +910,12 @@ struct Row16 {
 	f4 o[VD];
 	float M, l;
 	int E;
-	uint4 k[2][KL];
-	uint32_t v[8][VW];
-	float ks[8], vs[8];
+	// a step's codes and scales
+	struct Codes {
+		uint4 k[2][KL];
+		uint32_t v[8][VW];
+		float ks[8], vs[8];
+	};
 
 	// dims of step s, lane group g, place j: KL loads of 16 bytes at 16 g + 64 i
 	static __device__ __forceinline__ int dim0(int s, int g) {
@@ -950,47 +953,47 @@ struct Row16 {
 	}
 
 	// tile row i of key tile t is key 8 (i>>2) + 4 t + (i&3): a lane's eight scores are keys 8 g + 0..7
-	__device__ __forceinline__ void load_k(__amdgpu_buffer_rsrc_t kr, __amdgpu_buffer_rsrc_t ksr, int key0, int lane) {
+	static __device__ __forceinline__ void load_k(Codes &x, __amdgpu_buffer_rsrc_t kr, __amdgpu_buffer_rsrc_t ksr, int key0, int lane) {
 		const int i = lane & 15, g = lane >> 4;
 #pragma unroll
 		for (int t = 0; t < 2; t++) {
 			const uint32_t off = (uint32_t)(key0 + 8 * (i >> 2) + 4 * t + (i & 3)) * (HD * EB) + 16u * g;
 #pragma unroll
-			for (int n = 0; n < KL; n++) k[t][n] = ld_b128(kr, off + 64u * n);
+			for (int n = 0; n < KL; n++) x.k[t][n] = ld_b128(kr, off + 64u * n);
 		}
 #pragma unroll
 		for (int t = 0; t < 2; t++) {
-			const float4 x = __builtin_bit_cast(float4, ld_b128(ksr, 4u * (uint32_t)(key0 + 8 * g + 4 * t)));
-			ks[4 * t] = x.x, ks[4 * t + 1] = x.y, ks[4 * t + 2] = x.z, ks[4 * t + 3] = x.w;
+			const float4 y = __builtin_bit_cast(float4, ld_b128(ksr, 4u * (uint32_t)(key0 + 8 * g + 4 * t)));
+			x.ks[4 * t] = y.x, x.ks[4 * t + 1] = y.y, x.ks[4 * t + 2] = y.z, x.ks[4 * t + 3] = y.w;
 		}
 	}
-	__device__ __forceinline__ void load_v(__amdgpu_buffer_rsrc_t vr, __amdgpu_buffer_rsrc_t vsr, int key0, int lane) {
+	static __device__ __forceinline__ void load_v(Codes &x, __amdgpu_buffer_rsrc_t vr, __amdgpu_buffer_rsrc_t vsr, int key0, int lane) {
 		const int i = lane & 15, g = lane >> 4;
 #pragma unroll
 		for (int j = 0; j < 8; j++) {
 			const uint32_t off = ((uint32_t)(key0 + 8 * g + j) * HD + VD * i) * EB;
-			if (VW == 1) v[j][0] = __builtin_amdgcn_raw_buffer_load_b32(vr, (int)off, 0, 0);
+			if (VW == 1) x.v[j][0] = __builtin_amdgcn_raw_buffer_load_b32(vr, (int)off, 0, 0);
 			if (VW == 2) {
-				const uint2 x = ld_b64(vr, off);
-				v[j][0] = x.x;
-				v[j][VW - 1] = x.y;
+				const uint2 y = ld_b64(vr, off);
+				x.v[j][0] = y.x;
+				x.v[j][VW - 1] = y.y;
 			}
 			if (VW == 4) {
-				const uint4 x = ld_b128(vr, off);
-				v[j][0] = x.x;
-				v[j][1 % VW] = x.y;
-				v[j][2 % VW] = x.z;
-				v[j][VW - 1] = x.w;
+				const uint4 y = ld_b128(vr, off);
+				x.v[j][0] = y.x;
+				x.v[j][1 % VW] = y.y;
+				x.v[j][2 % VW] = y.z;
+				x.v[j][VW - 1] = y.w;
 			}
 		}
 #pragma unroll
 		for (int t = 0; t < 2; t++) {
-			const float4 x = __builtin_bit_cast(float4, ld_b128(vsr, 4u * (uint32_t)(key0 + 8 * g + 4 * t)));
-			vs[4 * t] = x.x, vs[4 * t + 1] = x.y, vs[4 * t + 2] = x.z, vs[4 * t + 3] = x.w;
+			const float4 y = __builtin_bit_cast(float4, ld_b128(vsr, 4u * (uint32_t)(key0 + 8 * g + 4 * t)));
+			x.vs[4 * t] = y.x, x.vs[4 * t + 1] = y.y, x.vs[4 * t + 2] = y.z, x.vs[4 * t + 3] = y.w;
 		}
 	}
 
-	__device__ __forceinline__ void scores(f4 sc[2]) {
+	__device__ __forceinline__ void scores(const Codes &c, f4 sc[2]) {
 #pragma unroll
 		for (int t = 0; t < 2; t++) {
 			sc[t] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
@@ -998,12 +1001,13 @@ struct Row16 {
 			for (int s = 0; s < KS; s++) {
 				h8 a;
 				if (Q8) {
-					const uint32_t w[4] = {k[t][s >> 1].x, k[t][s >> 1].y, k[t][s >> 1].z, k[t][s >> 1].w};
+					const uint4 &u4 = c.k[t][(s >> 1) % KL];
+					const uint32_t w[4] = {u4.x, u4.y, u4.z, u4.w};
 					const uint32_t x = w[2 * (s & 1)] ^ kFlip, y = w[2 * (s & 1) + 1] ^ kFlip;
 					const h2 p = bytes_h2(x, kLo2), q2 = bytes_h2(x, kHi2), r = bytes_h2(y, kLo2), u = bytes_h2(y, kHi2);
 					a = (h8){p.x, p.y, q2.x, q2.y, r.x, r.y, u.x, u.y};
 				} else {
-					a = __builtin_bit_cast(h8, k[t][s % KL]);
+					a = __builtin_bit_cast(h8, c.k[t][s % KL]);
 				}
 				sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[s], sc[t], 0, 0, 0);
 				sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[s], sc[t], 0, 0, 0);
@@ -1012,17 +1016,17 @@ struct Row16 {
 	}
 
 	// Weights of the 32 keys from key0, those at end and past it left out.
-	__device__ __forceinline__ void weigh(f4 sc[2], int key0, int end, int lane, h8 &ph, h8 &pl) {
+	__device__ __forceinline__ void weigh(Codes &cd, f4 sc[2], int key0, int end, int lane, h8 &ph, h8 &pl) {
 		const int g = lane >> 4;
 		float x[8], mx = -INFINITY, vm = 0.0f;
 #pragma unroll
 		for (int j = 0; j < 8; j++) {
 			// a value row that is not finite makes its score NaN
-			const bool fin = __builtin_isfinite(vs[j]);
-			x[j] = key0 + 8 * g + j < end ? (fin ? sc[j >> 2][j & 3] * ks[j] : __builtin_nanf("")) : -INFINITY;
-			vs[j] = fin ? vs[j] : 0.0f;
+			const bool fin = __builtin_isfinite(cd.vs[j]);
+			x[j] = key0 + 8 * g + j < end ? (fin ? sc[j >> 2][j & 3] * cd.ks[j] : __builtin_nanf("")) : -INFINITY;
+			cd.vs[j] = fin ? cd.vs[j] : 0.0f;
 			mx = __builtin_fmaxf(mx, x[j]);
-			vm = __builtin_fmaxf(vm, __builtin_fabsf(vs[j]));
+			vm = __builtin_fmaxf(vm, __builtin_fabsf(cd.vs[j]));
 		}
 		mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16));
 		vm = __builtin_fmaxf(vm, __shfl_xor(vm, 16));
@@ -1047,7 +1051,7 @@ struct Row16 {
 			for (int n = 0; n < 2; n++) {
 				const float p = exp2_(__builtin_fmaf(x[j + n], esc, c));
 				l += p;
-				w[n] = p * (vs[j + n] * vf);
+				w[n] = p * (cd.vs[j + n] * vf);
 			}
 			h2 a, b;
 			split2(w[0], w[1], a, b);
@@ -1057,13 +1061,13 @@ struct Row16 {
 	}
 
 	// tile row i of dim tile d is dim VD i + d
-	__device__ __forceinline__ void values(h8 ph, h8 pl) {
+	__device__ __forceinline__ void values(const Codes &c, h8 ph, h8 pl) {
 #pragma unroll
 		for (int d = 0; d < VD; d += 2) {
 			h2 t[2][4];
 #pragma unroll
 			for (int p = 0; p < 4; p++) {
-				const uint32_t a = v[2 * p][d * EB / 4], b = v[2 * p + 1][d * EB / 4];
+				const uint32_t a = c.v[2 * p][d * EB / 4], b = c.v[2 * p + 1][d * EB / 4];
 				if (Q8) {
 					const uint32_t m = __builtin_amdgcn_perm(b ^ kFlip, a ^ kFlip, d & 2 ? 0x07030602u : 0x05010400u);
 					t[0][p] = bytes_h2(m, kLo2);
@@ -1122,23 +1126,37 @@ __device__ __forceinline__ void decode_part(const AttnKv &c, DecodeLds<HD> &s, i
 	const __amdgpu_buffer_rsrc_t vr = stream_rsrc(uniform_ptr(c.v + r * HD * EB), rows * HD * EB);
 	const __amdgpu_buffer_rsrc_t ksr = stream_rsrc(uniform_ptr(c.ks + r), rows * 4);
 	const __amdgpu_buffer_rsrc_t vsr = stream_rsrc(uniform_ptr(c.vs + r), rows * 4);
+	// Codes on their way while others are used. 8 bits: two steps' in turn (64 sequences of 1000 positions 14.9 us, 16.6
+	// the other way). Halves, whose two steps would take 254 registers: the keys' of the next step once this one's
+	// weights are formed, the values' after their products (32768 and 20011 positions 18.0 us, 19.2 in turn). (Keys from
+	// `last` on read as zeros, from nowhere.)
+	typename Row16<HD, Q8>::Codes ca, cb;
 	int key0 = first + 32 * wave;
-	const bool any = key0 < last;   // (keys past the last read as zeros)
-	w.load_k(kr, ksr, any ? key0 : 0, lane);
-	w.load_v(vr, vsr, any ? key0 : 0, lane);
-	__builtin_amdgcn_sched_barrier(0);
+	auto load = [&](typename Row16<HD, Q8>::Codes &x, int key) {
+		w.load_k(x, kr, ksr, key, lane);
+		w.load_v(x, vr, vsr, key, lane);
+		__builtin_amdgcn_sched_barrier(0);
+	};
+	auto step = [&](typename Row16<HD, Q8>::Codes &x) {
+		f4 sc[2];
+		h8 ph, pl;
+		w.scores(x, sc);
+		w.weigh(x, sc, key0, last, lane, ph, pl);
+		key0 += 32 * kWaves;
+		if (!Q8) w.load_k(x, kr, ksr, key0, lane);
+		w.values(x, ph, pl);
+		if (!Q8) w.load_v(x, vr, vsr, key0, lane);
+		if (Q8) __builtin_amdgcn_sched_barrier(0);
+	};
+	load(ca, key0);
 	w.query(i < G ? q + sq * ldq + head * HD : nullptr, scale, lane);
-	if (any) {
-		for (; key0 < last; key0 += 32 * kWaves) {
-			f4 sc[2];
-			h8 ph, pl;
-			w.scores(sc);
-			w.weigh(sc, key0, last, lane, ph, pl);
-			const int next = key0 + 32 * kWaves;
-			if (next < last) w.load_k(kr, ksr, next, lane);
-			w.values(ph, pl);
-			if (next < last) w.load_v(vr, vsr, next, lane);
-		}
+	while (key0 < last) {
+		if (Q8) load(cb, key0 + 32 * kWaves);
+		step(ca);
+		if (!Q8) continue;
+		if (key0 >= last) break;
+		load(ca, key0 + 32 * kWaves);
+		step(cb);
 	}
 	w.l += __shfl_xor(w.l, 16);
 	w.l += __shfl_xor(w.l, 32);
