@@ -398,6 +398,86 @@ def test_prompt_many_sequences(gpu, prompt_kernel):
     c.free()
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hd,kvh,G,start,lens,prefix", [
+    (128, 4, 7, [0, 500], [4500, 700], 0),        # whole tiles and parts, in order of length
+    (64, 1, 16, [0], [8100], 0),                  # more items than the order's table holds
+    (128, 8, 4, [1000, 1000, 1000], [1500, 40, 900], 1000)])
+def test_prompt_long(gpu, prompt_kernel, kind, hd, kvh, G, start, lens, prefix):
+    """Long prompts, a sample of their tokens against float64: the first, the last, those at tile and chunk borders."""
+    if prompt_kernel == 1 and sum(lens) > 5000:
+        pytest.skip("the tiled kernel's range")
+    rng = np.random.default_rng(hd + G)
+    n_seq = len(lens)
+    c = ref.Cache(gpu, kind, n_seq + 1, max(a + m for a, m in zip(start, lens)), kvh, hd, rng)
+    q = rng.standard_normal((sum(lens), kvh * G, hd)).astype(np.float32)
+    got = run_prompt(gpu, c, q, None, start, lens, 1 / math.sqrt(hd), n_seq, prefix)
+    assert np.isfinite(got).all()
+    K, V = c.values()
+    row, at, want = 0, [], []
+    for s, (a, m) in enumerate(zip(start, lens)):
+        T = 256 // G
+        for i in {0, m - 1, m // 2, min(T, m) - 1, min(T, m - 1), max(0, m // T * T - 1), max(0, 64 - a - 1) % m, *rng.integers(0, m, 12)}:
+            at.append(row + int(i))
+            want.append(ref.attend(q[row + i], K, V, s, a + int(i) + 1, 1 / math.sqrt(hd), n_seq, prefix))
+        row += m
+    close(got[at], np.stack(want))
+    c.free()
+
+
+def test_decode_many_sequences(gpu):
+    """More sequences than CUs, one part each; with and without a prefix."""
+    rng = np.random.default_rng(50)
+    n = 300
+    c = ref.Cache(gpu, KV_Q8, 61, 260, 2, 64, rng)
+    slot, lens = [i % 60 for i in range(n)], [(i * 37) % 261 for i in range(n)]
+    q = rng.standard_normal((n, 6, 64)).astype(np.float32)
+    close(run_decode(gpu, c, q, slot, lens, 0.125), want_decode(c, q, slot, lens, 0.125))
+    close(run_decode(gpu, c, q, slot, lens, 0.125, 60, 111), want_decode(c, q, slot, lens, 0.125, 60, 111))
+    c.free()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_captured_prompt(gpu, prompt_kernel, kind):
+    """An append and a prompt in parts, captured: each replay equals the eager calls on the same rows."""
+    hd, kvh, H, n, at = 128, 2, 14, 90, 900
+    D, KV = H * hd, kvh * hd
+    ld = D + 2 * KV
+    rng = np.random.default_rng(60)
+    c = ref.Cache(gpu, kind, 2, 1000, kvh, hd, rng)
+    tab = ref.table(1000, hd)
+    bufs = [gpu.alloc(4 * n * ld), i32(gpu, [1] * n), i32(gpu, range(at, at + n)), gpu.alloc(4 * n * D), gpu.upload(tab)]
+    dx, ds, dp, dq, dt = bufs
+    host = [np.array([v], np.int32) for v in (1, at, n)]
+
+    def calls():
+        gpu.kv_append(c.kv, ds, dp, n, dx.offset(4 * D), dx.offset(4 * (D + KV)), ld, Rope(dt.ptr, 1000, hd, 1), dx, dq, H, ld, D)
+        gpu.attn_prompt(dq, D, dq, D, c.kv, *host, 1, H, 0.09)
+
+    gpu.h2d(dx, np.zeros((n, ld), np.float32))
+    calls()
+    gpu.capture_begin()
+    calls()
+    graph = gpu.capture_end()
+    for _ in range(3):
+        y = rng.standard_normal((n, ld)).astype(np.float32)
+        gpu.h2d(dx, y)
+        gpu.graph_launch(graph)
+        got = gpu.download(dq, np.float32, (n, H, hd))
+        calls()
+        np.testing.assert_array_equal(gpu.download(dq, np.float32, (n, H, hd)), got)
+        c.k[:], c.v[:], c.ks[:], c.vs[:] = c.pull()
+        pos = np.arange(at, at + n)
+        q = ref.rotate(y[:, :D].reshape(-1, H, hd), tab[pos], hd, 1)
+        rows = [0, 1, 45, n - 1]
+        K, V = c.values()
+        close(got[rows], np.stack([ref.attend(q[i], K, V, 1, at + i + 1, 0.09) for i in rows]))
+    gpu.graph_destroy(graph)
+    for b in bufs:
+        b.free()
+    c.free()
+
+
 def _dummy(gpu, c):
     return c.bufs[0], 128, c.bufs[1], 128
 
