@@ -39,9 +39,10 @@ constexpr int kWsAttn = 7;       // library workspace slot of the records
 constexpr int kKeys = 64;        // keys per chunk of the tiled kernel
 constexpr int kTileWaves = 8;    // its waves per workgroup, 32 rows each
 constexpr int kWaves = 4;        // waves per workgroup of the direct and the single-token kernel
-// M is a whole number not below the maximum it was taken from, so that what is
+// M is a whole number not below what it was taken from (the maximum of the
+// scores, in log2, plus the exponent of the value scales), so that what is
 // rescaled when it moves, and where sums meet, is so by exact powers of two;
-// it moves only when the maximum passes it by kSlack, which is rare.
+// it moves only when that passes it by kSlack, which is rare.
 constexpr float kNone = -FLT_MAX;   // M of a row that has seen no key
 constexpr float kUp = 6.0f;         // weights are 2^(u - M + 6): at most 2^14 while u <= M + kSlack
 constexpr float kSlack = 8.0f;
@@ -83,6 +84,9 @@ __device__ __forceinline__ int fresh(int v) {
 }
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+// The exponent m - to between two M, for ldexp: sums move by any power of two,
+// and to 0 from kNone.
+__device__ __forceinline__ int steps_down(float m, float to) { return (int)__builtin_fmaxf(m - to, -1000.0f); }
 
 // Four int8 codes as halves: byte + 128 under the exponent byte 0x64 is the
 // half 1024 + (code + 128).
@@ -112,8 +116,14 @@ __device__ __forceinline__ void split_q(const float *x, int e, h8 &hi, h8 &lo) {
 	}
 }
 
-// The exponent that value scales are divided by: that of their largest.
-__device__ __forceinline__ int scale_exp(float vmax) { return f16_split_exp(vmax); }
+// The exponent of the largest value scale of some keys. It goes into M, which
+// is not below any u_p + exponent of key p's step: weights times value scales
+// then fit a half whatever the scales are. Only scales that a row sees count
+// for it (those of a later token may be larger by any factor). Not below -88:
+// l, up to 2^(14 + 88) a key, stays finite.
+__device__ __forceinline__ float scale_exp(float vmax) {
+	return (float)max((int)(__builtin_bit_cast(uint32_t, vmax) >> 23) - 127, -88);
+}
 
 // ── tiled kernel: 256 query rows against chunks of 64 keys ──
 //
@@ -186,8 +196,8 @@ struct Stage {
 	}
 
 	// Converted into LDS: keys k_s [64][HD], values v_s [HD][64] halves, the
-	// scales; E follows the largest value scale (wave 0 keeps it).
-	__device__ __forceinline__ void store(uint8_t *k_s, uint8_t *v_s, float *ks_s, float *vs_s, int *e_s, int &E, int tid) {
+	// scales and the exponent of the largest value scale.
+	__device__ __forceinline__ void store(uint8_t *k_s, uint8_t *v_s, float *ks_s, float *vs_s, float *e_s, int tid) {
 #pragma unroll
 		for (int i = 0; i < KL; i++) {
 			const int u = tid + NT * i;
@@ -238,16 +248,17 @@ struct Stage {
 		if (tid < kKeys) {
 			// a value row that is not finite makes its scores NaN, which a row that may not see it masks
 			const bool fin = __builtin_isfinite(vs);
-			E = max(E, scale_exp(wave_max(fin ? __builtin_fabsf(vs) : 0.0f)));
+			vs = fin ? vs : 0.0f;
+			const float e = scale_exp(wave_max(__builtin_fabsf(vs)));
 			ks_s[tid] = fin ? ks : __builtin_nanf("");
-			vs_s[tid] = fin ? __builtin_ldexpf(vs, -E) : 0.0f;
-			if (tid == 0) *e_s = E;
+			vs_s[tid] = vs;
+			if (tid == 0) *e_s = e;
 		}
 	}
 };
 
 // One wave's 32 rows over the chunks of a part. lim: the lane's row sees keys
-// (positions) below it; out: O^T (value sums, times 2^E), M and l.
+// (positions) below it; out: O^T (value sums), M and l.
 template <int HD, bool Q8>
 struct Tile {
 	static constexpr int KS = HD / 16, DT = HD / 32;
@@ -257,13 +268,12 @@ struct Tile {
 		alignas(16) uint8_t v[2][kVB];
 		alignas(16) float ks[2][kKeys];
 		alignas(16) float vs[2][kKeys];
-		int e[2];
+		float e[2];
 	};
 	h8 qh[KS], ql[KS];
 	float esc;      // 2^e of the row
 	f16v o[DT];
 	float M, l;
-	int E;
 
 	// The lane's row q (null: an idle row), times scale log2(e).
 	__device__ __forceinline__ void query(const float *q, float scale, int lane) {
@@ -294,7 +304,6 @@ struct Tile {
 			for (int v = 0; v < 16; v++) o[d][v] = 0.0f;
 		M = kNone;
 		l = 0.0f;
-		E = -126;
 	}
 
 	// The 64 keys of the chunk in LDS buffer `b`, the first at position key0; mask: some row of the wave does not see
@@ -327,25 +336,37 @@ struct Tile {
 #pragma unroll
 				for (int j = 0; j < 4; j++) sc[t][4 * g + j] *= kv[j];
 			}
+		float e = s.e[b];
 		if (mask) {
 			const int n = lim - key0 - 8 * h;
+			float vm = 0.0f;
 #pragma unroll
 			for (int t = 0; t < 2; t++)
 #pragma unroll
-				for (int v = 0; v < 16; v++) sc[t][v] = 32 * t + 16 * (v >> 3) + (v & 7) < n ? sc[t][v] : -INFINITY;
+				for (int g = 0; g < 4; g++) {
+					const float4 vs = *(const float4 *)(s.vs[b] + 32 * t + 16 * (g >> 1) + 8 * h + 4 * (g & 1));
+					const float vv[4] = {vs.x, vs.y, vs.z, vs.w};
+#pragma unroll
+					for (int j = 0; j < 4; j++) {
+						const bool sees = 32 * t + 16 * (g >> 1) + 4 * (g & 1) + j < n;
+						sc[t][4 * g + j] = sees ? sc[t][4 * g + j] : -INFINITY;
+						vm = __builtin_fmaxf(vm, sees ? __builtin_fabsf(vv[j]) : 0.0f);
+					}
+				}
+			e = scale_exp(__builtin_fmaxf(vm, __shfl_xor(vm, 32)));
 		}
 #pragma unroll
 		for (int v = 0; v < 16; v++) mx = __builtin_fmaxf(__builtin_fmaxf(sc[0][v], sc[1][v]), mx);
-		mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32)) * esc;
+		mx = __builtin_fmaf(__builtin_fmaxf(mx, __shfl_xor(mx, 32)), esc, e);
 		if (__any(mx > M + kSlack)) {
 			const float mn = mx > M + kSlack ? __builtin_ceilf(mx) : M;
-			const float f = exp2_(M - mn);   // 0 from kNone
+			const int f = steps_down(M, mn);
 			M = mn;
-			l *= f;
+			l = __builtin_ldexpf(l, f);
 #pragma unroll
 			for (int d = 0; d < DT; d++)
 #pragma unroll
-				for (int v = 0; v < 16; v++) o[d][v] *= f;
+				for (int v = 0; v < 16; v++) o[d][v] = __builtin_ldexpf(o[d][v], f);
 		}
 		h8 ph[2][2], pl[2][2];
 		weigh(s, b, 0, sc[0], h, ph[0], pl[0]);
@@ -420,10 +441,9 @@ struct Tile {
 		};
 		// A wave's registers hold the codes two chunks on from the buffer that is read. The waves of a SIMD (w, w + 4)
 		// put them into LDS at opposite ends of a chunk, so that one has vector work while the other has matrix work.
-		int Es = -126;
 		if (c0 < c1) {
 			load(c0);
-			st.store(s.k[0], s.v[0], s.ks[0], s.vs[0], &s.e[0], Es, tid);
+			st.store(s.k[0], s.v[0], s.ks[0], s.vs[0], &s.e[0], tid);
 			if (c0 + 1 < c1) load(c0 + 1);
 		}
 		const bool early = __builtin_amdgcn_readfirstlane(tid >> 6) >= 4;
@@ -431,7 +451,7 @@ struct Tile {
 		for (int ch = c0; ch < c1; ch++) {
 			const int b = (ch - c0) & 1;
 			auto stage = [&] {
-				if (ch + 1 < c1) st.store(s.k[b ^ 1], s.v[b ^ 1], s.ks[b ^ 1], s.vs[b ^ 1], &s.e[b ^ 1], Es, fresh(tid));
+				if (ch + 1 < c1) st.store(s.k[b ^ 1], s.v[b ^ 1], s.ks[b ^ 1], s.vs[b ^ 1], &s.e[b ^ 1], fresh(tid));
 				if (ch + 2 < c1) load(ch + 2);
 				__builtin_amdgcn_sched_barrier(0);
 			};
@@ -440,15 +460,6 @@ struct Tile {
 			const int key0 = pre ? kKeys * ch : c.prefix_len + kKeys * (ch - nc1);
 			// rows see keys below min(lim, what the chunk holds)
 			const int top = pre ? pend : end;
-			const int e = s.e[b];
-			if (e != E) {
-				const float f = __builtin_ldexpf(1.0f, E - e);
-#pragma unroll
-				for (int d = 0; d < DT; d++)
-#pragma unroll
-					for (int v = 0; v < 16; v++) o[d][v] *= f;
-				E = e;
-			}
 			if (key0 < min(hi, top))   // some row of the wave sees some of these keys
 				chunk(s, b, key0, key0 + kKeys > min(lo, top), min(lim, top), lane);
 			if (!early) stage();
@@ -549,7 +560,6 @@ struct Direct {
 	float esc;
 	f16v o[DT];
 	float M, l;
-	int E;
 	uint4 k[KL];
 	uint32_t v[16][VW];
 	float sc1;   // lanes 0..31: the keys' scales, 32..63: the values'
@@ -594,7 +604,6 @@ struct Direct {
 			for (int v = 0; v < 16; v++) o[d][v] = 0.0f;
 		M = kNone;
 		l = 0.0f;
-		E = -126;
 	}
 
 	// Tile row i is the key of row i in key_row's order (an involution): register v of a lane's scores is key
@@ -646,22 +655,20 @@ struct Direct {
 		}
 	}
 
-	// The step's scales into the wave's own 64 floats of LDS, the values' divided by 2^E; 2^-(change of E).
+	// The step's scales into the wave's own 64 floats of LDS; the exponent of the values' largest.
 	__device__ __forceinline__ float scales(float *sx, int lane) {
 		const float other = __shfl_xor(sc1, 32);
 		const bool fin = __builtin_isfinite(lane < 32 ? other : sc1);   // the value row's scale
-		const int e = max(E, scale_exp(wave_max(lane >= 32 && fin ? __builtin_fabsf(sc1) : 0.0f)));
+		const float e = scale_exp(wave_max(lane >= 32 && fin ? __builtin_fabsf(sc1) : 0.0f));
 		// a value row that is not finite makes its score NaN
-		sx[lane] = lane < 32 ? (fin ? sc1 : __builtin_nanf("")) : (fin ? __builtin_ldexpf(sc1, -e) : 0.0f);
-		const float f = __builtin_ldexpf(1.0f, E - e);
-		E = e;
+		sx[lane] = fin ? sc1 : (lane < 32 ? __builtin_nanf("") : 0.0f);
 		__builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
 		__builtin_amdgcn_wave_barrier();
 		__builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-		return f;
+		return e;
 	}
 
-	__device__ __forceinline__ void weigh(f16v &sc, const float *sx, float fe, int key0, bool mask, int lim, int lane, h8 ph[2],
+	__device__ __forceinline__ void weigh(f16v &sc, const float *sx, float e, int key0, bool mask, int lim, int lane, h8 ph[2],
 	                                      h8 pl[2]) {
 		const int h = lane >> 5;
 		float mx = -INFINITY;
@@ -674,22 +681,32 @@ struct Direct {
 		}
 		if (mask) {
 			const int n = lim - key0 - 8 * h;
+			float vm = 0.0f;
 #pragma unroll
-			for (int v = 0; v < 16; v++) sc[v] = 16 * (v >> 3) + (v & 7) < n ? sc[v] : -INFINITY;
+			for (int g = 0; g < 4; g++) {
+				const float4 vs = *(const float4 *)(sx + 32 + 16 * (g >> 1) + 8 * h + 4 * (g & 1));
+				const float vv[4] = {vs.x, vs.y, vs.z, vs.w};
+#pragma unroll
+				for (int j = 0; j < 4; j++) {
+					const bool sees = 16 * (g >> 1) + 4 * (g & 1) + j < n;
+					sc[4 * g + j] = sees ? sc[4 * g + j] : -INFINITY;
+					vm = __builtin_fmaxf(vm, sees ? __builtin_fabsf(vv[j]) : 0.0f);
+				}
+			}
+			e = scale_exp(__builtin_fmaxf(vm, __shfl_xor(vm, 32)));
 		}
 #pragma unroll
 		for (int v = 0; v < 16; v++) mx = __builtin_fmaxf(mx, sc[v]);
-		mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32)) * esc;
-		if (__any(mx > M + kSlack || fe != 1.0f)) {
+		mx = __builtin_fmaf(__builtin_fmaxf(mx, __shfl_xor(mx, 32)), esc, e);
+		if (__any(mx > M + kSlack)) {
 			const float mn = mx > M + kSlack ? __builtin_ceilf(mx) : M;
-			const float f = exp2_(M - mn);   // 0 from kNone
+			const int f = steps_down(M, mn);
 			M = mn;
-			l *= f;
-			const float fo = f * fe;
+			l = __builtin_ldexpf(l, f);
 #pragma unroll
 			for (int d = 0; d < DT; d++)
 #pragma unroll
-				for (int v = 0; v < 16; v++) o[d][v] *= fo;
+				for (int v = 0; v < 16; v++) o[d][v] = __builtin_ldexpf(o[d][v], f);
 		}
 		const float c = kUp - M;
 #pragma unroll
@@ -789,10 +806,10 @@ __device__ __forceinline__ void direct_rows(const AttnKv &c, DirectLds<HD> &s, i
 		f16v sc;
 		h8 ph[2], pl[2];
 		w.scores(sc);
-		const float fe = w.scales(sx, lane);
+		const float e = w.scales(sx, lane);
 		if (ch + kWaves < c1) load_k(ch + kWaves);
 		__builtin_amdgcn_sched_barrier(0);
-		w.weigh(sc, sx, fe, key0, key0 + 32 > min(lo, top), min(lim, top), fresh(lane), ph, pl);
+		w.weigh(sc, sx, e, key0, key0 + 32 > min(lo, top), min(lim, top), fresh(lane), ph, pl);
 		w.values(ph, pl);
 		if (ch + kWaves < c1) load_v(ch + kWaves);
 		__builtin_amdgcn_sched_barrier(0);
@@ -800,14 +817,13 @@ __device__ __forceinline__ void direct_rows(const AttnKv &c, DirectLds<HD> &s, i
 	w.l += __shfl_xor(w.l, 32);
 	// the waves' sums meet: row i, dims DT (8 (v>>2) + 4 h + (v&3)) + d
 	const int i = lane & 31, h = lane >> 5;
-	const float f = __builtin_ldexpf(1.0f, w.E);
 #pragma unroll
 	for (int v = 0; v < 16; v++) {
 		float *at = &s.o[wave][i][w.DT * (8 * (v >> 2) + 4 * h + (v & 3))];
 		if (w.DT == 4)
-			*(float4 *)at = make_float4(w.o[0][v] * f, w.o[1][v] * f, w.o[2 % w.DT][v] * f, w.o[3 % w.DT][v] * f);
+			*(float4 *)at = make_float4(w.o[0][v], w.o[1][v], w.o[2 % w.DT][v], w.o[3 % w.DT][v]);
 		else
-			*(float2 *)at = make_float2(w.o[0][v] * f, w.o[1][v] * f);
+			*(float2 *)at = make_float2(w.o[0][v], w.o[1][v]);
 	}
 	if (h == 0) {
 		s.ml[wave][i][0] = w.M;
@@ -820,11 +836,12 @@ __device__ __forceinline__ void direct_rows(const AttnKv &c, DirectLds<HD> &s, i
 	float m = s.ml[0][row][0];
 #pragma unroll
 	for (int k = 1; k < kWaves; k++) m = __builtin_fmaxf(m, s.ml[k][row][0]);
-	float x[kWaves], ls = 0.0f;
+	int x[kWaves];
+	float ls = 0.0f;
 #pragma unroll
 	for (int k = 0; k < kWaves; k++) {
-		x[k] = exp2_(s.ml[k][row][0] - m);
-		ls = __builtin_fmaf(s.ml[k][row][1], x[k], ls);
+		x[k] = steps_down(s.ml[k][row][0], m);
+		ls += __builtin_ldexpf(s.ml[k][row][1], x[k]);
 	}
 	const float z = ro ? 1.0f : (ls == 0.0f ? 0.0f : 1.0f / ls);
 	float *to = ro ? ro : dst;
@@ -834,10 +851,10 @@ __device__ __forceinline__ void direct_rows(const AttnKv &c, DirectLds<HD> &s, i
 #pragma unroll
 		for (int k = 0; k < kWaves; k++) {
 			const float4 b = *(const float4 *)&s.o[k][row][d];
-			a.x = __builtin_fmaf(b.x, x[k], a.x);
-			a.y = __builtin_fmaf(b.y, x[k], a.y);
-			a.z = __builtin_fmaf(b.z, x[k], a.z);
-			a.w = __builtin_fmaf(b.w, x[k], a.w);
+			a.x += __builtin_ldexpf(b.x, x[k]);
+			a.y += __builtin_ldexpf(b.y, x[k]);
+			a.z += __builtin_ldexpf(b.z, x[k]);
+			a.w += __builtin_ldexpf(b.w, x[k]);
 		}
 		*(float4 *)(to + d) = make_float4(a.x * z, a.y * z, a.z * z, a.w * z);
 	}
@@ -864,11 +881,11 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void prompt_kernel(AttnKv c, Se
 	w.chunks(c, kvh, x.slot, x.end, x.c0, x.c1, lim, lo, hi, s, tid);
 	if (!on) return;
 	if (x.parts == 1) {
-		w.put(out + row * ldo + head * HD, __builtin_ldexpf(1.0f, w.E) / w.l, lane);
+		w.put(out + row * ldo + head * HD, 1.0f / w.l, lane);
 		return;
 	}
 	const size_t rec = record_of(t, x, tok, c.kvh * G, head);
-	w.put(rec_o + rec * HD, __builtin_ldexpf(1.0f, w.E), lane);
+	w.put(rec_o + rec * HD, 1.0f, lane);
 	if (lane < 32) rec_ml[rec] = make_float2(w.M, w.l);
 }
 
@@ -909,7 +926,6 @@ struct Row16 {
 	float esc;
 	f4 o[VD];
 	float M, l;
-	int E;
 	// a step's codes and scales
 	struct Codes {
 		uint4 k[2][KL];
@@ -949,7 +965,6 @@ struct Row16 {
 		for (int d = 0; d < VD; d++) o[d] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
 		M = kNone;
 		l = 0.0f;
-		E = -126;
 	}
 
 	// tile row i of key tile t is key 8 (i>>2) + 4 t + (i&3): a lane's eight scores are keys 8 g + 0..7
@@ -1030,20 +1045,19 @@ struct Row16 {
 		}
 		mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16));
 		vm = __builtin_fmaxf(vm, __shfl_xor(vm, 16));
-		mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32)) * esc;
 		vm = __builtin_fmaxf(vm, __shfl_xor(vm, 32));
-		const int e = max(E, scale_exp(vm));
-		if (__any(mx > M + kSlack || e != E)) {
+		mx = __builtin_fmaf(__builtin_fmaxf(mx, __shfl_xor(mx, 32)), esc, scale_exp(vm));
+		if (__any(mx > M + kSlack)) {
 			const float mn = mx > M + kSlack ? __builtin_ceilf(mx) : M;
-			const float f = exp2_(M - mn);
+			const int f = steps_down(M, mn);
 			M = mn;
-			l *= f;
-			const float fo = __builtin_ldexpf(f, E - e);
-			E = e;
+			l = __builtin_ldexpf(l, f);
 #pragma unroll
-			for (int d = 0; d < VD; d++) o[d] *= fo;
+			for (int d = 0; d < VD; d++)
+#pragma unroll
+				for (int v = 0; v < 4; v++) o[d][v] = __builtin_ldexpf(o[d][v], f);
 		}
-		const float c = kUp - M, vf = __builtin_ldexpf(1.0f, -E);
+		const float c = kUp - M;
 #pragma unroll
 		for (int j = 0; j < 8; j += 2) {
 			float w[2];
@@ -1051,7 +1065,7 @@ struct Row16 {
 			for (int n = 0; n < 2; n++) {
 				const float p = exp2_(__builtin_fmaf(x[j + n], esc, c));
 				l += p;
-				w[n] = p * (cd.vs[j + n] * vf);
+				w[n] = p * cd.vs[j + n];
 			}
 			h2 a, b;
 			split2(w[0], w[1], a, b);
@@ -1161,13 +1175,12 @@ __device__ __forceinline__ void decode_part(const AttnKv &c, DecodeLds<HD> &s, i
 	w.l += __shfl_xor(w.l, 16);
 	w.l += __shfl_xor(w.l, 32);
 	// the waves' sums meet: rows i, dims VD (4 g + v) + d
-	const float f = __builtin_ldexpf(1.0f, w.E);
 #pragma unroll
 	for (int v = 0; v < 4; v++)
 #pragma unroll
 		for (int d = 0; d < w.VD; d += 4)
 			*(float4 *)&s.o[wave][i][w.VD * (4 * g + v) + d] =
-			    make_float4(w.o[d][v] * f, w.o[d + 1][v] * f, w.o[d + 2][v] * f, w.o[d + 3][v] * f);
+			    make_float4(w.o[d][v], w.o[d + 1][v], w.o[d + 2][v], w.o[d + 3][v]);
 	if (g == 0) {
 		s.ml[wave][i][0] = w.M;
 		s.ml[wave][i][1] = w.l;
@@ -1182,13 +1195,13 @@ __device__ __forceinline__ void decode_part(const AttnKv &c, DecodeLds<HD> &s, i
 		float4 a = make_float4(0, 0, 0, 0);
 #pragma unroll
 		for (int k = 0; k < kWaves; k++) {
-			const float x = exp2_(s.ml[k][row][0] - m);
+			const int x = steps_down(s.ml[k][row][0], m);
 			const float4 b = *(const float4 *)&s.o[k][row][d];
-			ls = __builtin_fmaf(s.ml[k][row][1], x, ls);
-			a.x = __builtin_fmaf(b.x, x, a.x);
-			a.y = __builtin_fmaf(b.y, x, a.y);
-			a.z = __builtin_fmaf(b.z, x, a.z);
-			a.w = __builtin_fmaf(b.w, x, a.w);
+			ls += __builtin_ldexpf(s.ml[k][row][1], x);
+			a.x += __builtin_ldexpf(b.x, x);
+			a.y += __builtin_ldexpf(b.y, x);
+			a.z += __builtin_ldexpf(b.z, x);
+			a.w += __builtin_ldexpf(b.w, x);
 		}
 		const int hd = kvh * G + row;
 		if (nrec == 0) {
@@ -1276,19 +1289,19 @@ __device__ __forceinline__ void join(const float *__restrict__ ro, const float2 
 	__syncthreads();
 #pragma unroll
 	for (int k = 0; k < kJoin; k++) m = __builtin_fmaxf(m, m_s[k]);
-	const float f0 = exp2_(x0.x - m);
-	float ls = x0.y * f0;
-	float4 a = make_float4(b0.x * f0, b0.y * f0, b0.z * f0, b0.w * f0);
+	const int f0 = steps_down(x0.x, m);
+	float ls = __builtin_ldexpf(x0.y, f0);
+	float4 a = make_float4(__builtin_ldexpf(b0.x, f0), __builtin_ldexpf(b0.y, f0), __builtin_ldexpf(b0.z, f0), __builtin_ldexpf(b0.w, f0));
 #pragma unroll 4
 	for (int k = k0 + W; k < n; k += W) {
 		const float2 x = ml[k];
-		const float f = exp2_(x.x - m);
+		const int f = steps_down(x.x, m);
 		const float4 b = *(const float4 *)(ro + (size_t)k * HD + d);
-		ls = __builtin_fmaf(x.y, f, ls);
-		a.x = __builtin_fmaf(b.x, f, a.x);
-		a.y = __builtin_fmaf(b.y, f, a.y);
-		a.z = __builtin_fmaf(b.z, f, a.z);
-		a.w = __builtin_fmaf(b.w, f, a.w);
+		ls += __builtin_ldexpf(x.y, f);
+		a.x += __builtin_ldexpf(b.x, f);
+		a.y += __builtin_ldexpf(b.y, f);
+		a.z += __builtin_ldexpf(b.z, f);
+		a.w += __builtin_ldexpf(b.w, f);
 	}
 #pragma unroll
 	for (int k = L; k < 64; k <<= 1) {
@@ -1354,12 +1367,12 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(SeqTab t, int prefix_l
 	for (int k = 0; k < n; k++) {
 		const float4 b = *(const float4 *)(ro + (size_t)k * HD);
 		const float2 x = ml[k];
-		const float f = exp2_(x.x - m);
-		ls = __builtin_fmaf(x.y, f, ls);
-		a.x = __builtin_fmaf(b.x, f, a.x);
-		a.y = __builtin_fmaf(b.y, f, a.y);
-		a.z = __builtin_fmaf(b.z, f, a.z);
-		a.w = __builtin_fmaf(b.w, f, a.w);
+		const int f = steps_down(x.x, m);
+		ls += __builtin_ldexpf(x.y, f);
+		a.x += __builtin_ldexpf(b.x, f);
+		a.y += __builtin_ldexpf(b.y, f);
+		a.z += __builtin_ldexpf(b.z, f);
+		a.w += __builtin_ldexpf(b.w, f);
 	}
 	const float z = 1.0f / ls;
 	*(float4 *)(out + ((int64_t)t.row[sq] + tok) * ldo + (int64_t)h * HD + d) = make_float4(a.x * z, a.y * z, a.z * z, a.w * z);
@@ -1476,7 +1489,7 @@ int sort_items(const SeqTab &t, int prefix_len, ItemTab &order) {
 			const int nc = tile_steps<K>(t.start[s] + std::min((i + 1) * t.tile_tokens, t.len[s]), prefix_len);
 			const int parts = (nc + t.unit - 1) / t.unit, per = (nc + parts - 1) / parts;
 			if (n + parts > kItems) return 0;
-			for (int k = 0; k < parts; k++) len[n++] = {std::min(per, nc - k * per), (uint32_t)(s << 26 | i << 8 | k)};
+			for (int k = 0; k < parts; k++) len[n++] = {std::min(per, nc - k * per), (uint32_t)s << 26 | (uint32_t)(i << 8 | k)};
 		}
 	}
 	std::sort(len, len + n, [](const Len &a, const Len &b) { return a.steps != b.steps ? a.steps > b.steps : a.item < b.item; });

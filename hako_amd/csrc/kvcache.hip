@@ -91,7 +91,7 @@ __device__ __forceinline__ void put_row(const float v[8], int u0, int u1, uint8_
 		*(uint32_t *)(codes + 4 * u0) = w[0];
 		*(uint32_t *)(codes + 4 * u1) = w[1];
 	} else {
-		const int e = finite ? f16_split_exp(m < 0x00800000u ? 0.0f : __builtin_bit_cast(float, m)) : 0;
+		const int e = finite ? max((int)(m >> 23) - 127, -126) : 0;
 		sc = __builtin_ldexpf(1.0f, e);
 		uint2 w[2];
 #pragma unroll

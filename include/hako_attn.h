@@ -34,8 +34,8 @@ extern "C" {
  * HAKO_KV_Q8: int8 codes by the q8_32 rule of hako_gpu_quantize_q8_32 over
  *   the whole row: scale = max|x| * RN(1/127), code = x * RN(127 / max|x|)
  *   rounded half to even, subnormals taken as 0.
- * HAKO_KV_F16: scale = the power of two not above max|x| (1 for a row of
- *   zeros), code = the half nearest to x / scale: no row overflows.
+ * HAKO_KV_F16: scale = the power of two not above max|x| (2^-126 at least),
+ *   code = the half nearest to x / scale: no row overflows.
  *
  * A row that holds a NaN or an infinity gets codes 0 and the scale NaN: it
  * reads back as NaN throughout, and a query that sees it answers NaN. */

@@ -20,7 +20,7 @@ def rows(x, kind):
             inv = np.where(scale > 0, np.float32(127) / amax, np.float32(0)).astype(np.float32)
         c = np.clip(np.rint(np.where(a < FLT_MIN, np.float32(0), x) * inv[..., None]), -127, 127).astype(np.int8)
     else:
-        e = np.where(amax > 0, np.frexp(amax)[1] - 1, 0)
+        e = np.where(bad, 0, np.maximum(np.where(a.max(-1) > 0, np.frexp(a.max(-1))[1] - 1, -126), -126))
         scale = np.ldexp(np.float32(1), e).astype(np.float32)
         c = np.ldexp(x.astype(np.float64), -e[..., None]).astype(np.float16)
     return c, np.where(bad, np.float32(np.nan), scale).astype(np.float32)

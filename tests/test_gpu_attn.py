@@ -384,6 +384,58 @@ def test_prompt_masked_rows(gpu, prompt_kernel, kind):
     c.free()
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_prompt_later_rows_do_not_count(gpu, prompt_kernel, kind):
+    """A token's output does not depend on the rows after it by a bit, whatever their size."""
+    rng = np.random.default_rng(6)
+    c = ref.Cache(gpu, kind, 2, 200, 1, 128, rng)
+    start, lens, at = [0, 30], [100, 71], 60
+    q = rng.standard_normal((171, 4, 128)).astype(np.float32)
+    before = [i for i in range(171) if (i if i < 100 else i - 70) < at]
+    first = run_prompt(gpu, c, q, None, start, lens, 0.09)
+    close(first, want_prompt(c, q, None, start, lens, 0.09))
+    c.ks[:, :, at:] *= 2.0 ** 20
+    c.vs[:, :, at:] *= 2.0 ** 70
+    c.push()
+    got = run_prompt(gpu, c, q, None, start, lens, 0.09)
+    assert np.isfinite(got).all()
+    np.testing.assert_array_equal(got[before], first[before])
+    c.free()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_decode_prefix_rows_past_a_length_do_not_count(gpu, kind):
+    rng = np.random.default_rng(7)
+    c = ref.Cache(gpu, kind, 4, 400, 1, 128, rng)
+    lens, pl = [100, 77, 33], 300
+    q = rng.standard_normal((3, 4, 128)).astype(np.float32)
+    first = run_decode(gpu, c, q, None, lens, 0.09, 3, pl)
+    close(first, want_decode(c, q, None, lens, 0.09, 3, pl))
+    c.ks[3, :, 100:] *= 2.0 ** 20
+    c.vs[3, :, 100:] *= 2.0 ** 70
+    c.push()
+    np.testing.assert_array_equal(run_decode(gpu, c, q, None, lens, 0.09, 3, pl), first)
+    c.free()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("size", [2.0 ** 70, 2.0 ** -70])
+def test_values_of_any_size(gpu, prompt_kernel, kind, size):
+    """Large and small values, after rows of zeros and rows that are far smaller."""
+    rng = np.random.default_rng(17)
+    c = ref.Cache(gpu, kind, 1, 500, 2, 64, rng)
+    c.vs *= np.float32(size)
+    c.vs[:, :, :70] *= np.float32(2.0 ** -9)
+    c.v[:, :, :40], c.vs[:, :, :40] = 0, ref.rows(np.zeros(64, np.float32), kind)[1]
+    c.push()
+    q = rng.standard_normal((90, 6, 64)).astype(np.float32)
+    for start in (0, 45, 410):
+        close(run_prompt(gpu, c, q, None, [start], [90], 0.125), want_prompt(c, q, None, [start], [90], 0.125))
+    for n in (40, 60, 500):
+        close(run_decode(gpu, c, q[:1], None, [n], 0.125), want_decode(c, q[:1], None, [n], 0.125))
+    c.free()
+
+
 def test_prompt_many_sequences(gpu, prompt_kernel):
     """More sequences than one launch takes, most of them short or empty."""
     rng = np.random.default_rng(9)
