@@ -38,6 +38,7 @@ constexpr int kItems = 480;      // items of a launch whose order the host sets 
 constexpr int kWsAttn = 7;       // library workspace slot of the records
 constexpr int kKeys = 64;        // keys per chunk of the tiled kernel
 constexpr int kTileWaves = 8;    // its waves per workgroup, 32 rows each
+constexpr int kLongPart = 2048;  // keys of a part where sequences alone fill the chip
 constexpr int kWaves = 4;        // waves per workgroup of the direct and the single-token kernel
 // M is a whole number not below what it was taken from (the maximum of the
 // scores, in log2, plus the exponent of the value scales), so that what is
@@ -910,7 +911,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_direct_kernel(AttnKv c,
 
 // ── single tokens: the up to 16 query heads of a group over one sequence's own keys ──
 //
-// Workgroup (key/value head, part, sequence); each wave takes steps of 32
+// Workgroup (key/value head, sequence, part). Each wave takes steps of 32
 // keys, codes straight from memory into the matrix-core operands
 // (v_mfma_f32_16x16x32_f16: keys need no transposition, values are paired by
 // byte permutes), keys of the next step loaded while this one's weights form
@@ -1030,23 +1031,32 @@ struct Row16 {
 		}
 	}
 
-	// Weights of the 32 keys from key0, those at end and past it left out.
-	__device__ __forceinline__ void weigh(Codes &cd, f4 sc[2], int key0, int end, int lane, h8 &ph, h8 &pl) {
-		const int g = lane >> 4;
-		float x[8], mx = -INFINITY, vm = 0.0f;
+	// The exponent of the step's largest value scale. (Keys past the part read as zeros.) A value row that is not finite
+	// makes its score NaN, through its key's scale.
+	static __device__ __forceinline__ float exponent(Codes &cd) {
+		float vm = 0.0f;
 #pragma unroll
 		for (int j = 0; j < 8; j++) {
-			// a value row that is not finite makes its score NaN
 			const bool fin = __builtin_isfinite(cd.vs[j]);
-			x[j] = key0 + 8 * g + j < end ? (fin ? sc[j >> 2][j & 3] * cd.ks[j] : __builtin_nanf("")) : -INFINITY;
+			cd.ks[j] = fin ? cd.ks[j] : __builtin_nanf("");
 			cd.vs[j] = fin ? cd.vs[j] : 0.0f;
-			mx = __builtin_fmaxf(mx, x[j]);
 			vm = __builtin_fmaxf(vm, __builtin_fabsf(cd.vs[j]));
 		}
-		mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16));
 		vm = __builtin_fmaxf(vm, __shfl_xor(vm, 16));
-		vm = __builtin_fmaxf(vm, __shfl_xor(vm, 32));
-		mx = __builtin_fmaf(__builtin_fmaxf(mx, __shfl_xor(mx, 32)), esc, scale_exp(vm));
+		return scale_exp(__builtin_fmaxf(vm, __shfl_xor(vm, 32)));
+	}
+
+	// Weights of the 32 keys from key0, those at end and past it left out.
+	__device__ __forceinline__ void weigh(const Codes &cd, float e, f4 sc[2], int key0, int end, int lane, h8 &ph, h8 &pl) {
+		const int g = lane >> 4;
+		float x[8], mx = -INFINITY;
+#pragma unroll
+		for (int j = 0; j < 8; j++) {
+			x[j] = key0 + 8 * g + j < end ? sc[j >> 2][j & 3] * cd.ks[j] : -INFINITY;
+			mx = __builtin_fmaxf(mx, x[j]);
+		}
+		mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16));
+		mx = __builtin_fmaf(__builtin_fmaxf(mx, __shfl_xor(mx, 32)), esc, e);
 		if (__any(mx > M + kSlack)) {
 			const float mn = mx > M + kSlack ? __builtin_ceilf(mx) : M;
 			const int f = steps_down(M, mn);
@@ -1101,10 +1111,25 @@ struct Row16 {
 	}
 };
 
-// Keys per part of a sequence with n own keys in at most `parts` parts.
-__device__ __forceinline__ int part_keys(int n, int parts) {
-	const int per = (n + parts - 1) / parts;
+// Keys per part of a sequence with n own keys in at most `parts` parts of `least` keys or more.
+__device__ __forceinline__ int part_keys(int n, int parts, int least) {
+	const int per = max((n + parts - 1) / parts, least);
 	return (per + 32 * kWaves - 1) / (32 * kWaves) * (32 * kWaves);
+}
+// The part and sequence of workgroup b (of each key/value head). A sequence's
+// parts lie next to each other, on different CUs, while sequences are few.
+// Where they fill the chip most parts are empty: all first parts come first,
+// every next round shifted by one, so that the others go to all dies (64
+// sequences of 1000 positions, one of 32000: 38 us, 85 with a sequence's parts
+// together; but 8 of 1..8000 13.3 and 16.8).
+__device__ __forceinline__ void part_of(int b, int n_seq, int parts, int least, int &part, int &sq) {
+	if (least < kLongPart) {
+		part = b % parts;
+		sq = b / parts;
+	} else {
+		part = b / n_seq;
+		sq = (b + part) % n_seq;
+	}
 }
 // A sequence's own keys [prefix, end): end, 0 where it has no slot.
 __device__ __forceinline__ int own_end(const AttnKv &c, const int *slot, const int *len, int sq, int &sl) {
@@ -1121,15 +1146,16 @@ struct DecodeLds {
 template <int HD, bool Q8>
 __device__ __forceinline__ void decode_part(const AttnKv &c, DecodeLds<HD> &s, int kvh, int part, int sq, float *out, int64_t ldo,
                                             const float *q, int64_t ldq, const int *__restrict__ slot,
-                                            const int *__restrict__ len, int G, float scale, int parts, int rec0, int nrec,
+                                            const int *__restrict__ len, int G, float scale, int parts, int least, int rec0, int nrec,
                                             float *__restrict__ rec_o, float2 *__restrict__ rec_ml) {
 	constexpr int EB = Q8 ? 1 : 2;
 	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
 	int sl;
 	const int end = own_end(c, slot, len, sq, sl), n = max(end - c.prefix_len, 0);
-	const int per = part_keys(n, parts);
+	const int per = part_keys(n, parts, least);
 	const int first = c.prefix_len + part * per, last = min(end, first + per);   // this part's keys
-	if (first >= end && (part > 0 || nrec > 0)) return;   // a record that the merge does not read
+	if (first >= end && (part > 0 || nrec > 0)) return;   // a record that the join does not read
+	const bool whole = nrec == 0 || (rec0 == 0 && n <= per);   // (the join leaves it alone)
 	const int i = lane & 15, g = lane >> 4;
 	const int head = kvh * G + i;
 	// the first step's codes are on their way before the queries are asked for
@@ -1154,8 +1180,11 @@ __device__ __forceinline__ void decode_part(const AttnKv &c, DecodeLds<HD> &s, i
 	auto step = [&](typename Row16<HD, Q8>::Codes &x) {
 		f4 sc[2];
 		h8 ph, pl;
+		float e;
+		if (Q8) e = w.exponent(x);
 		w.scores(x, sc);
-		w.weigh(x, sc, key0, last, lane, ph, pl);
+		if (!Q8) e = w.exponent(x);
+		w.weigh(x, e, sc, key0, last, lane, ph, pl);
 		key0 += 32 * kWaves;
 		if (!Q8) w.load_k(x, kr, ksr, key0, lane);
 		w.values(x, ph, pl);
@@ -1204,7 +1233,7 @@ __device__ __forceinline__ void decode_part(const AttnKv &c, DecodeLds<HD> &s, i
 			a.w += __builtin_ldexpf(b.w, x);
 		}
 		const int hd = kvh * G + row;
-		if (nrec == 0) {
+		if (whole) {
 			const float z = ls == 0.0f ? 0.0f : 1.0f / ls;
 			*(float4 *)(out + sq * ldo + hd * HD + d) = make_float4(a.x * z, a.y * z, a.z * z, a.w * z);
 		} else {
@@ -1217,11 +1246,13 @@ __device__ __forceinline__ void decode_part(const AttnKv &c, DecodeLds<HD> &s, i
 
 template <int HD, bool Q8>
 __global__ __launch_bounds__(256) void decode_kernel(AttnKv c, float *out, int64_t ldo, const float *q, int64_t ldq,
-                                                     const int *__restrict__ slot, const int *__restrict__ len, int G,
-                                                     float scale, int parts, int nrec, float *__restrict__ rec_o,
+                                                     const int *__restrict__ slot, const int *__restrict__ len, int n_seq, int G,
+                                                     float scale, int parts, int least, int nrec, float *__restrict__ rec_o,
                                                      float2 *__restrict__ rec_ml) {
 	__shared__ DecodeLds<HD> s;
-	decode_part<HD, Q8>(c, s, blockIdx.x, blockIdx.y, blockIdx.z, out, ldo, q, ldq, slot, len, G, scale, parts, 0, nrec, rec_o,
+	int part, sq;
+	part_of(blockIdx.x / c.kvh, n_seq, parts, least, part, sq);
+	decode_part<HD, Q8>(c, s, blockIdx.x % c.kvh, part, sq, out, ldo, q, ldq, slot, len, G, scale, parts, least, 0, nrec, rec_o,
 	                    rec_ml);
 }
 
@@ -1232,7 +1263,7 @@ __global__ __launch_bounds__(256) void decode_kernel(AttnKv c, float *out, int64
 template <int HD, bool Q8>
 __global__ __launch_bounds__(64 * kWaves, 2) void prefix_kernel(AttnKv c, const float *q, int64_t ldq, const int *__restrict__ slot,
                                                         const int *__restrict__ len, int n_seq, int G, float scale,
-                                                        int tiles, int pparts, int unit, int parts, int nrec,
+                                                        int tiles, int pparts, int unit, int parts, int least, int nrec,
                                                         float *__restrict__ rec_o, float2 *__restrict__ rec_ml) {
 	__shared__ union Lds {
 		DirectLds<HD> a;
@@ -1243,7 +1274,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefix_kernel(AttnKv c, const 
 	int b = blockIdx.x / c.kvh;
 	if (b >= tiles * pparts) {
 		b -= tiles * pparts;
-		decode_part<HD, Q8>(c, s.b, kvh, b % parts, b / parts, nullptr, 0, q, ldq, slot, len, G, scale, parts, pparts, nrec, rec_o,
+		int own, sq;
+		part_of(b, n_seq, parts, least, own, sq);
+		decode_part<HD, Q8>(c, s.b, kvh, own, sq, nullptr, 0, q, ldq, slot, len, G, scale, parts, least, pparts, nrec, rec_o,
 		                    rec_ml);
 		return;
 	}
@@ -1329,13 +1362,14 @@ __device__ __forceinline__ void join(const float *__restrict__ ro, const float2 
 
 template <int HD>
 __global__ __launch_bounds__(64 * kJoin) void decode_join_kernel(AttnKv c, float *out, int64_t ldo, const int *__restrict__ slot,
-                                                         const int *__restrict__ len, int H, int parts, int rec0,
+                                                         const int *__restrict__ len, int H, int parts, int least, int rec0,
                                                          int nrec, const float *__restrict__ rec_o,
                                                          const float2 *__restrict__ rec_ml) {
 	const int h = blockIdx.x, sq = blockIdx.y;
 	int sl;
 	const int end = own_end(c, slot, len, sq, sl), n = max(end - c.prefix_len, 0);
-	const int per = part_keys(n, parts), used = n > 0 ? (n + per - 1) / per : 0;
+	const int per = part_keys(n, parts, least), used = n > 0 ? (n + per - 1) / per : 0;
+	if (rec0 == 0 && used == 1) return;   // written at once
 	const size_t rec = ((size_t)sq * H + h) * nrec;
 	join<HD>(rec_o + rec * HD, rec_ml + rec, rec0 + used, out + sq * ldo + h * HD);
 }
@@ -1411,24 +1445,26 @@ int records(size_t n, int HD, float **o, float2 **ml) {
 	return HAKO_GPU_OK;
 }
 
-// How the single tokens of a batch are shared out: own keys in `parts` parts,
-// the prefix (tiles of 32 rows) in pparts parts of `unit` steps, nrec records
-// to a query head (0: written at once).
+// How the single tokens of a batch are shared out: own keys in up to `parts`
+// parts of `least` keys or more, the prefix (tiles of 32 rows) in pparts parts
+// of `unit` steps, nrec records to a query head (0: written at once).
 struct DecodePlan {
 	int64_t tiles;
-	int parts, pparts, unit, nrec;
+	int parts, least, pparts, unit, nrec;
 };
 DecodePlan decode_plan(int max_seq, int prefix_len, int kvh, int n_seq, int H) {
 	DecodePlan p{};
 	const int own = max_seq - prefix_len;
 	const int slots = 2 * cu_count();   // workgroups that run at once
-	// own keys: parts of at least 32 keys a wave, until the workgroups fill the chip (one part from a workgroup per CU on:
-	// 64 sequences of 1000 positions, 256 pairs, 16.5 us against 19.1 with two parts and their join; 16 of 4096, 64 pairs:
-	// 18.4 us with 8 parts, 20.0 with 4, 23.5 with 12)
-	p.parts = (own + 32 * kWaves - 1) / (32 * kWaves);
+	// own keys: parts of 32 keys a wave or more, until the workgroups fill the chip (16 sequences of 4096, 64 pairs of
+	// sequence and head: 18.4 us with 8 parts, 20.0 with 4, 23.5 with 12). From a pair per CU on only long sequences are
+	// split, for one among short ones (64 sequences, 256 pairs: one of 8000 and 63 of 100..400 positions 27 us, 62 in one
+	// part; all of 4096 56 us, 50 in one part)
 	const int64_t pairs = (int64_t)n_seq * kvh;
-	const int fill = pairs >= cu_count() ? 1 : (int)((slots + pairs - 1) / pairs);
-	p.parts = std::max(1, std::min(p.parts, fill));
+	p.least = pairs >= cu_count() ? kLongPart : 32 * kWaves;
+	p.parts = (own + p.least - 1) / p.least;
+	if (pairs < cu_count()) p.parts = std::min(p.parts, (int)((slots + pairs - 1) / pairs));
+	p.parts = std::max(1, p.parts);
 	// the prefix: parts of at least a step for each wave, until its tiles fill the chip
 	p.tiles = ((int64_t)n_seq * (H / kvh) + 31) / 32;
 	const int nc = (prefix_len + 31) / 32;
@@ -1447,24 +1483,24 @@ int decode(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq
            int n_seq, int H, float scale) {
 	const int G = H / c.kvh;
 	const DecodePlan p = decode_plan(c.max_seq, c.prefix_len, c.kvh, n_seq, H);
-	const int parts = p.parts, pparts = p.pparts, unit = p.unit, nrec = p.nrec;
+	const int parts = p.parts, least = p.least, pparts = p.pparts, unit = p.unit, nrec = p.nrec;
 	const int64_t tiles = p.tiles;
 	float *ro = nullptr;
 	float2 *ml = nullptr;
 	if (nrec)
 		if (int rc = records((size_t)n_seq * H * nrec, HD, &ro, &ml)) return rc;
+	const int64_t blocks = (tiles * pparts + (int64_t)n_seq * parts) * c.kvh;
+	if (blocks > kMaxThreads / (64 * kWaves)) return set_error(HAKO_GPU_EINVAL, "%lld workgroups in one call", (long long)blocks);
 	if (pparts) {
-		const int64_t blocks = (tiles * pparts + (int64_t)n_seq * parts) * c.kvh;
-		if (blocks > 0x7FFFFFFF) return set_error(HAKO_GPU_EINVAL, "%lld workgroups in one call", (long long)blocks);
 		hipLaunchKernelGGL((prefix_kernel<HD, Q8>), dim3((unsigned)blocks), dim3(64 * kWaves), 0, stream(), c, q, ldq, slot, len,
-		                   n_seq, G, scale * kLog2e, (int)tiles, pparts, unit, parts, nrec, ro, ml);
+		                   n_seq, G, scale * kLog2e, (int)tiles, pparts, unit, parts, least, nrec, ro, ml);
 	} else {
-		hipLaunchKernelGGL((decode_kernel<HD, Q8>), dim3(c.kvh, parts, n_seq), dim3(256), 0, stream(), c, out, ldo, q, ldq, slot,
-		                   len, G, scale * kLog2e, parts, nrec, ro, ml);
+		hipLaunchKernelGGL((decode_kernel<HD, Q8>), dim3((unsigned)blocks), dim3(256), 0, stream(), c, out, ldo, q, ldq, slot,
+		                   len, n_seq, G, scale * kLog2e, parts, least, nrec, ro, ml);
 	}
 	HK_LAUNCHED("attention");
 	if (nrec) {
-		hipLaunchKernelGGL(decode_join_kernel<HD>, dim3(H, n_seq), dim3(64 * kJoin), 0, stream(), c, out, ldo, slot, len, H, parts,
+		hipLaunchKernelGGL(decode_join_kernel<HD>, dim3(H, n_seq), dim3(64 * kJoin), 0, stream(), c, out, ldo, slot, len, H, parts, least,
 		                   pparts, nrec, ro, ml);
 		HK_LAUNCHED("attention join");
 	}
@@ -1522,7 +1558,7 @@ int prompt_launch(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, int H, in
 		recs += (int64_t)(t.len[s] - first) * H * t.nsplit[s];
 	}
 	t.item[t.n] = (int)items;
-	if (items * c.kvh > 0x7FFFFFFF || recs > 0xFFFFFFFFll || (int64_t)t.join[t.n] * H > 0x7FFFFFFF)
+	if (items * c.kvh > kMaxThreads / (64 * kTileWaves) || recs > 0xFFFFFFFFll || (int64_t)t.join[t.n] * H * (HD / 4) > kMaxThreads)
 		return set_error(HAKO_GPU_EINVAL, "%lld tiles and %lld records in one call", (long long)(items * c.kvh), (long long)recs);
 	float *ro = nullptr;
 	float2 *ml = nullptr;

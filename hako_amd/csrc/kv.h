@@ -6,6 +6,8 @@
 
 namespace hako {
 
+// Threads of a launch's grid that HIP takes.
+constexpr int64_t kMaxThreads = 0xFFFFFFFFll;
 // Bytes of a code.
 inline int kv_elt(int type) { return type == HAKO_KV_Q8 ? 1 : 2; }
 // The checks every call makes of its cache; 0 or an error code.

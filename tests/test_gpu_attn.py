@@ -490,6 +490,22 @@ def test_decode_many_sequences(gpu):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+def test_decode_long_ones_among_many(gpu, kind):
+    """Sequences enough for every CU: the long ones in parts, the short ones written at once, in place too."""
+    rng = np.random.default_rng(51)
+    n = 260
+    c = ref.Cache(gpu, kind, 5, 4200, 1, 64, rng)
+    slot = [i % 5 for i in range(n)]
+    lens = [{3: 4200, 50: 2048, 51: 2049, 100: 0, 101: 4097}.get(i, 1 + (i * 53) % 300) for i in range(n)]
+    q = rng.standard_normal((n, 3, 64)).astype(np.float32)
+    want = want_decode(c, q, slot, lens, 0.125)
+    close(run_decode(gpu, c, q, slot, lens, 0.125), want)
+    close(run_decode(gpu, c, q, slot, lens, 0.125, in_place=True), want)
+    close(run_decode(gpu, c, q, slot, lens, 0.125, 4, 90), want_decode(c, q, slot, lens, 0.125, 4, 90))
+    c.free()
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_captured_prompt(gpu, prompt_kernel, kind):
     """An append and a prompt in parts, captured: each replay equals the eager calls on the same rows."""
     hd, kvh, H, n, at = 128, 2, 14, 90, 900
