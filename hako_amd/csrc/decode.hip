@@ -23,6 +23,8 @@
 #include <math.h>
 #include <string.h>
 
+#include <memory>
+#include <new>
 #include <vector>
 
 #include "../../include/hako_decode.h"
@@ -2187,10 +2189,12 @@ int prefill_chunk(hako_gpu_decoder *d, int seq, const int *tokens, int n, int po
 	for (int i = 0; i < n; i++) posv[i] = pos0 + i;
 	HK_HIP(hipMemcpyAsync(d->pf_tok, tokens, sizeof(int) * n, hipMemcpyHostToDevice, stream()));
 	HK_HIP(hipMemcpyAsync(d->pf_pos, posv.data(), sizeof(int) * n, hipMemcpyHostToDevice, stream()));
-	std::vector<int> slotv;
+	std::unique_ptr<int[]> slotv;
 	if (d->kv_type) {
-		slotv.assign(n, seq);
-		HK_HIP(hipMemcpyAsync(d->pf_slot, slotv.data(), sizeof(int) * n, hipMemcpyHostToDevice, stream()));
+		slotv.reset(new (std::nothrow) int[n]);
+		if (!slotv) return set_error(HAKO_GPU_ENOMEM, "host memory for %d tokens", n);
+		for (int i = 0; i < n; i++) slotv[i] = seq;
+		HK_HIP(hipMemcpyAsync(d->pf_slot, slotv.get(), sizeof(int) * n, hipMemcpyHostToDevice, stream()));
 	}
 	HK_HIP(hipStreamSynchronize(stream()));   // posv and slotv are this frame's
 	hipLaunchKernelGGL(embed_kernel, dim3(n), dim3(256), 0, stream(), (const uint8_t *)m.tok_embd, m.t_embd,
@@ -2319,6 +2323,11 @@ int typed_caches(hako_gpu_decoder *d) {
 	hako_gpu_kv kv{d->kv_type, d->n_seq, d->max_seq, m.n_kv_heads, m.head_dim, nullptr, nullptr, nullptr, nullptr};
 	size_t codes, scales;
 	if (int rc = hako_gpu_kv_bytes(&kv, &codes, &scales)) return rc;
+	try {
+		d->kv.reserve(m.n_layers);
+	} catch (const std::bad_alloc &) {
+		return set_error(HAKO_GPU_ENOMEM, "host memory for %d layers", m.n_layers);
+	}
 	uint8_t *p[4];
 	for (int i = 0; i < 4; i++) {
 		const size_t bytes = (size_t)m.n_layers * (i < 2 ? codes : scales);

@@ -4,7 +4,8 @@
 
 namespace hako {
 
-int kv_check(const hako_gpu_kv *kv) {
+// A cache's type and shape; 0 or an error code.
+static int kv_shape_check(const hako_gpu_kv *kv) {
 	if (!kv) return set_error(HAKO_GPU_EINVAL, "null cache");
 	if (kv->type != HAKO_KV_F16 && kv->type != HAKO_KV_Q8)
 		return set_error(HAKO_GPU_ETYPE, "cache type %d", kv->type);
@@ -16,6 +17,14 @@ int kv_check(const hako_gpu_kv *kv) {
 	if ((size_t)kv->max_seq * kv->head_dim * kv_elt(kv->type) >= kBufNone)
 		return set_error(HAKO_GPU_EINVAL, "max_seq %d x head_dim %d: one head's rows exceed 2 GiB", kv->max_seq,
 		                 kv->head_dim);
+	// (rows of one head fit 25 bits, heads 16)
+	if (((size_t)kv->max_seq * kv->n_kv_heads * kv->n_slots) >> 48)
+		return set_error(HAKO_GPU_EINVAL, "%d slots of %d positions of %d heads", kv->n_slots, kv->max_seq, kv->n_kv_heads);
+	return HAKO_GPU_OK;
+}
+
+int kv_check(const hako_gpu_kv *kv) {
+	if (int rc = kv_shape_check(kv)) return rc;
 	if (!kv->k || !kv->v || !kv->k_scale || !kv->v_scale) return set_error(HAKO_GPU_EINVAL, "null cache array");
 	if ((((uintptr_t)kv->k | (uintptr_t)kv->v) & 15) || (((uintptr_t)kv->k_scale | (uintptr_t)kv->v_scale) & 3))
 		return set_error(HAKO_GPU_EINVAL, "cache arrays need 16-byte (codes) and 4-byte (scales) alignment");
@@ -223,7 +232,7 @@ int tokens_check(const hako_gpu_kv *kv, const int *slot, const int *pos, int n_t
 // workgroups for `rows` head rows, `each` of them to one
 int row_blocks(int64_t rows, int each, dim3 *grid) {
 	const int64_t n = (rows + each - 1) / each;
-	if (rows > 0x7FFFFFFF) return set_error(HAKO_GPU_EINVAL, "%lld head rows in one call", (long long)rows);
+	if (n > kMaxThreads / 256) return set_error(HAKO_GPU_EINVAL, "%lld head rows in one call", (long long)rows);
 	*grid = dim3((unsigned)n);
 	return HAKO_GPU_OK;
 }
@@ -236,12 +245,8 @@ using namespace hako;
 extern "C" {
 
 int hako_gpu_kv_bytes(const hako_gpu_kv *kv, size_t *codes, size_t *scales) {
-	if (!kv || !codes || !scales) return set_error(HAKO_GPU_EINVAL, "null argument");
-	if (kv->type != HAKO_KV_F16 && kv->type != HAKO_KV_Q8)
-		return set_error(HAKO_GPU_ETYPE, "cache type %d", kv->type);
-	if (kv->n_slots < 1 || kv->max_seq < 1 || kv->n_kv_heads < 1 || (kv->head_dim != 64 && kv->head_dim != 128))
-		return set_error(HAKO_GPU_EINVAL, "unsupported cache shape: %d slots of %d positions, %d heads of %d",
-		                 kv->n_slots, kv->max_seq, kv->n_kv_heads, kv->head_dim);
+	if (!codes || !scales) return set_error(HAKO_GPU_EINVAL, "null argument");
+	if (int rc = kv_shape_check(kv)) return rc;
 	const size_t rows = (size_t)kv->n_slots * kv->n_kv_heads * kv->max_seq;
 	*codes = rows * kv->head_dim * kv_elt(kv->type);
 	*scales = rows * sizeof(float);

@@ -106,6 +106,12 @@ int hako_gpu_kv_read(const hako_gpu_kv *kv, const int *slot, const int *pos, int
  * slot prefix_slot for every sequence, the others its own slot's, so the
  * prefix is stored once and, for single tokens, read once for the batch.
  *
+ * Values that a token does not see have no part in its output, whatever they
+ * are; among those it sees, a contribution below 2^-24 of the largest value
+ * row times the largest weight may round away. Keys and values of magnitudes
+ * from 2^-80 to 2^80 are meant: outside, scores may overflow and small weights
+ * and values be lost.
+ *
  * The sums' order follows the shapes, not the timing: a call repeats itself
  * bit for bit. */
 

@@ -57,7 +57,7 @@ def prompt(lib, c=None, out=P, ldo=512, q=P, ldq=512, slot=(0, 1), start=(0, 3),
                                     *(None if x is None else x.ctypes.data for x in a), n, H, scale, ps, pl)
 
 
-BAD_KV = [dict(type=0), dict(type=3), dict(n_slots=0), dict(max_seq=0), dict(n_kv_heads=0), dict(n_kv_heads=65536),
+BAD_KV = [dict(n_slots=2 ** 31 - 1, n_kv_heads=65535, max_seq=2 ** 20), dict(type=0), dict(type=3), dict(n_slots=0), dict(max_seq=0), dict(n_kv_heads=0), dict(n_kv_heads=65536),
           dict(head_dim=96), dict(head_dim=0), dict(max_seq=1 << 24), dict(type=KV_F16, max_seq=1 << 23), dict(k=None),
           dict(v=None), dict(k_scale=None), dict(v_scale=None), dict(k=P + 8), dict(v=P + 4), dict(k_scale=P + 2),
           dict(v_scale=P + 1)]
