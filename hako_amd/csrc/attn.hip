@@ -67,10 +67,10 @@ struct AttnKv {
 // A prompt launch: sequence s has len[s] tokens from row row[s] of q and
 // out, at positions start[s].. of slot[s]; items item[s].. of the grid are
 // its tiles, the last tile first, each in nsplit[s] parts of its keys. The
-// tiles of more than `unit` chunks, whose parts are joined, hold the last
+// tiles of more than `unit` steps, whose parts are joined, hold the last
 // join[s + 1] - join[s] tokens.
 struct SeqTab {
-	int n, tile_tokens, unit;   // tokens per tile, chunks per part
+	int n, tile_tokens, unit;   // tokens per tile, steps per part
 	int row[kSeqs], len[kSeqs], slot[kSeqs], start[kSeqs], item[kSeqs + 1], nsplit[kSeqs];
 	int join[kSeqs + 1];
 	uint32_t rec[kSeqs];        // first record of a sequence's split tokens
@@ -551,6 +551,14 @@ __device__ __forceinline__ size_t record_of(const SeqTab &t, const Item &x, int 
 // converts every chunk once per 32 rows where the tiled kernel does once per
 // 256, and needs neither barriers nor long runs of keys: a call too small to
 // give every CU several of those tiles ends sooner with it.
+//
+// Bound: vector work. A step is 32 matrix operations of 16 passes and about
+// 390 vector ones, 176 of them codes to halves; with 2000 tokens of 7B heads
+// the vector pipes are busy 68% of the cycles, the matrix pipes 30% (that call
+// is the tiled kernel's for this reason: 98 and 86 us). Small calls: 77 tokens
+// of 3B heads 7.6 us, 512 of 7B heads 14.4, 16 x 77 22, 64 tokens at position
+// 8000 33.7. On the way: every wave converting all 32 queries for itself cost
+// 512 tokens 1.8 us more (a thread now converts an eighth of a row, once).
 template <int HD, bool Q8>
 struct Direct {
 	static constexpr int EB = Q8 ? 1 : 2;
@@ -914,8 +922,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_direct_kernel(AttnKv c,
 // Workgroup (key/value head, sequence, part). Each wave takes steps of 32
 // keys, codes straight from memory into the matrix-core operands
 // (v_mfma_f32_16x16x32_f16: keys need no transposition, values are paired by
-// byte permutes), keys of the next step loaded while this one's weights form
-// and values while the next scores do; the waves meet once, in LDS.
+// byte permutes), the next ones on their way while these are used; the waves
+// meet once, in LDS.
+//
+// Bound: memory behind a start of about 6 us (queries, first codes, the
+// record, the join's launch): 16 sequences of 4096 positions read 69 MB in
+// 19.4 us, 128 of 2000 270 MB in 52 us, 5.2 TB/s (a copy of 1 GiB runs at
+// 5.1). One sequence of 1025 takes 9.1 us, the kernel 6.4 and the join 3.3. On
+// the way: queries asked for before the first codes, and joins by one wave,
+// 32768 and 20011 positions in 16 bits 20.8 us, now 17.7 (13.1 and 4.9).
 template <int HD, bool Q8>
 struct Row16 {
 	static constexpr int EB = Q8 ? 1 : 2;
@@ -1588,9 +1603,9 @@ int64_t all_steps(const AttnKv &c, const SeqTab &t, int tokens) {
 	return n * c.kvh;
 }
 
-// Which kernel (7B heads, one MI355X, direct / tiled): 200 tokens 10 / 20 us,
-// 512 16 / 31, 512 at position 3000 (52 thousand wave-steps of 32 rows x 32
-// keys) 73 / 73, 2000 tokens (63 thousand) 98 / 86, 8192 tokens 1601 / 880.
+// Which kernel (7B heads, one MI355X, direct / tiled): 200 tokens 9 / 20 us,
+// 512 14 / 31, 512 at position 3000 (52 thousand wave-steps of 32 rows x 32
+// keys) 71 / 73, 2000 tokens (63 thousand) 98 / 86, 8192 tokens 1601 / 870.
 // So the direct one up to 55 wave-steps for each SIMD.
 //
 // Parts: the tiled kernel splits tiles of more than 1.5 times an equal share

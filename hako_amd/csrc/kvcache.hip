@@ -128,7 +128,13 @@ __device__ __forceinline__ void put4_past(float *dst, const float x[4]) {
 // A head row (token, one of its query, key or value heads) is L = head_dim/8
 // lanes of two float4 each. The two of a lane hold whole pairs: unit u (dims
 // 4u..4u+3) with unit u + rot/8 in the half layout, any two in the
-// interleaved one. Lanes on consecutive units keep both accesses contiguous.
+// interleaved one. Lanes on consecutive units keep both accesses contiguous;
+// a row's maximum is three or four lane permutes, nothing passes through LDS.
+//
+// Bound: memory, and below some thousand rows the launch (one token 3 us, 512
+// of 7B heads 5.7). 8192 packed tokens of 7B heads into 16 bits move 286 MB in
+// 51 us, 5.6 TB/s (a copy of 1 GiB runs at 5.1; part of the input is still in
+// the caches), the waves waiting 79% of their cycles.
 template <int HD, bool Q8>
 __global__ __launch_bounds__(256) void append_kernel(KvDev kv, const int *__restrict__ slot, const int *__restrict__ posv,
                                                      int n_tok, const float *__restrict__ k,
@@ -177,7 +183,8 @@ __global__ __launch_bounds__(256) void append_kernel(KvDev kv, const int *__rest
 }
 
 // A thread takes four consecutive dims of kReadRows rows, loads first; a wave's
-// accesses are whole rows.
+// accesses are whole rows. Bound: memory (32.7 thousand positions of 4 heads
+// from 8 bits: 169 MB in 25.5 us, 6.6 TB/s, four fifths of it stores).
 constexpr int kReadRows = 2;
 template <int HD, bool Q8>
 __global__ __launch_bounds__(256) void read_kernel(KvDev kv, const int *__restrict__ slot, const int *__restrict__ posv,
