@@ -927,10 +927,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_direct_kernel(AttnKv c,
 //
 // Bound: memory behind a start of about 6 us (queries, first codes, the
 // record, the join's launch): 16 sequences of 4096 positions read 69 MB in
-// 19.4 us, 128 of 2000 270 MB in 52 us, 5.2 TB/s (a copy of 1 GiB runs at
+// 19.2 us, 128 of 2000 270 MB in 52 us, 5.2 TB/s (a copy of 1 GiB runs at
 // 5.1). One sequence of 1025 takes 9.1 us, the kernel 6.4 and the join 3.3. On
 // the way: queries asked for before the first codes, and joins by one wave,
-// 32768 and 20011 positions in 16 bits 20.8 us, now 17.7 (13.1 and 4.9).
+// 32768 and 20011 positions in 16 bits 20.8 us, now 17.9.
 template <int HD, bool Q8>
 struct Row16 {
 	static constexpr int EB = Q8 ? 1 : 2;
@@ -1131,20 +1131,23 @@ __device__ __forceinline__ int part_keys(int n, int parts, int least) {
 	const int per = max((n + parts - 1) / parts, least);
 	return (per + 32 * kWaves - 1) / (32 * kWaves) * (32 * kWaves);
 }
-// The part and sequence of workgroup b (of each key/value head). A sequence's
+// The part and sequence of a workgroup (of each key/value head), by its place
+// (y, z) in a grid of own_grid, or the b-th in that order. A sequence's
 // parts lie next to each other, on different CUs, while sequences are few.
 // Where they fill the chip most parts are empty: all first parts come first,
 // every next round shifted by one, so that the others go to all dies (64
 // sequences of 1000 positions, one of 32000: 38 us, 85 with a sequence's parts
 // together; but 8 of 1..8000 13.3 and 16.8).
-__device__ __forceinline__ void part_of(int b, int n_seq, int parts, int least, int &part, int &sq) {
-	if (least < kLongPart) {
-		part = b % parts;
-		sq = b / parts;
-	} else {
-		part = b / n_seq;
-		sq = (b + part) % n_seq;
-	}
+dim3 own_grid(int kvh, int n_seq, int parts, int least) {
+	return least < kLongPart ? dim3(kvh, parts, n_seq) : dim3(kvh, n_seq, parts);
+}
+__device__ __forceinline__ void part_of(int y, int z, int n_seq, int least, int &part, int &sq) {
+	part = least < kLongPart ? y : z;
+	sq = least < kLongPart ? z : (y + z) % n_seq;
+}
+__device__ __forceinline__ void part_of_nth(int b, int n_seq, int parts, int least, int &part, int &sq) {
+	const int w = least < kLongPart ? parts : n_seq;
+	part_of(b % w, b / w, n_seq, least, part, sq);
 }
 // A sequence's own keys [prefix, end): end, 0 where it has no slot.
 __device__ __forceinline__ int own_end(const AttnKv &c, const int *slot, const int *len, int sq, int &sl) {
@@ -1266,8 +1269,8 @@ __global__ __launch_bounds__(256) void decode_kernel(AttnKv c, float *out, int64
                                                      float2 *__restrict__ rec_ml) {
 	__shared__ DecodeLds<HD> s;
 	int part, sq;
-	part_of(blockIdx.x / c.kvh, n_seq, parts, least, part, sq);
-	decode_part<HD, Q8>(c, s, blockIdx.x % c.kvh, part, sq, out, ldo, q, ldq, slot, len, G, scale, parts, least, 0, nrec, rec_o,
+	part_of(blockIdx.y, blockIdx.z, n_seq, least, part, sq);
+	decode_part<HD, Q8>(c, s, blockIdx.x, part, sq, out, ldo, q, ldq, slot, len, G, scale, parts, least, 0, nrec, rec_o,
 	                    rec_ml);
 }
 
@@ -1290,7 +1293,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefix_kernel(AttnKv c, const 
 	if (b >= tiles * pparts) {
 		b -= tiles * pparts;
 		int own, sq;
-		part_of(b, n_seq, parts, least, own, sq);
+		part_of_nth(b, n_seq, parts, least, own, sq);
 		decode_part<HD, Q8>(c, s.b, kvh, own, sq, nullptr, 0, q, ldq, slot, len, G, scale, parts, least, pparts, nrec, rec_o,
 		                    rec_ml);
 		return;
@@ -1513,7 +1516,7 @@ int decode(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq
 		hipLaunchKernelGGL((prefix_kernel<HD, Q8>), dim3((unsigned)blocks), dim3(64 * kWaves), 0, stream(), c, q, ldq, slot, len,
 		                   n_seq, G, scale * kLog2e, (int)tiles, pparts, unit, parts, least, nrec, ro, ml);
 	} else {
-		hipLaunchKernelGGL((decode_kernel<HD, Q8>), dim3((unsigned)blocks), dim3(256), 0, stream(), c, out, ldo, q, ldq, slot,
+		hipLaunchKernelGGL((decode_kernel<HD, Q8>), own_grid(c.kvh, n_seq, parts, least), dim3(256), 0, stream(), c, out, ldo, q, ldq, slot,
 		                   len, n_seq, G, scale * kLog2e, parts, least, nrec, ro, ml);
 	}
 	HK_LAUNCHED("attention");
