@@ -17,8 +17,9 @@ static int kv_shape_check(const hako_gpu_kv *kv) {
 	if ((size_t)kv->max_seq * kv->head_dim * kv_elt(kv->type) >= kBufNone)
 		return set_error(HAKO_GPU_EINVAL, "max_seq %d x head_dim %d: one head's rows exceed 2 GiB", kv->max_seq,
 		                 kv->head_dim);
-	// (rows of one head fit 25 bits, heads 16)
-	if (((size_t)kv->max_seq * kv->n_kv_heads * kv->n_slots) >> 48)
+	// at most 2^48 - 1 rows, so that no size in bytes overflows (a slot's rows, 25 bits by 16, do not; all slots' might)
+	const uint64_t slot_rows = (uint64_t)kv->max_seq * kv->n_kv_heads;
+	if ((uint64_t)kv->n_slots > ((1ull << 48) - 1) / slot_rows)
 		return set_error(HAKO_GPU_EINVAL, "%d slots of %d positions of %d heads", kv->n_slots, kv->max_seq, kv->n_kv_heads);
 	return HAKO_GPU_OK;
 }

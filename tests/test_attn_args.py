@@ -136,3 +136,30 @@ def test_kv_bytes(lib):
 def test_without_a_device(lib, call):
     """What is accepted goes on to the device, and says so where none was initialised."""
     assert call(lib) == ENODEV
+
+
+# Shapes whose number of rows is a multiple of 2^64, or wraps to a small one: no cache of theirs can be addressed.
+WRAPS = [dict(type=KV_Q8, head_dim=64, max_seq=1 << 24, n_kv_heads=1 << 15, n_slots=1 << 25),
+         dict(type=KV_F16, head_dim=64, max_seq=1 << 23, n_kv_heads=1 << 15, n_slots=1 << 26),
+         dict(type=KV_Q8, head_dim=64, max_seq=(1 << 24) + 1, n_kv_heads=1 << 15, n_slots=1 << 25)]
+
+
+@pytest.mark.parametrize("shape", WRAPS, ids=str)
+def test_shapes_that_wrap_are_refused(lib, shape):
+    assert (shape["max_seq"] * shape["n_kv_heads"] * shape["n_slots"]) % 2 ** 64 < 2 ** 48
+    codes, scales = C.c_size_t(7), C.c_size_t(7)
+    c = kv(k=None, v=None, k_scale=None, v_scale=None, **shape)
+    assert lib.hako_gpu_kv_bytes(C.byref(c), C.byref(codes), C.byref(scales)) == EINVAL
+    assert (codes.value, scales.value) == (7, 7)
+    c = kv(**shape)
+    assert append(lib, c, ldk=shape["n_kv_heads"] * 64) == EINVAL and read(lib, c, ldk=shape["n_kv_heads"] * 64) == EINVAL
+
+
+def test_the_largest_shapes_are_taken(lib):
+    """2^48 - 2^24 rows, and one slot more."""
+    codes, scales = C.c_size_t(), C.c_size_t()
+    c = kv(k=None, v=None, k_scale=None, v_scale=None, head_dim=64, max_seq=1 << 24, n_kv_heads=1, n_slots=(1 << 24) - 1)
+    assert lib.hako_gpu_kv_bytes(C.byref(c), C.byref(codes), C.byref(scales)) == 0
+    assert codes.value == ((1 << 48) - (1 << 24)) * 64 and scales.value == ((1 << 48) - (1 << 24)) * 4
+    c.n_slots += 1
+    assert lib.hako_gpu_kv_bytes(C.byref(c), C.byref(codes), C.byref(scales)) == EINVAL
