@@ -43,8 +43,10 @@ constexpr int kWaves = 4;        // waves per workgroup of the direct and the si
 // M is a whole number not below what it was taken from (the maximum of the
 // scores, in log2, plus the exponent of the value scales), so that what is
 // rescaled when it moves, and where sums meet, is so by exact powers of two;
-// it moves only when that passes it by kSlack, which is rare.
+// it moves only when that passes it by kSlack, which is rare. From kBig on a
+// float has no room for the exponent beside the score (see Base).
 constexpr float kNone = -FLT_MAX;   // M of a row that has seen no key
+constexpr float kBig = 4194304.0f;
 constexpr float kUp = 6.0f;         // weights are 2^(u - M + 6): at most 2^14 while u <= M + kSlack
 constexpr float kSlack = 8.0f;
 
@@ -85,9 +87,71 @@ __device__ __forceinline__ int fresh(int v) {
 }
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
-// The exponent m - to between two M, for ldexp: sums move by any power of two,
-// and to 0 from kNone.
-__device__ __forceinline__ int steps_down(float m, float to) { return (int)__builtin_fmaxf(m - to, -1000.0f); }
+
+// What a row's sums are taken against, M in two parts: weights are
+// 2^(u - m - e + kUp). A small base, |m| < kBig, has e = 0 and the exponent of
+// the value scales in m. A big one has the score's whole number in m and that
+// exponent in e: past 2^24 m + e would round to m (as would kUp), and weights
+// times value scales leave a half's range (before this was so, keys of 2^30
+// and values of 2^17 gave infinities). Steps with a big base go through a
+// block of their own, out of the way of the others, whose times stayed the same.
+struct Base {
+	float m, e;
+	__device__ __forceinline__ bool big() const { return (e != 0.0f || __builtin_fabsf(m) >= kBig) && m != kNone; }
+};
+// How far a lies above b, in powers of two: exact where they are near.
+__device__ __forceinline__ float above(Base a, Base b) { return (a.m - b.m) + (a.e - b.e); }
+// The same for ldexp, of sums that move from a to b >= a: any power of two, and to 0 from kNone.
+__device__ __forceinline__ int steps_down(Base a, Base b) { return (int)__builtin_fmaxf(above(a, b), -1000.0f); }
+
+// The sums of part of a row's keys: value sums o [record][HD], (M, l) in ml, and where e is not 0, which l's sign tells,
+// e (so that nobody reads it who need not).
+struct Records {
+	float *o;
+	float2 *ml;
+	float *e;
+	__device__ __forceinline__ void put(size_t r, Base b, float l) const {
+		ml[r] = make_float2(b.m, b.e != 0.0f ? -__builtin_fabsf(l) : __builtin_fabsf(l));
+		if (b.e != 0.0f) e[r] = b.e;
+	}
+};
+__device__ __forceinline__ bool has_e(float2 ml) { return __builtin_bit_cast(int, ml.y) < 0; }
+__device__ __forceinline__ Base base_of(float2 ml, const float *e) { return {ml.x, has_e(ml) ? *e : 0.0f}; }
+
+// Whether a step moves a small base M up, ue being the row's largest score there plus the exponent of the value scales.
+__device__ __forceinline__ bool passes(float ue, float M) { return ue > M + kSlack; }
+// ... and to a big one.
+__device__ __forceinline__ bool passes_big(float ue, float M) { return passes(ue, M) && !(__builtin_fabsf(__builtin_ceilf(ue)) < kBig); }
+// Moves a small base that stays small: the shift of the row's sums.
+__device__ __forceinline__ int move_up(float &M, float ue) {
+	const float n = passes(ue, M) ? __builtin_ceilf(ue) : M;
+	const int f = steps_down({M, 0.0f}, {n, 0.0f});
+	M = n;
+	return f;
+}
+// Moves any base: u is the largest score, e the exponent of the value scales, ue their sum. Small bases go as in
+// move_up, so that a row's answer is its own whatever the others of its wave do.
+__device__ __forceinline__ int move_up_any(Base &b, float u, float e, float ue) {
+	Base n = b;
+	if (b.big() ? (u - b.m) + (e - b.e) > kSlack : passes(ue, b.m)) {
+		const float c = __builtin_ceilf(ue);
+		n = __builtin_fabsf(c) < kBig ? Base{c, 0.0f} : Base{__builtin_ceilf(u), e};
+	}
+	const int f = steps_down(b, n);
+	b = n;
+	return f;
+}
+// N scores (in units of esc) against a big base: those whose weights are exp2(score esc). (esc is a power of two, and a
+// score that overflows here lies far below the base.)
+template <int N, class V>
+__device__ __forceinline__ void big_scores(V &sc, Base b, float esc) {
+	const float inv = __builtin_bit_cast(float, 0x7F000000u - __builtin_bit_cast(uint32_t, esc));   // 1 / esc
+#pragma unroll
+	for (int i = 0; i < N; i++) {
+		const float w = (__builtin_fmaf(sc[i], esc, -b.m) + (kUp - b.e)) * inv;
+		sc[i] = b.big() ? w : sc[i];
+	}
+}
 
 // Four int8 codes as halves: byte + 128 under the exponent byte 0x64 is the
 // half 1024 + (code + 128).
@@ -270,11 +334,13 @@ struct Tile {
 		alignas(16) float ks[2][kKeys];
 		alignas(16) float vs[2][kKeys];
 		float e[2];
+		float be[64 * kTileWaves];   // e of the rows' bases
 	};
 	h8 qh[KS], ql[KS];
 	float esc;      // 2^e of the row
 	f16v o[DT];
 	float M, l;
+	uint64_t big;   // lanes whose base is big; while there are any, every lane's e is in LDS, else it is 0
 
 	// The lane's row q (null: an idle row), times scale log2(e).
 	__device__ __forceinline__ void query(const float *q, float scale, int lane) {
@@ -305,12 +371,13 @@ struct Tile {
 			for (int v = 0; v < 16; v++) o[d][v] = 0.0f;
 		M = kNone;
 		l = 0.0f;
+		big = 0;
 	}
 
 	// The 64 keys of the chunk in LDS buffer `b`, the first at position key0; mask: some row of the wave does not see
 	// all of them. (Two instances of this, with and without the mask, cost a second set of the value sums' registers.)
 	// The weights of the second 32 keys form while the matrix cores add up the values of the first.
-	__device__ __forceinline__ void chunk(const Lds &s, int b, int key0, bool mask, int lim, int lane) {
+	__device__ __forceinline__ void chunk(Lds &s, int b, int key0, bool mask, int lim, int lane) {
 		lane = fresh(lane);
 		const int h = lane >> 5, i = lane & 31;
 		const uint8_t *kr = s.k[b] + i * kKeyRow<HD> + 16 * h;
@@ -358,11 +425,24 @@ struct Tile {
 		}
 #pragma unroll
 		for (int v = 0; v < 16; v++) mx = __builtin_fmaxf(__builtin_fmaxf(sc[0][v], sc[1][v]), mx);
-		mx = __builtin_fmaf(__builtin_fmaxf(mx, __shfl_xor(mx, 32)), esc, e);
-		if (__any(mx > M + kSlack)) {
-			const float mn = mx > M + kSlack ? __builtin_ceilf(mx) : M;
-			const int f = steps_down(M, mn);
-			M = mn;
+		mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32));
+		const float ue = __builtin_fmaf(mx, esc, e);
+		float c = kUp - M;
+		if (__ballot(passes(ue, M)) | big) {
+			int f;
+			if (__builtin_expect((__ballot(passes_big(ue, M)) | big) != 0, 0)) {
+				Base at = {M, big ? s.be[threadIdx.x] : 0.0f};
+				f = move_up_any(at, mx * esc, e, ue);
+				M = at.m;
+				s.be[threadIdx.x] = at.e;
+				big = __ballot(at.big());
+				big_scores<16>(sc[0], at, esc);
+				big_scores<16>(sc[1], at, esc);
+				c = at.big() ? 0.0f : kUp - M;
+			} else {
+				f = move_up(M, ue);
+				c = kUp - M;
+			}
 			l = __builtin_ldexpf(l, f);
 #pragma unroll
 			for (int d = 0; d < DT; d++)
@@ -370,16 +450,15 @@ struct Tile {
 				for (int v = 0; v < 16; v++) o[d][v] = __builtin_ldexpf(o[d][v], f);
 		}
 		h8 ph[2][2], pl[2][2];
-		weigh(s, b, 0, sc[0], h, ph[0], pl[0]);
-		weigh(s, b, 1, sc[1], h, ph[1], pl[1]);
+		weigh(s, b, 0, sc[0], c, h, ph[0], pl[0]);
+		weigh(s, b, 1, sc[1], c, h, ph[1], pl[1]);
 		add(s, b, 0, i, h, ph[0], pl[0]);
 		add(s, b, 1, i, h, ph[1], pl[1]);
 		__builtin_amdgcn_sched_barrier(0);
 	}
 
 	// Scores -> weights times the value scales, as halves, and their sum.
-	__device__ __forceinline__ void weigh(const Lds &s, int b, int t, const f16v &sc, int h, h8 ph[2], h8 pl[2]) {
-		const float c = kUp - M;
+	__device__ __forceinline__ void weigh(const Lds &s, int b, int t, const f16v &sc, float c, int h, h8 ph[2], h8 pl[2]) {
 #pragma unroll
 		for (int g = 0; g < 4; g++) {
 			const float4 vs = *(const float4 *)(s.vs[b] + 32 * t + 16 * (g >> 1) + 8 * h + 4 * (g & 1));
@@ -565,19 +644,23 @@ struct Direct {
 	static constexpr int KS = HD / 16, DT = HD / 32;
 	static constexpr int KL = HD * EB / 32;   // 16-byte loads of a key per lane (a key is two lanes)
 	static constexpr int VW = DT * EB / 4 > 0 ? DT * EB / 4 : 1;   // dwords of a value row per lane (DT dims; a row is 32 lanes)
+	// The last step's lo halves stay in LDS where registers do not hold all (in scratch memory they took 2 us of 32, 48
+	// sequences over 6000 positions in 16 bits).
+	static constexpr bool kKeep = !Q8 && HD == 128;
 	h8 qh[KS], ql[KS];
 	float esc;
 	f16v o[DT];
 	float M, l;
+	uint64_t big;   // as in Tile
 	uint4 k[KL];
 	uint32_t v[16][VW];
 	float sc1;   // lanes 0..31: the keys' scales, 32..63: the values'
 
 	// The rows' queries, times scale log2(e): a thread converts HD/8 dims of row tid/8 (src), once for all waves, and the
-	// operands go through LDS (buf: HD * 128 bytes, es: 32 floats, both free again when this returns). Step s of the
-	// score product takes dims 16 s + 8 h.. (halves) or 32 (s>>1) + 16 h + 8 (s&1).. (8 bits, as a 16-byte load brings
-	// them) in lane half h.
-	__device__ __forceinline__ void query(const float *src, float scale, uint8_t *buf, float *es, int tid) {
+	// operands go through LDS (buf: HD * 128 bytes, es: 32 floats, both free again when this returns; keep: 1 KB that
+	// stays). Step s of the score product takes dims 16 s + 8 h.. (halves) or 32 (s>>1) + 16 h + 8 (s&1).. (8 bits, as a
+	// 16-byte load brings them) in lane half h.
+	__device__ __forceinline__ void query(const float *src, float scale, uint8_t *buf, uint8_t *keep, float *es, int tid) {
 		constexpr int N = HD / 8;
 		const int t = tid & 7, row = tid >> 3, lane = tid & 63;
 		float x[N], a = 0.0f;
@@ -598,12 +681,13 @@ struct Direct {
 			split_q(x + 8 * j, e, hi, lo);
 			*(h8 *)(buf + 16 * (128 * s + 32 * h + row)) = hi;
 			*(h8 *)(buf + 16 * (128 * s + 64 + 32 * h + row)) = lo;
+			if (kKeep && s == KS - 1) *(h8 *)(keep + 16 * (32 * h + row)) = lo;
 		}
 		__syncthreads();
 #pragma unroll
 		for (int s = 0; s < KS; s++) {
 			qh[s] = *(const h8 *)(buf + 16 * (128 * s + lane));
-			ql[s] = *(const h8 *)(buf + 16 * (128 * s + 64 + lane));
+			if (!kKeep || s < KS - 1) ql[s] = *(const h8 *)(buf + 16 * (128 * s + 64 + lane));
 		}
 		esc = es[lane & 31];
 		__syncthreads();
@@ -613,6 +697,7 @@ struct Direct {
 			for (int v = 0; v < 16; v++) o[d][v] = 0.0f;
 		M = kNone;
 		l = 0.0f;
+		big = 0;
 	}
 
 	// Tile row i is the key of row i in key_row's order (an involution): register v of a lane's scores is key
@@ -644,8 +729,9 @@ struct Direct {
 		}
 	}
 
-	// The step's 32 keys from key0; mask: some row does not see all of them. sx: 64 floats of the wave's own in LDS.
-	__device__ __forceinline__ void scores(f16v &sc) {
+	// The step's 32 keys from key0; mask: some row does not see all of them. sx: 128 floats of the wave's own in LDS, the
+	// step's scales and every lane's base's e.
+	__device__ __forceinline__ void scores(f16v &sc, const uint8_t *keep, int lane) {
 #pragma unroll
 		for (int v = 0; v < 16; v++) sc[v] = 0.0f;
 #pragma unroll
@@ -660,11 +746,11 @@ struct Direct {
 				a = __builtin_bit_cast(h8, k[s % KL]);
 			}
 			sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[s], sc, 0, 0, 0);
-			sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[s], sc, 0, 0, 0);
+			sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, kKeep && s == KS - 1 ? *(const h8 *)(keep + 16 * lane) : ql[s], sc, 0, 0, 0);
 		}
 	}
 
-	// The step's scales into the wave's own 64 floats of LDS; the exponent of the values' largest.
+	// The step's scales into sx; the exponent of the values' largest.
 	__device__ __forceinline__ float scales(float *sx, int lane) {
 		const float other = __shfl_xor(sc1, 32);
 		const bool fin = __builtin_isfinite(lane < 32 ? other : sc1);   // the value row's scale
@@ -677,7 +763,7 @@ struct Direct {
 		return e;
 	}
 
-	__device__ __forceinline__ void weigh(f16v &sc, const float *sx, float e, int key0, bool mask, int lim, int lane, h8 ph[2],
+	__device__ __forceinline__ void weigh(f16v &sc, float *sx, float e, int key0, bool mask, int lim, int lane, h8 ph[2],
 	                                      h8 pl[2]) {
 		const int h = lane >> 5;
 		float mx = -INFINITY;
@@ -706,18 +792,29 @@ struct Direct {
 		}
 #pragma unroll
 		for (int v = 0; v < 16; v++) mx = __builtin_fmaxf(mx, sc[v]);
-		mx = __builtin_fmaf(__builtin_fmaxf(mx, __shfl_xor(mx, 32)), esc, e);
-		if (__any(mx > M + kSlack)) {
-			const float mn = mx > M + kSlack ? __builtin_ceilf(mx) : M;
-			const int f = steps_down(M, mn);
-			M = mn;
+		mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32));
+		const float ue = __builtin_fmaf(mx, esc, e);
+		float c = kUp - M;
+		if (__ballot(passes(ue, M)) | big) {
+			int f;
+			if (__builtin_expect((__ballot(passes_big(ue, M)) | big) != 0, 0)) {
+				Base at = {M, big ? sx[64 + lane] : 0.0f};
+				f = move_up_any(at, mx * esc, e, ue);
+				M = at.m;
+				sx[64 + lane] = at.e;
+				big = __ballot(at.big());
+				big_scores<16>(sc, at, esc);
+				c = at.big() ? 0.0f : kUp - M;
+			} else {
+				f = move_up(M, ue);
+				c = kUp - M;
+			}
 			l = __builtin_ldexpf(l, f);
 #pragma unroll
 			for (int d = 0; d < DT; d++)
 #pragma unroll
 				for (int v = 0; v < 16; v++) o[d][v] = __builtin_ldexpf(o[d][v], f);
 		}
-		const float c = kUp - M;
 #pragma unroll
 		for (int g = 0; g < 4; g++) {
 			const float4 vs = *(const float4 *)(sx + 32 + 16 * (g >> 1) + 8 * h + 4 * (g & 1));
@@ -766,17 +863,61 @@ struct Direct {
 	}
 };
 
+// The base and the sum that the waves' of a row meet at, and each wave's shift to it.
+template <int R>
+__device__ __forceinline__ Base meet(const float (&ml)[kWaves][R][4], int row, int x[kWaves], float &ls) {
+	Base k[kWaves];
+	float l[kWaves];
+	bool big = false;
+#pragma unroll
+	for (int i = 0; i < kWaves; i++) {
+		const float4 v = *(const float4 *)ml[i][row];
+		k[i] = {v.x, v.y};
+		l[i] = v.z;
+		big |= v.y != 0.0f;
+	}
+	Base b = k[0];
+#pragma unroll
+	for (int i = 1; i < kWaves; i++) b.m = __builtin_fmaxf(b.m, k[i].m);
+	if (__builtin_expect(big, 0)) {
+		b = k[0];
+#pragma unroll
+		for (int i = 1; i < kWaves; i++) b = above(k[i], b) > 0.0f ? k[i] : b;
+	}
+	ls = 0.0f;
+#pragma unroll
+	for (int i = 0; i < kWaves; i++) {
+		x[i] = steps_down(k[i], b);
+		ls += __builtin_ldexpf(l[i], x[i]);
+	}
+	return b;
+}
+
 template <int HD>
 struct DirectLds {
 	alignas(16) float o[kWaves][32][HD + 4];
-	float ml[kWaves][32][2];
-	alignas(16) float sx[kWaves][64];
+	alignas(16) float ml[kWaves][32][4];   // M, e and l
+	alignas(16) float sx[kWaves][128];   // a wave's scales, and e of its rows' bases
+	alignas(16) uint8_t keep[1024];
 };
 
-// 32 rows over steps [c0, c1) of their tile's keys. row: out row (null: idle row), or rec: its record.
+// Where rows go: row (token t, head g of the group) to o + t ot + g og, or to record first + t rt + g rg.
+struct Dest {
+	float *o;
+	int64_t ot, og;
+	Records rec;
+	size_t first;
+	int64_t rt, rg;
+	__device__ __forceinline__ Dest(float *out, int64_t ldo, int HD) : o(out), ot(ldo), og(HD), rec{}, first(0), rt(0), rg(0) {}
+	// (nrec to a query head, H heads to a token)
+	__device__ __forceinline__ Dest(const Records &r, size_t f, int H, int nrec) : o(nullptr), ot(0), og(0), rec(r), first(f), rt((int64_t)H * nrec), rg(nrec) {}
+};
+
+// 32 rows over steps [c0, c1) of their tile's keys. A lane's row: q (null: an idle row) and lim, tok << 4 | g its token
+// and head. (Places come from those two numbers after the steps: pointers held across them cost registers.)
 template <int HD, bool Q8>
 __device__ __forceinline__ void direct_rows(const AttnKv &c, DirectLds<HD> &s, int kvh, int slot, int end, int c0, int c1,
-                                            const float *q, float scale, int lim, float *out, float *rec_o, float2 *rec_ml) {
+                                            const float *q, float scale, int lim, int tok_g, const Dest &dest) {
 	constexpr int EB = Q8 ? 1 : 2;
 	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 	const int pend = min(c.prefix_len, end), nc1 = (pend + 31) / 32;
@@ -807,14 +948,14 @@ __device__ __forceinline__ void direct_rows(const AttnKv &c, DirectLds<HD> &s, i
 		const uint64_t x = (uint64_t)(uintptr_t)p;
 		return (uint64_t)(uint32_t)__shfl((int)(uint32_t)x, row) | ((uint64_t)(uint32_t)__shfl((int)(x >> 32), row) << 32);
 	};
-	w.query((const float *)(uintptr_t)from(q), scale, (uint8_t *)s.o, s.sx[0], tid);
-	const int lo = wave_min_i(q ? lim : 0x7FFFFFFF);
+	w.query((const float *)(uintptr_t)from(q), scale, (uint8_t *)s.o, s.keep, s.sx[0], tid);
+	const int lo = wave_min_i(tok_g >= 0 ? lim : 0x7FFFFFFF);
 	float *sx = s.sx[wave];
 	for (; ch < c1; ch += kWaves) {
 		const int key0 = first_key(ch), top = ch < nc1 ? pend : end;
 		f16v sc;
 		h8 ph[2], pl[2];
-		w.scores(sc);
+		w.scores(sc, s.keep, fresh(lane));
 		const float e = w.scales(sx, lane);
 		if (ch + kWaves < c1) load_k(ch + kWaves);
 		__builtin_amdgcn_sched_barrier(0);
@@ -825,56 +966,44 @@ __device__ __forceinline__ void direct_rows(const AttnKv &c, DirectLds<HD> &s, i
 	}
 	w.l += __shfl_xor(w.l, 32);
 	// the waves' sums meet: row i, dims DT (8 (v>>2) + 4 h + (v&3)) + d
-	const int i = lane & 31, h = lane >> 5;
+	const int at = fresh(tid), i = at & 31, h = (at >> 5) & 1, out = at >> 3;   // (out: this thread's row from here on)
 #pragma unroll
 	for (int v = 0; v < 16; v++) {
-		float *at = &s.o[wave][i][w.DT * (8 * (v >> 2) + 4 * h + (v & 3))];
+		float *to = &s.o[wave][i][w.DT * (8 * (v >> 2) + 4 * h + (v & 3))];
 		if (w.DT == 4)
-			*(float4 *)at = make_float4(w.o[0][v], w.o[1][v], w.o[2 % w.DT][v], w.o[3 % w.DT][v]);
+			*(float4 *)to = make_float4(w.o[0][v], w.o[1][v], w.o[2 % w.DT][v], w.o[3 % w.DT][v]);
 		else
-			*(float2 *)at = make_float2(w.o[0][v], w.o[1][v]);
+			*(float2 *)to = make_float2(w.o[0][v], w.o[1][v]);
 	}
-	if (h == 0) {
-		s.ml[wave][i][0] = w.M;
-		s.ml[wave][i][1] = w.l;
-	}
+	if (h == 0) *(float4 *)s.ml[wave][i] = make_float4(w.M, w.big ? sx[64 + (at & 63)] : 0.0f, w.l, 0.0f);
 	__syncthreads();
-	float *dst = (float *)(uintptr_t)from(out), *ro = (float *)(uintptr_t)from(rec_o);
-	float2 *rm = (float2 *)(uintptr_t)from(rec_ml);
-	if (!dst && !ro) return;
-	float m = s.ml[0][row][0];
-#pragma unroll
-	for (int k = 1; k < kWaves; k++) m = __builtin_fmaxf(m, s.ml[k][row][0]);
+	const int tg = __shfl(tok_g, out);
+	if (tg < 0) return;
+	const size_t r = dest.first + (tg >> 4) * dest.rt + (tg & 15) * dest.rg;
+	float *to = dest.o ? dest.o + (tg >> 4) * dest.ot + (tg & 15) * dest.og : dest.rec.o + r * HD;
 	int x[kWaves];
-	float ls = 0.0f;
+	float ls;
+	const Base b = meet(s.ml, out, x, ls);
+	const float z = !dest.o ? 1.0f : (ls == 0.0f ? 0.0f : 1.0f / ls);
 #pragma unroll
-	for (int k = 0; k < kWaves; k++) {
-		x[k] = steps_down(s.ml[k][row][0], m);
-		ls += __builtin_ldexpf(s.ml[k][row][1], x[k]);
-	}
-	const float z = ro ? 1.0f : (ls == 0.0f ? 0.0f : 1.0f / ls);
-	float *to = ro ? ro : dst;
-#pragma unroll
-	for (int d = 4 * (tid & 7); d < HD; d += 32) {
+	for (int d = 4 * (at & 7); d < HD; d += 32) {
 		float4 a = make_float4(0, 0, 0, 0);
 #pragma unroll
 		for (int k = 0; k < kWaves; k++) {
-			const float4 b = *(const float4 *)&s.o[k][row][d];
-			a.x += __builtin_ldexpf(b.x, x[k]);
-			a.y += __builtin_ldexpf(b.y, x[k]);
-			a.z += __builtin_ldexpf(b.z, x[k]);
-			a.w += __builtin_ldexpf(b.w, x[k]);
+			const float4 y = *(const float4 *)&s.o[k][out][d];
+			a.x += __builtin_ldexpf(y.x, x[k]);
+			a.y += __builtin_ldexpf(y.y, x[k]);
+			a.z += __builtin_ldexpf(y.z, x[k]);
+			a.w += __builtin_ldexpf(y.w, x[k]);
 		}
 		*(float4 *)(to + d) = make_float4(a.x * z, a.y * z, a.z * z, a.w * z);
 	}
-	if (ro && (tid & 7) == 0) *rm = make_float2(m, ls);
+	if (!dest.o && (at & 7) == 0) dest.rec.put(r, b, ls);
 }
 
-// Records: value sums rec_o [record][HD] and (M, l) rec_ml [record].
 template <int HD, bool Q8>
 __global__ __launch_bounds__(64 * kTileWaves, 2) void prompt_kernel(AttnKv c, SeqTab t, ItemTab order, float *out, int64_t ldo, const float *q,
-                                                        int64_t ldq, int G, float scale, float *__restrict__ rec_o,
-                                                        float2 *__restrict__ rec_ml) {
+                                                        int64_t ldq, int G, float scale, Records rec) {
 	__shared__ typename Tile<HD, Q8>::Lds s;
 	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
 	const int kvh = blockIdx.x % c.kvh;
@@ -893,28 +1022,28 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void prompt_kernel(AttnKv c, Se
 		w.put(out + row * ldo + head * HD, 1.0f / w.l, lane);
 		return;
 	}
-	const size_t rec = record_of(t, x, tok, c.kvh * G, head);
-	w.put(rec_o + rec * HD, 1.0f, lane);
-	if (lane < 32) rec_ml[rec] = make_float2(w.M, w.l);
+	const size_t r0 = record_of(t, x, tok, c.kvh * G, head);
+	w.put(rec.o + r0 * HD, 1.0f, lane);
+	if (lane < 32) rec.put(r0, {w.M, w.big ? s.be[tid] : 0.0f}, w.l);
 }
 
 // The direct kernel's items: tiles of 32 rows, parts of `unit` steps of 32 keys.
 template <int HD, bool Q8>
 __global__ __launch_bounds__(64 * kWaves, 2) void prompt_direct_kernel(AttnKv c, SeqTab t, float *out, int64_t ldo, const float *q,
-                                                               int64_t ldq, int G, float scale, float *__restrict__ rec_o,
-                                                               float2 *__restrict__ rec_ml) {
+                                                               int64_t ldq, int G, float scale, Records rec) {
 	__shared__ DirectLds<HD> s;
 	const int lane = threadIdx.x & 63;
 	const int kvh = blockIdx.x % c.kvh;
 	Item x;
 	if (!item_of<32>(t, nullptr, blockIdx.x / c.kvh, c.prefix_len, x)) return;
-	const int r = lane & 31, tok = r / G, head = kvh * G + r - tok * G;
-	const bool on = tok < x.ntok, whole = x.parts == 1;
-	const int64_t row = (int64_t)t.row[x.sq] + x.tok0 + tok;
-	const size_t rec = on && !whole ? record_of(t, x, tok, c.kvh * G, head) : 0;
-	direct_rows<HD, Q8>(c, s, kvh, x.slot, x.end, x.c0, x.c1, on ? q + row * ldq + head * HD : nullptr, scale,
-	                    on ? t.start[x.sq] + x.tok0 + tok + 1 : 0, on && whole ? out + row * ldo + head * HD : nullptr,
-	                    on && !whole ? rec_o + rec * HD : nullptr, rec_ml + rec);
+	const int r = lane & 31, tok = r / G, g = r - tok * G;
+	const bool on = tok < x.ntok;
+	const int64_t row = (int64_t)t.row[x.sq] + x.tok0;
+	const int head = kvh * G, H = c.kvh * G;
+	direct_rows<HD, Q8>(c, s, kvh, x.slot, x.end, x.c0, x.c1, on ? q + (row + tok) * ldq + (head + g) * HD : nullptr, scale,
+	                    on ? t.start[x.sq] + x.tok0 + tok + 1 : 0, on ? tok << 4 | g : -1,
+	                    x.parts == 1 ? Dest(out + row * ldo + head * HD, ldo, HD)
+	                                 : Dest(rec, record_of(t, x, 0, H, head), H, t.nsplit[x.sq]));
 }
 
 // ── single tokens: the up to 16 query heads of a group over one sequence's own keys ──
@@ -942,6 +1071,7 @@ struct Row16 {
 	float esc;
 	f4 o[VD];
 	float M, l;
+	uint64_t big;   // as in Tile
 	// a step's codes and scales
 	struct Codes {
 		uint4 k[2][KL];
@@ -981,6 +1111,7 @@ struct Row16 {
 		for (int d = 0; d < VD; d++) o[d] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
 		M = kNone;
 		l = 0.0f;
+		big = 0;
 	}
 
 	// tile row i of key tile t is key 8 (i>>2) + 4 t + (i&3): a lane's eight scores are keys 8 g + 0..7
@@ -1062,7 +1193,7 @@ struct Row16 {
 	}
 
 	// Weights of the 32 keys from key0, those at end and past it left out.
-	__device__ __forceinline__ void weigh(const Codes &cd, float e, f4 sc[2], int key0, int end, int lane, h8 &ph, h8 &pl) {
+	__device__ __forceinline__ void weigh(const Codes &cd, float *be, float e, f4 sc[2], int key0, int end, int lane, h8 &ph, h8 &pl) {
 		const int g = lane >> 4;
 		float x[8], mx = -INFINITY;
 #pragma unroll
@@ -1071,18 +1202,29 @@ struct Row16 {
 			mx = __builtin_fmaxf(mx, x[j]);
 		}
 		mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16));
-		mx = __builtin_fmaf(__builtin_fmaxf(mx, __shfl_xor(mx, 32)), esc, e);
-		if (__any(mx > M + kSlack)) {
-			const float mn = mx > M + kSlack ? __builtin_ceilf(mx) : M;
-			const int f = steps_down(M, mn);
-			M = mn;
+		mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32));
+		const float ue = __builtin_fmaf(mx, esc, e);
+		float c = kUp - M;
+		if (__ballot(passes(ue, M)) | big) {
+			int f;
+			if (__builtin_expect((__ballot(passes_big(ue, M)) | big) != 0, 0)) {
+				Base at = {M, big ? be[threadIdx.x] : 0.0f};
+				f = move_up_any(at, mx * esc, e, ue);
+				M = at.m;
+				be[threadIdx.x] = at.e;
+				big = __ballot(at.big());
+				big_scores<8>(x, at, esc);
+				c = at.big() ? 0.0f : kUp - M;
+			} else {
+				f = move_up(M, ue);
+				c = kUp - M;
+			}
 			l = __builtin_ldexpf(l, f);
 #pragma unroll
 			for (int d = 0; d < VD; d++)
 #pragma unroll
 				for (int v = 0; v < 4; v++) o[d][v] = __builtin_ldexpf(o[d][v], f);
 		}
-		const float c = kUp - M;
 #pragma unroll
 		for (int j = 0; j < 8; j += 2) {
 			float w[2];
@@ -1158,16 +1300,17 @@ __device__ __forceinline__ int own_end(const AttnKv &c, const int *slot, const i
 template <int HD>
 struct DecodeLds {
 	alignas(16) float o[kWaves][kMaxGroup][HD + 4];
-	float ml[kWaves][kMaxGroup][2];
+	alignas(16) float ml[kWaves][kMaxGroup][4];   // M, e and l
+	float be[64 * kWaves];   // e of the rows' bases
 };
 
 template <int HD, bool Q8>
 __device__ __forceinline__ void decode_part(const AttnKv &c, DecodeLds<HD> &s, int kvh, int part, int sq, float *out, int64_t ldo,
                                             const float *q, int64_t ldq, const int *__restrict__ slot,
                                             const int *__restrict__ len, int G, float scale, int parts, int least, int rec0, int nrec,
-                                            float *__restrict__ rec_o, float2 *__restrict__ rec_ml) {
+                                            Records rec) {
 	constexpr int EB = Q8 ? 1 : 2;
-	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 	int sl;
 	const int end = own_end(c, slot, len, sq, sl), n = max(end - c.prefix_len, 0);
 	const int per = part_keys(n, parts, least);
@@ -1202,7 +1345,7 @@ __device__ __forceinline__ void decode_part(const AttnKv &c, DecodeLds<HD> &s, i
 		if (Q8) e = w.exponent(x);
 		w.scores(x, sc);
 		if (!Q8) e = w.exponent(x);
-		w.weigh(x, e, sc, key0, last, lane, ph, pl);
+		w.weigh(x, s.be, e, sc, key0, last, lane, ph, pl);
 		key0 += 32 * kWaves;
 		if (!Q8) w.load_k(x, kr, ksr, key0, lane);
 		w.values(x, ph, pl);
@@ -1228,36 +1371,30 @@ __device__ __forceinline__ void decode_part(const AttnKv &c, DecodeLds<HD> &s, i
 		for (int d = 0; d < w.VD; d += 4)
 			*(float4 *)&s.o[wave][i][w.VD * (4 * g + v) + d] =
 			    make_float4(w.o[d][v], w.o[d + 1][v], w.o[d + 2][v], w.o[d + 3][v]);
-	if (g == 0) {
-		s.ml[wave][i][0] = w.M;
-		s.ml[wave][i][1] = w.l;
-	}
+	if (g == 0) *(float4 *)s.ml[wave][i] = make_float4(w.M, w.big ? s.be[tid] : 0.0f, w.l, 0.0f);
 	__syncthreads();
 	for (int t = tid; t < G * (HD / 4); t += 256) {
 		const int row = t / (HD / 4), d = t % (HD / 4) * 4;
-		float m = s.ml[0][row][0];
-#pragma unroll
-		for (int k = 1; k < kWaves; k++) m = __builtin_fmaxf(m, s.ml[k][row][0]);
-		float ls = 0.0f;
+		int x[kWaves];
+		float ls;
+		const Base b = meet(s.ml, row, x, ls);
 		float4 a = make_float4(0, 0, 0, 0);
 #pragma unroll
 		for (int k = 0; k < kWaves; k++) {
-			const int x = steps_down(s.ml[k][row][0], m);
-			const float4 b = *(const float4 *)&s.o[k][row][d];
-			ls += __builtin_ldexpf(s.ml[k][row][1], x);
-			a.x += __builtin_ldexpf(b.x, x);
-			a.y += __builtin_ldexpf(b.y, x);
-			a.z += __builtin_ldexpf(b.z, x);
-			a.w += __builtin_ldexpf(b.w, x);
+			const float4 y = *(const float4 *)&s.o[k][row][d];
+			a.x += __builtin_ldexpf(y.x, x[k]);
+			a.y += __builtin_ldexpf(y.y, x[k]);
+			a.z += __builtin_ldexpf(y.z, x[k]);
+			a.w += __builtin_ldexpf(y.w, x[k]);
 		}
 		const int hd = kvh * G + row;
 		if (whole) {
 			const float z = ls == 0.0f ? 0.0f : 1.0f / ls;
 			*(float4 *)(out + sq * ldo + hd * HD + d) = make_float4(a.x * z, a.y * z, a.z * z, a.w * z);
 		} else {
-			const size_t rec = ((size_t)sq * (c.kvh * G) + hd) * nrec + rec0 + part;
-			*(float4 *)(rec_o + rec * HD + d) = a;
-			if (d == 0) rec_ml[rec] = make_float2(m, ls);
+			const size_t r0 = ((size_t)sq * (c.kvh * G) + hd) * nrec + rec0 + part;
+			*(float4 *)(rec.o + r0 * HD + d) = a;
+			if (d == 0) rec.put(r0, b, ls);
 		}
 	}
 }
@@ -1265,13 +1402,11 @@ __device__ __forceinline__ void decode_part(const AttnKv &c, DecodeLds<HD> &s, i
 template <int HD, bool Q8>
 __global__ __launch_bounds__(256) void decode_kernel(AttnKv c, float *out, int64_t ldo, const float *q, int64_t ldq,
                                                      const int *__restrict__ slot, const int *__restrict__ len, int n_seq, int G,
-                                                     float scale, int parts, int least, int nrec, float *__restrict__ rec_o,
-                                                     float2 *__restrict__ rec_ml) {
+                                                     float scale, int parts, int least, int nrec, Records rec) {
 	__shared__ DecodeLds<HD> s;
 	int part, sq;
 	part_of(blockIdx.y, blockIdx.z, n_seq, least, part, sq);
-	decode_part<HD, Q8>(c, s, blockIdx.x, part, sq, out, ldo, q, ldq, slot, len, G, scale, parts, least, 0, nrec, rec_o,
-	                    rec_ml);
+	decode_part<HD, Q8>(c, s, blockIdx.x, part, sq, out, ldo, q, ldq, slot, len, G, scale, parts, least, 0, nrec, rec);
 }
 
 // A batch with a prefix in one launch, so that the two kinds of work fill each
@@ -1282,7 +1417,7 @@ template <int HD, bool Q8>
 __global__ __launch_bounds__(64 * kWaves, 2) void prefix_kernel(AttnKv c, const float *q, int64_t ldq, const int *__restrict__ slot,
                                                         const int *__restrict__ len, int n_seq, int G, float scale,
                                                         int tiles, int pparts, int unit, int parts, int least, int nrec,
-                                                        float *__restrict__ rec_o, float2 *__restrict__ rec_ml) {
+                                                        Records rec) {
 	__shared__ union Lds {
 		DirectLds<HD> a;
 		DecodeLds<HD> b;
@@ -1294,24 +1429,31 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefix_kernel(AttnKv c, const 
 		b -= tiles * pparts;
 		int own, sq;
 		part_of_nth(b, n_seq, parts, least, own, sq);
-		decode_part<HD, Q8>(c, s.b, kvh, own, sq, nullptr, 0, q, ldq, slot, len, G, scale, parts, least, pparts, nrec, rec_o,
-		                    rec_ml);
+		decode_part<HD, Q8>(c, s.b, kvh, own, sq, nullptr, 0, q, ldq, slot, len, G, scale, parts, least, pparts, nrec, rec);
 		return;
 	}
 	const int lane = threadIdx.x & 63, part = b / tiles;
 	const int64_t r = (int64_t)(b % tiles) * 32 + (lane & 31);
-	const int sq = (int)(r / G), head = kvh * G + (int)(r - (int64_t)sq * G);
+	const int sq = (int)(r / G), g = (int)(r - (int64_t)sq * G), head = kvh * G, H = c.kvh * G;
 	const bool on = sq < n_seq;
 	int lim = 0;
 	if (on) {
 		int sl;
 		lim = min(own_end(c, slot, len, sq, sl), c.prefix_len);
 	}
-	const size_t rec = on ? ((size_t)sq * (c.kvh * G) + head) * nrec + part : 0;
 	const int nc = (c.prefix_len + 31) / 32;
 	direct_rows<HD, Q8>(c, s.a, kvh, c.prefix_slot, c.prefix_len, part * unit, min(nc, part * unit + unit),
-	                    on ? q + (int64_t)sq * ldq + head * HD : nullptr, scale, lim, nullptr, on ? rec_o + rec * HD : nullptr,
-	                    rec_ml + rec);
+	                    on ? q + (int64_t)sq * ldq + (head + g) * HD : nullptr, scale, lim, on ? sq << 4 | g : -1,
+	                    Dest(rec, (size_t)head * nrec + part, H, nrec));
+}
+
+// a += y 2^f, ls += |l| 2^f
+__device__ __forceinline__ void add_record(float4 &a, float &ls, float4 y, float l, int f) {
+	ls += __builtin_ldexpf(__builtin_fabsf(l), f);
+	a.x += __builtin_ldexpf(y.x, f);
+	a.y += __builtin_ldexpf(y.y, f);
+	a.z += __builtin_ldexpf(y.z, f);
+	a.w += __builtin_ldexpf(y.w, f);
 }
 
 // One head's n records joined by a workgroup of kJoin waves: HD/4 lanes to a
@@ -1320,39 +1462,60 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefix_kernel(AttnKv c, const 
 // alone sets.
 constexpr int kJoin = 4;
 template <int HD>
-__device__ __forceinline__ void join(const float *__restrict__ ro, const float2 *__restrict__ ml, int n, float *dst) {
+__device__ __forceinline__ void join(const float *__restrict__ ro, const float2 *__restrict__ ml, const float *__restrict__ re, int n,
+                                     float *dst) {
 	constexpr int L = HD / 4, W = 64 * kJoin / L;
-	__shared__ float m_s[kJoin];
+	__shared__ float m_s[kJoin], e_s[kJoin];
+	__shared__ int big_s[kJoin];
 	__shared__ float a_s[kJoin][HD + 4];
 	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
 	const int d = tid % L * 4, k0 = tid / L;
 	// the first round's records and every thread's share of the maxima at once
-	float4 b0 = make_float4(0, 0, 0, 0);
-	float2 x0 = make_float2(kNone, 0.0f);
-	if (k0 < n) {
-		b0 = *(const float4 *)(ro + (size_t)k0 * HD + d);
-		x0 = ml[k0];
+	const int kf = max(min(k0, n - 1), 0);   // (there is room for a record where there is none)
+	const float4 b0 = *(const float4 *)(ro + (size_t)kf * HD + d);
+	const float2 x0 = ml[kf];
+	// the largest base: the largest m, and where some have an e the most that a record is above that
+	Base b = {kNone, 0.0f};
+	bool some = false;
+	for (int k = tid; k < n; k += 64 * kJoin) {
+		const float2 x = ml[k];
+		b.m = __builtin_fmaxf(b.m, x.x);
+		some |= has_e(x);
 	}
-	float m = kNone;
-	for (int k = tid; k < n; k += 64 * kJoin) m = __builtin_fmaxf(m, ml[k].x);
-	m = wave_max(m);
-	if (lane == 0) m_s[wave] = m;
+	b.m = wave_max(b.m);
+	int big = __any(some);
+	if (lane == 0) {
+		m_s[wave] = b.m;
+		big_s[wave] = big;
+	}
 	__syncthreads();
 #pragma unroll
-	for (int k = 0; k < kJoin; k++) m = __builtin_fmaxf(m, m_s[k]);
-	const int f0 = steps_down(x0.x, m);
-	float ls = __builtin_ldexpf(x0.y, f0);
-	float4 a = make_float4(__builtin_ldexpf(b0.x, f0), __builtin_ldexpf(b0.y, f0), __builtin_ldexpf(b0.z, f0), __builtin_ldexpf(b0.w, f0));
+	for (int k = 0; k < kJoin; k++) {
+		b.m = __builtin_fmaxf(b.m, m_s[k]);
+		big |= big_s[k];
+	}
+	big = __builtin_amdgcn_readfirstlane(big);
+	if (__builtin_expect(big, 0)) {
+		float e = kNone;
+		for (int k = tid; k < n; k += 64 * kJoin) e = __builtin_fmaxf(e, above(base_of(ml[k], re + k), b));
+		e = wave_max(e);
+		if (lane == 0) e_s[wave] = e;
+		__syncthreads();
+#pragma unroll
+		for (int k = 0; k < kJoin; k++) e = __builtin_fmaxf(e, e_s[k]);
+		b.e = e;
+	}
+	float ls = 0.0f;
+	float4 a = make_float4(0, 0, 0, 0);
+	if (__builtin_expect(big, 0)) {
+		for (int k = k0; k < n; k += W) add_record(a, ls, *(const float4 *)(ro + (size_t)k * HD + d), ml[k].y, steps_down(base_of(ml[k], re + k), b));
+	} else {
+		if (k0 < n) add_record(a, ls, b0, x0.y, steps_down({x0.x, 0.0f}, b));
 #pragma unroll 4
-	for (int k = k0 + W; k < n; k += W) {
-		const float2 x = ml[k];
-		const int f = steps_down(x.x, m);
-		const float4 b = *(const float4 *)(ro + (size_t)k * HD + d);
-		ls += __builtin_ldexpf(x.y, f);
-		a.x += __builtin_ldexpf(b.x, f);
-		a.y += __builtin_ldexpf(b.y, f);
-		a.z += __builtin_ldexpf(b.z, f);
-		a.w += __builtin_ldexpf(b.w, f);
+		for (int k = k0 + W; k < n; k += W) {
+			const float2 x = ml[k];
+			add_record(a, ls, *(const float4 *)(ro + (size_t)k * HD + d), x.y, steps_down({x.x, 0.0f}, b));
+		}
 	}
 #pragma unroll
 	for (int k = L; k < 64; k <<= 1) {
@@ -1381,15 +1544,15 @@ __device__ __forceinline__ void join(const float *__restrict__ ro, const float2 
 template <int HD>
 __global__ __launch_bounds__(64 * kJoin) void decode_join_kernel(AttnKv c, float *out, int64_t ldo, const int *__restrict__ slot,
                                                          const int *__restrict__ len, int H, int parts, int least, int rec0,
-                                                         int nrec, const float *__restrict__ rec_o,
-                                                         const float2 *__restrict__ rec_ml) {
+                                                         int nrec, const float *__restrict__ rec_o, const float2 *__restrict__ rec_ml,
+                                                         const float *__restrict__ rec_e) {
 	const int h = blockIdx.x, sq = blockIdx.y;
 	int sl;
 	const int end = own_end(c, slot, len, sq, sl), n = max(end - c.prefix_len, 0);
 	const int per = part_keys(n, parts, least), used = n > 0 ? (n + per - 1) / per : 0;
 	if (rec0 == 0 && used == 1) return;   // written at once
 	const size_t rec = ((size_t)sq * H + h) * nrec;
-	join<HD>(rec_o + rec * HD, rec_ml + rec, rec0 + used, out + sq * ldo + h * HD);
+	join<HD>(rec_o + rec * HD, rec_ml + rec, rec_e + rec, rec0 + used, out + sq * ldo + h * HD);
 }
 
 // The tokens whose tiles were split (the last ones of each sequence), few
@@ -1397,7 +1560,8 @@ __global__ __launch_bounds__(64 * kJoin) void decode_join_kernel(AttnKv c, float
 template <int HD, int K>
 __global__ __launch_bounds__(256) void prompt_join_kernel(SeqTab t, int prefix_len, float *out, int64_t ldo, int H,
                                                           const float *__restrict__ rec_o,
-                                                          const float2 *__restrict__ rec_ml) {
+                                                          const float2 *__restrict__ rec_ml,
+                                                          const float *__restrict__ rec_e) {
 	constexpr int L = HD / 4;
 	const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
 	const int js = (int)(row / H), h = (int)(row - (int64_t)js * H), d = threadIdx.x % L * 4;
@@ -1409,22 +1573,33 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(SeqTab t, int prefix_l
 	const int tile = tok / t.tile_tokens, ns = t.nsplit[sq];
 	const int nc = tile_steps<K>(t.start[sq] + min((tile + 1) * t.tile_tokens, t.len[sq]), prefix_len);
 	const int n = (nc + t.unit - 1) / t.unit;
-	const size_t rec = (size_t)t.rec[sq] + ((size_t)j * H + h) * ns;
-	const float2 *ml = rec_ml + rec;
-	const float *ro = rec_o + rec * HD + d;
-	float m = kNone, ls = 0.0f;
-	for (int k = 0; k < n; k++) m = __builtin_fmaxf(m, ml[k].x);
-	float4 a = make_float4(0, 0, 0, 0);
-#pragma unroll 4
+	const size_t first = (size_t)t.rec[sq] + ((size_t)j * H + h) * ns;
+	const float2 *ml = rec_ml + first;
+	const float *ro = rec_o + first * HD + d, *re = rec_e + first;
+	Base b = {kNone, 0.0f};
+	bool some = false;
 	for (int k = 0; k < n; k++) {
-		const float4 b = *(const float4 *)(ro + (size_t)k * HD);
 		const float2 x = ml[k];
-		const int f = steps_down(x.x, m);
-		ls += __builtin_ldexpf(x.y, f);
-		a.x += __builtin_ldexpf(b.x, f);
-		a.y += __builtin_ldexpf(b.y, f);
-		a.z += __builtin_ldexpf(b.z, f);
-		a.w += __builtin_ldexpf(b.w, f);
+		b.m = __builtin_fmaxf(b.m, x.x);
+		some |= has_e(x);
+	}
+	const bool big = __any(some);
+	if (__builtin_expect(big, 0)) {
+		float e = kNone;
+		for (int k = 0; k < n; k++) e = __builtin_fmaxf(e, above(base_of(ml[k], re + k), b));
+		b.e = e;
+	}
+	float ls = 0.0f;
+	float4 a = make_float4(0, 0, 0, 0);
+	if (__builtin_expect(big, 0)) {
+		for (int k = 0; k < n; k++) add_record(a, ls, *(const float4 *)(ro + (size_t)k * HD), ml[k].y, steps_down(base_of(ml[k], re + k), b));
+	} else {
+#pragma unroll 4
+		for (int k = 0; k < n; k++) {
+			const float4 y = *(const float4 *)(ro + (size_t)k * HD);
+			const float2 x = ml[k];
+			add_record(a, ls, y, x.y, steps_down({x.x, 0.0f}, b));
+		}
 	}
 	const float z = 1.0f / ls;
 	*(float4 *)(out + ((int64_t)t.row[sq] + tok) * ldo + (int64_t)h * HD + d) = make_float4(a.x * z, a.y * z, a.z * z, a.w * z);
@@ -1454,12 +1629,13 @@ AttnKv attn_kv(const hako_gpu_kv *kv, int prefix_slot, int prefix_len, int len_a
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
-// Room for n records of HD value sums and (M, l).
-int records(size_t n, int HD, float **o, float2 **ml) {
+// Room for n records.
+int records(size_t n, int HD, Records *r) {
 	void *p = nullptr;
-	if (int rc = workspace(kWsAttn, n * (HD + 2) * sizeof(float), &p)) return rc;
-	*o = (float *)p;
-	*ml = (float2 *)(*o + n * HD);
+	if (int rc = workspace(kWsAttn, n * (HD + 3) * sizeof(float), &p)) return rc;
+	r->o = (float *)p;
+	r->ml = (float2 *)(r->o + n * HD);
+	r->e = (float *)(r->ml + n);
 	return HAKO_GPU_OK;
 }
 
@@ -1506,23 +1682,22 @@ int decode(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq
 	const DecodePlan p = decode_plan(c.max_seq, c.prefix_len, c.kvh, n_seq, H);
 	const int parts = p.parts, least = p.least, pparts = p.pparts, unit = p.unit, nrec = p.nrec;
 	const int64_t tiles = p.tiles;
-	float *ro = nullptr;
-	float2 *ml = nullptr;
+	Records rec{};
 	if (nrec)
-		if (int rc = records((size_t)n_seq * H * nrec, HD, &ro, &ml)) return rc;
+		if (int rc = records((size_t)n_seq * H * nrec, HD, &rec)) return rc;
 	const int64_t blocks = (tiles * pparts + (int64_t)n_seq * parts) * c.kvh;
 	if (blocks > kMaxThreads / (64 * kWaves)) return set_error(HAKO_GPU_EINVAL, "%lld workgroups in one call", (long long)blocks);
 	if (pparts) {
 		hipLaunchKernelGGL((prefix_kernel<HD, Q8>), dim3((unsigned)blocks), dim3(64 * kWaves), 0, stream(), c, q, ldq, slot, len,
-		                   n_seq, G, scale * kLog2e, (int)tiles, pparts, unit, parts, least, nrec, ro, ml);
+		                   n_seq, G, scale * kLog2e, (int)tiles, pparts, unit, parts, least, nrec, rec);
 	} else {
 		hipLaunchKernelGGL((decode_kernel<HD, Q8>), own_grid(c.kvh, n_seq, parts, least), dim3(256), 0, stream(), c, out, ldo, q, ldq, slot,
-		                   len, n_seq, G, scale * kLog2e, parts, least, nrec, ro, ml);
+		                   len, n_seq, G, scale * kLog2e, parts, least, nrec, rec);
 	}
 	HK_LAUNCHED("attention");
 	if (nrec) {
 		hipLaunchKernelGGL(decode_join_kernel<HD>, dim3(H, n_seq), dim3(64 * kJoin), 0, stream(), c, out, ldo, slot, len, H, parts, least,
-		                   pparts, nrec, ro, ml);
+		                   pparts, nrec, rec.o, rec.ml, rec.e);
 		HK_LAUNCHED("attention join");
 	}
 	return HAKO_GPU_OK;
@@ -1581,16 +1756,14 @@ int prompt_launch(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, int H, in
 	t.item[t.n] = (int)items;
 	if (items * c.kvh > kMaxThreads / (64 * kTileWaves) || recs > 0xFFFFFFFFll || (int64_t)t.join[t.n] * H * (HD / 4) > kMaxThreads)
 		return set_error(HAKO_GPU_EINVAL, "%lld tiles and %lld records in one call", (long long)(items * c.kvh), (long long)recs);
-	float *ro = nullptr;
-	float2 *ml = nullptr;
+	Records rec{};
 	if (recs)
-		if (int rc = records((size_t)recs, HD, &ro, &ml)) return rc;
-	launch(items, ro, ml);
+		if (int rc = records((size_t)recs, HD, &rec)) return rc;
+	launch(items, rec);
 	HK_LAUNCHED("attention");
 	if (recs) {
 		const int64_t blocks = ((int64_t)t.join[t.n] * H * (HD / 4) + 255) / 256;
-		hipLaunchKernelGGL((prompt_join_kernel<HD, K>), dim3((unsigned)blocks), dim3(256), 0, stream(), t, c.prefix_len, out, ldo, H,
-		                   ro, ml);
+		hipLaunchKernelGGL((prompt_join_kernel<HD, K>), dim3((unsigned)blocks), dim3(256), 0, stream(), t, c.prefix_len, out, ldo, H, rec.o, rec.ml, rec.e);
 		HK_LAUNCHED("attention join");
 	}
 	return HAKO_GPU_OK;
@@ -1629,20 +1802,20 @@ int prompt(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, const float *q, 
 		const int64_t all = all_steps<kKeys>(c, t, 32 * kTileWaves / G);
 		return prompt_launch<HD, Q8, kKeys>(
 		    c, t, out, ldo, H, 32 * kTileWaves, std::max<int64_t>(4, (3 * all + 2 * cu - 1) / (2 * cu)),
-		    [&](int64_t items, float *ro, float2 *ml) {
+		    [&](int64_t items, const Records &rec) {
 			    ItemTab order;
 			    if (const int n = sort_items<kKeys>(t, c.prefix_len, order)) items = n;
 			    hipLaunchKernelGGL((prompt_kernel<HD, Q8>), dim3((unsigned)(items * c.kvh)), dim3(64 * kTileWaves), 0, stream(), c, t, order, out,
-			                       ldo, q, ldq, G, scale * kLog2e, ro, ml);
+			                       ldo, q, ldq, G, scale * kLog2e, rec);
 		    });
 	}
 	int64_t tiles = 0;
 	for (int s = 0; s < t.n; s++) tiles += (t.len[s] + 32 / G - 1) / (32 / G);
 	const int64_t share = (steps + slots - 1) / slots;
 	return prompt_launch<HD, Q8, 32>(c, t, out, ldo, H, 32, std::max<int64_t>(4 * kWaves, 2 * tiles * c.kvh <= slots ? share : 2 * share),
-	                                 [&](int64_t items, float *ro, float2 *ml) {
+	                                 [&](int64_t items, const Records &rec) {
 		                                 hipLaunchKernelGGL((prompt_direct_kernel<HD, Q8>), dim3((unsigned)(items * c.kvh)),
-		                                                    dim3(64 * kWaves), 0, stream(), c, t, out, ldo, q, ldq, G, scale * kLog2e, ro, ml);
+		                                                    dim3(64 * kWaves), 0, stream(), c, t, out, ldo, q, ldq, G, scale * kLog2e, rec);
 	                                 });
 }
 
@@ -1658,9 +1831,8 @@ int attn_decode(float *out, int64_t ldo, const float *q, int64_t ldq, const hako
 
 int attn_decode_reserve(const hako_gpu_kv *kv, int n_seq, int H, int prefix_len) {
 	const DecodePlan p = decode_plan(kv->max_seq, prefix_len, kv->n_kv_heads, n_seq, H);
-	float *o;
-	float2 *ml;
-	return p.nrec ? records((size_t)n_seq * H * p.nrec, kv->head_dim, &o, &ml) : HAKO_GPU_OK;
+	Records r;
+	return p.nrec ? records((size_t)n_seq * H * p.nrec, kv->head_dim, &r) : HAKO_GPU_OK;
 }
 
 void attn_set_prompt(int v) { g_attn_prompt = v == 1 || v == 2 ? v : 0; }

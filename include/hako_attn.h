@@ -10,7 +10,8 @@
  * reference: src/model.c:105-137 with an fp32 cache, one token at a time.
  *
  * Everything outside the cache is fp32, and so is the arithmetic: products
- * with cached codes are carried to 22 bits or more and summed in fp32.
+ * with cached codes are carried to 22 bits or more (of a query's values, those
+ * below 2^-16 of its head's largest to 2^-38 of that) and summed in fp32.
  * Conventions are those of hako_gpu.h: 0 or a negative HAKO_GPU_E* code with
  * hako_gpu_last_error() set, work enqueued on the library stream, device
  * pointers unless a comment says host. The attention calls use a library
