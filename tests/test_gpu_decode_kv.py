@@ -241,3 +241,67 @@ def test_refusals(gpu, tmp_path):
         assert (k.type, k.n_slots, k.max_seq, k.head_dim) == (KV_Q8, 2, 64, 64) and C.sizeof(k) > 0
     finally:
         typed.close()
+
+
+@pytest.mark.parametrize("kind", [KV_Q8, KV_F16])
+@pytest.mark.parametrize("cfg", [SMALL_128, TINY])
+def test_captured_steps_follow_the_prefix(gpu, tmp_path, kind, cfg):
+    """Captured steps against eager ones on the same decoder, bit for bit: without a prefix, under one (the step captured
+    before is not replayed), after its end (as a decoder that never shared one), and under one again. Besides the tokens
+    (a random model soon repeats one, whatever it sees) the rows that the steps write in the last layer's cache count:
+    they follow from the attention of the layers before it."""
+    path = str(tmp_path / "m.mlf2")
+    mlf2.write_qwen2(path, cfg, 9)
+    rng = np.random.default_rng(11)
+    prefix = rng.integers(0, cfg.vocab, 130)
+    turns = [rng.integers(0, cfg.vocab, m) for m in (5, 40, 17)]
+    plain = [rng.integers(0, cfg.vocab, m) for m in (60, 9, 33)]
+    tok, n = np.array([4, 5, 6], np.int32), 6
+    assert cfg.n_layers > 1
+
+    def written(dec, pos):
+        """Keys and values of the n positions from pos on."""
+        return np.stack([[x[p:] for x in rows_of(gpu, dec, dec.cache(cfg.n_layers - 1), s, p + n)] for s, p in enumerate(pos)])
+
+    def fed(dec, at, prompts):
+        """Prompts from position `at`, then n captured steps; the same steps eagerly, and captured again, write the same."""
+        dec.set_pos(at)
+        for s, p in enumerate(prompts):
+            dec.prefill(p, s)
+        pos = [at + len(p) for p in prompts]
+        gen = dec.generate(tok, n)
+        rows = written(dec, pos)
+        assert np.isfinite(rows).all()
+        dec.set_pos(pos)
+        cur, eager = tok, []
+        for _ in range(n):
+            cur = dec.step(cur)
+            eager.append(cur)
+        np.testing.assert_array_equal(gen, np.stack(eager))
+        np.testing.assert_array_equal(rows, written(dec, pos))
+        dec.set_pos(pos)
+        np.testing.assert_array_equal(dec.generate(tok, n), gen)
+        np.testing.assert_array_equal(rows, written(dec, pos))
+        return rows
+
+    other = Decoder(gpu, path, 3, 260, kind)
+    try:
+        want = fed(other, 0, plain)
+    finally:
+        other.close()
+    dec = Decoder(gpu, path, 3, 260, kind)
+    try:
+        np.testing.assert_array_equal(fed(dec, 0, plain), want)
+        shared = []
+        for owner in (1, 2):
+            dec.set_pos(0)
+            dec.prefill(prefix, owner)
+            dec.share_prefix(owner, len(prefix))
+            shared.append(fed(dec, len(prefix), turns))
+            dec.share_prefix(0, 0)
+            np.testing.assert_array_equal(fed(dec, 0, plain), want)
+        np.testing.assert_array_equal(shared[0], shared[1])
+        # and the prefix counts: without it every sequence's rows come out otherwise
+        assert (fed(dec, len(prefix), turns) != shared[0]).any((1, 2, 3)).all()
+    finally:
+        dec.close()
