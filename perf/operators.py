@@ -162,6 +162,8 @@ def _table(case, positions):
 
 
 def prepare(case, seed):
+    if own:
+        _lib()
     g, lens = _gen(seed), _ints(case["lens"])
     H, KVH, hd = case["heads"], case["kv_heads"], case["head_dim"]
     n_seq, max_seq = len(lens), _max_seq(case)
@@ -200,14 +202,19 @@ def prepare(case, seed):
 
 # ── the framework's calls ──
 
-_gpu = None
+_gpu = _stream = None
 
 
 def _lib():
-    global _gpu
+    """The library; torch's work goes to its stream from here on, as in a program that uses both."""
+    global _gpu, _stream
     if _gpu is None:
         from hako_amd.gpu import Gpu
-        _gpu = Gpu(0)
+        gpu = Gpu(0)
+        _stream = torch.cuda.ExternalStream(gpu.lib.hako_gpu_stream())
+        torch.cuda.current_stream().synchronize()
+        torch.cuda.set_stream(_stream)
+        _gpu = gpu
     return _gpu
 
 
@@ -220,7 +227,19 @@ def _view(s):
 
 
 def _own_run(s):
-    gpu, case = _lib(), s["case"]
+    """The calls, on the library's stream: in order with torch's work there, and made to be so for a caller on another."""
+    _lib()
+    if torch._C._cuda_getCurrentRawStream(0) == _stream.cuda_stream:   # (2.5 us less than torch.cuda.current_stream())
+        return _own_calls(s)
+    caller = torch.cuda.current_stream()
+    _stream.wait_stream(caller)
+    out = _own_calls(s)
+    caller.wait_stream(_stream)
+    return out
+
+
+def _own_calls(s):
+    gpu, case = _gpu, s["case"]
     H, KV, hd, kv = case["heads"], case["kv_heads"] * case["head_dim"], case["head_dim"], _view(s)
     D, scale = H * hd, 1.0 / math.sqrt(hd)
     if case["kind"] in ("append", "read"):
