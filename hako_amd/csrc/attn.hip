@@ -200,9 +200,9 @@ __device__ __forceinline__ float scale_exp(float vmax) {
 // chunk.
 //
 // Bound: matrix work at the chip's power. 8192 tokens of 7B heads (28 / 4 of
-// 128, 481 GFLOP, each product twice: 962) take 0.84-0.90 ms, 1.1 PFLOP/s of
+// 128, 481 GFLOP, each product twice: 962) take 0.84-0.86 ms, 1.1 PFLOP/s of
 // matrix operations; an 8192^3 fp16 product of the library runs at 1.09 here.
-// The matrix pipes are then busy 61% of the cycles, the vector pipes 57%, at
+// The matrix pipes are then busy 64% of the cycles, the vector pipes 59%, at
 // 1.8 GHz. On the way (the same call): 128-row tiles and one accumulator set
 // per masked and unmasked instance 1.51 ms; one instance, 16-byte LDS reads
 // 1.00; the weights of the second 32 keys formed under the values' products of
@@ -633,10 +633,10 @@ __device__ __forceinline__ size_t record_of(const SeqTab &t, const Item &x, int 
 //
 // Bound: vector work. A step is 32 matrix operations of 16 passes and about
 // 390 vector ones, 176 of them codes to halves; with 2000 tokens of 7B heads
-// the vector pipes are busy 68% of the cycles, the matrix pipes 30% (that call
-// is the tiled kernel's for this reason: 98 and 86 us). Small calls: 77 tokens
-// of 3B heads 7.6 us, 512 of 7B heads 14.4, 16 x 77 22, 64 tokens at position
-// 8000 33.7. On the way: every wave converting all 32 queries for itself cost
+// the vector pipes are busy 66% of the cycles, the matrix pipes 33% (that call
+// is the tiled kernel's for this reason: 92 and 87 us). Small calls: 77 tokens
+// of 3B heads 8.4 us, 512 of 7B heads 14.1, 16 x 77 22.3, 64 tokens at position
+// 8000 33.8. On the way: every wave converting all 32 queries for itself cost
 // 512 tokens 1.8 us more (a thread now converts an eighth of a row, once).
 template <int HD, bool Q8>
 struct Direct {
@@ -644,8 +644,8 @@ struct Direct {
 	static constexpr int KS = HD / 16, DT = HD / 32;
 	static constexpr int KL = HD * EB / 32;   // 16-byte loads of a key per lane (a key is two lanes)
 	static constexpr int VW = DT * EB / 4 > 0 ? DT * EB / 4 : 1;   // dwords of a value row per lane (DT dims; a row is 32 lanes)
-	// The last step's lo halves stay in LDS where registers do not hold all (in scratch memory they took 2 us of 32, 48
-	// sequences over 6000 positions in 16 bits).
+	// The last step's lo halves stay in LDS where registers do not hold all (48 sequences over 6000 positions in 16 bits
+	// 32.0 us, 33.8 with the compiler's choice in scratch memory).
 	static constexpr bool kKeep = !Q8 && HD == 128;
 	h8 qh[KS], ql[KS];
 	float esc;
@@ -1056,10 +1056,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_direct_kernel(AttnKv c,
 //
 // Bound: memory behind a start of about 6 us (queries, first codes, the
 // record, the join's launch): 16 sequences of 4096 positions read 69 MB in
-// 19.2 us, 128 of 2000 270 MB in 52 us, 5.2 TB/s (a copy of 1 GiB runs at
-// 5.1). One sequence of 1025 takes 9.1 us, the kernel 6.4 and the join 3.3. On
+// 19.1 us, 128 of 2000 270 MB in 52 us, 5.2 TB/s (a copy of 1 GiB runs at
+// 5.1). One sequence of 1025 takes 9.3 us, the kernel 6.3 and the join 3.5. On
 // the way: queries asked for before the first codes, and joins by one wave,
-// 32768 and 20011 positions in 16 bits 20.8 us, now 17.9.
+// 32768 and 20011 positions in 16 bits 20.8 us, then 17.9. The waves' number as
+// a scalar, so that the loop is one for the compiler too: 64 sequences of 1000
+// positions 15.1 us, now 14.8.
 template <int HD, bool Q8>
 struct Row16 {
 	static constexpr int EB = Q8 ? 1 : 2;
@@ -1327,9 +1329,9 @@ __device__ __forceinline__ void decode_part(const AttnKv &c, DecodeLds<HD> &s, i
 	const __amdgpu_buffer_rsrc_t vr = stream_rsrc(uniform_ptr(c.v + r * HD * EB), rows * HD * EB);
 	const __amdgpu_buffer_rsrc_t ksr = stream_rsrc(uniform_ptr(c.ks + r), rows * 4);
 	const __amdgpu_buffer_rsrc_t vsr = stream_rsrc(uniform_ptr(c.vs + r), rows * 4);
-	// Codes on their way while others are used. 8 bits: two steps' in turn (64 sequences of 1000 positions 14.9 us, 16.6
+	// Codes on their way while others are used. 8 bits: two steps' in turn (64 sequences of 1000 positions 1.7 us less than
 	// the other way). Halves, whose two steps would take 254 registers: the keys' of the next step once this one's
-	// weights are formed, the values' after their products (32768 and 20011 positions 18.0 us, 19.2 in turn). (Keys from
+	// weights are formed, the values' after their products (32768 and 20011 positions 1.2 us less than in turn). (Keys from
 	// `last` on read as zeros, from nowhere.)
 	typename Row16<HD, Q8>::Codes ca, cb;
 	int key0 = first + 32 * wave;
@@ -1651,17 +1653,18 @@ DecodePlan decode_plan(int max_seq, int prefix_len, int kvh, int n_seq, int H) {
 	const int own = max_seq - prefix_len;
 	const int slots = 2 * cu_count();   // workgroups that run at once
 	// own keys: parts of 32 keys a wave or more, until the workgroups fill the chip (16 sequences of 4096, 64 pairs of
-	// sequence and head: 18.4 us with 8 parts, 20.0 with 4, 23.5 with 12). From a pair per CU on only long sequences are
-	// split, for one among short ones (64 sequences, 256 pairs: one of 8000 and 63 of 100..400 positions 27 us, 62 in one
-	// part; all of 4096 56 us, 50 in one part)
+	// sequence and head: 19.0 us with 8 parts, 18.5 with 4, 22.8 with 12). From a pair per CU on only long sequences are
+	// split, for one among short ones (64 sequences, 256 pairs: one of 8000 and 63 of 100..400 positions 26 us, 63 in one
+	// part; all of 4096 56 to 58 us, 50 to 53 in one part). The lengths are not known here, so the parts are those of
+	// max_seq: 64 sequences of 1000 positions in slots of 2048 take 14.9 us, of 8192 17.4, of 32768 20.6
 	const int64_t pairs = (int64_t)n_seq * kvh;
 	p.least = pairs >= cu_count() ? kLongPart : 32 * kWaves;
 	p.parts = (own + p.least - 1) / p.least;
 	if (pairs < cu_count()) p.parts = std::min(p.parts, (int)(((prefix_len ? slots / 2 : slots) + pairs - 1) / pairs));
 	p.parts = std::max(1, p.parts);
 	// the prefix: parts of at least a step for each wave, until its tiles fill what the own keys leave, at least half the
-	// chip (all of it / this: 48 sequences over 6000 positions 28.8 / 27.4 us, 8 over 16000 22.0 / 19.6, 32 of 3B heads
-	// over 3000 20.8 / 15.3, 128 over 4000 37.7 / 38.9)
+	// chip (all of it / this: 48 sequences over 6000 positions 27.8 / 27.2 us, 8 over 16000 22.2 / 19.0, 32 of 3B heads
+	// over 3000 20.0 / 15.3, 128 over 4000 42.4 / 39.3)
 	p.tiles = ((int64_t)n_seq * (H / kvh) + 31) / 32;
 	const int nc = (prefix_len + 31) / 32;
 	p.unit = 1;
@@ -1782,17 +1785,27 @@ int64_t all_steps(const AttnKv &c, const SeqTab &t, int tokens) {
 	return n * c.kvh;
 }
 
-// Which kernel (7B heads, one MI355X, direct / tiled): 200 tokens 9 / 20 us,
-// 512 14 / 31, 512 at position 3000 (52 thousand wave-steps of 32 rows x 32
-// keys) 71 / 73, 2000 tokens (63 thousand) 98 / 86, 8192 tokens 1601 / 870.
-// So the direct one up to 55 wave-steps for each SIMD.
+// Which kernel (one MI355X, heads of 128, us by the direct / the tiled one):
+//   tokens        wave-steps (32 rows x 32 keys)   8 bits        16 bits
+//   7B heads  200       0.8 thousand               9.3 / 20.5    9.9 / 20.5
+//            1000      16.5                       33.6 / 41.2   37.5 / 41.2
+//             512 at 3000   52                    70.6 / 72.8   79.6 / 73.6
+//            2000      64                         92.0 / 87.2    109 / 88.5
+//            3000     143                          187 / 153     221 / 156
+//   3B heads 2000      32                         52.7 / 59.9   58.6 / 60.4
+//            3000      71                         98.7 / 103     116 / 105
+//             512 at 3000   26                    59.8 / 51.4   73.0 / 51.7
+// So the direct one up to 55 wave-steps for each SIMD. (One query group of 16
+// goes as 3B heads, heads of 64 cross at about the same work. Some hundred
+// tokens far on in a slot of few heads are better off with the tiled one, the
+// last row; the rule does not see that.)
 //
 // Parts: the tiled kernel splits tiles of more than 1.5 times an equal share
-// of the work (1, 1.5, 2 times: packed prompts of 4096 tokens 104 / 98 / 109
-// us, 2 x 1500 tokens 99 / 84 / 85: a part costs its record's way to memory and
+// of the work (1, 1.5, 2 times: packed prompts of 4097 tokens 109 / 100 / 106
+// us, 2 x 1500 tokens 98 / 83 / 83: a part costs its record's way to memory and
 // back); the direct one tiles of more than a share where they are too few for
-// the chip (64 tokens at position 8000: 35 us, 40 at two shares), else of more
-// than two (512 at 3000: 73, 90 at one).
+// the chip (64 tokens at position 8000: 34 us, 37 at two shares), else of more
+// than two (512 at 3000: 70, 115 at one).
 template <int HD, bool Q8>
 int prompt(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, const float *q, int64_t ldq, int H, float scale) {
 	const int G = H / c.kvh;

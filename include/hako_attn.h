@@ -16,7 +16,11 @@
  * hako_gpu_last_error() set, work enqueued on the library stream, device
  * pointers unless a comment says host. The attention calls use a library
  * workspace (see hako_gpu_capture_begin): make one call of a shape before
- * capturing it. Calls are made from one thread at a time.
+ * capturing it. It follows the cache's max_seq, not the lengths: for n_seq
+ * sequences of single tokens up to n_seq * n_heads * (max_seq / 2048 + 1)
+ * records of (head_dim + 3) * 4 bytes where n_seq * n_kv_heads fills the chip
+ * (64 sequences of 28 heads of 128 in slots of 32768: 15 MB; 1024 in slots of
+ * 131072: 1 GB), else a few MB. Calls are made from one thread at a time.
  */
 #pragma once
 #include <stddef.h>
