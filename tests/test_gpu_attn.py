@@ -665,3 +665,59 @@ def test_refused_calls_say_why(gpu):
     with pytest.raises(HakoGpuError, match="positions"):
         gpu.attn_prompt(c.bufs[0], 64, c.bufs[1], 64, c.kv, None, np.array([60], np.int32), np.array([5], np.int32), 1, 1, 1.0)
     c.free()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_two_graphs_and_a_growing_workspace(gpu, kind):
+    """A captured call, a call that needs a larger workspace, a second captured one, and replays of both in turn, with eager
+    calls and a read-back captured too: each answers as the eager call on the same inputs."""
+    rng = np.random.default_rng(70)
+    small = ref.Cache(gpu, kind, 3, 900, 2, 64, rng)
+    large = ref.Cache(gpu, kind, 1, 131072 if kind == KV_Q8 else 140000, 4, 64, fill=0)
+    n, H, m = 3, 8, 128
+    lens = [900, 333, 1]
+    dq, do, dl = gpu.alloc(4 * n * H * 64), gpu.alloc(4 * n * H * 64), i32(gpu, lens)
+    ds, dp, dk = i32(gpu, [0, 1, 2]), i32(gpu, [5, 332, 0]), gpu.alloc(4 * n * 2 * 64)
+    bq, bo, bl, bs = gpu.upload(rng.standard_normal((m, 64, 64)).astype(np.float32)), gpu.alloc(4 * m * 64 * 64), i32(gpu, [40] * m), i32(gpu, [0] * m)
+    q = rng.standard_normal((n, H, 64)).astype(np.float32)
+
+    def one():
+        gpu.attn_decode(do, H * 64, dq, H * 64, small.kv, None, dl, n, H, 0.125)
+
+    def two():
+        gpu.attn_decode(do, H * 64, dq, H * 64, small.kv, None, dl, n, H, 0.125, 2, 100)
+        gpu.kv_read(small.kv, ds, dp, n, dk, None, 2 * 64)
+
+    def captured(call):
+        call()
+        gpu.capture_begin()
+        call()
+        return gpu.capture_end()
+
+    def of(x):
+        return gpu.download(x, np.float32, (n, H if x is do else 2, 64))
+
+    gpu.h2d(dq, q)
+    first = captured(one)
+    gpu.attn_decode(bo, 64 * 64, bq, 64 * 64, large.kv, bs, bl, m, 64, 0.125)   # 64 records a head
+    second = captured(two)
+    for r in range(3):
+        q = rng.standard_normal((n, H, 64)).astype(np.float32)
+        gpu.h2d(dq, q)
+        gpu.graph_launch(first)
+        got = of(do)
+        close(got, want_decode(small, q, None, lens, 0.125))
+        gpu.graph_launch(second)
+        got2, rows = of(do), of(dk)
+        close(got2, want_decode(small, q, None, lens, 0.125, 2, 100))
+        np.testing.assert_array_equal(rows, np.stack([small.k[s, :, p].astype(np.float32) * small.ks[s, :, p, None] for s, p in ((0, 5), (1, 332), (2, 0))]))
+        one()
+        np.testing.assert_array_equal(of(do), got)
+        two()
+        np.testing.assert_array_equal(of(do), got2)
+    for g in (first, second):
+        gpu.graph_destroy(g)
+    for b in (dq, do, dl, ds, dp, dk, bq, bo, bl, bs):
+        b.free()
+    small.free()
+    large.free()

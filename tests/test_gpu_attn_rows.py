@@ -129,3 +129,56 @@ def test_rows_that_see_nothing(gpu, kind):
         assert (want[[1, 2, 3, 5]] == 0).all() and (want[[0, 4]] != 0).any((1, 2)).all()
         assert off(run_decode(gpu, c, q, slot, lens, 0.09, ps, pl, pad=4, in_place=in_place), want) < TOL
     c.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+def test_queries_that_are_not_finite(gpu, prompt_kernel, kind):   # noqa: F811
+    """A query head with a NaN or an infinity answers NaN; the other heads and tokens do not move by a bit."""
+    rng = np.random.default_rng(8)
+    c = ref.Cache(gpu, kind, 3, 900, 2, 128, rng)
+    q = rng.standard_normal((150, 8, 128)).astype(np.float32)
+    bad = [(0, 0, np.nan), (1, 3, np.inf), (2, 7, -np.inf), (100, 5, np.nan), (149, 0, np.inf)]
+    hurt = q.copy()
+    for t, h, x in bad:
+        hurt[t, h, (t + h) % 128] = x
+    where = np.zeros(q.shape[:2], bool)
+    for t, h, _ in bad:
+        where[t, h] = True
+
+    def check(first, got):
+        assert np.isnan(got[where[:len(got)]]).all()
+        np.testing.assert_array_equal(got[~where[:len(got)]], first[~where[:len(got)]])
+        assert np.isfinite(first).all()
+
+    for ps, pl in ((0, 0), (2, 300)):
+        check(*(run_prompt(gpu, c, x, None, [0, 700], [70, 80], 0.09, ps, pl) for x in (q, hurt)))
+        check(*(run_decode(gpu, c, x[:3], None, [900, 400, 30], 0.09, ps, pl) for x in (q, hurt)))
+    c.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("scale", [-0.09, 0.0])
+def test_scales(gpu, prompt_kernel, kind, scale):   # noqa: F811
+    """A negative scale, and 0: the mean of the values seen."""
+    rng = np.random.default_rng(9)
+    c = ref.Cache(gpu, kind, 2, 500, 2, 64, rng)
+    q = rng.standard_normal((130, 6, 64)).astype(np.float32)
+    assert off(run_prompt(gpu, c, q, None, [0, 440], [70, 60], scale), want_prompt(c, q, None, [0, 440], [70, 60], scale)) < TOL
+    assert off(run_decode(gpu, c, q[:2], None, [500, 3], scale), want_decode(c, q[:2], None, [500, 3], scale)) < TOL
+    c.free()
+
+
+@pytest.mark.gpu
+def test_many_prompts_in_place(gpu, prompt_kernel):   # noqa: F811
+    """More sequences than a launch takes, in place, over a prefix: a launch does not touch the rows of the others."""
+    rng = np.random.default_rng(10)
+    n = 130
+    c = ref.Cache(gpu, KV_F16, 11, 400, 1, 64, rng)
+    lens, start = [1 + (i * 7) % 23 for i in range(n)], [(i * 31) % 370 for i in range(n)]
+    slot = [i % 10 for i in range(n)]
+    q = rng.standard_normal((sum(lens), 4, 64)).astype(np.float32)
+    want = want_prompt(c, q, slot, start, lens, 0.125, 10, 150)
+    assert off(run_prompt(gpu, c, q, slot, start, lens, 0.125, 10, 150, pad=4, in_place=True), want) < TOL
+    c.free()

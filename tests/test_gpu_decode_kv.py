@@ -305,3 +305,41 @@ def test_captured_steps_follow_the_prefix(gpu, tmp_path, kind, cfg):
         assert (fed(dec, len(prefix), turns) != shared[0]).any((1, 2, 3)).all()
     finally:
         dec.close()
+
+
+class Model(C.Structure):
+    """hakm_model (include/hako_mlf2.h)."""
+    _fields_ = [("h", C.c_char * 128), ("tensors", C.c_void_p), ("data", C.c_void_p), ("tok", C.c_void_p), ("map", C.c_void_p),
+                ("map_size", C.c_size_t)]
+
+
+@pytest.mark.parametrize("kind", [0, KV_Q8, KV_F16])
+def test_decoder_from_a_mapped_model(gpu, tmp_path, kind):
+    """hako_decoder_from_model_kv over a model in host memory: the decoder of the same file and cache type, bit for bit."""
+    from dropin import host_lib
+    path = str(tmp_path / "m.mlf2")
+    mlf2.write_qwen2(path, SMALL_128, 13)
+    prompt, tok = np.random.default_rng(1).integers(0, SMALL_128.vocab, 40).astype(np.int32), np.array([5], np.int32)
+    dec = Decoder(gpu, path, 1, 64, kind)
+    try:
+        dec.prefill(prompt, 0)
+        want = dec.step(tok, logits=True)[1]
+    finally:
+        dec.close()
+    image = np.fromfile(path, np.uint8)
+    at = {n: int(np.frombuffer(image[o:o + 8].tobytes(), np.uint64)[0]) for n, o in (("tensors", 60), ("tok", 68), ("data", 76))}
+    m = Model(image[:128].tobytes(), *(image.ctypes.data + at[n] for n in ("tensors", "data", "tok")), image.ctypes.data, image.nbytes)
+    C.memmove(C.byref(m), image.ctypes.data, 128)   # (a char array field stops at a 0)
+    host, lib, d = host_lib(), gpu.lib, C.c_void_p()
+    host.hako_decoder_from_model_kv.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_void_p)]
+    assert host.hako_decoder_from_model_kv(C.byref(m), 1, 64, 9, C.byref(d)) == -6 and not d.value
+    assert host.hako_decoder_from_model_kv(C.byref(m), 1, 64, kind, C.byref(d)) == 0
+    try:
+        assert host.hako_model_release(C.byref(m)) != 0   # its weights are in use
+        lg = np.empty((1, SMALL_128.vocab), np.float32)
+        assert lib.hako_gpu_decoder_prefill(d, 0, prompt.ctypes.data, len(prompt), None, None) == 0
+        assert lib.hako_gpu_decoder_step(d, tok.ctypes.data, lg.ctypes.data, None) == 0
+        np.testing.assert_array_equal(lg, want)
+    finally:
+        assert lib.hako_gpu_decoder_destroy(d) == 0
+        assert host.hako_model_release(C.byref(m)) == 0
