@@ -132,7 +132,7 @@ def bounded(c, q, slot, end, scale):
 
 
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("size", SIZES, ids=str)
+@pytest.mark.parametrize("size", SIZES + [(77, 77), (77, -77), (-77, 77), (-77, -77)], ids=str)   # (N(0, 1) to the ends of the range)
 def test_random_keys(gpu, prompt_kernel, kind, size):   # noqa: F811
     rng = np.random.default_rng(size[0] + 77)
     c = ref.Cache(gpu, kind, 3, 700, 2, 128, rng)
