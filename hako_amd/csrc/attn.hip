@@ -64,6 +64,7 @@ struct AttnKv {
 	int n_slots, max_seq, kvh;
 	int prefix_slot, prefix_len;
 	int len_add;   // added to every length (single tokens)
+	int window, sinks;   // a token's last positions and the first ones that stay (window 0: it sees every one before it)
 };
 
 // A prompt launch: sequence s has len[s] tokens from row row[s] of q and
@@ -76,6 +77,64 @@ struct SeqTab {
 	int row[kSeqs], len[kSeqs], slot[kSeqs], start[kSeqs], item[kSeqs + 1], nsplit[kSeqs];
 	int join[kSeqs + 1];
 	uint32_t rec[kSeqs];        // first record of a sequence's split tokens
+};
+
+// Positions that a tile of tokens looks at, in steps of K: those of [0, pend)
+// of row r0's slot and head, n0 steps, then those of [b0, end) of r1's.
+struct Span {
+	size_t r0, r1;
+	int pend, n0, b0, end;
+	__device__ __forceinline__ bool first(int step) const { return step < n0; }
+	template <int K>
+	__device__ __forceinline__ int key(int step) const { return step < n0 ? K * step : b0 + K * (step - n0); }
+	// positions from here on are not the step's
+	__device__ __forceinline__ int top(int step) const { return step < n0 ? pend : end; }
+};
+
+// Which keys of a step a row sees: at(k, ..) turns to those from key k on,
+// sees(i) tells of the i-th of them. lim: the row sees keys below it.
+// Every one:
+struct Below {
+	static constexpr bool kHi = false, kBlanks = false;
+	int lim;
+	__device__ __forceinline__ void at(int k, int top, bool) { lim = min(lim, top) - k; }
+	__device__ __forceinline__ bool sees(int i) const { return i < lim; }
+	// whether keys before k are of use to rows of the least lim lo (those from k on may be)
+	__device__ __forceinline__ bool reaches(int, bool, int) const { return true; }
+	// whether a step of K keys at k needs the mask; lo, hi: the least and greatest lim of the rows
+	template <int K>
+	__device__ __forceinline__ bool masks(int k, int top, bool, int lo, int) const { return k + K > min(lo, top); }
+};
+// The last `window`, and in a span's first steps every one:
+struct Within {
+	static constexpr bool kHi = true, kBlanks = false;
+	int lim, window, from;
+	__device__ __forceinline__ void at(int k, int top, bool first) {
+		from = first ? 0 : lim - window - k;
+		lim = min(lim, top) - k;
+	}
+	__device__ __forceinline__ bool sees(int i) const { return i < lim && i >= from; }
+	__device__ __forceinline__ bool reaches(int k, bool first, int lo) const { return first || k > lo - window; }
+	template <int K>
+	__device__ __forceinline__ bool masks(int k, int top, bool first, int lo, int hi) const {
+		return k + K > min(lo, top) || (!first && k < hi - window);
+	}
+};
+// Those below lim, and of the 64 from there on those of its bits:
+struct Nodes {
+	static constexpr bool kHi = false, kBlanks = true;
+	int lim;
+	uint64_t bits;
+	uint32_t w;
+	__device__ __forceinline__ void at(int k, int top, bool) {
+		const int s = k - lim, n = top - k;
+		if (s >= 0) w = s < 64 ? (uint32_t)(bits >> s) : 0;
+		else w = s > -32 ? (uint32_t)(bits << -s) | ((1u << -s) - 1) : ~0u;
+		w = n >= 32 ? w : n > 0 ? w & ((1u << n) - 1) : 0;
+	}
+	__device__ __forceinline__ bool sees(int i) const { return w >> i & 1; }
+	template <int K>
+	__device__ __forceinline__ bool masks(int k, int top, bool, int lo, int) const { return k + K > min(lo, top); }
 };
 
 // The same value, made anew where this stands: addresses and masks that
@@ -374,10 +433,11 @@ struct Tile {
 		big = 0;
 	}
 
-	// The 64 keys of the chunk in LDS buffer `b`, the first at position key0; mask: some row of the wave does not see
-	// all of them. (Two instances of this, with and without the mask, cost a second set of the value sums' registers.)
+	// The 64 keys of the chunk in LDS buffer `b`; mask: some row of the wave does not see all of them, see (at the lane
+	// half's first key) tells which. (Two instances of this, with and without the mask, cost a second set of the value sums' registers.)
 	// The weights of the second 32 keys form while the matrix cores add up the values of the first.
-	__device__ __forceinline__ void chunk(Lds &s, int b, int key0, bool mask, int lim, int lane) {
+	template <class See>
+	__device__ __forceinline__ void chunk(Lds &s, int b, bool mask, const See &see, int lane) {
 		lane = fresh(lane);
 		const int h = lane >> 5, i = lane & 31;
 		const uint8_t *kr = s.k[b] + i * kKeyRow<HD> + 16 * h;
@@ -406,7 +466,6 @@ struct Tile {
 			}
 		float e = s.e[b];
 		if (mask) {
-			const int n = lim - key0 - 8 * h;
 			float vm = 0.0f;
 #pragma unroll
 			for (int t = 0; t < 2; t++)
@@ -416,7 +475,7 @@ struct Tile {
 					const float vv[4] = {vs.x, vs.y, vs.z, vs.w};
 #pragma unroll
 					for (int j = 0; j < 4; j++) {
-						const bool sees = 32 * t + 16 * (g >> 1) + 4 * (g & 1) + j < n;
+						const bool sees = see.sees(32 * t + 16 * (g >> 1) + 4 * (g & 1) + j);
 						sc[t][4 * g + j] = sees ? sc[t][4 * g + j] : -INFINITY;
 						vm = __builtin_fmaxf(vm, sees ? __builtin_fabsf(vv[j]) : 0.0f);
 					}
@@ -501,23 +560,18 @@ struct Tile {
 		}
 	}
 
-	// Chunks [c0, c1) of a tile that sees positions below `end`: first the prefix's, then the slot's own from
-	// prefix_len on. lo, hi: the least and greatest lim of the wave's rows.
-	__device__ __forceinline__ void chunks(const AttnKv &c, int kvh, int slot, int end, int c0, int c1, int lim, int lo,
-	                                       int hi, Lds &s, int tid) {
+	// Chunks [c0, c1) of a tile's span. lo, hi: the least and greatest lim of the wave's rows.
+	template <class See>
+	__device__ __forceinline__ void chunks(const AttnKv &c, const Span &sp, int c0, int c1, const See &row, int lo, int hi, Lds &s,
+	                                       int tid) {
 		constexpr int EB = Q8 ? 1 : 2;
 		const int lane = tid & 63;
-		const int pend = min(c.prefix_len, end), nc1 = (pend + kKeys - 1) / kKeys;
-		auto base = [&](int sl) { return ((size_t)sl * c.kvh + kvh) * c.max_seq; };
-		const size_t b0 = base(c.prefix_len > 0 ? c.prefix_slot : slot), b1 = base(slot);
 		Stage<HD, Q8> st;
 		auto load = [&](int ch) {
-			const bool pre = ch < nc1;
-			const size_t r = pre ? b0 : b1;
-			const uint32_t n = (uint32_t)(pre ? pend : end);   // rows past it read as zeros
+			const size_t r = sp.first(ch) ? sp.r0 : sp.r1;
+			const uint32_t n = (uint32_t)sp.top(ch);   // rows past it read as zeros
 			st.load(stream_rsrc(uniform_ptr(c.k + r * HD * EB), n * HD * EB), stream_rsrc(uniform_ptr(c.v + r * HD * EB), n * HD * EB),
-			        stream_rsrc(uniform_ptr(c.ks + r), n * 4), stream_rsrc(uniform_ptr(c.vs + r), n * 4),
-			        pre ? kKeys * ch : c.prefix_len + kKeys * (ch - nc1), fresh(tid));
+			        stream_rsrc(uniform_ptr(c.ks + r), n * 4), stream_rsrc(uniform_ptr(c.vs + r), n * 4), sp.key<kKeys>(ch), fresh(tid));
 		};
 		// A wave's registers hold the codes two chunks on from the buffer that is read. The waves of a SIMD (w, w + 4)
 		// put them into LDS at opposite ends of a chunk, so that one has vector work while the other has matrix work.
@@ -536,12 +590,13 @@ struct Tile {
 				__builtin_amdgcn_sched_barrier(0);
 			};
 			if (early) stage();
-			const bool pre = ch < nc1;
-			const int key0 = pre ? kKeys * ch : c.prefix_len + kKeys * (ch - nc1);
-			// rows see keys below min(lim, what the chunk holds)
-			const int top = pre ? pend : end;
-			if (key0 < min(hi, top))   // some row of the wave sees some of these keys
-				chunk(s, b, key0, key0 + kKeys > min(lo, top), min(lim, top), lane);
+			const bool first = sp.first(ch);
+			const int key0 = sp.key<kKeys>(ch), top = sp.top(ch);
+			if (key0 < min(hi, top) && row.reaches(key0 + kKeys, first, lo)) {   // some row of the wave sees some of these keys
+				See see = row;
+				see.at(key0 + 8 * (fresh(lane) >> 5), top, first);
+				chunk(s, b, row.template masks<kKeys>(key0, top, first, lo, hi), see, lane);
+			}
 			if (!early) stage();
 			__syncthreads();
 		}
@@ -578,6 +633,37 @@ __host__ __device__ __forceinline__ int tile_steps(int end, int prefix) {
 	return (p + K - 1) / K + (end - p + K - 1) / K;
 }
 
+// What a launch's tokens see.
+struct Reach {
+	int prefix, window, sinks;
+};
+// Steps of a tile of `tokens` tokens from position `first` (as if it were full: the steps of a sequence's tiles then never
+// fall), the last of them at end - 1. With a window whose last token leaves some positions past the sinks behind these are
+// the sinks' and those from the first token's window on; else all before it.
+__host__ __device__ __forceinline__ bool two_spans(const Reach &r, int first, int tokens) { return first + tokens - r.window > r.sinks; }
+__host__ __device__ __forceinline__ int span_start(const Reach &r, int first) {
+	return first - r.window + 1 > r.sinks ? first - r.window + 1 : r.sinks;
+}
+template <int K, bool WIN>
+__host__ __device__ __forceinline__ int reach_steps(const Reach &r, int first, int tokens, int end) {
+	if (!WIN) return tile_steps<K>(end, r.prefix);
+	const int e = first + tokens;
+	if (!two_spans(r, first, tokens)) return (e + K - 1) / K;
+	return (r.sinks + K - 1) / K + (e - span_start(r, first) + K - 1) / K;
+}
+template <int K, bool WIN>
+__device__ __forceinline__ Span span_of(const AttnKv &c, int kvh, int slot, int first, int tokens, int end) {
+	auto base = [&](int sl) { return ((size_t)sl * c.kvh + kvh) * c.max_seq; };
+	if (!WIN) {
+		const int pend = min(c.prefix_len, end);
+		return {base(c.prefix_len > 0 ? c.prefix_slot : slot), base(slot), pend, (pend + K - 1) / K, c.prefix_len, end};
+	}
+	const Reach r = {0, c.window, c.sinks};
+	const bool two = two_spans(r, first, tokens);
+	const int s = two ? c.sinks : first + tokens;   // what every token sees of what comes before it
+	return {base(slot), base(slot), min(s, end), (s + K - 1) / K, two ? span_start(r, first) : end, end};
+}
+
 // The items of a launch, the longest first: sequence << 26 | tile << 8 | part.
 // Without (n 0) they go by sequence, tile and part.
 struct ItemTab {
@@ -590,8 +676,8 @@ struct ItemTab {
 struct Item {
 	int sq, slot, tok0, ntok, end, part, parts, c0, c1;
 };
-template <int K>
-__device__ __forceinline__ bool item_of(const SeqTab &t, const ItemTab *order, int item, int prefix_len, Item &x) {
+template <int K, bool WIN>
+__device__ __forceinline__ bool item_of(const SeqTab &t, const ItemTab *order, int item, const Reach &reach, Item &x) {
 	int tile;
 	if (order && order->n) {
 		const uint32_t v = order->item[item];
@@ -609,7 +695,7 @@ __device__ __forceinline__ bool item_of(const SeqTab &t, const ItemTab *order, i
 	x.tok0 = tile * t.tile_tokens;
 	x.ntok = min(t.tile_tokens, t.len[x.sq] - x.tok0);
 	x.end = t.start[x.sq] + x.tok0 + x.ntok;
-	const int nc = tile_steps<K>(x.end, prefix_len);
+	const int nc = reach_steps<K, WIN>(reach, t.start[x.sq] + x.tok0, t.tile_tokens, x.end);
 	x.parts = (nc + t.unit - 1) / t.unit;
 	const int per = (nc + x.parts - 1) / x.parts;
 	x.c0 = x.part * per;
@@ -763,8 +849,8 @@ struct Direct {
 		return e;
 	}
 
-	__device__ __forceinline__ void weigh(f16v &sc, float *sx, float e, int key0, bool mask, int lim, int lane, h8 ph[2],
-	                                      h8 pl[2]) {
+	template <class See>
+	__device__ __forceinline__ void weigh(f16v &sc, float *sx, float e, bool mask, const See &see, int lane, h8 ph[2], h8 pl[2]) {
 		const int h = lane >> 5;
 		float mx = -INFINITY;
 #pragma unroll
@@ -775,7 +861,6 @@ struct Direct {
 			for (int j = 0; j < 4; j++) sc[4 * g + j] *= kv[j];
 		}
 		if (mask) {
-			const int n = lim - key0 - 8 * h;
 			float vm = 0.0f;
 #pragma unroll
 			for (int g = 0; g < 4; g++) {
@@ -783,7 +868,7 @@ struct Direct {
 				const float vv[4] = {vs.x, vs.y, vs.z, vs.w};
 #pragma unroll
 				for (int j = 0; j < 4; j++) {
-					const bool sees = 16 * (g >> 1) + 4 * (g & 1) + j < n;
+					const bool sees = see.sees(16 * (g >> 1) + 4 * (g & 1) + j);
 					sc[4 * g + j] = sees ? sc[4 * g + j] : -INFINITY;
 					vm = __builtin_fmaxf(vm, sees ? __builtin_fabsf(vv[j]) : 0.0f);
 				}
@@ -913,28 +998,26 @@ struct Dest {
 	__device__ __forceinline__ Dest(const Records &r, size_t f, int H, int nrec) : o(nullptr), ot(0), og(0), rec(r), first(f), rt((int64_t)H * nrec), rg(nrec) {}
 };
 
-// 32 rows over steps [c0, c1) of their tile's keys. A lane's row: q (null: an idle row) and lim, tok << 4 | g its token
-// and head. (Places come from those two numbers after the steps: pointers held across them cost registers.)
-template <int HD, bool Q8>
-__device__ __forceinline__ void direct_rows(const AttnKv &c, DirectLds<HD> &s, int kvh, int slot, int end, int c0, int c1,
-                                            const float *q, float scale, int lim, int tok_g, const Dest &dest) {
+// 32 rows over steps [c0, c1) of their tile's span. A lane's row: q (null: an idle row) and what it sees, tok << 4 | g its
+// token and head (with kBlank: a row that sees nothing, whatever `row` says). (Places come from those two numbers after the
+// steps: pointers held across them cost registers.)
+constexpr int kBlank = 1 << 30;
+template <int HD, bool Q8, class See>
+__device__ __forceinline__ void direct_rows(const AttnKv &c, DirectLds<HD> &s, const Span &sp, int c0, int c1, const float *q,
+                                            float scale, const See &seen, int tok_g, const Dest &dest) {
 	constexpr int EB = Q8 ? 1 : 2;
 	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-	const int pend = min(c.prefix_len, end), nc1 = (pend + 31) / 32;
-	auto base = [&](int sl) { return ((size_t)sl * c.kvh + kvh) * c.max_seq; };
-	const size_t b0 = base(c.prefix_len > 0 ? c.prefix_slot : slot), b1 = base(slot);
 	Direct<HD, Q8> w;
-	auto first_key = [&](int ch) { return ch < nc1 ? 32 * ch : c.prefix_len + 32 * (ch - nc1); };
 	auto load_k = [&](int ch) {
-		const size_t r = ch < nc1 ? b0 : b1;
-		const uint32_t n = (uint32_t)(ch < nc1 ? pend : end);   // rows past it read as zeros
+		const size_t r = sp.first(ch) ? sp.r0 : sp.r1;
+		const uint32_t n = (uint32_t)sp.top(ch);   // rows past it read as zeros
 		w.load_k(stream_rsrc(uniform_ptr(c.k + r * HD * EB), n * HD * EB), stream_rsrc(uniform_ptr(c.ks + r), n * 4),
-		         stream_rsrc(uniform_ptr(c.vs + r), n * 4), first_key(ch), fresh(lane));
+		         stream_rsrc(uniform_ptr(c.vs + r), n * 4), sp.key<32>(ch), fresh(lane));
 	};
 	auto load_v = [&](int ch) {
-		const size_t r = ch < nc1 ? b0 : b1;
-		const uint32_t n = (uint32_t)(ch < nc1 ? pend : end);
-		w.load_v(stream_rsrc(uniform_ptr(c.v + r * HD * EB), n * HD * EB), first_key(ch), fresh(lane));
+		const size_t r = sp.first(ch) ? sp.r0 : sp.r1;
+		const uint32_t n = (uint32_t)sp.top(ch);
+		w.load_v(stream_rsrc(uniform_ptr(c.v + r * HD * EB), n * HD * EB), sp.key<32>(ch), fresh(lane));
 	};
 	int ch = c0 + wave;
 	if (ch < c1) {
@@ -949,17 +1032,19 @@ __device__ __forceinline__ void direct_rows(const AttnKv &c, DirectLds<HD> &s, i
 		return (uint64_t)(uint32_t)__shfl((int)(uint32_t)x, row) | ((uint64_t)(uint32_t)__shfl((int)(x >> 32), row) << 32);
 	};
 	w.query((const float *)(uintptr_t)from(q), scale, (uint8_t *)s.o, s.keep, s.sx[0], tid);
-	const int lo = wave_min_i(tok_g >= 0 ? lim : 0x7FFFFFFF);
+	const int lo = wave_min_i(tok_g >= 0 ? seen.lim : 0x7FFFFFFF), hi = seen.kHi ? wave_max_i(seen.lim) : 0;
 	float *sx = s.sx[wave];
 	for (; ch < c1; ch += kWaves) {
-		const int key0 = first_key(ch), top = ch < nc1 ? pend : end;
+		const int key0 = sp.key<32>(ch), top = sp.top(ch);
 		f16v sc;
 		h8 ph[2], pl[2];
 		w.scores(sc, s.keep, fresh(lane));
 		const float e = w.scales(sx, lane);
 		if (ch + kWaves < c1) load_k(ch + kWaves);
 		__builtin_amdgcn_sched_barrier(0);
-		w.weigh(sc, sx, e, key0, key0 + 32 > min(lo, top), min(lim, top), fresh(lane), ph, pl);
+		See see = seen;
+		see.at(key0 + 8 * (fresh(lane) >> 5), top, sp.first(ch));
+		w.weigh(sc, sx, e, seen.template masks<32>(key0, top, sp.first(ch), lo, hi), see, fresh(lane), ph, pl);
 		w.values(ph, pl);
 		if (ch + kWaves < c1) load_v(ch + kWaves);
 		__builtin_amdgcn_sched_barrier(0);
@@ -979,11 +1064,17 @@ __device__ __forceinline__ void direct_rows(const AttnKv &c, DirectLds<HD> &s, i
 	__syncthreads();
 	const int tg = __shfl(tok_g, out);
 	if (tg < 0) return;
-	const size_t r = dest.first + (tg >> 4) * dest.rt + (tg & 15) * dest.rg;
-	float *to = dest.o ? dest.o + (tg >> 4) * dest.ot + (tg & 15) * dest.og : dest.rec.o + r * HD;
+	const bool blank = seen.kBlanks && tg & kBlank;
+	const int tok = (seen.kBlanks ? tg & ~kBlank : tg) >> 4;
+	const size_t r = dest.first + tok * dest.rt + (tg & 15) * dest.rg;
+	float *to = dest.o ? dest.o + tok * dest.ot + (tg & 15) * dest.og : dest.rec.o + r * HD;
 	int x[kWaves];
 	float ls;
-	const Base b = meet(s.ml, out, x, ls);
+	Base b = meet(s.ml, out, x, ls);
+	if (blank) {
+		b = {kNone, 0.0f};
+		ls = 0.0f;
+	}
 	const float z = !dest.o ? 1.0f : (ls == 0.0f ? 0.0f : 1.0f / ls);
 #pragma unroll
 	for (int d = 4 * (at & 7); d < HD; d += 32) {
@@ -996,19 +1087,27 @@ __device__ __forceinline__ void direct_rows(const AttnKv &c, DirectLds<HD> &s, i
 			a.z += __builtin_ldexpf(y.z, x[k]);
 			a.w += __builtin_ldexpf(y.w, x[k]);
 		}
+		if (blank) a = make_float4(0, 0, 0, 0);
 		*(float4 *)(to + d) = make_float4(a.x * z, a.y * z, a.z * z, a.w * z);
 	}
 	if (!dest.o && (at & 7) == 0) dest.rec.put(r, b, ls);
 }
 
-template <int HD, bool Q8>
+// What a prompt's row sees, lim its position and those before it.
+template <bool WIN>
+__device__ __forceinline__ auto row_sees(const AttnKv &c, int lim) {
+	if constexpr (WIN) return Within{lim, c.window, 0};
+	else return Below{lim};
+}
+
+template <int HD, bool Q8, bool WIN>
 __global__ __launch_bounds__(64 * kTileWaves, 2) void prompt_kernel(AttnKv c, SeqTab t, ItemTab order, float *out, int64_t ldo, const float *q,
                                                         int64_t ldq, int G, float scale, Records rec) {
 	__shared__ typename Tile<HD, Q8>::Lds s;
 	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
 	const int kvh = blockIdx.x % c.kvh;
 	Item x;
-	if (!item_of<kKeys>(t, &order, blockIdx.x / c.kvh, c.prefix_len, x)) return;
+	if (!item_of<kKeys, WIN>(t, &order, blockIdx.x / c.kvh, {c.prefix_len, c.window, c.sinks}, x)) return;
 	const int r = 32 * wave + (lane & 31), tok = r / G, head = kvh * G + r - tok * G;
 	const bool on = tok < x.ntok;
 	const int lim = on ? t.start[x.sq] + x.tok0 + tok + 1 : 0;
@@ -1016,7 +1115,8 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void prompt_kernel(AttnKv c, Se
 	const int64_t row = (int64_t)t.row[x.sq] + x.tok0 + tok;
 	Tile<HD, Q8> w;
 	w.query(on ? q + row * ldq + head * HD : nullptr, scale, lane);
-	w.chunks(c, kvh, x.slot, x.end, x.c0, x.c1, lim, lo, hi, s, tid);
+	w.chunks(c, span_of<kKeys, WIN>(c, kvh, x.slot, t.start[x.sq] + x.tok0, t.tile_tokens, x.end), x.c0, x.c1, row_sees<WIN>(c, lim), lo, hi,
+	         s, tid);
 	if (!on) return;
 	if (x.parts == 1) {
 		w.put(out + row * ldo + head * HD, 1.0f / w.l, lane);
@@ -1028,20 +1128,21 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void prompt_kernel(AttnKv c, Se
 }
 
 // The direct kernel's items: tiles of 32 rows, parts of `unit` steps of 32 keys.
-template <int HD, bool Q8>
+template <int HD, bool Q8, bool WIN>
 __global__ __launch_bounds__(64 * kWaves, 2) void prompt_direct_kernel(AttnKv c, SeqTab t, float *out, int64_t ldo, const float *q,
                                                                int64_t ldq, int G, float scale, Records rec) {
 	__shared__ DirectLds<HD> s;
 	const int lane = threadIdx.x & 63;
 	const int kvh = blockIdx.x % c.kvh;
 	Item x;
-	if (!item_of<32>(t, nullptr, blockIdx.x / c.kvh, c.prefix_len, x)) return;
+	if (!item_of<32, WIN>(t, nullptr, blockIdx.x / c.kvh, {c.prefix_len, c.window, c.sinks}, x)) return;
 	const int r = lane & 31, tok = r / G, g = r - tok * G;
 	const bool on = tok < x.ntok;
 	const int64_t row = (int64_t)t.row[x.sq] + x.tok0;
 	const int head = kvh * G, H = c.kvh * G;
-	direct_rows<HD, Q8>(c, s, kvh, x.slot, x.end, x.c0, x.c1, on ? q + (row + tok) * ldq + (head + g) * HD : nullptr, scale,
-	                    on ? t.start[x.sq] + x.tok0 + tok + 1 : 0, on ? tok << 4 | g : -1,
+	direct_rows<HD, Q8>(c, s, span_of<32, WIN>(c, kvh, x.slot, t.start[x.sq] + x.tok0, t.tile_tokens, x.end), x.c0, x.c1,
+	                    on ? q + (row + tok) * ldq + (head + g) * HD : nullptr, scale,
+	                    row_sees<WIN>(c, on ? t.start[x.sq] + x.tok0 + tok + 1 : 0), on ? tok << 4 | g : -1,
 	                    x.parts == 1 ? Dest(out + row * ldo + head * HD, ldo, HD)
 	                                 : Dest(rec, record_of(t, x, 0, H, head), H, t.nsplit[x.sq]));
 }
@@ -1299,6 +1400,19 @@ __device__ __forceinline__ int own_end(const AttnKv &c, const int *slot, const i
 	return sl < 0 || sl >= c.n_slots ? 0 : min(max(len[sq] + c.len_add, 0), c.max_seq);
 }
 
+// A sequence's own keys in the order that its parts take them: n of them, the first `sinks` (whole steps, if any) those
+// from position 0, then those from b0 on.
+struct Keys {
+	int n, sinks, b0;
+};
+template <bool WIN>
+__device__ __forceinline__ Keys own_keys(const AttnKv &c, int end) {
+	if (!WIN) return {max(end - c.prefix_len, 0), 0, c.prefix_len};
+	if (end - c.window <= c.sinks) return {end, 0, 0};
+	const int s = (c.sinks + 31) / 32 * 32;
+	return {s + c.window, s, end - c.window};
+}
+
 template <int HD>
 struct DecodeLds {
 	alignas(16) float o[kWaves][kMaxGroup][HD + 4];
@@ -1306,7 +1420,7 @@ struct DecodeLds {
 	float be[64 * kWaves];   // e of the rows' bases
 };
 
-template <int HD, bool Q8>
+template <int HD, bool Q8, bool WIN>
 __device__ __forceinline__ void decode_part(const AttnKv &c, DecodeLds<HD> &s, int kvh, int part, int sq, float *out, int64_t ldo,
                                             const float *q, int64_t ldq, const int *__restrict__ slot,
                                             const int *__restrict__ len, int G, float scale, int parts, int least, int rec0, int nrec,
@@ -1314,10 +1428,12 @@ __device__ __forceinline__ void decode_part(const AttnKv &c, DecodeLds<HD> &s, i
 	constexpr int EB = Q8 ? 1 : 2;
 	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 	int sl;
-	const int end = own_end(c, slot, len, sq, sl), n = max(end - c.prefix_len, 0);
-	const int per = part_keys(n, parts, least);
-	const int first = c.prefix_len + part * per, last = min(end, first + per);   // this part's keys
-	if (first >= end && (part > 0 || nrec > 0)) return;   // a record that the join does not read
+	const int end = own_end(c, slot, len, sq, sl);
+	const Keys own = own_keys<WIN>(c, end);
+	const int n = own.n, per = part_keys(n, parts, least);
+	const int k0 = part * per, k1 = min(n, k0 + per);   // this part's keys
+	if (k0 >= n && (part > 0 || nrec > 0)) return;   // a record that the join does not read
+	const int first = own.b0 + k0, last = WIN ? end : min(end, first + per);   // (with a window: positions in at())
 	const bool whole = nrec == 0 || (rec0 == 0 && n <= per);   // (the join leaves it alone)
 	const int i = lane & 15, g = lane >> 4;
 	const int head = kvh * G + i;
@@ -1325,19 +1441,26 @@ __device__ __forceinline__ void decode_part(const AttnKv &c, DecodeLds<HD> &s, i
 	Row16<HD, Q8> w;
 	const size_t r = ((size_t)(end > 0 ? sl : 0) * c.kvh + kvh) * c.max_seq;
 	const uint32_t rows = (uint32_t)max(last, 0);
-	const __amdgpu_buffer_rsrc_t kr = stream_rsrc(uniform_ptr(c.k + r * HD * EB), rows * HD * EB);
-	const __amdgpu_buffer_rsrc_t vr = stream_rsrc(uniform_ptr(c.v + r * HD * EB), rows * HD * EB);
-	const __amdgpu_buffer_rsrc_t ksr = stream_rsrc(uniform_ptr(c.ks + r), rows * 4);
-	const __amdgpu_buffer_rsrc_t vsr = stream_rsrc(uniform_ptr(c.vs + r), rows * 4);
+	auto kr = [&](uint32_t n) { return stream_rsrc(uniform_ptr(c.k + r * HD * EB), n * HD * EB); };
+	auto vr = [&](uint32_t n) { return stream_rsrc(uniform_ptr(c.v + r * HD * EB), n * HD * EB); };
+	auto ksr = [&](uint32_t n) { return stream_rsrc(uniform_ptr(c.ks + r), n * 4); };
+	auto vsr = [&](uint32_t n) { return stream_rsrc(uniform_ptr(c.vs + r), n * 4); };
 	// Codes on their way while others are used. 8 bits: two steps' in turn (64 sequences of 1000 positions 1.7 us less than
 	// the other way). Halves, whose two steps would take 254 registers: the keys' of the next step once this one's
 	// weights are formed, the values' after their products (32768 and 20011 positions 1.2 us less than in turn). (Keys from
 	// `last` on read as zeros, from nowhere.)
 	typename Row16<HD, Q8>::Codes ca, cb;
-	int key0 = first + 32 * wave;
+	// With a window key0 counts the part's keys in their order: at() is the position of the first of a step, top() that
+	// past its last (a step past the part reads from nowhere).
+	int key0 = WIN ? k0 + 32 * wave : first + 32 * wave;
+	const int stop = WIN ? k1 : last;
+	auto at = [&](int key) { return !WIN ? key : key >= k1 ? (int)rows : key < own.sinks ? key : own.b0 + (key - own.sinks); };
+	auto top = [&](int key) { return WIN && key < own.sinks ? c.sinks : (int)rows; };
+	auto load_k = [&](typename Row16<HD, Q8>::Codes &x, int key) { w.load_k(x, kr(top(key)), ksr(top(key)), at(key), lane); };
+	auto load_v = [&](typename Row16<HD, Q8>::Codes &x, int key) { w.load_v(x, vr(top(key)), vsr(top(key)), at(key), lane); };
 	auto load = [&](typename Row16<HD, Q8>::Codes &x, int key) {
-		w.load_k(x, kr, ksr, key, lane);
-		w.load_v(x, vr, vsr, key, lane);
+		load_k(x, key);
+		load_v(x, key);
 		__builtin_amdgcn_sched_barrier(0);
 	};
 	auto step = [&](typename Row16<HD, Q8>::Codes &x) {
@@ -1347,20 +1470,20 @@ __device__ __forceinline__ void decode_part(const AttnKv &c, DecodeLds<HD> &s, i
 		if (Q8) e = w.exponent(x);
 		w.scores(x, sc);
 		if (!Q8) e = w.exponent(x);
-		w.weigh(x, s.be, e, sc, key0, last, lane, ph, pl);
+		w.weigh(x, s.be, e, sc, at(key0), top(key0), lane, ph, pl);
 		key0 += 32 * kWaves;
-		if (!Q8) w.load_k(x, kr, ksr, key0, lane);
+		if (!Q8) load_k(x, key0);
 		w.values(x, ph, pl);
-		if (!Q8) w.load_v(x, vr, vsr, key0, lane);
+		if (!Q8) load_v(x, key0);
 		if (Q8) __builtin_amdgcn_sched_barrier(0);
 	};
 	load(ca, key0);
 	w.query(i < G ? q + sq * ldq + head * HD : nullptr, scale, lane);
-	while (key0 < last) {
+	while (key0 < stop) {
 		if (Q8) load(cb, key0 + 32 * kWaves);
 		step(ca);
 		if (!Q8) continue;
-		if (key0 >= last) break;
+		if (key0 >= stop) break;
 		load(ca, key0 + 32 * kWaves);
 		step(cb);
 	}
@@ -1401,14 +1524,14 @@ __device__ __forceinline__ void decode_part(const AttnKv &c, DecodeLds<HD> &s, i
 	}
 }
 
-template <int HD, bool Q8>
+template <int HD, bool Q8, bool WIN>
 __global__ __launch_bounds__(256) void decode_kernel(AttnKv c, float *out, int64_t ldo, const float *q, int64_t ldq,
                                                      const int *__restrict__ slot, const int *__restrict__ len, int n_seq, int G,
                                                      float scale, int parts, int least, int nrec, Records rec) {
 	__shared__ DecodeLds<HD> s;
 	int part, sq;
 	part_of(blockIdx.y, blockIdx.z, n_seq, least, part, sq);
-	decode_part<HD, Q8>(c, s, blockIdx.x, part, sq, out, ldo, q, ldq, slot, len, G, scale, parts, least, 0, nrec, rec);
+	decode_part<HD, Q8, WIN>(c, s, blockIdx.x, part, sq, out, ldo, q, ldq, slot, len, G, scale, parts, least, 0, nrec, rec);
 }
 
 // A batch with a prefix in one launch, so that the two kinds of work fill each
@@ -1431,7 +1554,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefix_kernel(AttnKv c, const 
 		b -= tiles * pparts;
 		int own, sq;
 		part_of_nth(b, n_seq, parts, least, own, sq);
-		decode_part<HD, Q8>(c, s.b, kvh, own, sq, nullptr, 0, q, ldq, slot, len, G, scale, parts, least, pparts, nrec, rec);
+		decode_part<HD, Q8, false>(c, s.b, kvh, own, sq, nullptr, 0, q, ldq, slot, len, G, scale, parts, least, pparts, nrec, rec);
 		return;
 	}
 	const int lane = threadIdx.x & 63, part = b / tiles;
@@ -1444,8 +1567,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefix_kernel(AttnKv c, const 
 		lim = min(own_end(c, slot, len, sq, sl), c.prefix_len);
 	}
 	const int nc = (c.prefix_len + 31) / 32;
-	direct_rows<HD, Q8>(c, s.a, kvh, c.prefix_slot, c.prefix_len, part * unit, min(nc, part * unit + unit),
-	                    on ? q + (int64_t)sq * ldq + (head + g) * HD : nullptr, scale, lim, on ? sq << 4 | g : -1,
+	direct_rows<HD, Q8>(c, s.a, span_of<32, false>(c, kvh, c.prefix_slot, 0, 0, c.prefix_len), part * unit, min(nc, part * unit + unit),
+	                    on ? q + (int64_t)sq * ldq + (head + g) * HD : nullptr, scale, Below{lim}, on ? sq << 4 | g : -1,
 	                    Dest(rec, (size_t)head * nrec + part, H, nrec));
 }
 
@@ -1543,41 +1666,23 @@ __device__ __forceinline__ void join(const float *__restrict__ ro, const float2 
 	}
 }
 
-template <int HD>
+template <int HD, bool WIN>
 __global__ __launch_bounds__(64 * kJoin) void decode_join_kernel(AttnKv c, float *out, int64_t ldo, const int *__restrict__ slot,
                                                          const int *__restrict__ len, int H, int parts, int least, int rec0,
                                                          int nrec, const float *__restrict__ rec_o, const float2 *__restrict__ rec_ml,
                                                          const float *__restrict__ rec_e) {
 	const int h = blockIdx.x, sq = blockIdx.y;
 	int sl;
-	const int end = own_end(c, slot, len, sq, sl), n = max(end - c.prefix_len, 0);
+	const int n = own_keys<WIN>(c, own_end(c, slot, len, sq, sl)).n;
 	const int per = part_keys(n, parts, least), used = n > 0 ? (n + per - 1) / per : 0;
 	if (rec0 == 0 && used == 1) return;   // written at once
 	const size_t rec = ((size_t)sq * H + h) * nrec;
 	join<HD>(rec_o + rec * HD, rec_ml + rec, rec_e + rec, rec0 + used, out + sq * ldo + h * HD);
 }
 
-// The tokens whose tiles were split (the last ones of each sequence), few
-// records each: HD/4 lanes to a query head, 1024/HD heads to a workgroup.
-template <int HD, int K>
-__global__ __launch_bounds__(256) void prompt_join_kernel(SeqTab t, int prefix_len, float *out, int64_t ldo, int H,
-                                                          const float *__restrict__ rec_o,
-                                                          const float2 *__restrict__ rec_ml,
-                                                          const float *__restrict__ rec_e) {
-	constexpr int L = HD / 4;
-	const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-	const int js = (int)(row / H), h = (int)(row - (int64_t)js * H), d = threadIdx.x % L * 4;
-	if (js >= t.join[t.n]) return;
-	int sq = 0;
-	while (js >= t.join[sq + 1]) sq++;
-	const int split = t.join[sq + 1] - t.join[sq];   // split tokens of the sequence
-	const int j = js - t.join[sq], tok = t.len[sq] - split + j;
-	const int tile = tok / t.tile_tokens, ns = t.nsplit[sq];
-	const int nc = tile_steps<K>(t.start[sq] + min((tile + 1) * t.tile_tokens, t.len[sq]), prefix_len);
-	const int n = (nc + t.unit - 1) / t.unit;
-	const size_t first = (size_t)t.rec[sq] + ((size_t)j * H + h) * ns;
-	const float2 *ml = rec_ml + first;
-	const float *ro = rec_o + first * HD + d, *re = rec_e + first;
+// n records, few, of one head joined for the four dims of ro.. (of each record HD floats).
+__device__ __forceinline__ void join_few(const float *__restrict__ ro, int HD, const float2 *__restrict__ ml, const float *__restrict__ re,
+                                         int n, float *dst) {
 	Base b = {kNone, 0.0f};
 	bool some = false;
 	for (int k = 0; k < n; k++) {
@@ -1603,8 +1708,31 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(SeqTab t, int prefix_l
 			add_record(a, ls, y, x.y, steps_down({x.x, 0.0f}, b));
 		}
 	}
-	const float z = 1.0f / ls;
-	*(float4 *)(out + ((int64_t)t.row[sq] + tok) * ldo + (int64_t)h * HD + d) = make_float4(a.x * z, a.y * z, a.z * z, a.w * z);
+	const float z = ls == 0.0f ? 0.0f : 1.0f / ls;
+	*(float4 *)dst = make_float4(a.x * z, a.y * z, a.z * z, a.w * z);
+}
+
+// The tokens whose tiles were split (the last ones of each sequence), few
+// records each: HD/4 lanes to a query head, 1024/HD heads to a workgroup.
+template <int HD, int K, bool WIN>
+__global__ __launch_bounds__(256) void prompt_join_kernel(SeqTab t, Reach reach, float *out, int64_t ldo, int H,
+                                                          const float *__restrict__ rec_o,
+                                                          const float2 *__restrict__ rec_ml,
+                                                          const float *__restrict__ rec_e) {
+	constexpr int L = HD / 4;
+	const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+	const int js = (int)(row / H), h = (int)(row - (int64_t)js * H), d = threadIdx.x % L * 4;
+	if (js >= t.join[t.n]) return;
+	int sq = 0;
+	while (js >= t.join[sq + 1]) sq++;
+	const int split = t.join[sq + 1] - t.join[sq];   // split tokens of the sequence
+	const int j = js - t.join[sq], tok = t.len[sq] - split + j;
+	const int tile = tok / t.tile_tokens, ns = t.nsplit[sq];
+	const int nc = reach_steps<K, WIN>(reach, t.start[sq] + tile * t.tile_tokens, t.tile_tokens,
+	                                   t.start[sq] + min((tile + 1) * t.tile_tokens, t.len[sq]));
+	const int n = (nc + t.unit - 1) / t.unit;
+	const size_t first = (size_t)t.rec[sq] + ((size_t)j * H + h) * ns;
+	join_few(rec_o + first * HD + d, HD, rec_ml + first, rec_e + first, n, out + ((int64_t)t.row[sq] + tok) * ldo + (int64_t)h * HD + d);
 }
 
 int attn_check(float *out, int64_t ldo, const float *q, int64_t ldq, const hako_gpu_kv *kv, int n_seq, int H,
@@ -1626,7 +1754,15 @@ int attn_check(float *out, int64_t ldo, const float *q, int64_t ldq, const hako_
 
 AttnKv attn_kv(const hako_gpu_kv *kv, int prefix_slot, int prefix_len, int len_add) {
 	return {(const uint8_t *)kv->k, (const uint8_t *)kv->v, kv->k_scale, kv->v_scale, kv->n_slots, kv->max_seq,
-	        kv->n_kv_heads, prefix_slot, prefix_len, len_add};
+	        kv->n_kv_heads, prefix_slot, prefix_len, len_add, 0, 0};
+}
+
+// (a window or sinks past the cache's end are all of it)
+AttnKv attn_kv_window(const hako_gpu_kv *kv, int len_add, int window, int sinks) {
+	AttnKv c = attn_kv(kv, 0, 0, len_add);
+	c.window = std::min(window, kv->max_seq);
+	c.sinks = std::min(sinks, kv->max_seq);
+	return c;
 }
 
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -1641,16 +1777,15 @@ int records(size_t n, int HD, Records *r) {
 	return HAKO_GPU_OK;
 }
 
-// How the single tokens of a batch are shared out: own keys in up to `parts`
+// How the single tokens of a batch are shared out: own keys (at most `own`) in up to `parts`
 // parts of `least` keys or more, the prefix (tiles of 32 rows) in pparts parts
 // of `unit` steps, nrec records to a query head (0: written at once).
 struct DecodePlan {
 	int64_t tiles;
 	int parts, least, pparts, unit, nrec;
 };
-DecodePlan decode_plan(int max_seq, int prefix_len, int kvh, int n_seq, int H) {
+DecodePlan decode_plan(int own, int prefix_len, int kvh, int n_seq, int H) {
 	DecodePlan p{};
-	const int own = max_seq - prefix_len;
 	const int slots = 2 * cu_count();   // workgroups that run at once
 	// own keys: parts of 32 keys a wave or more, until the workgroups fill the chip (16 sequences of 4096, 64 pairs of
 	// sequence and head: 19.0 us with 8 parts, 18.5 with 4, 22.8 with 12). From a pair per CU on only long sequences are
@@ -1678,11 +1813,16 @@ DecodePlan decode_plan(int max_seq, int prefix_len, int kvh, int n_seq, int H) {
 	return p;
 }
 
-template <int HD, bool Q8>
+// The most keys of its own that a sequence's token sees, a window's in whole steps after the sinks'.
+int most_keys(const AttnKv &c) {
+	return c.window ? (int)std::min<int64_t>(c.max_seq, ((int64_t)c.sinks + 31) / 32 * 32 + c.window) : c.max_seq - c.prefix_len;
+}
+
+template <int HD, bool Q8, bool WIN>
 int decode(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq, const int *slot, const int *len,
            int n_seq, int H, float scale) {
 	const int G = H / c.kvh;
-	const DecodePlan p = decode_plan(c.max_seq, c.prefix_len, c.kvh, n_seq, H);
+	const DecodePlan p = decode_plan(most_keys(c), c.prefix_len, c.kvh, n_seq, H);
 	const int parts = p.parts, least = p.least, pparts = p.pparts, unit = p.unit, nrec = p.nrec;
 	const int64_t tiles = p.tiles;
 	Records rec{};
@@ -1690,16 +1830,16 @@ int decode(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq
 		if (int rc = records((size_t)n_seq * H * nrec, HD, &rec)) return rc;
 	const int64_t blocks = (tiles * pparts + (int64_t)n_seq * parts) * c.kvh;
 	if (blocks > kMaxThreads / (64 * kWaves)) return set_error(HAKO_GPU_EINVAL, "%lld workgroups in one call", (long long)blocks);
-	if (pparts) {
+	if (!WIN && pparts) {
 		hipLaunchKernelGGL((prefix_kernel<HD, Q8>), dim3((unsigned)blocks), dim3(64 * kWaves), 0, stream(), c, q, ldq, slot, len,
 		                   n_seq, G, scale * kLog2e, (int)tiles, pparts, unit, parts, least, nrec, rec);
 	} else {
-		hipLaunchKernelGGL((decode_kernel<HD, Q8>), own_grid(c.kvh, n_seq, parts, least), dim3(256), 0, stream(), c, out, ldo, q, ldq, slot,
+		hipLaunchKernelGGL((decode_kernel<HD, Q8, WIN>), own_grid(c.kvh, n_seq, parts, least), dim3(256), 0, stream(), c, out, ldo, q, ldq, slot,
 		                   len, n_seq, G, scale * kLog2e, parts, least, nrec, rec);
 	}
 	HK_LAUNCHED("attention");
 	if (nrec) {
-		hipLaunchKernelGGL(decode_join_kernel<HD>, dim3(H, n_seq), dim3(64 * kJoin), 0, stream(), c, out, ldo, slot, len, H, parts, least,
+		hipLaunchKernelGGL((decode_join_kernel<HD, WIN>), dim3(H, n_seq), dim3(64 * kJoin), 0, stream(), c, out, ldo, slot, len, H, parts, least,
 		                   pparts, nrec, rec.o, rec.ml, rec.e);
 		HK_LAUNCHED("attention join");
 	}
@@ -1709,8 +1849,8 @@ int decode(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq
 // A launch's items in order of their length, so that the last ones to start
 // are the shortest, where there are few enough for the table; their number,
 // or 0.
-template <int K>
-int sort_items(const SeqTab &t, int prefix_len, ItemTab &order) {
+template <int K, bool WIN>
+int sort_items(const SeqTab &t, const Reach &reach, ItemTab &order) {
 	struct Len {
 		int steps;
 		uint32_t item;
@@ -1721,7 +1861,8 @@ int sort_items(const SeqTab &t, int prefix_len, ItemTab &order) {
 		const int tiles = (t.len[s] + t.tile_tokens - 1) / t.tile_tokens;
 		if (tiles > kItems || t.nsplit[s] > 256) return 0;
 		for (int i = tiles - 1; i >= 0; i--) {
-			const int nc = tile_steps<K>(t.start[s] + std::min((i + 1) * t.tile_tokens, t.len[s]), prefix_len);
+			const int nc = reach_steps<K, WIN>(reach, t.start[s] + i * t.tile_tokens, t.tile_tokens,
+			                                   t.start[s] + std::min((i + 1) * t.tile_tokens, t.len[s]));
 			const int parts = (nc + t.unit - 1) / t.unit, per = (nc + parts - 1) / parts;
 			if (n + parts > kItems) return 0;
 			for (int k = 0; k < parts; k++) len[n++] = {std::min(per, nc - k * per), (uint32_t)s << 26 | (uint32_t)(i << 8 | k)};
@@ -1734,22 +1875,26 @@ int sort_items(const SeqTab &t, int prefix_len, ItemTab &order) {
 
 // One launch of up to kSeqs sequences, in the order given (the longest
 // first): tiles of `rows` query rows, steps of K keys, parts of `unit` steps.
-template <int HD, bool Q8, int K, class Launch>
-int prompt_launch(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, int H, int rows, int64_t unit, Launch launch) {
+template <int HD, bool Q8, int K, bool WIN, class Launch>
+int prompt_launch(const AttnKv &c, const Reach &reach, SeqTab &t, float *out, int64_t ldo, int H, int rows, int64_t unit, Launch launch) {
 	t.tile_tokens = rows / (H / c.kvh);
 	t.unit = (int)std::min<int64_t>(unit, 0x7FFFFFFF);
 	int64_t items = 0, recs = 0;
 	for (int s = 0; s < t.n; s++) {
-		t.nsplit[s] = (tile_steps<K>(t.start[s] + t.len[s], c.prefix_len) + t.unit - 1) / t.unit;
+		const int tiles = (t.len[s] + t.tile_tokens - 1) / t.tile_tokens;
+		auto steps = [&](int tile) {
+			return reach_steps<K, WIN>(reach, t.start[s] + tile * t.tile_tokens, t.tile_tokens,
+			                           (int)(t.start[s] + std::min<int64_t>((int64_t)(tile + 1) * t.tile_tokens, t.len[s])));
+		};
+		t.nsplit[s] = (steps(tiles - 1) + t.unit - 1) / t.unit;
 		t.item[s] = (int)items;
-		items += (int64_t)((t.len[s] + t.tile_tokens - 1) / t.tile_tokens) * t.nsplit[s];
+		items += (int64_t)tiles * t.nsplit[s];
 		t.rec[s] = (uint32_t)recs;
 		// the first tile of more than `unit` steps (a tile sees no fewer than those before it)
-		int lo = 0, hi = (t.len[s] + t.tile_tokens - 1) / t.tile_tokens;
+		int lo = 0, hi = tiles;
 		while (lo < hi) {
 			const int mid = (lo + hi) / 2;
-			const int64_t end = t.start[s] + std::min<int64_t>((int64_t)(mid + 1) * t.tile_tokens, t.len[s]);
-			if (tile_steps<K>((int)end, c.prefix_len) <= t.unit) lo = mid + 1;
+			if (steps(mid) <= t.unit) lo = mid + 1;
 			else hi = mid;
 		}
 		const int first = (int)std::min<int64_t>((int64_t)lo * t.tile_tokens, t.len[s]);
@@ -1766,21 +1911,31 @@ int prompt_launch(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, int H, in
 	HK_LAUNCHED("attention");
 	if (recs) {
 		const int64_t blocks = ((int64_t)t.join[t.n] * H * (HD / 4) + 255) / 256;
-		hipLaunchKernelGGL((prompt_join_kernel<HD, K>), dim3((unsigned)blocks), dim3(256), 0, stream(), t, c.prefix_len, out, ldo, H, rec.o, rec.ml, rec.e);
+		hipLaunchKernelGGL((prompt_join_kernel<HD, K, WIN>), dim3((unsigned)blocks), dim3(256), 0, stream(), t, reach, out, ldo, H, rec.o, rec.ml, rec.e);
 		HK_LAUNCHED("attention join");
 	}
 	return HAKO_GPU_OK;
 }
 
 // Steps of K keys over all tiles of `tokens` tokens: a sequence's tiles at the
-// mean of its first and last one's.
-template <int K>
-int64_t all_steps(const AttnKv &c, const SeqTab &t, int tokens) {
+// mean of its first and last one's; with a window the tiles that still see
+// everything so, the others at the last one's.
+template <int K, bool WIN>
+int64_t all_steps(const AttnKv &c, const Reach &reach, const SeqTab &t, int tokens) {
 	int64_t n = 0;
 	for (int s = 0; s < t.n; s++) {
 		const int64_t tiles = (t.len[s] + tokens - 1) / tokens;
-		n += (tiles * (tile_steps<K>(t.start[s] + std::min(tokens, t.len[s]), c.prefix_len) +
-		               tile_steps<K>(t.start[s] + t.len[s], c.prefix_len)) + 1) / 2;
+		auto steps = [&](int64_t tile) {
+			const int first = (int)(t.start[s] + tile * tokens);
+			return (int64_t)reach_steps<K, WIN>(reach, first, tokens, std::min(first + tokens, t.start[s] + t.len[s]));
+		};
+		int64_t grow = tiles;
+		if (WIN) {   // tiles with start + (tile + 1) tokens - window <= sinks
+			const int64_t room = (int64_t)reach.sinks + reach.window - t.start[s];
+			grow = std::min(tiles, room < 0 ? 0 : room / tokens);
+		}
+		if (grow) n += (grow * (steps(0) + steps(grow - 1)) + 1) / 2;
+		n += (tiles - grow) * steps(tiles - 1);
 	}
 	return n * c.kvh;
 }
@@ -1806,30 +1961,117 @@ int64_t all_steps(const AttnKv &c, const SeqTab &t, int tokens) {
 // back); the direct one tiles of more than a share where they are too few for
 // the chip (64 tokens at position 8000: 34 us, 37 at two shares), else of more
 // than two (512 at 3000: 70, 115 at one).
-template <int HD, bool Q8>
+template <int HD, bool Q8, bool WIN>
 int prompt(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, const float *q, int64_t ldq, int H, float scale) {
 	const int G = H / c.kvh;
 	const int64_t cu = cu_count(), slots = 2 * cu;   // workgroups of the direct kernel that run at once
-	const int64_t steps = all_steps<32>(c, t, 32 / G);
+	const Reach reach = {c.prefix_len, c.window, c.sinks};
+	const int64_t steps = all_steps<32, WIN>(c, reach, t, 32 / G);
 	if (g_attn_prompt ? g_attn_prompt == 2 : steps > 55 * 4 * cu) {
-		const int64_t all = all_steps<kKeys>(c, t, 32 * kTileWaves / G);
-		return prompt_launch<HD, Q8, kKeys>(
-		    c, t, out, ldo, H, 32 * kTileWaves, std::max<int64_t>(4, (3 * all + 2 * cu - 1) / (2 * cu)),
+		const int64_t all = all_steps<kKeys, WIN>(c, reach, t, 32 * kTileWaves / G);
+		return prompt_launch<HD, Q8, kKeys, WIN>(
+		    c, reach, t, out, ldo, H, 32 * kTileWaves, std::max<int64_t>(4, (3 * all + 2 * cu - 1) / (2 * cu)),
 		    [&](int64_t items, const Records &rec) {
 			    ItemTab order;
-			    if (const int n = sort_items<kKeys>(t, c.prefix_len, order)) items = n;
-			    hipLaunchKernelGGL((prompt_kernel<HD, Q8>), dim3((unsigned)(items * c.kvh)), dim3(64 * kTileWaves), 0, stream(), c, t, order, out,
-			                       ldo, q, ldq, G, scale * kLog2e, rec);
+			    if (const int n = sort_items<kKeys, WIN>(t, reach, order)) items = n;
+			    hipLaunchKernelGGL((prompt_kernel<HD, Q8, WIN>), dim3((unsigned)(items * c.kvh)), dim3(64 * kTileWaves), 0, stream(), c, t, order,
+			                       out, ldo, q, ldq, G, scale * kLog2e, rec);
 		    });
 	}
 	int64_t tiles = 0;
 	for (int s = 0; s < t.n; s++) tiles += (t.len[s] + 32 / G - 1) / (32 / G);
 	const int64_t share = (steps + slots - 1) / slots;
-	return prompt_launch<HD, Q8, 32>(c, t, out, ldo, H, 32, std::max<int64_t>(4 * kWaves, 2 * tiles * c.kvh <= slots ? share : 2 * share),
-	                                 [&](int64_t items, const Records &rec) {
-		                                 hipLaunchKernelGGL((prompt_direct_kernel<HD, Q8>), dim3((unsigned)(items * c.kvh)),
-		                                                    dim3(64 * kWaves), 0, stream(), c, t, out, ldo, q, ldq, G, scale * kLog2e, rec);
-	                                 });
+	return prompt_launch<HD, Q8, 32, WIN>(c, reach, t, out, ldo, H, 32,
+	                                      std::max<int64_t>(4 * kWaves, 2 * tiles * c.kvh <= slots ? share : 2 * share),
+	                                      [&](int64_t items, const Records &rec) {
+		                                      hipLaunchKernelGGL((prompt_direct_kernel<HD, Q8, WIN>), dim3((unsigned)(items * c.kvh)),
+		                                                         dim3(64 * kWaves), 0, stream(), c, t, out, ldo, q, ldq, G, scale * kLog2e, rec);
+	                                      });
+}
+
+// ── drafted trees: 32 rows of (node, head of the group) of one sequence by the direct kernel ──
+
+// Where a sequence's nodes go: rows [base, end), base 0 and no rows where it has no place.
+__device__ __forceinline__ bool tree_place(const AttnKv &c, const int *slot, const int *base, int sq, int N, int &sl, int &b, int &end) {
+	sl = slot ? slot[sq] : sq;
+	b = base[sq];
+	const bool on = sl >= 0 && sl < c.n_slots && b >= 0;
+	sl = on ? sl : 0;
+	b = on ? min(b, c.max_seq) : 0;
+	end = on ? min(b + N, c.max_seq) : 0;
+	return on;
+}
+// Steps per part of a tile with nc steps, at least one for each wave.
+__device__ __forceinline__ int tree_part(int nc, int parts) {
+	return max(((nc + parts - 1) / parts + kWaves - 1) / kWaves * kWaves, kWaves);
+}
+
+template <int HD, bool Q8>
+__global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(AttnKv c, float *out, int64_t ldo, const float *q, int64_t ldq,
+                                                              const int *__restrict__ slot, const int *__restrict__ base,
+                                                              const uint64_t *__restrict__ seen, int n_seq, int N, int G, float scale,
+                                                              int parts, Records rec) {
+	__shared__ DirectLds<HD> s;
+	const int kvh = blockIdx.x % c.kvh, pair = blockIdx.x / c.kvh;
+	const int sq = pair % n_seq, part = pair / n_seq % parts, tile = pair / n_seq / parts;
+	const int lane = threadIdx.x & 63, r = 32 * tile + (lane & 31), node = r / G, g = r - node * G;
+	const int head = kvh * G, H = c.kvh * G;
+	const bool on = node < N;
+	int sl, b, end;
+	const bool placed = tree_place(c, slot, base, sq, N, sl, b, end);
+	const Span sp = span_of<32, false>(c, kvh, sl, 0, 0, end);
+	const int nc = sp.n0 + (max(end - sp.b0, 0) + 31) / 32;
+	const int per = tree_part(nc, parts), c0 = part * per;
+	if (c0 >= nc && part > 0) return;   // a record that the join does not read
+	const int64_t row = (int64_t)sq * N + node;
+	uint64_t bits = on && placed ? seen[row] : 0;
+	if (N < 64) bits &= (1ull << N) - 1;
+	direct_rows<HD, Q8>(c, s, sp, c0, min(nc, c0 + per), on && bits ? q + row * ldq + (head + g) * HD : nullptr, scale, Nodes{b, bits, 0},
+	                    on ? node << 4 | g | (bits ? 0 : kBlank) : -1,
+	                    parts == 1 ? Dest(out + (int64_t)sq * N * ldo + head * HD, ldo, HD)
+	                               : Dest(rec, ((size_t)sq * N * H + head) * parts + part, H, parts));
+}
+
+template <int HD>
+__global__ __launch_bounds__(256) void tree_join_kernel(AttnKv c, float *out, int64_t ldo, const int *__restrict__ slot,
+                                                        const int *__restrict__ base, int n_seq, int N, int H, int parts,
+                                                        const float *__restrict__ rec_o, const float2 *__restrict__ rec_ml,
+                                                        const float *__restrict__ rec_e) {
+	constexpr int L = HD / 4;
+	const int64_t i = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+	const int64_t row = i / H;
+	const int h = (int)(i - row * H), d = threadIdx.x % L * 4, sq = (int)(row / N);
+	if (sq >= n_seq) return;
+	int sl, b, end;
+	tree_place(c, slot, base, sq, N, sl, b, end);
+	const int nc = tile_steps<32>(end, c.prefix_len), per = tree_part(nc, parts);
+	const size_t first = (size_t)i * parts;
+	join_few(rec_o + first * HD + d, HD, rec_ml + first, rec_e + first, max((nc + per - 1) / per, 1), out + row * ldo + (int64_t)h * HD + d);
+}
+
+// Trees of N nodes: parts of the keys (a step for each wave or more) until the workgroups fill the chip.
+template <int HD, bool Q8>
+int tree(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq, const int *slot, const int *base, const uint64_t *seen,
+         int n_seq, int N, int H, float scale) {
+	const int G = H / c.kvh;
+	const int64_t slots = 2 * cu_count(), tiles = ((int64_t)N * G + 31) / 32, wgs = tiles * n_seq * c.kvh;
+	const int most = (tile_steps<32>(c.max_seq, c.prefix_len) + kWaves - 1) / kWaves;
+	const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(most, slots / wgs));
+	if (wgs * parts > kMaxThreads / (64 * kWaves) || (int64_t)n_seq * N * H * (HD / 4) > kMaxThreads)
+		return set_error(HAKO_GPU_EINVAL, "%lld workgroups in one call", (long long)(wgs * parts));
+	Records rec{};
+	if (parts > 1)
+		if (int rc = records((size_t)n_seq * N * H * parts, HD, &rec)) return rc;
+	hipLaunchKernelGGL((tree_kernel<HD, Q8>), dim3((unsigned)(wgs * parts)), dim3(64 * kWaves), 0, stream(), c, out, ldo, q, ldq, slot, base,
+	                   seen, n_seq, N, G, scale * kLog2e, parts, rec);
+	HK_LAUNCHED("attention");
+	if (parts > 1) {
+		const int64_t blocks = ((int64_t)n_seq * N * H * (HD / 4) + 255) / 256;
+		hipLaunchKernelGGL(tree_join_kernel<HD>, dim3((unsigned)blocks), dim3(256), 0, stream(), c, out, ldo, slot, base, n_seq, N, H, parts,
+		                   rec.o, rec.ml, rec.e);
+		HK_LAUNCHED("attention join");
+	}
+	return HAKO_GPU_OK;
 }
 
 }  // namespace
@@ -1837,13 +2079,22 @@ int prompt(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, const float *q, 
 int attn_decode(float *out, int64_t ldo, const float *q, int64_t ldq, const hako_gpu_kv *kv, const int *slot,
                 const int *len, int len_add, int n_seq, int H, float scale, int prefix_slot, int prefix_len) {
 	const AttnKv c = attn_kv(kv, prefix_slot, prefix_len, len_add);
-#define HK_DECODE(HD, Q8) decode<HD, Q8>(c, out, ldo, q, ldq, slot, len, n_seq, H, scale)
+#define HK_DECODE(HD, Q8) decode<HD, Q8, false>(c, out, ldo, q, ldq, slot, len, n_seq, H, scale)
 	return HK_KV_SWITCH(kv, HK_DECODE);
 #undef HK_DECODE
 }
 
-int attn_decode_reserve(const hako_gpu_kv *kv, int n_seq, int H, int prefix_len) {
-	const DecodePlan p = decode_plan(kv->max_seq, prefix_len, kv->n_kv_heads, n_seq, H);
+int attn_decode_window(float *out, int64_t ldo, const float *q, int64_t ldq, const hako_gpu_kv *kv, const int *slot,
+                       const int *len, int len_add, int n_seq, int H, float scale, int window, int sinks) {
+	const AttnKv c = attn_kv_window(kv, len_add, window, sinks);
+#define HK_DECODE(HD, Q8) decode<HD, Q8, true>(c, out, ldo, q, ldq, slot, len, n_seq, H, scale)
+	return HK_KV_SWITCH(kv, HK_DECODE);
+#undef HK_DECODE
+}
+
+int attn_decode_reserve(const hako_gpu_kv *kv, int n_seq, int H, int prefix_len, int window, int sinks) {
+	const AttnKv c = window ? attn_kv_window(kv, 0, window, sinks) : attn_kv(kv, 0, prefix_len, 0);
+	const DecodePlan p = decode_plan(most_keys(c), prefix_len, kv->n_kv_heads, n_seq, H);
 	Records r;
 	return p.nrec ? records((size_t)n_seq * H * p.nrec, kv->head_dim, &r) : HAKO_GPU_OK;
 }
@@ -1854,27 +2105,23 @@ void attn_set_prompt(int v) { g_attn_prompt = v == 1 || v == 2 ? v : 0; }
 
 using namespace hako;
 
-extern "C" {
+namespace {
 
-int hako_gpu_attn_decode(float *out, int64_t out_stride, const float *q, int64_t q_stride, const hako_gpu_kv *kv,
-                         const int *slot, const int *len, int n_seq, int n_heads, float scale, int prefix_slot,
-                         int prefix_len) {
-	if (int rc = attn_check(out, out_stride, q, q_stride, kv, n_seq, n_heads, prefix_slot, prefix_len)) return rc;
+int decode_check(const hako_gpu_kv *kv, const int *slot, const int *len, int n_seq) {
 	if (!len && n_seq) return set_error(HAKO_GPU_EINVAL, "null lengths");
 	if (!slot && n_seq > kv->n_slots)
 		return set_error(HAKO_GPU_EINVAL, "%d sequences without slots in a cache of %d", n_seq, kv->n_slots);
 	if (n_seq > 65535) return set_error(HAKO_GPU_EINVAL, "%d sequences in one call (at most 65535)", n_seq);
-	if (int rc = require_device()) return rc;
-	if (n_seq == 0) return ok();
-	if (int rc = attn_decode(out, out_stride, q, q_stride, kv, slot, len, 0, n_seq, n_heads, scale, prefix_slot, prefix_len))
-		return rc;
-	return ok();
+	return HAKO_GPU_OK;
 }
 
-int hako_gpu_attn_prompt(float *out, int64_t out_stride, const float *q, int64_t q_stride, const hako_gpu_kv *kv,
-                         const int *slot, const int *start, const int *len, int n_seq, int n_heads, float scale,
-                         int prefix_slot, int prefix_len) {
-	if (int rc = attn_check(out, out_stride, q, q_stride, kv, n_seq, n_heads, prefix_slot, prefix_len)) return rc;
+int window_check(int window, int sinks) {
+	if (window < 1 || sinks < 0) return set_error(HAKO_GPU_EINVAL, "a window of %d positions after %d sinks", window, sinks);
+	return HAKO_GPU_OK;
+}
+
+// The prompts of a call, checked but for q, out and the cache; rows of q and out.
+int prompt_check(const hako_gpu_kv *kv, const int *slot, const int *start, const int *len, int n_seq) {
 	if (n_seq && (!start || !len)) return set_error(HAKO_GPU_EINVAL, "null starts or lengths");
 	int64_t rows = 0;
 	for (int s = 0; s < n_seq; s++) {
@@ -1886,8 +2133,11 @@ int hako_gpu_attn_prompt(float *out, int64_t out_stride, const float *q, int64_t
 		rows += len[s];
 	}
 	if (rows > 0x7FFFFFFF) return set_error(HAKO_GPU_EINVAL, "%lld tokens in one call", (long long)rows);
-	if (int rc = require_device()) return rc;
-	const AttnKv c = attn_kv(kv, prefix_slot, prefix_len, 0);
+	return HAKO_GPU_OK;
+}
+
+int prompts(const AttnKv &c, const hako_gpu_kv *kv, float *out, int64_t ldo, const float *q, int64_t ldq, const int *slot,
+            const int *start, const int *len, int n_seq, int H, float scale) {
 	// the sequences with tokens, those that end last (the longest tiles) first
 	std::vector<int> order, row;
 	try {
@@ -1913,10 +2163,79 @@ int hako_gpu_attn_prompt(float *out, int64_t out_stride, const float *q, int64_t
 			t.slot[t.n] = slot ? slot[s] : s;
 			t.start[t.n] = start[s];
 		}
-#define HK_PROMPT(HD, Q8) prompt<HD, Q8>(c, t, out, out_stride, q, q_stride, n_heads, scale)
+#define HK_PROMPT(HD, Q8) (c.window ? prompt<HD, Q8, true>(c, t, out, ldo, q, ldq, H, scale) : prompt<HD, Q8, false>(c, t, out, ldo, q, ldq, H, scale))
 		if (int rc = HK_KV_SWITCH(kv, HK_PROMPT)) return rc;
 #undef HK_PROMPT
 	}
+	return HAKO_GPU_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int hako_gpu_attn_decode(float *out, int64_t out_stride, const float *q, int64_t q_stride, const hako_gpu_kv *kv,
+                         const int *slot, const int *len, int n_seq, int n_heads, float scale, int prefix_slot,
+                         int prefix_len) {
+	if (int rc = attn_check(out, out_stride, q, q_stride, kv, n_seq, n_heads, prefix_slot, prefix_len)) return rc;
+	if (int rc = decode_check(kv, slot, len, n_seq)) return rc;
+	if (int rc = require_device()) return rc;
+	if (n_seq == 0) return ok();
+	if (int rc = attn_decode(out, out_stride, q, q_stride, kv, slot, len, 0, n_seq, n_heads, scale, prefix_slot, prefix_len))
+		return rc;
+	return ok();
+}
+
+int hako_gpu_attn_decode_window(float *out, int64_t out_stride, const float *q, int64_t q_stride, const hako_gpu_kv *kv,
+                                const int *slot, const int *len, int n_seq, int n_heads, float scale, int window,
+                                int sinks) {
+	if (int rc = attn_check(out, out_stride, q, q_stride, kv, n_seq, n_heads, 0, 0)) return rc;
+	if (int rc = decode_check(kv, slot, len, n_seq)) return rc;
+	if (int rc = window_check(window, sinks)) return rc;
+	if (int rc = require_device()) return rc;
+	if (n_seq == 0) return ok();
+	if (int rc = attn_decode_window(out, out_stride, q, q_stride, kv, slot, len, 0, n_seq, n_heads, scale, window, sinks)) return rc;
+	return ok();
+}
+
+int hako_gpu_attn_prompt(float *out, int64_t out_stride, const float *q, int64_t q_stride, const hako_gpu_kv *kv,
+                         const int *slot, const int *start, const int *len, int n_seq, int n_heads, float scale,
+                         int prefix_slot, int prefix_len) {
+	if (int rc = attn_check(out, out_stride, q, q_stride, kv, n_seq, n_heads, prefix_slot, prefix_len)) return rc;
+	if (int rc = prompt_check(kv, slot, start, len, n_seq)) return rc;
+	if (int rc = require_device()) return rc;
+	if (int rc = prompts(attn_kv(kv, prefix_slot, prefix_len, 0), kv, out, out_stride, q, q_stride, slot, start, len, n_seq, n_heads, scale))
+		return rc;
+	return ok();
+}
+
+int hako_gpu_attn_prompt_window(float *out, int64_t out_stride, const float *q, int64_t q_stride, const hako_gpu_kv *kv,
+                                const int *slot, const int *start, const int *len, int n_seq, int n_heads, float scale,
+                                int window, int sinks) {
+	if (int rc = attn_check(out, out_stride, q, q_stride, kv, n_seq, n_heads, 0, 0)) return rc;
+	if (int rc = prompt_check(kv, slot, start, len, n_seq)) return rc;
+	if (int rc = window_check(window, sinks)) return rc;
+	if (int rc = require_device()) return rc;
+	if (int rc = prompts(attn_kv_window(kv, 0, window, sinks), kv, out, out_stride, q, q_stride, slot, start, len, n_seq, n_heads, scale))
+		return rc;
+	return ok();
+}
+
+int hako_gpu_attn_tree(float *out, int64_t out_stride, const float *q, int64_t q_stride, const hako_gpu_kv *kv,
+                       const int *slot, const int *base, const uint64_t *seen, int n_seq, int n_tree, int n_heads,
+                       float scale, int prefix_slot, int prefix_len) {
+	if (int rc = attn_check(out, out_stride, q, q_stride, kv, n_seq, n_heads, prefix_slot, prefix_len)) return rc;
+	if (int rc = tree_check(n_seq, n_tree)) return rc;
+	if (n_seq && (!base || !seen)) return set_error(HAKO_GPU_EINVAL, "null bases or masks");
+	if ((uintptr_t)seen & 7) return set_error(HAKO_GPU_EINVAL, "masks are not 8-byte aligned");
+	if (!slot && n_seq > kv->n_slots)
+		return set_error(HAKO_GPU_EINVAL, "%d sequences without slots in a cache of %d", n_seq, kv->n_slots);
+	if (int rc = require_device()) return rc;
+	if (n_seq == 0) return ok();
+	const AttnKv c = attn_kv(kv, prefix_slot, prefix_len, 0);
+#define HK_TREE(HD, Q8) tree<HD, Q8>(c, out, out_stride, q, q_stride, slot, base, seen, n_seq, n_tree, n_heads, scale)
+	if (int rc = HK_KV_SWITCH(kv, HK_TREE)) return rc;
+#undef HK_TREE
 	return ok();
 }
 

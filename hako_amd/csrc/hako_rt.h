@@ -44,7 +44,8 @@ void dec_set_merge_rows(int v);
 void dec_set_qkv_items(int v);
 void dec_set_attn_parts(int v);
 void attn_set_prompt(int v);
-// Grow-only device workspace slot `slot` (0..7) of at least `bytes`.
+// Grow-only device workspace slot `slot` (0..kWorkspaces-1) of at least `bytes`.
+constexpr int kWorkspaces = 9;
 int workspace(int slot, size_t bytes, void **ptr);
 // Look up this device's address of the no-allocation scratch array (with
 // the device current; once per device).

@@ -19,7 +19,12 @@ int rows_check(const char *what, const void *p, int64_t stride, int64_t width);
 // n_seq >= 1.
 int attn_decode(float *out, int64_t ldo, const float *q, int64_t ldq, const hako_gpu_kv *kv, const int *slot,
                 const int *len, int len_add, int n_seq, int H, float scale, int prefix_slot, int prefix_len);
-// The workspace of such calls, taken now (before a capture).
-int attn_decode_reserve(const hako_gpu_kv *kv, int n_seq, int H, int prefix_len);
+// hako_gpu_attn_decode_window likewise.
+int attn_decode_window(float *out, int64_t ldo, const float *q, int64_t ldq, const hako_gpu_kv *kv, const int *slot,
+                       const int *len, int len_add, int n_seq, int H, float scale, int window, int sinks);
+// The workspace of such calls, taken now (before a capture); window 0: none.
+int attn_decode_reserve(const hako_gpu_kv *kv, int n_seq, int H, int prefix_len, int window = 0, int sinks = 0);
+// The sizes of a batch of drafted trees.
+int tree_check(int n_seq, int n_tree);
 
 }  // namespace hako

@@ -138,7 +138,7 @@ __device__ __forceinline__ void put4_past(float *dst, const float x[4]) {
 // the caches), the waves waiting 79% of their cycles.
 template <int HD, bool Q8>
 __global__ __launch_bounds__(256) void append_kernel(KvDev kv, const int *__restrict__ slot, const int *__restrict__ posv,
-                                                     int n_tok, const float *__restrict__ k,
+                                                     const int *__restrict__ turnv, int n_tok, const float *__restrict__ k,
                                                      const float *__restrict__ v, int64_t kv_stride, RopeDev rope,
                                                      const float *q, float *q_out, int H, int64_t q_stride,
                                                      int64_t q_out_stride) {
@@ -146,8 +146,8 @@ __global__ __launch_bounds__(256) void append_kernel(KvDev kv, const int *__rest
 	const uint32_t row = blockIdx.x * (256 / L) + threadIdx.x / L, per = H + 2 * kv.kvh;
 	const int tok = (int)(row / per), h = (int)(row - tok * per), t = threadIdx.x % L;
 	if (tok >= n_tok) return;
-	const int sl = slot ? slot[tok] : tok, pos = posv[tok];
-	if (sl < 0 || sl >= kv.n_slots || pos < 0 || pos >= kv.max_seq || (rope.table && pos >= rope.n_pos)) return;
+	const int sl = slot ? slot[tok] : tok, pos = posv[tok], at = turnv ? turnv[tok] : pos;
+	if (sl < 0 || sl >= kv.n_slots || pos < 0 || pos >= kv.max_seq || (rope.table && (at < 0 || at >= rope.n_pos))) return;
 	const bool is_q = h < H, is_v = h >= H + kv.kvh;
 	const float *src = is_q ? q + tok * q_stride + (int64_t)h * HD
 	                        : (is_v ? v + tok * kv_stride + (int64_t)(h - H - kv.kvh) * HD
@@ -157,7 +157,7 @@ __global__ __launch_bounds__(256) void append_kernel(KvDev kv, const int *__rest
 	const float4 a = *(const float4 *)(src + 4 * u0), b = *(const float4 *)(src + 4 * u1);
 	float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 	if (t < ru) {
-		const float *tb = rope.table + (size_t)pos * rope.rot;
+		const float *tb = rope.table + (size_t)at * rope.rot;
 		if (rope.interleaved) {
 			const float4 c0 = *(const float4 *)(tb + 4 * u0), c1 = *(const float4 *)(tb + 4 * u1);
 			turn(x[0], x[1], c0.x, c0.y);
@@ -261,9 +261,9 @@ int hako_gpu_kv_bytes(const hako_gpu_kv *kv, size_t *codes, size_t *scales) {
 	return ok();
 }
 
-int hako_gpu_kv_append(const hako_gpu_kv *kv, const int *slot, const int *pos, int n_tok, const float *k,
-                       const float *v, int64_t kv_stride, const hako_gpu_rope *rope, const float *q, float *q_out,
-                       int n_heads, int64_t q_stride, int64_t q_out_stride) {
+static int append(const hako_gpu_kv *kv, const int *slot, const int *pos, const int *turn, int n_tok, const float *k,
+                  const float *v, int64_t kv_stride, const hako_gpu_rope *rope, const float *q, float *q_out, int n_heads,
+                  int64_t q_stride, int64_t q_out_stride) {
 	if (int rc = kv_check(kv)) return rc;
 	if (int rc = tokens_check(kv, slot, pos, n_tok)) return rc;
 	const int64_t kvw = (int64_t)kv->n_kv_heads * kv->head_dim;
@@ -294,8 +294,8 @@ int hako_gpu_kv_append(const hako_gpu_kv *kv, const int *slot, const int *pos, i
 	dim3 grid;
 	if (int rc = row_blocks((int64_t)n_tok * (H + 2 * kv->n_kv_heads), 256 / (kv->head_dim / 8), &grid)) return rc;
 #define HK_APPEND(HD, Q8)                                                                                          \
-	hipLaunchKernelGGL((append_kernel<HD, Q8>), grid, dim3(256), 0, stream(), kv_dev(kv), slot, pos, n_tok, k, v,    \
-	                   kv_stride, r, q, q_out, H, q_stride, q_out_stride)
+	hipLaunchKernelGGL((append_kernel<HD, Q8>), grid, dim3(256), 0, stream(), kv_dev(kv), slot, pos, turn, n_tok, k, \
+	                   v, kv_stride, r, q, q_out, H, q_stride, q_out_stride)
 	if (kv->head_dim == 128) {
 		if (kv->type == HAKO_KV_Q8) HK_APPEND(128, true);
 		else HK_APPEND(128, false);
@@ -306,6 +306,20 @@ int hako_gpu_kv_append(const hako_gpu_kv *kv, const int *slot, const int *pos, i
 #undef HK_APPEND
 	HK_LAUNCHED("kv append");
 	return ok();
+}
+
+int hako_gpu_kv_append(const hako_gpu_kv *kv, const int *slot, const int *pos, int n_tok, const float *k,
+                       const float *v, int64_t kv_stride, const hako_gpu_rope *rope, const float *q, float *q_out,
+                       int n_heads, int64_t q_stride, int64_t q_out_stride) {
+	return append(kv, slot, pos, nullptr, n_tok, k, v, kv_stride, rope, q, q_out, n_heads, q_stride, q_out_stride);
+}
+
+int hako_gpu_kv_append_turned(const hako_gpu_kv *kv, const int *slot, const int *pos, const int *turn, int n_tok,
+                              const float *k, const float *v, int64_t kv_stride, const hako_gpu_rope *rope,
+                              const float *q, float *q_out, int n_heads, int64_t q_stride, int64_t q_out_stride) {
+	if (!turn && n_tok > 0) return set_error(HAKO_GPU_EINVAL, "null turns");
+	if (!rope) return set_error(HAKO_GPU_EINVAL, "turns without a rotation");
+	return append(kv, slot, pos, turn, n_tok, k, v, kv_stride, rope, q, q_out, n_heads, q_stride, q_out_stride);
 }
 
 int hako_gpu_kv_read(const hako_gpu_kv *kv, const int *slot, const int *pos, int n_tok, float *k, float *v,

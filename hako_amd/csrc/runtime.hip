@@ -44,8 +44,8 @@ struct State {
 	hipStream_t stream = nullptr;
 	hipDeviceProp_t prop{};
 	std::vector<Mirror> mirrors;
-	void *ws[8] = {};
-	size_t ws_bytes[8] = {};
+	void *ws[kWorkspaces] = {};
+	size_t ws_bytes[kWorkspaces] = {};
 	// workspaces outgrown by a later call: a graph captured earlier may still
 	// address them, so they live until hako_gpu_shutdown
 	std::vector<void *> ws_retired;
@@ -89,7 +89,7 @@ int require_device() {
 
 int workspace(int slot, size_t bytes, void **ptr) {
 	State &s = st();
-	if (slot < 0 || slot >= 8) return set_error(HAKO_GPU_EINVAL, "workspace slot %d", slot);
+	if (slot < 0 || slot >= kWorkspaces) return set_error(HAKO_GPU_EINVAL, "workspace slot %d", slot);
 	if (s.ws_bytes[slot] < bytes) {
 		// Grow by at least half again, so the retired buffers of a slot stay
 		// below twice its size.
@@ -145,7 +145,7 @@ int hako_gpu_shutdown(void) {
 	HK_HIP(hipStreamSynchronize(s.stream));
 	for (auto &m : s.mirrors) HK_HIP(hipFree(m.dev));
 	s.mirrors.clear();
-	for (int i = 0; i < 8; i++) {
+	for (int i = 0; i < kWorkspaces; i++) {
 		if (s.ws[i]) HK_HIP(hipFree(s.ws[i]));
 		s.ws[i] = nullptr;
 		s.ws_bytes[i] = 0;

@@ -1,4 +1,4 @@
-"""ctypes view of the hako_gpu C ABI (include/hako_gpu.h, include/hako_attn.h) for tests and the bench.
+"""ctypes view of the hako_gpu C ABI (include/hako_gpu.h, hako_attn.h, hako_search.h) for tests and the bench.
 
 Python never computes here: every call below is a C-ABI call into
 ``lib/libhako_gpu.so``. Loading fails loudly if the library has not been
@@ -81,6 +81,19 @@ ATTN_SIGNATURES = {
     "hako_gpu_kv_read": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _i64]),
     "hako_gpu_attn_decode": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i, _i, C.c_float, _i, _i]),
     "hako_gpu_attn_prompt": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i, _i, C.c_float, _i, _i]),
+    "hako_gpu_kv_append_turned": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _vp, _i64, _vp, _vp, _vp, _i, _i64, _i64]),
+    "hako_gpu_attn_decode_window": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i, _i, C.c_float, _i, _i]),
+    "hako_gpu_attn_prompt_window": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i, _i, C.c_float, _i, _i]),
+    "hako_gpu_attn_tree": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i, _i, _i, C.c_float, _i, _i]),
+}
+
+# ... and include/hako_search.h.
+SEARCH_SIGNATURES = {
+    "hako_gpu_beam_select": (_i, [_vp, _i64, _i, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
+    "hako_gpu_kv_reorder": (_i, [_vp, _i, _vp, _vp, _i, _i, _vp, _vp]),
+    "hako_gpu_tree_plan": (_i, [_vp, _vp, _vp, _i, _i, _vp, _vp, _vp, _vp]),
+    "hako_gpu_tree_accept": (_i, [_vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _vp, _vp]),
+    "hako_gpu_kv_keep": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _i, _i]),
 }
 
 
@@ -114,7 +127,7 @@ def load_library() -> C.CDLL:
         if not os.path.exists(GPU_LIB):
             raise HakoGpuError(f"{GPU_LIB} is not built; run __graft_entry__.build() (make -C hako_amd)")
         lib = C.CDLL(GPU_LIB)
-        for name, (res, args) in {**SIGNATURES, **ATTN_SIGNATURES}.items():
+        for name, (res, args) in {**SIGNATURES, **ATTN_SIGNATURES, **SEARCH_SIGNATURES}.items():
             fn = getattr(lib, name)
             fn.restype, fn.argtypes = res, args
         _lib = lib
@@ -293,6 +306,61 @@ class Gpu:
         self.check(self.lib.hako_gpu_attn_prompt(_ptr(out), out_stride, _ptr(q), q_stride, C.byref(kv), _ptr(slot),
                                                  _ptr(start), _ptr(length), n_seq, n_heads, scale, prefix_slot,
                                                  prefix_len), "attn_prompt")
+
+    def kv_append_turned(self, kv: Kv, slot, pos, turn, n_tok: int, k, v, kv_stride: int, rope: Rope, q=None, q_out=None,
+                         n_heads: int = 0, q_stride: int = 0, q_out_stride: int = 0):
+        self.check(self.lib.hako_gpu_kv_append_turned(C.byref(kv), _ptr(slot), _ptr(pos), _ptr(turn), n_tok, _ptr(k),
+                                                      _ptr(v), kv_stride, None if rope is None else C.byref(rope),
+                                                      _ptr(q), _ptr(q_out), n_heads, q_stride, q_out_stride),
+                   "kv_append_turned")
+
+    def attn_decode_window(self, out, out_stride: int, q, q_stride: int, kv: Kv, slot, length, n_seq: int, n_heads: int,
+                           scale: float, window: int, sinks: int = 0):
+        self.check(self.lib.hako_gpu_attn_decode_window(_ptr(out), out_stride, _ptr(q), q_stride, C.byref(kv), _ptr(slot),
+                                                        _ptr(length), n_seq, n_heads, scale, window, sinks),
+                   "attn_decode_window")
+
+    def attn_prompt_window(self, out, out_stride: int, q, q_stride: int, kv: Kv, slot, start, length, n_seq: int,
+                           n_heads: int, scale: float, window: int, sinks: int = 0):
+        """slot, start, length: host int32 arrays (slot may be None)."""
+        self.check(self.lib.hako_gpu_attn_prompt_window(_ptr(out), out_stride, _ptr(q), q_stride, C.byref(kv), _ptr(slot),
+                                                        _ptr(start), _ptr(length), n_seq, n_heads, scale, window, sinks),
+                   "attn_prompt_window")
+
+    def attn_tree(self, out, out_stride: int, q, q_stride: int, kv: Kv, slot, base, seen, n_seq: int, n_tree: int,
+                  n_heads: int, scale: float, prefix_slot: int = 0, prefix_len: int = 0):
+        self.check(self.lib.hako_gpu_attn_tree(_ptr(out), out_stride, _ptr(q), q_stride, C.byref(kv), _ptr(slot),
+                                               _ptr(base), _ptr(seen), n_seq, n_tree, n_heads, scale, prefix_slot,
+                                               prefix_len), "attn_tree")
+
+    # beams and drafted trees
+    @staticmethod
+    def kv_layers(kvs):
+        """The caches of several layers, as the calls over all of them take them."""
+        return (Kv * len(kvs))(*kvs)
+
+    def beam_select(self, logits, ld: int, vocab: int, score, done, eos: int, n_req: int, n_beams: int, n_pick: int,
+                    arrange: bool, parent, token, score_out, done_out=None):
+        self.check(self.lib.hako_gpu_beam_select(_ptr(logits), ld, vocab, _ptr(score), _ptr(done), eos, n_req, n_beams,
+                                                 n_pick, arrange, _ptr(parent), _ptr(token), _ptr(score_out),
+                                                 _ptr(done_out)), "beam_select")
+
+    def kv_reorder(self, layers, slot, parent, n_req: int, n_beams: int, since, length):
+        """layers: kv_layers()."""
+        self.check(self.lib.hako_gpu_kv_reorder(layers, len(layers), _ptr(slot), _ptr(parent), n_req, n_beams, _ptr(since),
+                                                _ptr(length)), "kv_reorder")
+
+    def tree_plan(self, slot, base, parent, n_seq: int, n_tree: int, seen=None, node_slot=None, row=None, turn=None):
+        self.check(self.lib.hako_gpu_tree_plan(_ptr(slot), _ptr(base), _ptr(parent), n_seq, n_tree, _ptr(seen),
+                                               _ptr(node_slot), _ptr(row), _ptr(turn)), "tree_plan")
+
+    def tree_accept(self, parent, token, pick, base, n_seq: int, n_tree: int, path, n_path, nxt, new_base=None):
+        self.check(self.lib.hako_gpu_tree_accept(_ptr(parent), _ptr(token), _ptr(pick), _ptr(base), n_seq, n_tree,
+                                                 _ptr(path), _ptr(n_path), _ptr(nxt), _ptr(new_base)), "tree_accept")
+
+    def kv_keep(self, layers, slot, base, path, n_path, n_seq: int, n_tree: int):
+        self.check(self.lib.hako_gpu_kv_keep(layers, len(layers), _ptr(slot), _ptr(base), _ptr(path), _ptr(n_path), n_seq,
+                                             n_tree), "kv_keep")
 
     def matmul_host(self, out: np.ndarray, x: np.ndarray, qtype: int, w_host: np.ndarray,
                     bias: np.ndarray | None, n_out: int, n_in: int):

@@ -91,6 +91,16 @@ int hako_gpu_kv_append(const hako_gpu_kv *kv, const int *slot, const int *pos, i
                        const float *k, const float *v, int64_t kv_stride, const hako_gpu_rope *rope,
                        const float *q, float *q_out, int n_heads, int64_t q_stride, int64_t q_out_stride);
 
+/* The same with the rotation apart from the row: token i's keys and values go
+ * to row pos[i], its key and queries are turned as at position turn[i]. For
+ * rows that do not lie in the order of the text: drafted trees
+ * (hako_search.h), where several nodes share a place in the text, or a slot
+ * used as a ring, whose rows the window of a long text passes through. A token
+ * whose turn lies outside the rope's table is left out too. */
+int hako_gpu_kv_append_turned(const hako_gpu_kv *kv, const int *slot, const int *pos, const int *turn, int n_tok,
+                              const float *k, const float *v, int64_t kv_stride, const hako_gpu_rope *rope,
+                              const float *q, float *q_out, int n_heads, int64_t q_stride, int64_t q_out_stride);
+
 /* The values of cached rows: token i's keys to k + i*kv_stride, its values to
  * v + i*kv_stride (either may be NULL), from position pos[i] of slot slot[i]
  * (slot NULL: slot i). The rows of a token outside the cache are left as they
@@ -137,6 +147,35 @@ int hako_gpu_attn_decode(float *out, int64_t out_stride, const float *q, int64_t
 int hako_gpu_attn_prompt(float *out, int64_t out_stride, const float *q, int64_t q_stride, const hako_gpu_kv *kv,
                          const int *slot, const int *start, const int *len, int n_seq, int n_heads, float scale,
                          int prefix_slot, int prefix_len);
+
+/* ── a window, and a few first positions that stay ──
+ * The same two for models (or layers) whose tokens look back a limited way: a
+ * token at position t sees the positions p <= t with p > t - window (window
+ * >= 1: its own and the window - 1 before it) or p < sinks (>= 0). Rows outside
+ * that are not read, so a token's work does not grow with its position, and
+ * the workspace of single tokens follows min(max_seq, sinks + window) in the
+ * place of max_seq. Prefixes are not shared here. */
+int hako_gpu_attn_decode_window(float *out, int64_t out_stride, const float *q, int64_t q_stride, const hako_gpu_kv *kv,
+                                const int *slot, const int *len, int n_seq, int n_heads, float scale, int window,
+                                int sinks);
+int hako_gpu_attn_prompt_window(float *out, int64_t out_stride, const float *q, int64_t q_stride, const hako_gpu_kv *kv,
+                                const int *slot, const int *start, const int *len, int n_seq, int n_heads, float scale,
+                                int window, int sinks);
+
+/* ── trees of drafted tokens ──
+ * n_tree (1..64) nodes of each of n_seq sequences: node j of sequence s is row
+ * s*n_tree + j of q and out, its keys and values are in row base[s] + j of slot
+ * slot[s] (NULL: slot s). It sees the positions below base[s], and of the rows
+ * from base[s] on those whose bits are set in seen[s*n_tree + j] (8-byte
+ * aligned): bit i is node i. A node whose mask is 0 is not there: it gets
+ * zeros. slot, base and seen are device arrays, read when the kernels run; a
+ * base above max_seq counts as max_seq, and no row at max_seq or past it is
+ * seen; a base below 0 or a slot outside the cache: the sequence gets zeros.
+ * hako_gpu_tree_plan (hako_search.h) makes the masks of a tree from its
+ * parents. A prefix in common as above. */
+int hako_gpu_attn_tree(float *out, int64_t out_stride, const float *q, int64_t q_stride, const hako_gpu_kv *kv,
+                       const int *slot, const int *base, const uint64_t *seen, int n_seq, int n_tree, int n_heads,
+                       float scale, int prefix_slot, int prefix_len);
 
 #pragma GCC visibility pop
 
