@@ -26,20 +26,31 @@ __device__ __forceinline__ int lanes_below(uint64_t m) {
 //
 // Values come in tiles of 64 E, position (i 64 + lane) 4 + c of a tile in
 // register 4 i + c; equal ones rank by position. Of a tile only what may still
-// be among the n best is looked at one by one: values above the n-th best so
-// far, and where more than n lanes have such values, above the n-th largest of
-// the lanes' own maxima (found bit by bit, a ballot each), which at most n - 1
-// lanes exceed. So no tile has more than n (E + 1) candidates, whatever the
-// values are, and an ordinary one has about n at first and hardly any later.
-// Candidates and the list so far rank each other in LDS.
+// be among the n best is kept: values above the n-th best known so far, and
+// where more than n lanes have such values, above the n-th largest of the
+// lanes' own maxima, or what tells it from the next (found bit by bit, a ballot
+// each), which at most n lanes exceed. So no tile adds more than n (E + 1), whatever the values are, and an
+// ordinary one about n at first and hardly any later. What is kept waits in LDS
+// until there are more than 64, and is then ranked: a lane a value, each
+// against all, as 64-bit keys of value and position.
 template <int E>
 struct Best {
 	struct Lds {
-		float v[HAKO_MAX_PICK * (E + 2)], lv[HAKO_MAX_PICK];
-		int i[HAKO_MAX_PICK * (E + 2)], li[HAKO_MAX_PICK];   // li, lv: the list, best first
+		alignas(16) uint64_t key[64 + HAKO_MAX_PICK * (E + 1) + 4], list[HAKO_MAX_PICK];
 	};
-	int n, count;   // wanted, in the list
+	int n, count;   // wanted, waiting
 	float least;    // a later value has to be larger
+
+	// (zeros of both signs are equal)
+	static __device__ __forceinline__ uint64_t key_of(float v, int pos) {
+		const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.0f);
+		return (uint64_t)(b >> 31 ? ~b : b | 0x80000000u) << 32 | (uint32_t)~pos;
+	}
+	static __device__ __forceinline__ float value(uint64_t key) {
+		const uint32_t k = (uint32_t)(key >> 32);
+		return __builtin_bit_cast(float, k >> 31 ? k & 0x7FFFFFFFu : ~k);
+	}
+	static __device__ __forceinline__ int place(uint64_t key) { return (int)~(uint32_t)key; }
 
 	__device__ __forceinline__ void start(int want) {
 		n = want;
@@ -47,38 +58,30 @@ struct Best {
 		least = -kInf;
 	}
 
-	__device__ __forceinline__ void tile(const float (&x)[E], int pos0, Lds &s, int lane) {
-		float mx = -kInf;
-#pragma unroll
-		for (int e = 0; e < E; e++) mx = __builtin_fmaxf(mx, x[e]);
+	// mx: the lane's largest value
+	__device__ __forceinline__ void tile(const float (&x)[E], float mx, int pos0, Lds &s, int lane) {
 		const uint64_t hits = __ballot(mx > least);
 		if (!hits) return;
 		float t = least;
 		int ties = 0;   // values equal to t that may come in, the first ones
 		if (__popcll(hits) > n) {
-			const uint32_t b = __builtin_bit_cast(uint32_t, mx), key = b >> 31 ? ~b : b | 0x80000000u;
+			const uint32_t key = (uint32_t)(key_of(mx, 0) >> 32);
 			uint32_t k = 0;
 			for (int bit = 31; bit >= 0; bit--) {
 				const uint32_t up = k | 1u << bit;
-				k = __popcll(__ballot(key >= up)) >= n ? up : k;
+				const int above = __popcll(__ballot(key >= up));
+				k = above >= n ? up : k;
+				if (above == n) break;
 			}
-			t = __builtin_bit_cast(float, k >> 31 ? k & 0x7FFFFFFFu : ~k);
+			t = value((uint64_t)k << 32);
 			ties = n;
 		}
 		int c = count;
-		if (lane < count) {
-			s.v[lane] = s.lv[lane];
-			s.i[lane] = s.li[lane];
-		}
 #pragma unroll
 		for (int e = 0; e < E; e++) {
 			const uint64_t m = __ballot(x[e] > t);
 			if (!m) continue;
-			if (x[e] > t) {
-				const int at = c + lanes_below(m);
-				s.v[at] = x[e];
-				s.i[at] = pos0 + ((e >> 2) * 64 + lane) * 4 + (e & 3);
-			}
+			if (x[e] > t) s.key[c + lanes_below(m)] = key_of(x[e], pos0 + ((e >> 2) * 64 + lane) * 4 + (e & 3));
 			c += __popcll(m);
 		}
 		if (ties) {
@@ -96,30 +99,34 @@ struct Best {
 #pragma unroll
 				for (int e = 0; e < 4; e++)
 					if (x[g + e] == t) {
-						if (before < ties) {
-							s.v[c + before] = t;
-							s.i[c + before] = pos0 + ((g >> 2) * 64 + lane) * 4 + e;
-						}
+						if (before < ties) s.key[c + before] = key_of(t, pos0 + ((g >> 2) * 64 + lane) * 4 + e);
 						before++;
 					}
 				c += min(all, ties);
 				ties -= all;
 			}
 		}
+		count = c;
+		if (c > 64 || (c >= n && least == -kInf)) settle(s, lane);
+	}
+
+	// The n best of what waits, in order, in list (and waiting again).
+	__device__ __forceinline__ void settle(Lds &s, int lane) {
+		if (lane < 4) s.key[count + lane] = 0;
 		wave_sync();
-		for (int j = lane; j < c; j += 64) {
-			const float v = s.v[j];
-			const int i = s.i[j];
+		for (int j = lane; j < count; j += 64) {
+			const uint64_t mine = s.key[j];
 			int rank = 0;
-			for (int k = 0; k < c; k++) rank += s.v[k] > v || (s.v[k] == v && s.i[k] < i);
-			if (rank < n) {
-				s.lv[rank] = v;
-				s.li[rank] = i;
+			for (int k = 0; k < count; k += 4) {
+				const ulonglong2 a = *(const ulonglong2 *)(s.key + k), b = *(const ulonglong2 *)(s.key + k + 2);
+				rank += (a.x > mine) + (a.y > mine) + (b.x > mine) + (b.y > mine);
 			}
+			if (rank < n) s.list[rank] = mine;
 		}
 		wave_sync();
-		count = min(c, n);
-		if (count == n) least = s.lv[n - 1];
+		count = min(count, n);
+		if (lane < count) s.key[lane] = s.list[lane];
+		if (count == n) least = value(s.list[n - 1]);
 	}
 };
 
@@ -131,6 +138,7 @@ struct Best {
 constexpr int kPickE = 16;                 // values of a lane's tile
 constexpr int kPickTile = 64 * kPickE;
 constexpr int kPickWaves = 4;
+constexpr int kPickFill = 16;              // waves a CU
 
 // Per row and part: the largest value, the sum of exp(x - it), n_pick values
 // and their tokens, best first, -inf where there are fewer.
@@ -140,13 +148,16 @@ struct Parts {
 	int *i;
 };
 
-__device__ __forceinline__ float exp_(float d) {   // exp(d), d <= 0; NaN stays NaN
-	d = d < -104.0f ? -104.0f : d;   // (0 from there on, -inf among them)
-	const float t = d * 1.44269502f;
-	const float r = __builtin_fmaf(d, 1.44269502f, -t) + d * 1.925963e-8f;   // log2(e) d - t
+// exp(d), d <= 0: 2^t (1 + s), s = d - t log(2) what t's rounding left out.
+__device__ __forceinline__ float exp_(float d) {
+	d = __builtin_fmaxf(d, -104.0f);   // (0 from there on, -inf among them)
+	const float t = d * 1.44269504f;
 	const float e = __builtin_amdgcn_exp2f(t);
-	return __builtin_fmaf(e, r * 0.693147180f, e);
+	return __builtin_fmaf(e, __builtin_fmaf(t, -0.693147181f, d), e);
 }
+
+// The larger of two, NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 __global__ __launch_bounds__(64 * kPickWaves) void beam_part_kernel(const float *__restrict__ logits, int64_t ld, int vocab,
                                                                     const int *__restrict__ done, int parts, int span,
@@ -156,14 +167,12 @@ __global__ __launch_bounds__(64 * kPickWaves) void beam_part_kernel(const float 
 	const int part = blockIdx.x * kPickWaves + wave;
 	const int64_t row = blockIdx.y;
 	if (part >= parts || (done && done[row])) return;
-	const int from = part * span, to = min(vocab, from + span);
-	const float *src = logits + row * ld + from;
-	const __amdgpu_buffer_rsrc_t r = stream_rsrc(uniform_ptr(src), (uint32_t)(to - from) * 4u);
+	const int from = part * span, n = min(vocab - from, span);
+	const __amdgpu_buffer_rsrc_t r = stream_rsrc(uniform_ptr(logits + row * ld + from), (uint32_t)n * 4u);
 	Best<kPickE> best;
 	best.start(n_pick);
 	float top = -kInf;
 	double sum = 0.0;
-	bool bad = false;
 	float x[kPickE], y[kPickE];
 	auto load = [&](float(&z)[kPickE], int t) {
 #pragma unroll
@@ -176,29 +185,29 @@ __global__ __launch_bounds__(64 * kPickWaves) void beam_part_kernel(const float 
 		}
 	};
 	auto use = [&](float(&z)[kPickE], int t) {
-		if (t + kPickTile > to - from) {
+		if (t + kPickTile > n) {
 #pragma unroll
-			for (int e = 0; e < kPickE; e++) z[e] = t + ((e >> 2) * 64 + lane) * 4 + (e & 3) < to - from ? z[e] : -kInf;
+			for (int e = 0; e < kPickE; e++) z[e] = t + ((e >> 2) * 64 + lane) * 4 + (e & 3) < n ? z[e] : -kInf;
 		}
-		float mx = -kInf;
+		float mx = z[0];
 #pragma unroll
-		for (int e = 0; e < kPickE; e++) mx = __builtin_fmaxf(mx, z[e]);
-		mx = wave_max(mx);
-		if (mx > top) {
-			sum *= exp((double)top - (double)mx);
-			top = mx;
+		for (int e = 1; e < kPickE; e++) mx = max_nan(mx, z[e]);
+		if (__any(mx != mx)) {   // the row has no continuations, whatever else it holds
+			sum = __builtin_nan("");
+			return;
+		}
+		const float m = wave_max(mx);
+		if (m > top) {
+			sum *= exp((double)top - (double)m);
+			top = m;
 		}
 		if (top > -kInf) {
 #pragma unroll
 			for (int e = 0; e < kPickE; e += 4)
 				sum += (double)((exp_(z[e] - top) + exp_(z[e + 1] - top)) + (exp_(z[e + 2] - top) + exp_(z[e + 3] - top)));
-		} else {
-#pragma unroll
-			for (int e = 0; e < kPickE; e++) bad |= z[e] != z[e];
 		}
-		best.tile(z, from + t, lds[wave], lane);
+		best.tile(z, mx, from + t, lds[wave], lane);
 	};
-	const int n = to - from;
 	load(x, 0);
 	for (int t = 0; t < n; t += 2 * kPickTile) {
 		if (t + kPickTile < n) load(y, t + kPickTile);
@@ -207,21 +216,22 @@ __global__ __launch_bounds__(64 * kPickWaves) void beam_part_kernel(const float 
 		if (t + 2 * kPickTile < n) load(x, t + 2 * kPickTile);
 		use(y, t + kPickTile);
 	}
+	best.settle(lds[wave], lane);
 #pragma unroll
 	for (int k = 1; k < 64; k <<= 1) sum += __shfl_xor(sum, k);
-	if (__any(bad)) sum = __builtin_nan("");
 	const int64_t rec = row * parts + part;
 	if (lane == 0) {
 		out.top[rec] = top;
 		out.sum[rec] = sum;
 	}
 	if (lane < n_pick) {
-		out.v[rec * n_pick + lane] = lane < best.count ? lds[wave].lv[lane] : -kInf;
-		out.i[rec * n_pick + lane] = lane < best.count ? lds[wave].li[lane] : -1;
+		const uint64_t key = lane < best.count ? lds[wave].list[lane] : 0;
+		out.v[rec * n_pick + lane] = lane < best.count ? best.value(key) : -kInf;
+		out.i[rec * n_pick + lane] = best.place(key);
 	}
 }
 
-constexpr int kJoinE = 4;
+constexpr int kJoinE = 8;
 
 // A wave a beam: its sum and its n_pick best; then the request's best of those.
 __global__ __launch_bounds__(64 * HAKO_MAX_BEAMS) void beam_join_kernel(const float *__restrict__ score, const int *__restrict__ done,
@@ -234,42 +244,62 @@ __global__ __launch_bounds__(64 * HAKO_MAX_BEAMS) void beam_join_kernel(const fl
 	const int lane = threadIdx.x & 63, b = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	const int64_t req = blockIdx.x, row = req * n_beams + b;
 	const double old = (double)score[row];
+	const int ended = done ? done[row] : 0;
+	// the parts' lists in the order of their tokens; in a list equal values are in that order too
+	const int64_t rec = row * parts;
+	const int n_list = parts * n_pick;
+	const __amdgpu_buffer_rsrc_t r = stream_rsrc(uniform_ptr(in.v + rec * n_pick), (uint32_t)n_list * 4u);
+	float x[kJoinE];
+	auto load = [&](int t) {
+#pragma unroll
+		for (int g = 0; g < kJoinE / 4; g++) {
+			const uint4 w = ld_b128(r, 4u * (uint32_t)(t + (g * 64 + lane) * 4));
+			const float z[4] = {__builtin_bit_cast(float, w.x), __builtin_bit_cast(float, w.y), __builtin_bit_cast(float, w.z), __builtin_bit_cast(float, w.w)};
+#pragma unroll
+			for (int e = 0; e < 4; e++) x[4 * g + e] = z[e];
+		}
+	};
+	load(0);
+	// (an ended beam's are whatever was there)
+	const float top0 = lane < parts ? in.top[rec + lane] : -kInf;
+	const double sum0 = lane < parts ? in.sum[rec + lane] : 0.0;
 	if (threadIdx.x < HAKO_MAX_PICK) pick[threadIdx.x] = -1;
-	if (done && done[row]) {
+	if (ended) {
 		if (lane < n_pick) {
 			val[b * n_pick + lane] = lane == 0 ? old : -(double)kInf;
 			tok[b * n_pick + lane] = eos;
 		}
 	} else {
-		const int64_t rec = row * parts;
-		float top = -kInf;
-		for (int p = lane; p < parts; p += 64) top = __builtin_fmaxf(top, in.top[rec + p]);
+		float top = top0;
+		for (int p = lane + 64; p < parts; p += 64) top = __builtin_fmaxf(top, in.top[rec + p]);
 		top = wave_max(top);
-		double sum = 0.0;
-		for (int p = lane; p < parts; p += 64) {
+		double sum = top0 == -kInf ? sum0 : sum0 * (double)exp_(top0 - top);
+		for (int p = lane + 64; p < parts; p += 64) {
 			const float t = in.top[rec + p];
-			sum += t == -kInf ? in.sum[rec + p] : in.sum[rec + p] * exp((double)t - (double)top);
+			const double w = in.sum[rec + p];
+			sum += t == -kInf ? w : w * (double)exp_(t - top);
 		}
 #pragma unroll
 		for (int k = 1; k < 64; k <<= 1) sum += __shfl_xor(sum, k);
 		const double lse = (double)top + log(sum);
-		// the parts' lists in the order of their tokens; in a list equal values are in that order too
 		Best<kJoinE> best;
 		best.start(n_pick);
-		const int n = parts * n_pick;
-		for (int t = 0; t < n; t += 64 * kJoinE) {
-			float x[kJoinE];
+		for (int t = 0; t < n_list; t += 64 * kJoinE) {
+			float mx = -kInf;
 #pragma unroll
 			for (int e = 0; e < kJoinE; e++) {
-				const int at = t + lane * 4 + e;
-				x[e] = at < n ? in.v[rec * n_pick + at] : -kInf;
+				x[e] = t + ((e >> 2) * 64 + lane) * 4 + (e & 3) < n_list ? x[e] : -kInf;
+				mx = __builtin_fmaxf(mx, x[e]);
 			}
-			best.tile(x, t, lds[b], lane);
+			best.tile(x, mx, t, lds[b], lane);
+			if (t + 64 * kJoinE < n_list) load(t + 64 * kJoinE);
 		}
+		best.settle(lds[b], lane);
 		if (lane < n_pick) {
 			const bool on = lane < best.count;
-			val[b * n_pick + lane] = on ? old + ((double)lds[b].lv[lane] - lse) : -(double)kInf;
-			tok[b * n_pick + lane] = on ? in.i[rec * n_pick + lds[b].li[lane]] : -1;
+			const uint64_t key = on ? lds[b].list[lane] : 0;
+			val[b * n_pick + lane] = on ? old + ((double)best.value(key) - lse) : -(double)kInf;
+			tok[b * n_pick + lane] = on ? in.i[rec * n_pick + best.place(key)] : -1;
 		}
 	}
 	__syncthreads();
@@ -279,6 +309,7 @@ __global__ __launch_bounds__(64 * HAKO_MAX_BEAMS) void beam_join_kernel(const fl
 		const double v = val[f];
 		if (!(v > -(double)kInf)) continue;
 		int rank = 0;
+#pragma unroll 8
 		for (int g = 0; g < n; g++) rank += val[g] > v || (val[g] == v && g < f);
 		if (rank < n_pick) pick[rank] = f;
 	}
@@ -322,6 +353,7 @@ struct Shape {
 // A workgroup takes units of 16 bytes (and scales) of one head's rows in all
 // of a request's slots at once: every load comes before the first store, so any
 // map of places is good.
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 template <int B>
 __global__ __launch_bounds__(256) void reorder_kernel(Layers layers, Shape c, const int *__restrict__ slot,
                                                       const int *__restrict__ parent, int n_beams,
@@ -349,13 +381,13 @@ __global__ __launch_bounds__(256) void reorder_kernel(Layers layers, Shape c, co
 	float *scales = is_v ? layers.vs[layer] : layers.ks[layer];
 	const int64_t units = (int64_t)(to - from) * (c.row / 16), first = (int64_t)from * (c.row / 16);
 	for (int64_t u = (int64_t)blockIdx.z * 256 + threadIdx.x; u < units; u += (int64_t)gridDim.z * 256) {
-		uint4 x[B];
+		u4 x[B];
 #pragma unroll
 		for (int b = 0; b < B; b++)
-			if (src[b] >= 0) x[b] = *(const uint4 *)(codes + src[b] * c.row + 16 * (first + u));
+			if (src[b] >= 0) x[b] = *(const u4 *)(codes + src[b] * c.row + 16 * (first + u));
 #pragma unroll
 		for (int b = 0; b < B; b++)
-			if (src[b] >= 0) *(uint4 *)(codes + dst[b] * c.row + 16 * (first + u)) = x[b];
+			if (src[b] >= 0) __builtin_nontemporal_store(x[b], (u4 *)(codes + dst[b] * c.row + 16 * (first + u)));
 	}
 	for (int64_t u = (int64_t)blockIdx.z * 256 + threadIdx.x; u < to - from; u += (int64_t)gridDim.z * 256) {
 		float x[B];
@@ -394,18 +426,17 @@ __global__ __launch_bounds__(64 * kKeepWaves) void keep_kernel(Layers layers, Sh
 	uint4 x[16];
 #pragma unroll
 	for (int i = 0; i < 16; i++) {
-		if (i * 64 >= rows * units) break;
 		const int u = i * 64 + lane, d = u >> lg, f = __shfl(from, d & 63);
-		if (d < rows && f >= 0) x[i] = *(const uint4 *)(codes + (int64_t)f * c.row + 16 * (u & (units - 1)));
+		x[i] = make_uint4(0, 0, 0, 0);
+		if (i * 64 < rows * units && d < rows && f >= 0) x[i] = *(const uint4 *)(codes + (int64_t)f * c.row + 16 * (u & (units - 1)));
 	}
 	// every load's data is here before the first store
 	asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 	if (from >= 0) scales[lane] = y;
 #pragma unroll
 	for (int i = 0; i < 16; i++) {
-		if (i * 64 >= rows * units) break;
 		const int u = i * 64 + lane, d = u >> lg, f = __shfl(from, d & 63);
-		if (d < rows && f >= 0) *(uint4 *)(codes + (int64_t)d * c.row + 16 * (u & (units - 1))) = x[i];
+		if (i * 64 < rows * units && d < rows && f >= 0) *(uint4 *)(codes + (int64_t)d * c.row + 16 * (u & (units - 1))) = x[i];
 	}
 }
 
@@ -545,7 +576,7 @@ int hako_gpu_beam_select(const float *logits, int64_t ld, int vocab, const float
 	if (n_req == 0) return ok();
 	const int rows = n_req * n_beams;
 	// parts of whole tiles, until the waves fill the chip
-	const int tiles = (vocab + kPickTile - 1) / kPickTile, want = (8 * cu_count() + rows - 1) / rows;
+	const int tiles = (vocab + kPickTile - 1) / kPickTile, want = (kPickFill * cu_count() + rows - 1) / rows;
 	const int span = (tiles + want - 1) / want * kPickTile, parts = (vocab + span - 1) / span;
 	const size_t recs = (size_t)rows * parts;
 	void *p = nullptr;
@@ -578,7 +609,7 @@ int hako_gpu_kv_reorder(const hako_gpu_kv *kv, int n_kv, const int *slot, const 
 	if (int rc = heads_check(n_kv, c, n_req)) return rc;
 	if (int rc = each_layers(kv, n_kv, [&](const Layers &l, int n) {
 		    const int64_t heads = (int64_t)n * c.kvh * 2;
-		    const int64_t most = ((int64_t)c.max_seq * (c.row / 16) + 255) / 256, fill = 8 * cu_count() / (heads * n_req) + 1;
+		    const int64_t most = ((int64_t)c.max_seq * (c.row / 16) + 255) / 256, fill = 16 * cu_count() / (heads * n_req) + 1;
 		    const dim3 grid((unsigned)heads, n_req, (unsigned)(fill < most ? fill : most));
 		    if (n_beams <= 4)
 			    hipLaunchKernelGGL(reorder_kernel<4>, grid, dim3(256), 0, stream(), l, c, slot, parent, n_beams, since, len);
