@@ -28,11 +28,12 @@ __device__ __forceinline__ int lanes_below(uint64_t m) {
 // register 4 i + c; equal ones rank by position. Of a tile only what may still
 // be among the n best is kept: values above the n-th best known so far, and
 // where more than n lanes have such values, above the n-th largest of the
-// lanes' own maxima, or what tells it from the next (found bit by bit, a ballot
-// each), which at most n lanes exceed. So no tile adds more than n (E + 1), whatever the values are, and an
-// ordinary one about n at first and hardly any later. What is kept waits in LDS
-// until there are more than 64, and is then ranked: a lane a value, each
-// against all, as 64-bit keys of value and position.
+// lanes' own maxima, or what tells it from the next (found bit by bit, a
+// ballot each), which at most n lanes exceed. So no tile adds more than
+// n (E + 1), whatever the values are, and an ordinary one about n at first and
+// hardly any later. What is kept waits in LDS until there are more than 64, and
+// is then ranked: a lane a value, each against all, as 64-bit keys of value and
+// position.
 template <int E>
 struct Best {
 	struct Lds {
@@ -240,7 +241,7 @@ __global__ __launch_bounds__(64 * HAKO_MAX_BEAMS) void beam_join_kernel(const fl
                                                                         float *__restrict__ score_out, int *__restrict__ done_out) {
 	__shared__ typename Best<kJoinE>::Lds lds[HAKO_MAX_BEAMS];
 	__shared__ double val[HAKO_MAX_BEAMS * HAKO_MAX_PICK];
-	__shared__ int tok[HAKO_MAX_BEAMS * HAKO_MAX_PICK], pick[HAKO_MAX_PICK];
+	__shared__ int tok[HAKO_MAX_BEAMS * HAKO_MAX_PICK], rank[HAKO_MAX_BEAMS * HAKO_MAX_PICK], pick[HAKO_MAX_PICK];
 	const int lane = threadIdx.x & 63, b = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	const int64_t req = blockIdx.x, row = req * n_beams + b;
 	const double old = (double)score[row];
@@ -302,17 +303,25 @@ __global__ __launch_bounds__(64 * HAKO_MAX_BEAMS) void beam_join_kernel(const fl
 			tok[b * n_pick + lane] = on ? in.i[rec * n_pick + best.place(key)] : -1;
 		}
 	}
-	__syncthreads();
-	// a beam's list falls, so that the place in it stands for logits and tokens
 	const int n = n_beams * n_pick;
-	for (int f = threadIdx.x; f < n; f += blockDim.x) {
+	if (lane < n_pick) rank[b * n_pick + lane] = 0;
+	__syncthreads();
+	// How many of this wave's list go before each value: the lists fall (so that a place in one stands for logits and
+	// tokens), and equal values go by list.
+	for (int f = lane; f < n; f += 64) {
 		const double v = val[f];
-		if (!(v > -(double)kInf)) continue;
-		int rank = 0;
-#pragma unroll 8
-		for (int g = 0; g < n; g++) rank += val[g] > v || (val[g] == v && g < f);
-		if (rank < n_pick) pick[rank] = f;
+		const int own = f - b * n_pick;
+		int before = 0;
+#pragma unroll
+		for (int step = HAKO_MAX_PICK; step; step >>= 1) {
+			const double x = val[b * n_pick + min(before + step, n_pick) - 1];
+			before += before + step <= n_pick && (x > v || (x == v && own >= 0)) ? step : 0;
+		}
+		atomicAdd(&rank[f], own >= 0 && own < n_pick ? own : before);
 	}
+	__syncthreads();
+	for (int f = threadIdx.x; f < n; f += blockDim.x)
+		if (val[f] > -(double)kInf && rank[f] < n_pick) pick[rank[f]] = f;
 	__syncthreads();
 	if (threadIdx.x >= 64) return;
 	const int f = lane < n_pick ? pick[lane] : -1, from = f < 0 ? -1 : f / n_pick;
