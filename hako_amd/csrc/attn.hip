@@ -22,6 +22,8 @@
 #include <algorithm>
 #include <float.h>
 #include <new>
+#include <stddef.h>
+#include <type_traits>
 #include <vector>
 
 // CALL(HD, Q8) for a cache's head size and type.
@@ -37,7 +39,6 @@ constexpr int kSeqs = 48;        // sequences of one prompt launch (by value in 
 constexpr int kItems = 480;      // items of a launch whose order the host sets (likewise)
 constexpr int kWsAttn = 7;       // library workspace slot of the records
 constexpr int kKeys = 64;        // keys per chunk of the tiled kernel
-constexpr int kTileWaves = 8;    // its waves per workgroup, 32 rows each
 constexpr int kLongPart = 2048;  // keys of a part where sequences alone fill the chip
 constexpr int kWaves = 4;        // waves per workgroup of the direct and the single-token kernel
 // M is a whole number not below what it was taken from (the maximum of the
@@ -124,15 +125,15 @@ struct Within {
 struct Nodes {
 	static constexpr bool kHi = false, kBlanks = true;
 	int lim;
-	uint64_t bits;
-	uint32_t w;
+	uint64_t bits, w;
 	__device__ __forceinline__ void at(int k, int top, bool) {
 		const int s = k - lim, n = top - k;
-		if (s >= 0) w = s < 64 ? (uint32_t)(bits >> s) : 0;
-		else w = s > -32 ? (uint32_t)(bits << -s) | ((1u << -s) - 1) : ~0u;
-		w = n >= 32 ? w : n > 0 ? w & ((1u << n) - 1) : 0;
+		if (s >= 0) w = s < 64 ? bits >> s : 0;
+		else w = s > -64 ? bits << -s | ((1ull << -s) - 1) : ~0ull;
+		w = n >= 64 ? w : n > 0 ? w & ((1ull << n) - 1) : 0;
 	}
 	__device__ __forceinline__ bool sees(int i) const { return w >> i & 1; }
+	__device__ __forceinline__ bool reaches(int, bool, int) const { return true; }
 	template <int K>
 	__device__ __forceinline__ bool masks(int k, int top, bool, int lo, int) const { return k + K > min(lo, top); }
 };
@@ -143,6 +144,13 @@ struct Nodes {
 __device__ __forceinline__ int fresh(int v) {
 	asm volatile("" : "+v"(v));
 	return v;
+}
+
+// What a wave wrote to LDS is there for its other lanes.
+__device__ __forceinline__ void wave_sync() {
+	__builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+	__builtin_amdgcn_wave_barrier();
+	__builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -283,14 +291,14 @@ __device__ __forceinline__ int key_row(int key) { return (key & ~12) | ((key >> 
 template <int HD>
 __device__ __forceinline__ int dim_row(int dim) { return (dim & 3) * (HD / 4) + (dim >> 2); }
 
-template <int HD, bool Q8>
+template <int HD, bool Q8, int W>
 struct Stage {
-	static constexpr int EB = Q8 ? 1 : 2, NT = 64 * kTileWaves;
+	static constexpr int EB = Q8 ? 1 : 2, NT = 64 * W;
 	static constexpr int KU = kKeys * HD * EB / 16, KL = (KU + NT - 1) / NT;   // 16-byte key loads of a chunk, per thread
 	static constexpr int VQ = HD / 4, VK = 4;                                  // dim quads; a thread takes 4 keys x 4 dims
-	static constexpr int VT = kKeys / VK * VQ;                                 // threads that stage values (512 or 256)
+	static constexpr int VT = kKeys / VK * VQ, VL = (VT + NT - 1) / NT;        // such pieces of the values (512 or 256), per thread
 	uint4 k[KL];
-	uint32_t v[VK][EB];
+	uint32_t v[VL][VK][EB];
 	float ks, vs;
 
 	__device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t kr, __amdgpu_buffer_rsrc_t vr, __amdgpu_buffer_rsrc_t ksr,
@@ -300,19 +308,21 @@ struct Stage {
 			const int u = tid + NT * i;   // 16-byte unit of the chunk
 			k[i] = ld_b128(kr, KU % NT && u >= KU ? kBufNone : (uint32_t)key0 * (HD * EB) + 16u * u);
 		}
-		if (VT == NT || tid < VT) {
-			const int d = tid % VQ, kg = tid / VQ;
-			const uint32_t off = ((uint32_t)(key0 + VK * kg) * HD + 4 * d) * EB;
 #pragma unroll
-			for (int j = 0; j < VK; j++) {
-				if (Q8) v[j][0] = __builtin_amdgcn_raw_buffer_load_b32(vr, (int)(off + j * HD), 0, 0);
-				else {
-					const uint2 t = ld_b64(vr, off + j * HD * 2);
-					v[j][0] = t.x;
-					v[j][EB - 1] = t.y;
+		for (int i = 0; i < VL; i++)
+			if (VT % NT == 0 || tid < VT) {
+				const int d = (tid + NT * i) % VQ, kg = (tid + NT * i) / VQ;
+				const uint32_t off = ((uint32_t)(key0 + VK * kg) * HD + 4 * d) * EB;
+#pragma unroll
+				for (int j = 0; j < VK; j++) {
+					if (Q8) v[i][j][0] = __builtin_amdgcn_raw_buffer_load_b32(vr, (int)(off + j * HD), 0, 0);
+					else {
+						const uint2 t = ld_b64(vr, off + j * HD * 2);
+						v[i][j][0] = t.x;
+						v[i][j][EB - 1] = t.y;
+					}
 				}
 			}
-		}
 		if (tid < kKeys) {
 			ks = ld_f32(ksr, 4u * (uint32_t)(key0 + tid));
 			vs = ld_f32(vsr, 4u * (uint32_t)(key0 + tid));
@@ -341,13 +351,15 @@ struct Stage {
 				*(uint4 *)(k_s + key_row(key) * kKeyRow<HD> + 16 * c) = k[i];
 			}
 		}
-		if (VT == NT || tid < VT) {
-			const int d = tid % VQ, kg = tid / VQ;
+#pragma unroll
+		for (int n = 0; n < VL; n++) {
+			if (VT % NT && tid >= VT) break;
+			const int d = (tid + NT * n) % VQ, kg = (tid + NT * n) / VQ;
 			h2 t[4][VK / 2];   // [dim][key pair]
 #pragma unroll
 			for (int p = 0; p < VK / 2; p++) {
 				if (Q8) {
-					const uint32_t a = v[2 * p][0] ^ kFlip, b = v[2 * p + 1][0] ^ kFlip;
+					const uint32_t a = v[n][2 * p][0] ^ kFlip, b = v[n][2 * p + 1][0] ^ kFlip;
 					const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x05010400u), hi = __builtin_amdgcn_perm(b, a, 0x07030602u);
 					t[0][p] = bytes_h2(lo, kLo2);
 					t[1][p] = bytes_h2(lo, kHi2);
@@ -356,7 +368,7 @@ struct Stage {
 				} else {
 #pragma unroll
 					for (int w = 0; w < 2; w++) {
-						const uint32_t a = v[2 * p][w * (EB - 1)], b = v[2 * p + 1][w * (EB - 1)];
+						const uint32_t a = v[n][2 * p][w * (EB - 1)], b = v[n][2 * p + 1][w * (EB - 1)];
 						t[2 * w][p] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(b, a, 0x05040100u));
 						t[2 * w + 1][p] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(b, a, 0x07060302u));
 					}
@@ -383,7 +395,7 @@ struct Stage {
 
 // One wave's 32 rows over the chunks of a part. lim: the lane's row sees keys
 // (positions) below it; out: O^T (value sums), M and l.
-template <int HD, bool Q8>
+template <int HD, bool Q8, int W>
 struct Tile {
 	static constexpr int KS = HD / 16, DT = HD / 32;
 	static constexpr int kKB = kKeys * kKeyRow<HD>, kVB = HD * kDimRow;
@@ -393,7 +405,7 @@ struct Tile {
 		alignas(16) float ks[2][kKeys];
 		alignas(16) float vs[2][kKeys];
 		float e[2];
-		float be[64 * kTileWaves];   // e of the rows' bases
+		float be[64 * W];   // e of the rows' bases
 	};
 	h8 qh[KS], ql[KS];
 	float esc;      // 2^e of the row
@@ -424,12 +436,7 @@ struct Tile {
 		esc = __builtin_ldexpf(1.0f, e);
 #pragma unroll
 		for (int s = 0; s < KS; s++) split_q(x + 8 * s, e, qh[s], ql[s]);
-#pragma unroll
-		for (int d = 0; d < DT; d++)
-#pragma unroll
-			for (int v = 0; v < 16; v++) o[d][v] = 0.0f;
-		M = kNone;
-		l = 0.0f;
+		clear();
 		big = 0;
 	}
 
@@ -560,13 +567,14 @@ struct Tile {
 		}
 	}
 
-	// Chunks [c0, c1) of a tile's span. lo, hi: the least and greatest lim of the wave's rows.
-	template <class See>
+	// Chunks [c0, c1) of a tile's span for the queries that ask(lane) takes up while the first chunk's codes are on their
+	// way. lo, hi: the least and greatest lim of the wave's rows.
+	template <class See, class Ask>
 	__device__ __forceinline__ void chunks(const AttnKv &c, const Span &sp, int c0, int c1, const See &row, int lo, int hi, Lds &s,
-	                                       int tid) {
+	                                       int tid, Ask ask) {
 		constexpr int EB = Q8 ? 1 : 2;
 		const int lane = tid & 63;
-		Stage<HD, Q8> st;
+		Stage<HD, Q8, W> st;
 		auto load = [&](int ch) {
 			const size_t r = sp.first(ch) ? sp.r0 : sp.r1;
 			const uint32_t n = (uint32_t)sp.top(ch);   // rows past it read as zeros
@@ -575,8 +583,10 @@ struct Tile {
 		};
 		// A wave's registers hold the codes two chunks on from the buffer that is read. The waves of a SIMD (w, w + 4)
 		// put them into LDS at opposite ends of a chunk, so that one has vector work while the other has matrix work.
+		if (c0 < c1) load(c0);
+		__builtin_amdgcn_sched_barrier(0);
+		ask(lane);
 		if (c0 < c1) {
-			load(c0);
 			st.store(s.k[0], s.v[0], s.ks[0], s.vs[0], &s.e[0], tid);
 			if (c0 + 1 < c1) load(c0 + 1);
 		}
@@ -603,14 +613,42 @@ struct Tile {
 		l += __shfl_xor(l, 32);
 	}
 
-	// The row's value sums times f to dst: row 8 a + 4 h + b of tile d is dim_row 32 d + ..
-	__device__ __forceinline__ void put(float *dst, float f, int lane) const {
-		const int h = lane >> 5;
+	// A row that has seen nothing.
+	__device__ __forceinline__ void clear() {
 #pragma unroll
-		for (int v = 0; v < 4 * DT; v++) {
-			const int r = 8 * (v >> 2) + 4 * h + (v & 3);   // quad of dims
-			*(float4 *)(dst + 4 * r) = DT == 4 ? make_float4(o[0][v] * f, o[1][v] * f, o[2 % DT][v] * f, o[3 % DT][v] * f)
-			                                   : make_float4(o[0][v] * f, o[0][v + 8] * f, o[1][v] * f, o[1][v + 8] * f);
+		for (int d = 0; d < DT; d++)
+#pragma unroll
+			for (int v = 0; v < 16; v++) o[d][v] = 0.0f;
+		M = kNone;
+		l = 0.0f;
+	}
+
+	// The rows' value sums times f to their places, dst for the lane's (null: nowhere): row 8 a + 4 h + b of tile d is
+	// dim_row 32 d + .. Half of the dims at a time pass through LDS, the chunks' place, so that stores are of whole lines
+	// (a lane's own stores, 16 bytes to each of 64 rows, took 5 us of an item of 148, these 1.5).
+	__device__ __forceinline__ void put(float *dst, float f, Lds &s, int tid) const {
+		constexpr int L = HD / 8, R = 2 * HD + 16, NV = 2 * DT;
+		static_assert(W * 32 * R <= 2 * kKB + 2 * kVB && offsetof(Lds, v) == 2 * kKB, "rows in the place of the chunks");
+		const int lane = tid & 63, i = lane & 31, h = lane >> 5;
+		uint8_t *buf = s.k[0] + (tid >> 6) * (32 * R);
+		const uint64_t at = (uint64_t)(uintptr_t)dst;
+#pragma unroll
+		for (int p = 0; p < 2; p++) {
+#pragma unroll
+			for (int v = NV * p; v < NV * p + NV; v++) {
+				const int r = 8 * (v >> 2) + 4 * h + (v & 3) - HD / 8 * p;   // quad of dims
+				*(float4 *)(buf + i * R + 16 * r) = DT == 4 ? make_float4(o[0][v] * f, o[1][v] * f, o[2 % DT][v] * f, o[3 % DT][v] * f)
+				                                            : make_float4(o[0][v] * f, o[0][v + 8] * f, o[1][v] * f, o[1][v + 8] * f);
+			}
+			wave_sync();
+#pragma unroll
+			for (int j = 0; j < L / 2; j++) {
+				const int row = j * (64 / L) + lane / L;
+				const float4 x = *(const float4 *)(buf + row * R + 16 * (lane % L));
+				const uint64_t to = (uint64_t)(uint32_t)__shfl((int)(uint32_t)at, row) | ((uint64_t)(uint32_t)__shfl((int)(at >> 32), row) << 32);
+				if (to) *(float4 *)((float *)(uintptr_t)to + HD / 2 * p + 4 * (lane % L)) = x;
+			}
+			wave_sync();
 		}
 	}
 };
@@ -1100,10 +1138,10 @@ __device__ __forceinline__ auto row_sees(const AttnKv &c, int lim) {
 	else return Below{lim};
 }
 
-template <int HD, bool Q8, bool WIN>
-__global__ __launch_bounds__(64 * kTileWaves, 2) void prompt_kernel(AttnKv c, SeqTab t, ItemTab order, float *out, int64_t ldo, const float *q,
+template <int HD, bool Q8, bool WIN, int W>
+__global__ __launch_bounds__(64 * W, 2) void prompt_kernel(AttnKv c, SeqTab t, ItemTab order, float *out, int64_t ldo, const float *q,
                                                         int64_t ldq, int G, float scale, Records rec) {
-	__shared__ typename Tile<HD, Q8>::Lds s;
+	__shared__ typename Tile<HD, Q8, W>::Lds s;
 	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
 	const int kvh = blockIdx.x % c.kvh;
 	Item x;
@@ -1113,18 +1151,16 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void prompt_kernel(AttnKv c, Se
 	const int lim = on ? t.start[x.sq] + x.tok0 + tok + 1 : 0;
 	const int lo = wave_min_i(on ? lim : 0x7FFFFFFF), hi = wave_max_i(lim);
 	const int64_t row = (int64_t)t.row[x.sq] + x.tok0 + tok;
-	Tile<HD, Q8> w;
-	w.query(on ? q + row * ldq + head * HD : nullptr, scale, lane);
+	Tile<HD, Q8, W> w;
 	w.chunks(c, span_of<kKeys, WIN>(c, kvh, x.slot, t.start[x.sq] + x.tok0, t.tile_tokens, x.end), x.c0, x.c1, row_sees<WIN>(c, lim), lo, hi,
-	         s, tid);
-	if (!on) return;
+	         s, tid, [&](int ln) { w.query(on ? q + row * ldq + head * HD : nullptr, scale, ln); });
 	if (x.parts == 1) {
-		w.put(out + row * ldo + head * HD, 1.0f / w.l, lane);
+		w.put(on ? out + row * ldo + head * HD : nullptr, 1.0f / w.l, s, tid);
 		return;
 	}
 	const size_t r0 = record_of(t, x, tok, c.kvh * G, head);
-	w.put(rec.o + r0 * HD, 1.0f, lane);
-	if (lane < 32) rec.put(r0, {w.M, w.big ? s.be[tid] : 0.0f}, w.l);
+	w.put(on ? rec.o + r0 * HD : nullptr, 1.0f, s, tid);
+	if (on && lane < 32) rec.put(r0, {w.M, w.big ? s.be[tid] : 0.0f}, w.l);
 }
 
 // The direct kernel's items: tiles of 32 rows, parts of `unit` steps of 32 keys.
@@ -1902,7 +1938,7 @@ int prompt_launch(const AttnKv &c, const Reach &reach, SeqTab &t, float *out, in
 		recs += (int64_t)(t.len[s] - first) * H * t.nsplit[s];
 	}
 	t.item[t.n] = (int)items;
-	if (items * c.kvh > kMaxThreads / (64 * kTileWaves) || recs > 0xFFFFFFFFll || (int64_t)t.join[t.n] * H * (HD / 4) > kMaxThreads)
+	if (items * c.kvh > kMaxThreads / 512 || recs > 0xFFFFFFFFll || (int64_t)t.join[t.n] * H * (HD / 4) > kMaxThreads)
 		return set_error(HAKO_GPU_EINVAL, "%lld tiles and %lld records in one call", (long long)(items * c.kvh), (long long)recs);
 	Records rec{};
 	if (recs)
@@ -1940,6 +1976,21 @@ int64_t all_steps(const AttnKv &c, const Reach &reach, const SeqTab &t, int toke
 	return n * c.kvh;
 }
 
+// The tiled kernel of W waves; as many workgroups run at once as fill a CU with eight.
+template <int HD, bool Q8, bool WIN, int W>
+int prompt_tiled(const AttnKv &c, const Reach &reach, SeqTab &t, float *out, int64_t ldo, const float *q, int64_t ldq, int H, float scale) {
+	const int G = H / c.kvh;
+	const int64_t slots = 8 / W * cu_count(), all = all_steps<kKeys, WIN>(c, reach, t, 32 * W / G);
+	return prompt_launch<HD, Q8, kKeys, WIN>(
+	    c, reach, t, out, ldo, H, 32 * W, std::max<int64_t>(4, (3 * all + 2 * slots - 1) / (2 * slots)),
+	    [&](int64_t items, const Records &rec) {
+		    ItemTab order;
+		    if (const int n = sort_items<kKeys, WIN>(t, reach, order)) items = n;
+		    hipLaunchKernelGGL((prompt_kernel<HD, Q8, WIN, W>), dim3((unsigned)(items * c.kvh)), dim3(64 * W), 0, stream(), c, t, order, out,
+		                       ldo, q, ldq, G, scale * kLog2e, rec);
+	    });
+}
+
 // Which kernel (one MI355X, heads of 128, us by the direct / the tiled one):
 //   tokens        wave-steps (32 rows x 32 keys)   8 bits        16 bits
 //   7B heads  200       0.8 thousand               9.3 / 20.5    9.9 / 20.5
@@ -1967,17 +2018,8 @@ int prompt(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, const float *q, 
 	const int64_t cu = cu_count(), slots = 2 * cu;   // workgroups of the direct kernel that run at once
 	const Reach reach = {c.prefix_len, c.window, c.sinks};
 	const int64_t steps = all_steps<32, WIN>(c, reach, t, 32 / G);
-	if (g_attn_prompt ? g_attn_prompt == 2 : steps > 55 * 4 * cu) {
-		const int64_t all = all_steps<kKeys, WIN>(c, reach, t, 32 * kTileWaves / G);
-		return prompt_launch<HD, Q8, kKeys, WIN>(
-		    c, reach, t, out, ldo, H, 32 * kTileWaves, std::max<int64_t>(4, (3 * all + 2 * cu - 1) / (2 * cu)),
-		    [&](int64_t items, const Records &rec) {
-			    ItemTab order;
-			    if (const int n = sort_items<kKeys, WIN>(t, reach, order)) items = n;
-			    hipLaunchKernelGGL((prompt_kernel<HD, Q8, WIN>), dim3((unsigned)(items * c.kvh)), dim3(64 * kTileWaves), 0, stream(), c, t, order,
-			                       out, ldo, q, ldq, G, scale * kLog2e, rec);
-		    });
-	}
+	if (WIN && g_attn_prompt == 3) return prompt_tiled<HD, Q8, WIN, WIN ? 4 : 8>(c, reach, t, out, ldo, q, ldq, H, scale);
+	if (g_attn_prompt ? g_attn_prompt == 2 : steps > 55 * 4 * cu) return prompt_tiled<HD, Q8, WIN, 8>(c, reach, t, out, ldo, q, ldq, H, scale);
 	int64_t tiles = 0;
 	for (int s = 0; s < t.n; s++) tiles += (t.len[s] + 32 / G - 1) / (32 / G);
 	const int64_t share = (steps + slots - 1) / slots;
@@ -2001,9 +2043,10 @@ __device__ __forceinline__ bool tree_place(const AttnKv &c, const int *slot, con
 	end = on ? min(b + N, c.max_seq) : 0;
 	return on;
 }
-// Steps per part of a tile with nc steps, at least one for each wave.
+// Steps per part of a tile with nc steps, in whole rounds of R.
+template <int R>
 __device__ __forceinline__ int tree_part(int nc, int parts) {
-	return max(((nc + parts - 1) / parts + kWaves - 1) / kWaves * kWaves, kWaves);
+	return max(((nc + parts - 1) / parts + R - 1) / R * R, R);
 }
 
 template <int HD, bool Q8>
@@ -2021,7 +2064,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(AttnKv c, float *o
 	const bool placed = tree_place(c, slot, base, sq, N, sl, b, end);
 	const Span sp = span_of<32, false>(c, kvh, sl, 0, 0, end);
 	const int nc = sp.n0 + (max(end - sp.b0, 0) + 31) / 32;
-	const int per = tree_part(nc, parts), c0 = part * per;
+	const int per = tree_part<kWaves>(nc, parts), c0 = part * per;
 	if (c0 >= nc && part > 0) return;   // a record that the join does not read
 	const int64_t row = (int64_t)sq * N + node;
 	uint64_t bits = on && placed ? seen[row] : 0;
@@ -2032,7 +2075,42 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(AttnKv c, float *o
 	                               : Dest(rec, ((size_t)sq * N * H + head) * parts + part, H, parts));
 }
 
-template <int HD>
+// The same by the tiled kernel, tiles of 32 W rows.
+template <int HD, bool Q8, int W>
+__global__ __launch_bounds__(64 * W, 2) void tree_tiled_kernel(AttnKv c, float *out, int64_t ldo, const float *q, int64_t ldq,
+                                                               const int *__restrict__ slot, const int *__restrict__ base,
+                                                               const uint64_t *__restrict__ seen, int n_seq, int N, int G, float scale,
+                                                               int parts, Records rec) {
+	__shared__ typename Tile<HD, Q8, W>::Lds s;
+	const int kvh = blockIdx.x % c.kvh, pair = blockIdx.x / c.kvh;
+	const int sq = pair % n_seq, part = pair / n_seq % parts, tile = pair / n_seq / parts;
+	const int tid = threadIdx.x, lane = tid & 63, r = 32 * (W * tile + (tid >> 6)) + (lane & 31), node = r / G, g = r - node * G;
+	const int head = kvh * G + g, H = c.kvh * G;
+	int sl, b, end;
+	const bool on = node < N, placed = tree_place(c, slot, base, sq, N, sl, b, end);
+	const Span sp = span_of<kKeys, false>(c, kvh, sl, 0, 0, end);
+	const int nc = sp.n0 + (max(end - sp.b0, 0) + kKeys - 1) / kKeys;
+	const int per = tree_part<1>(nc, parts), c0 = part * per;
+	if (c0 >= nc && part > 0) return;   // a record that the join does not read
+	const int64_t row = (int64_t)sq * N + node;
+	uint64_t bits = on && placed ? seen[row] : 0;
+	if (N < 64) bits &= (1ull << N) - 1;
+	// a wave without nodes sees nothing
+	const int hi = __any(bits != 0) ? end : 0;
+	Tile<HD, Q8, W> w;
+	w.chunks(c, sp, c0, min(nc, c0 + per), Nodes{b, bits, 0}, b, hi, s, tid,
+	         [&](int ln) { w.query(on ? q + row * ldq + head * HD : nullptr, scale, ln); });
+	if (!bits) w.clear();
+	if (parts == 1) {
+		w.put(on ? out + row * ldo + head * HD : nullptr, w.l == 0.0f ? 0.0f : 1.0f / w.l, s, tid);
+		return;
+	}
+	const size_t r0 = ((size_t)row * H + head) * parts + part;
+	w.put(on ? rec.o + r0 * HD : nullptr, 1.0f, s, tid);
+	if (on && lane < 32) rec.put(r0, {w.M, bits && w.big ? s.be[tid] : 0.0f}, w.l);
+}
+
+template <int HD, int K, int R>
 __global__ __launch_bounds__(256) void tree_join_kernel(AttnKv c, float *out, int64_t ldo, const int *__restrict__ slot,
                                                         const int *__restrict__ base, int n_seq, int N, int H, int parts,
                                                         const float *__restrict__ rec_o, const float2 *__restrict__ rec_ml,
@@ -2044,34 +2122,53 @@ __global__ __launch_bounds__(256) void tree_join_kernel(AttnKv c, float *out, in
 	if (sq >= n_seq) return;
 	int sl, b, end;
 	tree_place(c, slot, base, sq, N, sl, b, end);
-	const int nc = tile_steps<32>(end, c.prefix_len), per = tree_part(nc, parts);
+	const int nc = tile_steps<K>(end, c.prefix_len), per = tree_part<R>(nc, parts);
 	const size_t first = (size_t)i * parts;
 	join_few(rec_o + first * HD + d, HD, rec_ml + first, rec_e + first, max((nc + per - 1) / per, 1), out + row * ldo + (int64_t)h * HD + d);
 }
 
-// Trees of N nodes: parts of the keys (a step for each wave or more) until the workgroups fill the chip.
-template <int HD, bool Q8>
-int tree(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq, const int *slot, const int *base, const uint64_t *seen,
-         int n_seq, int N, int H, float scale) {
-	const int G = H / c.kvh;
-	const int64_t slots = 2 * cu_count(), tiles = ((int64_t)N * G + 31) / 32, wgs = tiles * n_seq * c.kvh;
-	const int most = (tile_steps<32>(c.max_seq, c.prefix_len) + kWaves - 1) / kWaves;
+// Trees of N nodes over parts of their keys, `slots` workgroups in all or fewer; launch(parts, blocks, records) of tiles
+// of `rows` rows.
+template <int HD, int K, int R, class Launch>
+int tree_launch(const AttnKv &c, float *out, int64_t ldo, const int *slot, const int *base, int n_seq, int N, int H, int rows, int64_t slots,
+                Launch launch) {
+	const int64_t wgs = ((int64_t)N * (H / c.kvh) + rows - 1) / rows * n_seq * c.kvh;
+	const int most = (tile_steps<K>(c.max_seq, c.prefix_len) + R - 1) / R;
 	const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(most, slots / wgs));
-	if (wgs * parts > kMaxThreads / (64 * kWaves) || (int64_t)n_seq * N * H * (HD / 4) > kMaxThreads)
+	if (wgs * parts > kMaxThreads / 512 || (int64_t)n_seq * N * H * (HD / 4) > kMaxThreads)
 		return set_error(HAKO_GPU_EINVAL, "%lld workgroups in one call", (long long)(wgs * parts));
 	Records rec{};
 	if (parts > 1)
 		if (int rc = records((size_t)n_seq * N * H * parts, HD, &rec)) return rc;
-	hipLaunchKernelGGL((tree_kernel<HD, Q8>), dim3((unsigned)(wgs * parts)), dim3(64 * kWaves), 0, stream(), c, out, ldo, q, ldq, slot, base,
-	                   seen, n_seq, N, G, scale * kLog2e, parts, rec);
+	launch(parts, dim3((unsigned)(wgs * parts)), rec);
 	HK_LAUNCHED("attention");
 	if (parts > 1) {
 		const int64_t blocks = ((int64_t)n_seq * N * H * (HD / 4) + 255) / 256;
-		hipLaunchKernelGGL(tree_join_kernel<HD>, dim3((unsigned)blocks), dim3(256), 0, stream(), c, out, ldo, slot, base, n_seq, N, H, parts,
-		                   rec.o, rec.ml, rec.e);
+		hipLaunchKernelGGL((tree_join_kernel<HD, K, R>), dim3((unsigned)blocks), dim3(256), 0, stream(), c, out, ldo, slot, base, n_seq, N, H,
+		                   parts, rec.o, rec.ml, rec.e);
 		HK_LAUNCHED("attention join");
 	}
 	return HAKO_GPU_OK;
+}
+
+template <int HD, bool Q8>
+int tree(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq, const int *slot, const int *base, const uint64_t *seen,
+         int n_seq, int N, int H, float scale) {
+	const int G = H / c.kvh;
+	auto tiled = [&](auto waves) {
+		constexpr int W = decltype(waves)::value;
+		return tree_launch<HD, kKeys, 1>(c, out, ldo, slot, base, n_seq, N, H, 32 * W, 8 / W * cu_count(),
+		                                 [&](int parts, dim3 grid, const Records &rec) {
+			                                 hipLaunchKernelGGL((tree_tiled_kernel<HD, Q8, W>), grid, dim3(64 * W), 0, stream(), c, out, ldo, q, ldq,
+			                                                    slot, base, seen, n_seq, N, G, scale * kLog2e, parts, rec);
+		                                 });
+	};
+	if (g_attn_prompt == 2) return tiled(std::integral_constant<int, 8>());
+	if (g_attn_prompt == 3) return tiled(std::integral_constant<int, 4>());
+	return tree_launch<HD, 32, kWaves>(c, out, ldo, slot, base, n_seq, N, H, 32, 2 * cu_count(), [&](int parts, dim3 grid, const Records &rec) {
+		hipLaunchKernelGGL((tree_kernel<HD, Q8>), grid, dim3(64 * kWaves), 0, stream(), c, out, ldo, q, ldq, slot, base, seen, n_seq, N, G,
+		                   scale * kLog2e, parts, rec);
+	});
 }
 
 }  // namespace
@@ -2099,7 +2196,7 @@ int attn_decode_reserve(const hako_gpu_kv *kv, int n_seq, int H, int prefix_len,
 	return p.nrec ? records((size_t)n_seq * H * p.nrec, kv->head_dim, &r) : HAKO_GPU_OK;
 }
 
-void attn_set_prompt(int v) { g_attn_prompt = v == 1 || v == 2 ? v : 0; }
+void attn_set_prompt(int v) { g_attn_prompt = v >= 1 && v <= 3 ? v : 0; }
 
 }  // namespace hako
 

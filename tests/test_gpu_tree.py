@@ -10,8 +10,17 @@ from hako_amd.gpu import KV_F16, KV_Q8, Rope
 
 pytestmark = pytest.mark.gpu
 
+TUNE_ATTN_PROMPT = 21
 TOL = 1e-5
 KINDS = [KV_Q8, KV_F16]
+
+
+@pytest.fixture(params=[1, 2, 3], ids=["direct", "tiled256", "tiled128"])
+def kernel(gpu, request):
+    """Each kernel of the attention in turn."""
+    gpu.tune(TUNE_ATTN_PROMPT, request.param)
+    yield request.param
+    gpu.tune(TUNE_ATTN_PROMPT, 0)
 
 
 def close(got, want):
@@ -78,7 +87,7 @@ def run_tree(gpu, c, q, slot, base, seen, N, scale, prefix=(0, 0), ldo=None):
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("H,KVH,hd", [(28, 4, 128), (16, 1, 64), (4, 4, 128), (14, 2, 64)])
 @pytest.mark.parametrize("N", [1, 2, 7, 26, 63, 64])
-def test_attention(gpu, kind, H, KVH, hd, N):
+def test_attention(gpu, kernel, kind, H, KVH, hd, N):
     """Texts of none to several steps, trees whole and padded, drafted rows that cross a step, a slot's last rows, past them."""
     rng = np.random.default_rng(N * H)
     base = [0, 1, 5, 31, 32, 33, 63, 100, 129, 200, 288, 299, 300, 1000]
@@ -96,7 +105,7 @@ def test_attention(gpu, kind, H, KVH, hd, N):
 
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("prefix", [1, 64, 100, 101, 160])
-def test_attention_over_a_prefix(gpu, kind, prefix):
+def test_attention_over_a_prefix(gpu, kernel, kind, prefix):
     """Also bases below the prefix, whose drafted rows are then the prefix slot's."""
     H, KVH, hd, N = 28, 4, 128, 9
     rng = np.random.default_rng(prefix)
@@ -112,7 +121,7 @@ def test_attention_over_a_prefix(gpu, kind, prefix):
 
 
 @pytest.mark.parametrize("n,N,base,H,KVH", [(1, 26, 5000, 16, 2), (2, 64, 5000, 28, 4), (40, 16, 900, 28, 4), (3, 1, 5000, 8, 8)])
-def test_attention_in_parts(gpu, n, N, base, H, KVH):
+def test_attention_in_parts(gpu, kernel, n, N, base, H, KVH):
     hd = 128
     rng = np.random.default_rng(n)
     c = ref.Cache(gpu, KV_Q8, n, base + 100, KVH, hd, rng)
@@ -127,7 +136,7 @@ def test_attention_in_parts(gpu, n, N, base, H, KVH):
     c.free()
 
 
-def test_masks_of_any_bits(gpu):
+def test_masks_of_any_bits(gpu, kernel):
     """Bits past the tree are nothing; a node may see any others; NaN and huge rows reach those who see them alone."""
     H, KVH, hd, N, base = 8, 2, 128, 20, 70
     rng = np.random.default_rng(4)
@@ -152,7 +161,7 @@ def test_masks_of_any_bits(gpu):
     c.free()
 
 
-def test_sequences_without_a_place(gpu):
+def test_sequences_without_a_place(gpu, kernel):
     """A base below 0, a slot outside the cache, an empty mask: zeros, whatever the context holds."""
     H, KVH, hd, N = 8, 2, 64, 3
     rng = np.random.default_rng(6)

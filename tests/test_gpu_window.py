@@ -142,11 +142,11 @@ def run_prompt(gpu, c, q, slot, start, lens, scale, window, sinks):
     return got[:n]
 
 
-@pytest.mark.parametrize("knob", [1, 2])
+@pytest.mark.parametrize("knob", [1, 2, 3])
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("H,KVH,hd", [(28, 4, 128), (16, 1, 64), (6, 6, 128), (8, 2, 64)])
 def test_prompt(gpu, kind, knob, H, KVH, hd):
-    """Both kernels: tiles and parts that end anywhere, starts of 0 and later, a prompt of one token and of none."""
+    """Each kernel: tiles and parts that end anywhere, starts of 0 and later, a prompt of one token and of none."""
     rng = np.random.default_rng(H + knob)
     lens, start, slot = [1, 77, 0, 300, 33, 64, 130], [0, 20, 5, 0, 400, 100, 230], [3, 0, 6, 2, 1, 5, 4]
     c = ref.Cache(gpu, kind, 7, 450, KVH, hd, rng)
@@ -164,7 +164,7 @@ def test_prompt(gpu, kind, knob, H, KVH, hd):
     c.free()
 
 
-@pytest.mark.parametrize("knob", [0, 1, 2])
+@pytest.mark.parametrize("knob", [0, 1, 2, 3])
 @pytest.mark.parametrize("lens,start,window,sinks", [([40], [5000], 4000, 4), ([700, 5], [0, 4200], 300, 0), ([257, 1], [3900, 5038], 4000, 100)])
 def test_prompt_in_parts(gpu, knob, lens, start, window, sinks):
     """Few tokens under a long window: the keys in parts, the last tile not full."""
@@ -185,7 +185,7 @@ def test_prompt_in_parts(gpu, knob, lens, start, window, sinks):
     c.free()
 
 
-@pytest.mark.parametrize("knob", [1, 2])
+@pytest.mark.parametrize("knob", [1, 2, 3])
 def test_prompt_leaves_out_what_is_not_in_sight(gpu, knob):
     """A row that is NaN or huge reaches the tokens whose window holds it and no other, whatever else their tile sees."""
     H, KVH, hd, n, W, S, bad = 8, 2, 128, 200, 50, 4, 90
