@@ -413,23 +413,38 @@ struct Tile {
 	float M, l;
 	uint64_t big;   // lanes whose base is big; while there are any, every lane's e is in LDS, else it is 0
 
-	// The lane's row q (null: an idle row), times scale log2(e).
-	__device__ __forceinline__ void query(const float *q, float scale, int lane) {
-		const int h = lane >> 5;
+	// The lane's row q (null: an idle row), times scale log2(e). Rows come as whole lines, half of the dims at a time
+	// through LDS, the chunks' place.
+	__device__ __forceinline__ void query(const float *q, float scale, Lds &lds, int tid) {
+		constexpr int L = HD / 8, R = 2 * HD + 16;
+		const int lane = tid & 63, h = lane >> 5;
+		uint8_t *buf = lds.k[0] + (tid >> 6) * (32 * R);
+		const uint64_t at = (uint64_t)(uintptr_t)q;
 		float x[KS * 8], a = 0.0f;
+		float4 y[L];
 #pragma unroll
-		for (int s = 0; s < KS; s++) {
-			float4 u = make_float4(0, 0, 0, 0), w = u;
-			if (q) {
-				u = *(const float4 *)(q + 16 * s + 8 * h);
-				w = *(const float4 *)(q + 16 * s + 8 * h + 4);
-			}
-			const float y[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+		for (int j = 0; j < L; j++) {
+			const int row = j % (L / 2) * (64 / L) + lane / L;
+			const uint64_t from = (uint64_t)(uint32_t)__shfl((int)(uint32_t)at, row) | ((uint64_t)(uint32_t)__shfl((int)(at >> 32), row) << 32);
+			y[j] = make_float4(0, 0, 0, 0);
+			if (from) y[j] = *(const float4 *)((const float *)(uintptr_t)from + HD / 2 * (j / (L / 2)) + 4 * (lane % L));
+		}
 #pragma unroll
-			for (int j = 0; j < 8; j++) {
-				x[8 * s + j] = y[j] * scale;
-				a = __builtin_fmaxf(a, __builtin_fabsf(x[8 * s + j]));
+		for (int p = 0; p < 2; p++) {
+#pragma unroll
+			for (int j = 0; j < L / 2; j++) *(float4 *)(buf + (j * (64 / L) + lane / L) * R + 16 * (lane % L)) = y[p * (L / 2) + j];
+			wave_sync();
+#pragma unroll
+			for (int s = 0; s < KS / 2; s++) {
+				const float4 u = *(const float4 *)(buf + (lane & 31) * R + 64 * s + 32 * h), w = *(const float4 *)(buf + (lane & 31) * R + 64 * s + 32 * h + 16);
+				const float z[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+#pragma unroll
+				for (int j = 0; j < 8; j++) {
+					x[8 * (p * (KS / 2) + s) + j] = z[j] * scale;
+					a = __builtin_fmaxf(a, __builtin_fabsf(z[j] * scale));
+				}
 			}
+			wave_sync();
 		}
 		a = __builtin_fmaxf(a, __shfl_xor(a, 32));
 		const int e = row_exp(a);
@@ -567,7 +582,7 @@ struct Tile {
 		}
 	}
 
-	// Chunks [c0, c1) of a tile's span for the queries that ask(lane) takes up while the first chunk's codes are on their
+	// Chunks [c0, c1) of a tile's span for the queries that ask() takes up while the first chunk's codes are on their
 	// way. lo, hi: the least and greatest lim of the wave's rows.
 	template <class See, class Ask>
 	__device__ __forceinline__ void chunks(const AttnKv &c, const Span &sp, int c0, int c1, const See &row, int lo, int hi, Lds &s,
@@ -585,7 +600,8 @@ struct Tile {
 		// put them into LDS at opposite ends of a chunk, so that one has vector work while the other has matrix work.
 		if (c0 < c1) load(c0);
 		__builtin_amdgcn_sched_barrier(0);
-		ask(lane);
+		ask();
+		__syncthreads();
 		if (c0 < c1) {
 			st.store(s.k[0], s.v[0], s.ks[0], s.vs[0], &s.e[0], tid);
 			if (c0 + 1 < c1) load(c0 + 1);
@@ -1153,7 +1169,7 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_kernel(AttnKv c, SeqTab t, I
 	const int64_t row = (int64_t)t.row[x.sq] + x.tok0 + tok;
 	Tile<HD, Q8, W> w;
 	w.chunks(c, span_of<kKeys, WIN>(c, kvh, x.slot, t.start[x.sq] + x.tok0, t.tile_tokens, x.end), x.c0, x.c1, row_sees<WIN>(c, lim), lo, hi,
-	         s, tid, [&](int ln) { w.query(on ? q + row * ldq + head * HD : nullptr, scale, ln); });
+	         s, tid, [&] { w.query(on ? q + row * ldq + head * HD : nullptr, scale, s, tid); });
 	if (x.parts == 1) {
 		w.put(on ? out + row * ldo + head * HD : nullptr, 1.0f / w.l, s, tid);
 		return;
@@ -2099,7 +2115,7 @@ __global__ __launch_bounds__(64 * W, 2) void tree_tiled_kernel(AttnKv c, float *
 	const int hi = __any(bits != 0) ? end : 0;
 	Tile<HD, Q8, W> w;
 	w.chunks(c, sp, c0, min(nc, c0 + per), Nodes{b, bits, 0}, b, hi, s, tid,
-	         [&](int ln) { w.query(on ? q + row * ldq + head * HD : nullptr, scale, ln); });
+	         [&] { w.query(on ? q + row * ldq + head * HD : nullptr, scale, s, tid); });
 	if (!bits) w.clear();
 	if (parts == 1) {
 		w.put(on ? out + row * ldo + head * HD : nullptr, w.l == 0.0f ? 0.0f : 1.0f / w.l, s, tid);
