@@ -21,9 +21,9 @@
 
 #include <algorithm>
 #include <float.h>
+#include <math.h>
 #include <new>
 #include <stddef.h>
-#include <type_traits>
 #include <vector>
 
 // CALL(HD, Q8) for a cache's head size and type.
@@ -1992,19 +1992,74 @@ int64_t all_steps(const AttnKv &c, const Reach &reach, const SeqTab &t, int toke
 	return n * c.kvh;
 }
 
+// The tiles of `tokens` tokens of a launch, with their key/value heads, and the steps of the longest.
+struct Tiles {
+	int64_t items, most;
+};
+template <int K, bool WIN>
+Tiles tiles_of(const AttnKv &c, const Reach &reach, const SeqTab &t, int tokens) {
+	Tiles x{};
+	for (int s = 0; s < t.n; s++) {
+		const int64_t n = (t.len[s] + tokens - 1) / tokens;
+		const int first = (int)(t.start[s] + (n - 1) * tokens);
+		x.items += n * c.kvh;
+		x.most = std::max<int64_t>(x.most, reach_steps<K, WIN>(reach, first, tokens, t.start[s] + t.len[s]));
+	}
+	return x;
+}
+
 // The tiled kernel of W waves; as many workgroups run at once as fill a CU with eight.
 template <int HD, bool Q8, bool WIN, int W>
 int prompt_tiled(const AttnKv &c, const Reach &reach, SeqTab &t, float *out, int64_t ldo, const float *q, int64_t ldq, int H, float scale) {
 	const int G = H / c.kvh;
 	const int64_t slots = 8 / W * cu_count(), all = all_steps<kKeys, WIN>(c, reach, t, 32 * W / G);
+	int64_t unit = (3 * all + 2 * slots - 1) / (2 * slots);
+	if (WIN) {
+		// tiles under a window are much alike: as many parts as the chip takes at once, and none where half a share is in
+		// question (1500 tokens under 512, two thirds of the chip: 62 us in two parts, 43 in one)
+		const Tiles x = tiles_of<kKeys, WIN>(c, reach, t, 32 * W / G);
+		const int64_t parts = x.items ? slots / x.items : 0;
+		unit = parts > 1 ? (x.most + parts - 1) / parts : 2 * ((all + slots - 1) / slots);
+	}
 	return prompt_launch<HD, Q8, kKeys, WIN>(
-	    c, reach, t, out, ldo, H, 32 * W, std::max<int64_t>(4, (3 * all + 2 * slots - 1) / (2 * slots)),
+	    c, reach, t, out, ldo, H, 32 * W, std::max<int64_t>(4, unit),
 	    [&](int64_t items, const Records &rec) {
 		    ItemTab order;
 		    if (const int n = sort_items<kKeys, WIN>(t, reach, order)) items = n;
 		    hipLaunchKernelGGL((prompt_kernel<HD, Q8, WIN, W>), dim3((unsigned)(items * c.kvh)), dim3(64 * W), 0, stream(), c, t, order, out,
 		                       ldo, q, ldq, G, scale * kLog2e, rec);
 	    });
+}
+
+// Which kernel under a window, 1 the direct one, 2 or 3 the tiled one of eight or four waves: the least of their times by
+// a model of a start, rounds of items and steps. Its constants, in us, are fits to heads of 128 / 64 on one MI355X: an
+// item takes 9 / 4.2 and 1.35 / 1 a step of a wave (16 bits and 128: 1.6) in the direct kernel, 13 / 8.5 and 2.8 / 1.85 a
+// chunk in the tiled one, where tiles of four waves, two at a time on a CU, cost (0.96 + 0.0065 chunks) times as much for
+// the same rows but end in half rounds. Model / measured for 7B heads, 8 bits, by the three: 512 tokens at 3000 under 512
+// 20 30 - / 20 36 33; 2000 under 512 63 46 - / 58 44 52; 4096 under 256 100 65 60 / 90 67 66; 8192 under 2048 576 440 510
+// / 573 416 436.
+template <int HD, bool Q8>
+int window_kernel(const AttnKv &c, const Reach &reach, const SeqTab &t, int G) {
+	const double cu = cu_count(), slots = 2 * cu, start = 5.0, join = 4.0;
+	const double di = HD == 128 ? 9.0 : 4.2, ds = HD == 64 ? 1.0 : Q8 ? 1.35 : 1.6, ti = HD == 128 ? 13.0 : 8.5, ts = HD == 128 ? 2.8 : 1.85;
+	const Tiles d = tiles_of<32, true>(c, reach, t, 32 / G), x = tiles_of<kKeys, true>(c, reach, t, 256 / G);
+	const double dn = (double)d.items, n = (double)x.items, all = (double)all_steps<kKeys, true>(c, reach, t, 256 / G);
+	double direct, tiled, small = 1e30;
+	if (dn >= slots) {
+		direct = start + (dn * di + ds * (double)all_steps<32, true>(c, reach, t, 32 / G) / kWaves) / slots;
+	} else {
+		const double parts = std::max(1.0, floor(slots / dn));
+		direct = start + di + ds * ceil(d.most / (kWaves * parts)) + (parts > 1 ? join : 0.0);
+	}
+	if (n > cu) {
+		const double item = ti + ts * all / n, r = n / cu, part = r - floor(r);
+		tiled = start + ceil(r) * item;
+		small = start + (floor(r) + (part > 0.0 ? std::max(part, 0.5) : 0.0)) * (0.96 + 0.0065 * all / n) * item;
+	} else {
+		const double parts = std::max(1.0, floor(cu / n));
+		tiled = start + ti + ts * ceil(x.most / parts) + (parts > 1 ? join : 0.0);
+	}
+	return direct <= std::min(tiled, small) ? 1 : tiled <= small ? 2 : 3;
 }
 
 // Which kernel (one MI355X, heads of 128, us by the direct / the tiled one):
@@ -2034,8 +2089,9 @@ int prompt(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, const float *q, 
 	const int64_t cu = cu_count(), slots = 2 * cu;   // workgroups of the direct kernel that run at once
 	const Reach reach = {c.prefix_len, c.window, c.sinks};
 	const int64_t steps = all_steps<32, WIN>(c, reach, t, 32 / G);
-	if (WIN && g_attn_prompt == 3) return prompt_tiled<HD, Q8, WIN, WIN ? 4 : 8>(c, reach, t, out, ldo, q, ldq, H, scale);
-	if (g_attn_prompt ? g_attn_prompt == 2 : steps > 55 * 4 * cu) return prompt_tiled<HD, Q8, WIN, 8>(c, reach, t, out, ldo, q, ldq, H, scale);
+	const int kernel = g_attn_prompt ? g_attn_prompt : WIN ? window_kernel<HD, Q8>(c, reach, t, G) : steps > 55 * 4 * cu ? 2 : 1;
+	if (WIN && kernel == 3) return prompt_tiled<HD, Q8, WIN, WIN ? 4 : 8>(c, reach, t, out, ldo, q, ldq, H, scale);
+	if (kernel != 1) return prompt_tiled<HD, Q8, WIN, 8>(c, reach, t, out, ldo, q, ldq, H, scale);
 	int64_t tiles = 0;
 	for (int s = 0; s < t.n; s++) tiles += (t.len[s] + 32 / G - 1) / (32 / G);
 	const int64_t share = (steps + slots - 1) / slots;
@@ -2065,14 +2121,41 @@ __device__ __forceinline__ int tree_part(int nc, int parts) {
 	return max(((nc + parts - 1) / parts + R - 1) / R * R, R);
 }
 
+// A workgroup's key/value head, sequence, part and tile. Workgroups go to the eight dies in turn: the tiles of a part,
+// which read the same keys, follow one another on one die.
+__device__ __forceinline__ bool tree_item(int n_kvh, int n_seq, int parts, int tiles, int &kvh, int &sq, int &part, int &tile) {
+	const int g = blockIdx.x / (8 * tiles), r = blockIdx.x - g * (8 * tiles);
+	const int p = 8 * g + r % 8;   // (part, sequence, head)
+	tile = r / 8;
+	kvh = p % n_kvh;
+	sq = p / n_kvh % n_seq;
+	part = p / n_kvh / n_seq;
+	return part < parts;
+}
+unsigned tree_blocks(int64_t items, int64_t tiles) { return (unsigned)((items + 7) / 8 * 8 * tiles); }
+
+// Zeros, or records of nothing, for the 32 rows (node, g) that a wave's lanes hold (node -1: none), by a workgroup whose
+// waves hold the same.
+template <int HD>
+__device__ __forceinline__ void tree_blank(int node, int g, int sq, int N, int head, float *out, int64_t ldo, int H, int parts, int part,
+                                           const Records &rec) {
+	const int row = threadIdx.x >> 3, n = __shfl(node, row), hd = head + __shfl(g, row);
+	if (n < 0) return;
+	const size_t r = (((size_t)sq * N + n) * H + hd) * parts + part;
+	float *to = parts == 1 ? out + ((int64_t)sq * N + n) * ldo + (int64_t)hd * HD : rec.o + r * HD;
+#pragma unroll
+	for (int d = 4 * (threadIdx.x & 7); d < HD; d += 32) *(float4 *)(to + d) = make_float4(0, 0, 0, 0);
+	if (parts > 1 && (threadIdx.x & 7) == 0) rec.put(r, {kNone, 0.0f}, 0.0f);
+}
+
 template <int HD, bool Q8>
 __global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(AttnKv c, float *out, int64_t ldo, const float *q, int64_t ldq,
                                                               const int *__restrict__ slot, const int *__restrict__ base,
                                                               const uint64_t *__restrict__ seen, int n_seq, int N, int G, float scale,
                                                               int parts, Records rec) {
 	__shared__ DirectLds<HD> s;
-	const int kvh = blockIdx.x % c.kvh, pair = blockIdx.x / c.kvh;
-	const int sq = pair % n_seq, part = pair / n_seq % parts, tile = pair / n_seq / parts;
+	int kvh, sq, part, tile;
+	if (!tree_item(c.kvh, n_seq, parts, (N * G + 31) / 32, kvh, sq, part, tile)) return;
 	const int lane = threadIdx.x & 63, r = 32 * tile + (lane & 31), node = r / G, g = r - node * G;
 	const int head = kvh * G, H = c.kvh * G;
 	const bool on = node < N;
@@ -2085,6 +2168,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(AttnKv c, float *o
 	const int64_t row = (int64_t)sq * N + node;
 	uint64_t bits = on && placed ? seen[row] : 0;
 	if (N < 64) bits &= (1ull << N) - 1;
+	if (!__any(bits != 0)) {   // nodes that are not there, as in the last tiles of a padded tree
+		tree_blank<HD>(on ? node : -1, g, sq, N, head, out, ldo, H, parts, part, rec);
+		return;
+	}
 	direct_rows<HD, Q8>(c, s, sp, c0, min(nc, c0 + per), on && bits ? q + row * ldq + (head + g) * HD : nullptr, scale, Nodes{b, bits, 0},
 	                    on ? node << 4 | g | (bits ? 0 : kBlank) : -1,
 	                    parts == 1 ? Dest(out + (int64_t)sq * N * ldo + head * HD, ldo, HD)
@@ -2098,8 +2185,8 @@ __global__ __launch_bounds__(64 * W, 2) void tree_tiled_kernel(AttnKv c, float *
                                                                const uint64_t *__restrict__ seen, int n_seq, int N, int G, float scale,
                                                                int parts, Records rec) {
 	__shared__ typename Tile<HD, Q8, W>::Lds s;
-	const int kvh = blockIdx.x % c.kvh, pair = blockIdx.x / c.kvh;
-	const int sq = pair % n_seq, part = pair / n_seq % parts, tile = pair / n_seq / parts;
+	int kvh, sq, part, tile;
+	if (!tree_item(c.kvh, n_seq, parts, (N * G + 32 * W - 1) / (32 * W), kvh, sq, part, tile)) return;
 	const int tid = threadIdx.x, lane = tid & 63, r = 32 * (W * tile + (tid >> 6)) + (lane & 31), node = r / G, g = r - node * G;
 	const int head = kvh * G + g, H = c.kvh * G;
 	int sl, b, end;
@@ -2111,10 +2198,10 @@ __global__ __launch_bounds__(64 * W, 2) void tree_tiled_kernel(AttnKv c, float *
 	const int64_t row = (int64_t)sq * N + node;
 	uint64_t bits = on && placed ? seen[row] : 0;
 	if (N < 64) bits &= (1ull << N) - 1;
-	// a wave without nodes sees nothing
-	const int hi = __any(bits != 0) ? end : 0;
+	// a wave without nodes sees nothing, a workgroup without any passes no chunk
+	const int hi = __any(bits != 0) ? end : 0, stop = __syncthreads_or(hi) ? min(nc, c0 + per) : c0;
 	Tile<HD, Q8, W> w;
-	w.chunks(c, sp, c0, min(nc, c0 + per), Nodes{b, bits, 0}, b, hi, s, tid,
+	w.chunks(c, sp, c0, stop, Nodes{b, bits, 0}, b, hi, s, tid,
 	         [&] { w.query(on ? q + row * ldq + head * HD : nullptr, scale, s, tid); });
 	if (!bits) w.clear();
 	if (parts == 1) {
@@ -2148,15 +2235,15 @@ __global__ __launch_bounds__(256) void tree_join_kernel(AttnKv c, float *out, in
 template <int HD, int K, int R, class Launch>
 int tree_launch(const AttnKv &c, float *out, int64_t ldo, const int *slot, const int *base, int n_seq, int N, int H, int rows, int64_t slots,
                 Launch launch) {
-	const int64_t wgs = ((int64_t)N * (H / c.kvh) + rows - 1) / rows * n_seq * c.kvh;
+	const int64_t tiles = ((int64_t)N * (H / c.kvh) + rows - 1) / rows, wgs = tiles * n_seq * c.kvh;
 	const int most = (tile_steps<K>(c.max_seq, c.prefix_len) + R - 1) / R;
 	const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(most, slots / wgs));
-	if (wgs * parts > kMaxThreads / 512 || (int64_t)n_seq * N * H * (HD / 4) > kMaxThreads)
+	if ((wgs * parts + 8 * tiles) > kMaxThreads / 512 || (int64_t)n_seq * N * H * (HD / 4) > kMaxThreads)
 		return set_error(HAKO_GPU_EINVAL, "%lld workgroups in one call", (long long)(wgs * parts));
 	Records rec{};
 	if (parts > 1)
 		if (int rc = records((size_t)n_seq * N * H * parts, HD, &rec)) return rc;
-	launch(parts, dim3((unsigned)(wgs * parts)), rec);
+	launch(parts, dim3(tree_blocks((int64_t)n_seq * c.kvh * parts, tiles)), rec);
 	HK_LAUNCHED("attention");
 	if (parts > 1) {
 		const int64_t blocks = ((int64_t)n_seq * N * H * (HD / 4) + 255) / 256;
@@ -2167,20 +2254,27 @@ int tree_launch(const AttnKv &c, float *out, int64_t ldo, const int *slot, const
 	return HAKO_GPU_OK;
 }
 
+// Which kernel (one MI355X, us by the direct / the tiled one; the texts fill their slots). Lengths are known on the device
+// alone, so the work is taken as if slots were full: shorter texts may then take the tiled kernel, at up to 10 us more.
+//   rows of a sequence and head   wave-steps a SIMD (32 rows x 32 keys)   8 bits       16 bits
+//   7B  8 trees of 64 at 1000  448 rows     14                          29 / 38      32 / 37
+//       8 of 32 at 4000        224          28                          51 / 46      57 / 47
+//       16 of 64 at 4096       448         112                         166 / 125    190 / 126
+//       32 of 16 at 3400       112          54                          63 / 76      78 / 73
+//       64 of 16 at 2000       112          64                          95 / 84     118 / 92
+//       64 of 8 at 2000         56          32                          49 / 78      62 / 77
+//   3B  8 of 64 at 4000        512          32                          52 / 50      58 / 50
+// So the tiled one from 27 on where its tiles of 256 rows are full or nearly, from 58 on where they are half full.
 template <int HD, bool Q8>
 int tree(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq, const int *slot, const int *base, const uint64_t *seen,
          int n_seq, int N, int H, float scale) {
-	const int G = H / c.kvh;
-	auto tiled = [&](auto waves) {
-		constexpr int W = decltype(waves)::value;
-		return tree_launch<HD, kKeys, 1>(c, out, ldo, slot, base, n_seq, N, H, 32 * W, 8 / W * cu_count(),
-		                                 [&](int parts, dim3 grid, const Records &rec) {
-			                                 hipLaunchKernelGGL((tree_tiled_kernel<HD, Q8, W>), grid, dim3(64 * W), 0, stream(), c, out, ldo, q, ldq,
-			                                                    slot, base, seen, n_seq, N, G, scale * kLog2e, parts, rec);
-		                                 });
-	};
-	if (g_attn_prompt == 2) return tiled(std::integral_constant<int, 8>());
-	if (g_attn_prompt == 3) return tiled(std::integral_constant<int, 4>());
+	const int G = H / c.kvh, rows = N * G;
+	const int64_t steps = (int64_t)(rows + 31) / 32 * n_seq * c.kvh * tile_steps<32>(c.max_seq, c.prefix_len);
+	if (g_attn_prompt ? g_attn_prompt >= 2 : rows > 64 && steps >= (rows >= 192 ? 27 : 58) * 4 * (int64_t)cu_count())
+		return tree_launch<HD, kKeys, 1>(c, out, ldo, slot, base, n_seq, N, H, 256, cu_count(), [&](int parts, dim3 grid, const Records &rec) {
+			hipLaunchKernelGGL((tree_tiled_kernel<HD, Q8, 8>), grid, dim3(512), 0, stream(), c, out, ldo, q, ldq, slot, base, seen, n_seq, N, G,
+			                   scale * kLog2e, parts, rec);
+		});
 	return tree_launch<HD, 32, kWaves>(c, out, ldo, slot, base, n_seq, N, H, 32, 2 * cu_count(), [&](int parts, dim3 grid, const Records &rec) {
 		hipLaunchKernelGGL((tree_kernel<HD, Q8>), grid, dim3(64 * kWaves), 0, stream(), c, out, ldo, q, ldq, slot, base, seen, n_seq, N, G,
 		                   scale * kLog2e, parts, rec);
