@@ -56,7 +56,7 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 
-// prompts: 1 = direct kernel, 2 = tiled kernel, 0 = by shape (tuning knob)
+// prompts and trees: 1 = direct kernel, 2 and 3 = tiled kernel of 256 and 128 rows, 0 = by shape (tuning knob)
 int g_attn_prompt = 0;
 
 struct AttnKv {
@@ -2260,19 +2260,30 @@ int tree_launch(const AttnKv &c, float *out, int64_t ldo, const int *slot, const
 //   7B  8 trees of 64 at 1000  448 rows     14                          29 / 38      32 / 37
 //       8 of 32 at 4000        224          28                          51 / 46      57 / 47
 //       16 of 64 at 4096       448         112                         166 / 125    190 / 126
-//       32 of 16 at 3400       112          54                          63 / 76      78 / 73
-//       64 of 16 at 2000       112          64                          95 / 84     118 / 92
-//       64 of 8 at 2000         56          32                          49 / 78      62 / 77
+//       8 of 16 at 2000        112           8                          22 / 32      24 / 30
+//       16 of 12 at 4000        84          24                          50 / 46      56 / 48
+//       32 of 16 at 3400       112          54                          78 / 77      89 / 81
+//       64 of 16 at 2000       112          64                          93 / 83     118 / 92
+//       64 of 8 at 2000         56          32                          49 / 72      62 / 72
 //   3B  8 of 64 at 4000        512          32                          52 / 50      58 / 50
-// So the tiled one from 27 on where its tiles of 256 rows are full or nearly, from 58 on where they are half full.
+// So the tiled one from 24 on for more than 64 rows. Its tiles are of 128 rows where these hold them all and sequences and
+// heads do not give every other CU a tile (32 ragged trees of 16 over a prefix in 16 bits 66 us, 73 in tiles of 256, 8
+// bits 67 and 76; 64 of 16 at 2000 96 and 90, 87 and 83).
 template <int HD, bool Q8>
 int tree(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq, const int *slot, const int *base, const uint64_t *seen,
          int n_seq, int N, int H, float scale) {
 	const int G = H / c.kvh, rows = N * G;
 	const int64_t steps = (int64_t)(rows + 31) / 32 * n_seq * c.kvh * tile_steps<32>(c.max_seq, c.prefix_len);
-	if (g_attn_prompt ? g_attn_prompt >= 2 : rows > 64 && steps >= (rows >= 192 ? 27 : 58) * 4 * (int64_t)cu_count())
+	const bool tiled = rows > 64 && steps >= 24 * 4 * (int64_t)cu_count();
+	const int kernel = g_attn_prompt ? g_attn_prompt : !tiled ? 1 : rows > 128 || 2 * n_seq * c.kvh > cu_count() ? 2 : 3;
+	if (kernel == 2)
 		return tree_launch<HD, kKeys, 1>(c, out, ldo, slot, base, n_seq, N, H, 256, cu_count(), [&](int parts, dim3 grid, const Records &rec) {
 			hipLaunchKernelGGL((tree_tiled_kernel<HD, Q8, 8>), grid, dim3(512), 0, stream(), c, out, ldo, q, ldq, slot, base, seen, n_seq, N, G,
+			                   scale * kLog2e, parts, rec);
+		});
+	if (kernel == 3)
+		return tree_launch<HD, kKeys, 1>(c, out, ldo, slot, base, n_seq, N, H, 128, 2 * cu_count(), [&](int parts, dim3 grid, const Records &rec) {
+			hipLaunchKernelGGL((tree_tiled_kernel<HD, Q8, 4>), grid, dim3(256), 0, stream(), c, out, ldo, q, ldq, slot, base, seen, n_seq, N, G,
 			                   scale * kLog2e, parts, rec);
 		});
 	return tree_launch<HD, 32, kWaves>(c, out, ldo, slot, base, n_seq, N, H, 32, 2 * cu_count(), [&](int parts, dim3 grid, const Records &rec) {

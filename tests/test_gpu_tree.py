@@ -15,7 +15,7 @@ TOL = 1e-5
 KINDS = [KV_Q8, KV_F16]
 
 
-@pytest.fixture(params=[1, 2], ids=["direct", "tiled"])
+@pytest.fixture(params=[1, 2, 3], ids=["direct", "tiled256", "tiled128"])
 def kernel(gpu, request):
     """Each kernel of the attention in turn."""
     gpu.tune(TUNE_ATTN_PROMPT, request.param)
