@@ -2275,7 +2275,7 @@ int tree(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq, 
 	const int G = H / c.kvh, rows = N * G;
 	const int64_t steps = (int64_t)(rows + 31) / 32 * n_seq * c.kvh * tile_steps<32>(c.max_seq, c.prefix_len);
 	const bool tiled = rows > 64 && steps >= 24 * 4 * (int64_t)cu_count();
-	const int kernel = g_attn_prompt ? g_attn_prompt : !tiled ? 1 : rows > 128 || 2 * n_seq * c.kvh > cu_count() ? 2 : 3;
+	const int kernel = g_attn_prompt ? g_attn_prompt : !tiled ? 1 : rows > 128 || 2 * (int64_t)n_seq * c.kvh > cu_count() ? 2 : 3;
 	if (kernel == 2)
 		return tree_launch<HD, kKeys, 1>(c, out, ldo, slot, base, n_seq, N, H, 256, cu_count(), [&](int parts, dim3 grid, const Records &rec) {
 			hipLaunchKernelGGL((tree_tiled_kernel<HD, Q8, 8>), grid, dim3(512), 0, stream(), c, out, ldo, q, ldq, slot, base, seen, n_seq, N, G,

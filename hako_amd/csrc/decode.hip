@@ -1473,6 +1473,20 @@ struct hako_gpu_decoder {
 	int kv_type = 0, prefix_seq = 0, prefix_len = 0;
 	std::vector<hako_gpu_kv> kv;
 	int *pf_slot = nullptr;   // the sequence of a pass's tokens
+	int window = 0, sinks = 0;   // positions that a token sees (window 0: all before it)
+	// beam search: beams of a request while its step is enqueued (0: a greedy step), the scores and ends of the beams as the
+	// step reads and as it writes them, parents and tokens of every step so far, and the rows that follow the beams
+	int beams = 0, beam_eos = 0;
+	float *b_score = nullptr, *b_next = nullptr;
+	int *b_done = nullptr, *b_ended = nullptr, *b_parent = nullptr, *b_hist = nullptr, *b_since = nullptr, *b_len = nullptr;
+	hipGraphExec_t b_exec = nullptr;
+	hipGraph_t b_graph = nullptr;
+	int b_exec_beams = 0, b_exec_eos = 0;   // what it was captured for
+	// a drafted tree (allocated on first use): arrays of HAKO_MAX_TREE nodes, logits of all
+	uint64_t *tr_seen = nullptr;
+	int *tr_parent = nullptr, *tr_turn = nullptr, *tr_pick = nullptr, *tr_path = nullptr, *tr_one = nullptr;
+	float *tr_logits = nullptr;
+	float2 *tr_apart = nullptr;
 	int *tok = nullptr, *pos = nullptr, *ring = nullptr, *nout = nullptr;
 	// one sequence: the output projection's fixed-point residual accumulators
 	// (three: by layer parity, and the last layer of an odd count; then one
@@ -1713,8 +1727,10 @@ int attention(hako_gpu_decoder *d, int l, int8_t *mxq = nullptr, float *mxs = nu
 		if (int rc = hako_gpu_kv_append(kv, nullptr, d->pos, d->n_seq, d->qkv + D, d->qkv + D + KV, d->qkv_dim, &rope, d->qkv,
 		                                d->qkv, m.n_heads, d->qkv_dim, d->qkv_dim))
 			return rc;
-		if (int rc = attn_decode(d->att, D, d->qkv, d->qkv_dim, kv, nullptr, d->pos, 1, d->n_seq, m.n_heads, scale,
-		                         d->prefix_seq, d->prefix_len))
+		if (int rc = d->window ? attn_decode_window(d->att, D, d->qkv, d->qkv_dim, kv, nullptr, d->pos, 1, d->n_seq, m.n_heads, scale,
+		                                            d->window, d->sinks)
+		                       : attn_decode(d->att, D, d->qkv, d->qkv_dim, kv, nullptr, d->pos, 1, d->n_seq, m.n_heads, scale,
+		                                     d->prefix_seq, d->prefix_len))
 			return rc;
 		return mxq ? hako_gpu_quantize_q8_32(d->att, d->n_seq, D, mxq, mxs) : HAKO_GPU_OK;
 	}
@@ -1759,6 +1775,39 @@ int argmax(hako_gpu_decoder *d) {
 	HK_LAUNCHED("argmax final");
 	return HAKO_GPU_OK;
 }
+
+// The end of a beam search's step: what it wrote becomes what the next one reads.
+__global__ __launch_bounds__(64) void beam_commit_kernel(int n_seq, int beams, const float *__restrict__ next, const int *__restrict__ ended,
+                                                         const int *__restrict__ parent, const int *__restrict__ tok, float *score,
+                                                         int *done, int *hist, int hist_len, int *pos, int *nout, int *len) {
+	const int sq = threadIdx.x;
+	if (sq >= n_seq) return;
+	score[sq] = next[sq];
+	done[sq] = ended[sq];
+	const int n = nout[sq];
+	if (n < hist_len) {
+		hist[(size_t)n * 2 * n_seq + sq] = parent[sq];
+		hist[(size_t)(n * 2 + 1) * n_seq + sq] = tok[sq];
+	}
+	nout[sq] = n + 1;
+	pos[sq] += 1;
+	if (sq % beams == 0) len[sq / beams] += 1;
+}
+
+// The beams' continuations in the place of the greedy pick, and the caches after them.
+int beam_pick(hako_gpu_decoder *d) {
+	const int K = d->beams, n_req = d->n_seq / K;
+	if (int rc = hako_gpu_beam_select(d->logits, d->m.vocab, d->m.vocab, d->b_score, d->b_done, d->beam_eos, n_req, K, K, 1, d->b_parent,
+	                                  d->tok, d->b_next, d->b_ended))
+		return rc;
+	if (int rc = hako_gpu_kv_reorder(d->kv.data(), (int)d->kv.size(), nullptr, d->b_parent, n_req, K, d->b_since, d->b_len)) return rc;
+	hipLaunchKernelGGL(beam_commit_kernel, dim3(1), dim3(64), 0, stream(), d->n_seq, K, d->b_next, d->b_ended, d->b_parent, d->tok,
+	                   d->b_score, d->b_done, d->b_hist, d->max_seq, d->pos, d->nout, d->b_len);
+	HK_LAUNCHED("beam commit");
+	return HAKO_GPU_OK;
+}
+
+int pick(hako_gpu_decoder *d) { return d->beams ? beam_pick(d) : argmax(d); }
 
 // x += the pending split partials (part, nsplit; none when part is null),
 // then rmsnorm (w) and q8 rows of x into d->xq / d->xs.
@@ -1926,7 +1975,7 @@ int enqueue_batched_step(hako_gpu_decoder *d) {
 		if (int rc = rmsnorm(d->x, m.out_norm, d->xn, D, m.rms_eps, M)) return rc;
 		if (int rc = batch_matmul(d, d->logits, m.vocab, d->xn, m.t_out, m.out_weight, nullptr, m.vocab, D)) return rc;
 	}
-	if (int rc = argmax(d)) return rc;
+	if (int rc = pick(d)) return rc;
 	return HAKO_GPU_OK;
 }
 
@@ -2085,8 +2134,8 @@ int enqueue_step(hako_gpu_decoder *d) {
 	return HAKO_GPU_OK;
 }
 
-int capture(hako_gpu_decoder *d) {
-	if (d->exec) return HAKO_GPU_OK;
+// The step as a graph.
+int capture_step(hako_gpu_decoder *d, hipGraph_t *graph, hipGraphExec_t *exec) {
 	HK_HIP(hipStreamBeginCapture(stream(), hipStreamCaptureModeThreadLocal));
 	const int rc = enqueue_step(d);
 	hipGraph_t g = nullptr;
@@ -2096,8 +2145,24 @@ int capture(hako_gpu_decoder *d) {
 		return rc;
 	}
 	if (e != hipSuccess) return hip_fail(e, "hipStreamEndCapture", __FILE__, __LINE__);
-	d->graph = g;
-	HK_HIP(hipGraphInstantiate(&d->exec, g, nullptr, nullptr, 0));
+	*graph = g;
+	HK_HIP(hipGraphInstantiate(exec, g, nullptr, nullptr, 0));
+	return HAKO_GPU_OK;
+}
+
+int capture(hako_gpu_decoder *d) { return d->exec ? HAKO_GPU_OK : capture_step(d, &d->graph, &d->exec); }
+
+// The captured steps hold what they were captured with.
+int drop_graphs(hako_gpu_decoder *d) {
+	HK_HIP(hipStreamSynchronize(stream()));
+	for (hipGraphExec_t *e : {&d->exec, &d->b_exec}) {
+		if (*e) HK_HIP(hipGraphExecDestroy(*e));
+		*e = nullptr;
+	}
+	for (hipGraph_t *g : {&d->graph, &d->b_graph}) {
+		if (*g) HK_HIP(hipGraphDestroy(*g));
+		*g = nullptr;
+	}
 	return HAKO_GPU_OK;
 }
 
@@ -2180,8 +2245,10 @@ int prefill_alloc(hako_gpu_decoder *d) {
 
 // Tokens [0, n) of sequence seq at positions pos0.. (n <= pf_chunk):
 // every layer for all of them, each matmul one multi-token launch, causal
-// attention over the cache (the chunk's keys and values appended first).
-int prefill_chunk(hako_gpu_decoder *d, int seq, const int *tokens, int n, int pos0) {
+// attention over the cache (the chunk's keys and values appended first). With
+// `parent` the tokens are a tree's nodes (n <= HAKO_MAX_TREE), at rows pos0..
+// and turned by their depth.
+int prefill_chunk(hako_gpu_decoder *d, int seq, const int *tokens, int n, int pos0, const int *parent = nullptr) {
 	const hako_gpu_model &m = d->m;
 	const int D = m.d_model, F = m.ffn_dim, KV = d->kv_dim, HD = m.head_dim, KVH = m.n_kv_heads;
 	const int G = m.n_heads / KVH;
@@ -2196,7 +2263,13 @@ int prefill_chunk(hako_gpu_decoder *d, int seq, const int *tokens, int n, int po
 		for (int i = 0; i < n; i++) slotv[i] = seq;
 		HK_HIP(hipMemcpyAsync(d->pf_slot, slotv.get(), sizeof(int) * n, hipMemcpyHostToDevice, stream()));
 	}
-	HK_HIP(hipStreamSynchronize(stream()));   // posv and slotv are this frame's
+	const int one[2] = {pos0, seq};
+	if (parent) {
+		HK_HIP(hipMemcpyAsync(d->tr_parent, parent, sizeof(int) * n, hipMemcpyHostToDevice, stream()));
+		HK_HIP(hipMemcpyAsync(d->tr_one, one, sizeof one, hipMemcpyHostToDevice, stream()));
+		if (int rc = hako_gpu_tree_plan(d->tr_one + 1, d->tr_one, d->tr_parent, 1, n, d->tr_seen, nullptr, nullptr, d->tr_turn)) return rc;
+	}
+	HK_HIP(hipStreamSynchronize(stream()));   // posv, slotv and one are this frame's
 	hipLaunchKernelGGL(embed_kernel, dim3(n), dim3(256), 0, stream(), (const uint8_t *)m.tok_embd, m.t_embd,
 	                   row_bytes(m.t_embd, D), d->pf_tok, d->pf_x, D, m.vocab);
 	HK_LAUNCHED("embed");
@@ -2244,11 +2317,17 @@ int prefill_chunk(hako_gpu_decoder *d, int seq, const int *tokens, int n, int po
 		if (d->kv_type) {
 			const hako_gpu_kv *kv = &d->kv[l];
 			const hako_gpu_rope rope = {(const float *)d->rope, d->max_seq, HD, 0};
-			if (int rc = hako_gpu_kv_append(kv, d->pf_slot, d->pf_pos, n, d->pf_k, d->pf_v, KV, &rope, d->pf_q, d->pf_q, m.n_heads,
-			                                D, D))
+			if (int rc = parent ? hako_gpu_kv_append_turned(kv, d->pf_slot, d->pf_pos, d->tr_turn, n, d->pf_k, d->pf_v, KV, &rope, d->pf_q,
+			                                                d->pf_q, m.n_heads, D, D)
+			                    : hako_gpu_kv_append(kv, d->pf_slot, d->pf_pos, n, d->pf_k, d->pf_v, KV, &rope, d->pf_q, d->pf_q,
+			                                         m.n_heads, D, D))
 				return rc;
-			if (int rc = hako_gpu_attn_prompt(d->pf_att, D, d->pf_q, D, kv, &seq, &pos0, &n, 1, m.n_heads, scale, d->prefix_seq,
-			                                  d->prefix_len))
+			if (int rc = parent ? hako_gpu_attn_tree(d->pf_att, D, d->pf_q, D, kv, d->tr_one + 1, d->tr_one, d->tr_seen, 1, n, m.n_heads,
+			                                         scale, d->prefix_seq, d->prefix_len)
+			             : d->window ? hako_gpu_attn_prompt_window(d->pf_att, D, d->pf_q, D, kv, &seq, &pos0, &n, 1, m.n_heads, scale,
+			                                                       d->window, d->sinks)
+			                         : hako_gpu_attn_prompt(d->pf_att, D, d->pf_q, D, kv, &seq, &pos0, &n, 1, m.n_heads, scale,
+			                                                d->prefix_seq, d->prefix_len))
 				return rc;
 			if (mxq)
 				if (int rc = hako_gpu_quantize_q8_32(d->pf_att, n, D, mxq, mxs)) return rc;
@@ -2315,6 +2394,52 @@ int prefill_chunk(hako_gpu_decoder *d, int seq, const int *tokens, int n, int po
 		}
 	}
 	return HAKO_GPU_OK;
+}
+
+// Grid (rows), one wave: the token of the blocks' best of a row, by the rule of argmax_final_kernel.
+__global__ __launch_bounds__(64) void argmax_row_kernel(const float2 *__restrict__ part, const float *__restrict__ logits, int V,
+                                                        int *__restrict__ pick) {
+	const float2 p = part[blockIdx.x * kArgBlocks + threadIdx.x];
+	const float l0 = logits[(size_t)blockIdx.x * V];
+	float v = p.x;
+	int i = __builtin_bit_cast(int, p.y);
+	argmax_wave(v, i);
+	if (threadIdx.x == 0) pick[blockIdx.x] = (i == 0x7FFFFFFF || l0 != l0) ? 0 : i;
+}
+
+int tree_alloc(hako_gpu_decoder *d) {
+	if (d->tr_logits) return HAKO_GPU_OK;
+	int rc = 0;
+#define HK_ALLOC(ptr, bytes) rc = rc ? rc : dalloc(d, (bytes), (void **)&(ptr))
+	HK_ALLOC(d->tr_seen, sizeof(uint64_t) * HAKO_MAX_TREE);
+	HK_ALLOC(d->tr_parent, sizeof(int) * HAKO_MAX_TREE);
+	HK_ALLOC(d->tr_turn, sizeof(int) * HAKO_MAX_TREE);
+	HK_ALLOC(d->tr_pick, sizeof(int) * HAKO_MAX_TREE);
+	HK_ALLOC(d->tr_path, sizeof(int) * HAKO_MAX_TREE);
+	HK_ALLOC(d->tr_one, sizeof(int) * 5);   // base, slot, nodes of the path, next token, new base
+	HK_ALLOC(d->tr_apart, sizeof(float2) * HAKO_MAX_TREE * kArgBlocks);
+	HK_ALLOC(d->tr_logits, sizeof(float) * HAKO_MAX_TREE * (size_t)d->m.vocab);
+#undef HK_ALLOC
+	if (rc) d->tr_logits = nullptr;   // retried on the next call; the others stay tracked for destroy
+	return rc;
+}
+
+int beam_alloc(hako_gpu_decoder *d) {
+	if (d->b_hist) return HAKO_GPU_OK;
+	const size_t n = sizeof(int) * d->n_seq;
+	int rc = 0;
+#define HK_ALLOC(ptr, bytes) rc = rc ? rc : dalloc(d, (bytes), (void **)&(ptr))
+	HK_ALLOC(d->b_score, n);
+	HK_ALLOC(d->b_next, n);
+	HK_ALLOC(d->b_done, n);
+	HK_ALLOC(d->b_ended, n);
+	HK_ALLOC(d->b_parent, n);
+	HK_ALLOC(d->b_since, n);
+	HK_ALLOC(d->b_len, n);
+	HK_ALLOC(d->b_hist, 2 * n * d->max_seq);
+#undef HK_ALLOC
+	if (rc) d->b_hist = nullptr;
+	return rc;
 }
 
 // The caches of a decoder in 8 or 16 bits: one layer after the other, zeros.
@@ -2472,6 +2597,8 @@ int hako_gpu_decoder_destroy(hako_gpu_decoder *d) {
 	if (stream()) (void)hipStreamSynchronize(stream());
 	if (d->exec) (void)hipGraphExecDestroy(d->exec);
 	if (d->graph) (void)hipGraphDestroy(d->graph);
+	if (d->b_exec) (void)hipGraphExecDestroy(d->b_exec);
+	if (d->b_graph) (void)hipGraphDestroy(d->b_graph);
 	for (hipEvent_t e : d->stage_ev)
 		if (e) (void)hipEventDestroy(e);
 	if (d->stage) (void)hipHostFree(d->stage);
@@ -2510,15 +2637,23 @@ int hako_gpu_decoder_share_prefix(hako_gpu_decoder *d, int seq, int n) {
 	if (seq < 0 || seq >= d->n_seq || n < 0 || n > d->max_seq)
 		return set_error(HAKO_GPU_EINVAL, "prefix of %d positions of sequence %d: %d sequences of %d", n, seq, d->n_seq,
 		                 d->max_seq);
+	if (n > 0 && d->window) return set_error(HAKO_GPU_EINVAL, "a prefix is not shared under a window");
 	if (int rc = attn_decode_reserve(&d->kv[0], d->n_seq, d->m.n_heads, n)) return rc;
-	// the captured step holds the prefix it was captured with
-	HK_HIP(hipStreamSynchronize(stream()));
-	if (d->exec) HK_HIP(hipGraphExecDestroy(d->exec));
-	if (d->graph) HK_HIP(hipGraphDestroy(d->graph));
-	d->exec = nullptr;
-	d->graph = nullptr;
+	if (int rc = drop_graphs(d)) return rc;
 	d->prefix_seq = seq;
 	d->prefix_len = n;
+	return ok();
+}
+
+int hako_gpu_decoder_window(hako_gpu_decoder *d, int window, int sinks) {
+	if (!d) return set_error(HAKO_GPU_EINVAL, "null decoder");
+	if (!d->kv_type) return set_error(HAKO_GPU_EINVAL, "a window needs a cache of 8 or 16 bits");
+	if (window < 0 || sinks < 0) return set_error(HAKO_GPU_EINVAL, "a window of %d positions after %d sinks", window, sinks);
+	if (window && d->prefix_len) return set_error(HAKO_GPU_EINVAL, "a prefix is not shared under a window");
+	if (int rc = attn_decode_reserve(&d->kv[0], d->n_seq, d->m.n_heads, 0, window, sinks)) return rc;
+	if (int rc = drop_graphs(d)) return rc;
+	d->window = window;
+	d->sinks = sinks;
 	return ok();
 }
 
@@ -2606,6 +2741,129 @@ int hako_gpu_decoder_prefill(hako_gpu_decoder *d, int seq, const int *tokens, in
 	HK_HIP(hipStreamSynchronize(stream()));
 	// greedy pick as the device argmax: NaN never wins, ties take the lowest index
 	if (next) *next = first_max(dst, m.vocab);
+	return ok();
+}
+
+int hako_gpu_decoder_beam(hako_gpu_decoder *d, int n_beams, const int *tokens, int n, int eos, int *out, float *score) {
+	if (!d || !tokens || !out || !score || n <= 0) return set_error(HAKO_GPU_EINVAL, "null argument or n <= 0");
+	if (!d->kv_type) return set_error(HAKO_GPU_EINVAL, "beams need a cache of 8 or 16 bits");
+	if (n_beams < 2 || d->n_seq % n_beams)
+		return set_error(HAKO_GPU_EINVAL, "%d beams a request in a decoder of %d sequences", n_beams, d->n_seq);
+	if (n > d->max_seq) return set_error(HAKO_GPU_EINVAL, "%d steps in sequences of %d positions", n, d->max_seq);
+	const int S = d->n_seq, K = n_beams, R = S / K, V = d->m.vocab;
+	// arrays of S: tokens, positions, parents, since, rows, ends; scores
+	std::unique_ptr<int[]> host(new (std::nothrow) int[6 * S]);
+	std::unique_ptr<int[]> hist(new (std::nothrow) int[(size_t)2 * n * S]);
+	if (!host || !hist) return set_error(HAKO_GPU_ENOMEM, "host memory for %d steps", n);
+	int *tok = host.get(), *pos = tok + S, *parent = pos + S, *since = parent + S, *len = since + S, *done = len + S;
+	HK_HIP(hipMemcpyAsync(pos, d->pos, sizeof(int) * S, hipMemcpyDeviceToHost, stream()));
+	HK_HIP(hipStreamSynchronize(stream()));
+	for (int r = 0; r < R; r++) {
+		const int p = pos[r * K];
+		if (tokens[r] < 0 || tokens[r] >= V) return set_error(HAKO_GPU_EINVAL, "token %d of request %d outside the vocabulary", tokens[r], r);
+		if (p < 0 || p > d->max_seq - n)
+			return set_error(HAKO_GPU_EINVAL, "request %d at position %d has no room for %d steps (max_seq %d)", r, p, n, d->max_seq);
+		if (p < d->prefix_len)
+			return set_error(HAKO_GPU_EINVAL, "request %d at position %d would write inside the prefix of %d positions", r, p, d->prefix_len);
+		since[r] = d->prefix_len;
+		len[r] = p;
+		for (int b = 0; b < K; b++) {
+			tok[r * K + b] = tokens[r];
+			pos[r * K + b] = p;
+			parent[r * K + b] = 0;
+			done[r * K + b] = 0;
+			score[r * K + b] = b ? -__builtin_inff() : 0.0f;
+		}
+	}
+	if (int rc = beam_alloc(d)) return rc;
+	if (int rc = beam_reserve(S, V, K)) return rc;
+	if (!d->b_exec || d->b_exec_beams != K || d->b_exec_eos != eos) {
+		HK_HIP(hipStreamSynchronize(stream()));
+		if (d->b_exec) HK_HIP(hipGraphExecDestroy(d->b_exec));
+		d->b_exec = nullptr;
+		if (d->b_graph) HK_HIP(hipGraphDestroy(d->b_graph));
+		d->b_graph = nullptr;
+		d->beams = K;
+		d->beam_eos = eos;
+		const int rc = capture_step(d, &d->b_graph, &d->b_exec);
+		d->beams = 0;
+		if (rc) return rc;
+		d->b_exec_beams = K;
+		d->b_exec_eos = eos;
+	}
+	// every beam starts from the rows of its request's first sequence; only that one is a beam before the first step
+	auto put = [&](void *dst, const void *src, int k) { return hipMemcpyAsync(dst, src, sizeof(int) * k, hipMemcpyHostToDevice, stream()); };
+	HK_HIP(put(d->b_parent, parent, S));
+	HK_HIP(put(d->b_since, since, R));
+	HK_HIP(put(d->b_len, len, R));
+	if (int rc = hako_gpu_kv_reorder(d->kv.data(), (int)d->kv.size(), nullptr, d->b_parent, R, K, d->b_since, d->b_len)) return rc;
+	HK_HIP(hipStreamSynchronize(stream()));
+	for (int r = 0; r < R; r++) {
+		since[r] = len[r];
+		len[r]++;
+	}
+	HK_HIP(put(d->b_since, since, R));
+	HK_HIP(put(d->b_len, len, R));
+	HK_HIP(put(d->b_score, score, S));
+	HK_HIP(put(d->b_done, done, S));
+	HK_HIP(put(d->nout, done, S));
+	HK_HIP(put(d->tok, tok, S));
+	HK_HIP(put(d->pos, pos, S));
+	for (int i = 0; i < n; i++) HK_HIP(hipGraphLaunch(d->b_exec, stream()));
+	HK_HIP(hipMemcpyAsync(hist.get(), d->b_hist, sizeof(int) * 2 * n * S, hipMemcpyDeviceToHost, stream()));
+	HK_HIP(hipMemcpyAsync(score, d->b_score, sizeof(float) * S, hipMemcpyDeviceToHost, stream()));
+	HK_HIP(hipStreamSynchronize(stream()));
+	// a beam's tokens, from its last one back through the parents
+	for (int s = 0; s < S; s++) {
+		int at = s;
+		for (int i = n - 1; i >= 0; i--) {
+			const int p = hist[(size_t)i * 2 * S + at];
+			out[(size_t)s * n + i] = hist[(size_t)(i * 2 + 1) * S + at];
+			at = p < 0 ? at : s / K * K + p;
+		}
+	}
+	return ok();
+}
+
+int hako_gpu_decoder_verify(hako_gpu_decoder *d, int seq, const int *tokens, const int *parent, int n, int *out, int *n_out) {
+	if (!d || !tokens || !parent || !out || !n_out) return set_error(HAKO_GPU_EINVAL, "null argument");
+	if (!d->kv_type) return set_error(HAKO_GPU_EINVAL, "drafted trees need a cache of 8 or 16 bits");
+	if (d->window) return set_error(HAKO_GPU_EINVAL, "a drafted tree is not verified under a window");
+	if (seq < 0 || seq >= d->n_seq) return set_error(HAKO_GPU_EINVAL, "sequence %d of %d", seq, d->n_seq);
+	if (n < 1 || n > HAKO_MAX_TREE) return set_error(HAKO_GPU_EINVAL, "a tree of %d nodes (1 to %d)", n, HAKO_MAX_TREE);
+	const hako_gpu_model &m = d->m;
+	for (int i = 0; i < n; i++) {
+		if (tokens[i] < 0 || tokens[i] >= m.vocab) return set_error(HAKO_GPU_EINVAL, "token %d of node %d outside the vocabulary", tokens[i], i);
+		if (i ? parent[i] < 0 || parent[i] >= i : parent[i] != -1) return set_error(HAKO_GPU_EINVAL, "node %d with parent %d", i, parent[i]);
+	}
+	int pos0 = 0;
+	HK_HIP(hipMemcpyAsync(&pos0, d->pos + seq, sizeof(int), hipMemcpyDeviceToHost, stream()));
+	HK_HIP(hipStreamSynchronize(stream()));
+	if (pos0 < 0 || pos0 > d->max_seq - n)
+		return set_error(HAKO_GPU_EINVAL, "sequence %d at position %d has no room for %d nodes (max_seq %d)", seq, pos0, n, d->max_seq);
+	if (pos0 < d->prefix_len)
+		return set_error(HAKO_GPU_EINVAL, "sequence %d at position %d would write inside the prefix of %d positions", seq, pos0,
+		                 d->prefix_len);
+	if (int rc = prefill_alloc(d)) return rc;
+	if (int rc = tree_alloc(d)) return rc;
+	if (int rc = prefill_chunk(d, seq, tokens, n, pos0, parent)) return rc;
+	if (int rc = rmsnorm(d->pf_x, m.out_norm, d->pf_xn, m.d_model, m.rms_eps, n)) return rc;
+	if (int rc = hako_gpu_matmul_batch(d->tr_logits, d->pf_xn, m.t_out, m.out_weight, nullptr, n, m.vocab, m.d_model)) return rc;
+	hipLaunchKernelGGL(argmax_part_kernel, dim3(kArgBlocks, n), dim3(256), 0, stream(), d->tr_logits, m.vocab, d->tr_apart);
+	HK_LAUNCHED("argmax");
+	hipLaunchKernelGGL(argmax_row_kernel, dim3(n), dim3(64), 0, stream(), d->tr_apart, d->tr_logits, m.vocab, d->tr_pick);
+	HK_LAUNCHED("argmax rows");
+	int *const one = d->tr_one;
+	if (int rc = hako_gpu_tree_accept(d->tr_parent, d->pf_tok, d->tr_pick, one, 1, n, d->tr_path, one + 2, one + 3, one + 4)) return rc;
+	if (int rc = hako_gpu_kv_keep(d->kv.data(), (int)d->kv.size(), one + 1, one, d->tr_path, one + 2, 1, n)) return rc;
+	HK_HIP(hipMemcpyAsync(d->pos + seq, one + 4, sizeof(int), hipMemcpyDeviceToDevice, stream()));
+	int path[HAKO_MAX_TREE], picks[HAKO_MAX_TREE], count = 0;
+	HK_HIP(hipMemcpyAsync(path, d->tr_path, sizeof(int) * n, hipMemcpyDeviceToHost, stream()));
+	HK_HIP(hipMemcpyAsync(picks, d->tr_pick, sizeof(int) * n, hipMemcpyDeviceToHost, stream()));
+	HK_HIP(hipMemcpyAsync(&count, one + 2, sizeof(int), hipMemcpyDeviceToHost, stream()));
+	HK_HIP(hipStreamSynchronize(stream()));
+	for (int i = 0; i < count; i++) out[i] = picks[path[i]];
+	*n_out = count;
 	return ok();
 }
 

@@ -24,6 +24,8 @@ int attn_decode_window(float *out, int64_t ldo, const float *q, int64_t ldq, con
                        const int *len, int len_add, int n_seq, int H, float scale, int window, int sinks);
 // The workspace of such calls, taken now (before a capture); window 0: none.
 int attn_decode_reserve(const hako_gpu_kv *kv, int n_seq, int H, int prefix_len, int window = 0, int sinks = 0);
+// The workspace of hako_gpu_beam_select over `rows` beams, taken now.
+int beam_reserve(int rows, int vocab, int n_pick);
 // The sizes of a batch of drafted trees.
 int tree_check(int n_seq, int n_tree);
 

@@ -549,6 +549,21 @@ int each_layers(const hako_gpu_kv *kv, int n_kv, Launch launch) {
 
 Shape shape_of(const hako_gpu_kv *kv) { return {kv->n_slots, kv->max_seq, kv->n_kv_heads, kv->head_dim * kv_elt(kv->type)}; }
 
+// How the rows of a selection are shared out, parts of whole tiles until the waves fill the chip, and the room for them.
+int beam_parts(int rows, int vocab, int n_pick, int *span, int *parts, Parts *out) {
+	const int tiles = (vocab + kPickTile - 1) / kPickTile, want = (kPickFill * cu_count() + rows - 1) / rows;
+	*span = (tiles + want - 1) / want * kPickTile;
+	*parts = (vocab + *span - 1) / *span;
+	const size_t recs = (size_t)rows * *parts;
+	void *p = nullptr;
+	if (int rc = workspace(kWsSearch, recs * (12 + 8 * (size_t)n_pick), &p)) return rc;
+	out->sum = (double *)p;
+	out->top = (float *)(out->sum + recs);
+	out->v = out->top + recs;
+	out->i = (int *)(out->v + recs * n_pick);
+	return HAKO_GPU_OK;
+}
+
 // Workgroups of a launch over the heads of its caches, each with n sequences' rows, some to spare.
 int heads_check(int n_kv, const Shape &c, int n) {
 	const int64_t heads = (int64_t)(n_kv < kLayers ? n_kv : kLayers) * c.kvh * 2 * n;
@@ -557,6 +572,12 @@ int heads_check(int n_kv, const Shape &c, int n) {
 }
 
 }  // namespace
+
+int beam_reserve(int rows, int vocab, int n_pick) {
+	int span, parts;
+	Parts out;
+	return beam_parts(rows, vocab, n_pick, &span, &parts, &out);
+}
 
 int tree_check(int n_seq, int n_tree) {
 	if (n_seq < 0 || n_seq > 0x7FFFFFFF / HAKO_MAX_TREE || n_tree < 1 || n_tree > HAKO_MAX_TREE)
@@ -584,17 +605,9 @@ int hako_gpu_beam_select(const float *logits, int64_t ld, int vocab, const float
 	if (int rc = require_device()) return rc;
 	if (n_req == 0) return ok();
 	const int rows = n_req * n_beams;
-	// parts of whole tiles, until the waves fill the chip
-	const int tiles = (vocab + kPickTile - 1) / kPickTile, want = (kPickFill * cu_count() + rows - 1) / rows;
-	const int span = (tiles + want - 1) / want * kPickTile, parts = (vocab + span - 1) / span;
-	const size_t recs = (size_t)rows * parts;
-	void *p = nullptr;
-	if (int rc = workspace(kWsSearch, recs * (12 + 8 * (size_t)n_pick), &p)) return rc;
+	int span, parts;
 	Parts out;
-	out.sum = (double *)p;
-	out.top = (float *)(out.sum + recs);
-	out.v = out.top + recs;
-	out.i = (int *)(out.v + recs * n_pick);
+	if (int rc = beam_parts(rows, vocab, n_pick, &span, &parts, &out)) return rc;
 	hipLaunchKernelGGL(beam_part_kernel, dim3((parts + kPickWaves - 1) / kPickWaves, rows), dim3(64 * kPickWaves), 0, stream(), logits, ld,
 	                   vocab, done, parts, span, n_pick, out);
 	HK_LAUNCHED("beam parts");

@@ -114,6 +114,10 @@ class Decoder:
         """Positions below n of every sequence become those of sequence `seq`."""
         self.gpu.check(self.lib.hako_gpu_decoder_share_prefix(self.d, seq, n), "decoder_share_prefix")
 
+    def window(self, window: int, sinks: int = 0):
+        """A token sees the last `window` positions and the first `sinks` from now on (0: all again)."""
+        self.gpu.check(self.lib.hako_gpu_decoder_window(self.d, window, sinks), "decoder_window")
+
     def kv_offset(self, seq: int, layer: int, pos: int) -> int:
         """Byte offset of (seq, layer, pos) in either cache."""
         return 4 * ((seq * self.cfg["n_layers"] + layer) * self.max_seq + pos) * self.kv_dim
@@ -147,6 +151,23 @@ class Decoder:
                                                          None if lg is None else lg.ctypes.data, nxt.ctypes.data),
                        "decoder_prefill")
         return (int(nxt[0]), lg) if logits else int(nxt[0])
+
+    def beam(self, n_beams: int, tokens, n: int, eos: int = -1):
+        """n steps of a beam search; (tokens [n_seq][n], scores [n_seq])."""
+        t = np.ascontiguousarray(np.broadcast_to(np.asarray(tokens, np.int32), (self.n_seq // max(n_beams, 1),)))
+        out, score = np.empty((self.n_seq, max(n, 0)), np.int32), np.empty(self.n_seq, np.float32)
+        self.gpu.check(self.lib.hako_gpu_decoder_beam(self.d, n_beams, t.ctypes.data, n, eos, out.ctypes.data,
+                                                      score.ctypes.data), "decoder_beam")
+        return out, score
+
+    def verify(self, tokens, parent, seq: int = 0) -> np.ndarray:
+        """One pass over a drafted tree of sequence `seq`; the tokens that the model follows."""
+        t, p = (np.ascontiguousarray(np.asarray(x, np.int32).reshape(-1)) for x in (tokens, parent))
+        assert t.size == p.size
+        out, count = np.empty(t.size, np.int32), np.zeros(1, np.int32)
+        self.gpu.check(self.lib.hako_gpu_decoder_verify(self.d, seq, t.ctypes.data, p.ctypes.data, t.size, out.ctypes.data,
+                                                        count.ctypes.data), "decoder_verify")
+        return out[:int(count[0])].copy()
 
     def replay(self, n: int):
         self.gpu.check(self.lib.hako_gpu_decoder_replay(self.d, n), "decoder_replay")

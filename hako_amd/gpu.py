@@ -72,6 +72,9 @@ SIGNATURES = {
     "hako_gpu_decoder_replay": (_i, [_vp, _i]),
     "hako_gpu_decoder_prefill": (_i, [_vp, _i, _vp, _i, _vp, _vp]),
     "hako_gpu_decoder_on_destroy": (_i, [_vp, _vp, _vp]),
+    "hako_gpu_decoder_window": (_i, [_vp, _i, _i]),
+    "hako_gpu_decoder_beam": (_i, [_vp, _i, _vp, _i, _i, _vp, _vp]),
+    "hako_gpu_decoder_verify": (_i, [_vp, _i, _vp, _vp, _i, _vp, _vp]),
 }
 
 # ... and include/hako_attn.h.

@@ -20,7 +20,7 @@
 #include <stddef.h>
 #include <stdint.h>
 
-#include "hako_attn.h"
+#include "hako_search.h"
 
 #ifdef __cplusplus
 extern "C" {
@@ -90,6 +90,12 @@ int hako_gpu_decoder_cache(hako_gpu_decoder *dec, int layer, hako_gpu_kv *kv);
  * below n is refused. Needs a cache of 8 or 16 bits. */
 int hako_gpu_decoder_share_prefix(hako_gpu_decoder *dec, int seq, int n);
 
+/* From the next call on, a token sees the `window` positions that end with its
+ * own and the first `sinks` of its sequence, in every layer (hako_attn.h); the
+ * caches keep all positions. window 0 ends this. Needs a cache of 8 or 16 bits
+ * and no shared prefix. */
+int hako_gpu_decoder_window(hako_gpu_decoder *dec, int window, int sinks);
+
 /* Device addresses of the fp32 KV caches, laid out as the reference's
  * (src/model.c:71-72, 117-118) once per sequence:
  * [n_seq][n_layers][max_seq][n_kv_heads*head_dim]. A caller may fill
@@ -122,6 +128,33 @@ int hako_gpu_decoder_generate(hako_gpu_decoder *dec, const int *tokens, int n, i
  * with their greedy id in *next (may be NULL). Synchronous. The other
  * sequences are untouched. */
 int hako_gpu_decoder_prefill(hako_gpu_decoder *dec, int seq, const int *tokens, int n, float *logits, int *next);
+
+/* n steps of a beam search (hako_search.h) for n_seq / n_beams requests of
+ * n_beams (2..16) sequences each; needs a cache of 8 or 16 bits. Request r
+ * starts from the text of its first sequence, r*n_beams, with the next token
+ * tokens[r] (host): the request's other sequences take that text's rows and
+ * position. A beam ends with token eos (-1: none does) and then repeats it at
+ * its score. out[n_seq][n] (host) receives the tokens of each sequence's beam
+ * after tokens[r], score[n_seq] (host) the sums of their log probabilities, in
+ * no order of worth; the caches hold their texts, the positions advance by n.
+ * Where a request has too few continuations (logits that are not finite) a
+ * sequence's last tokens are -1 and its score is -inf. The step is captured as
+ * a HIP graph for its n_beams and eos and replayed. Synchronous. */
+int hako_gpu_decoder_beam(hako_gpu_decoder *dec, int n_beams, const int *tokens, int n, int eos, int *out, float *score);
+
+/* One pass of sequence seq over a drafted tree (hako_search.h) of n
+ * (1..HAKO_MAX_TREE) nodes (host): tokens[0] is the token that comes next,
+ * parent[0] = -1, the others are guesses after their parents, 0 <= parent[j] <
+ * j. Greedy: out (host, room for n) receives the *n_out tokens that the model
+ * picks along the path it follows, the same that as many greedy steps from
+ * tokens[0] would (but for what the last bits of the sums of a pass of n
+ * tokens decide); the last of them is the next call's tokens[0]. The path's
+ * keys and values stay in the caches and the position advances by *n_out.
+ * Needs a cache of 8 or 16 bits, room for n more positions, and no window. The
+ * first call allocates the buffers of hako_gpu_decoder_prefill and the logits of
+ * HAKO_MAX_TREE tokens. Synchronous. */
+int hako_gpu_decoder_verify(hako_gpu_decoder *dec, int seq, const int *tokens, const int *parent, int n, int *out,
+                            int *n_out);
 
 /* Replays the captured step n times from the current device state (no host
  * transfer, no synchronization): the timed loop of a benchmark. */

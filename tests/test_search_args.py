@@ -149,3 +149,9 @@ def test_binding_covers_the_header():
 def test_without_a_device(lib, call, args):
     """What is accepted goes on to the device, and says so where none was initialised."""
     assert call(lib, **args) == ENODEV
+
+
+@pytest.mark.parametrize("call,args", [("hako_gpu_decoder_window", (None, 8, 4)), ("hako_gpu_decoder_beam", (None, 2, P, 3, -1, P, P)),
+                                       ("hako_gpu_decoder_verify", (None, 0, P, P, 3, P, P))])
+def test_decoder_calls_refuse(lib, call, args):
+    assert getattr(lib, call)(*args) == EINVAL
