@@ -2230,6 +2230,20 @@ __global__ __launch_bounds__(256) void tree_join_kernel(AttnKv c, float *out, in
 	join_few(rec_o + first * HD + d, HD, rec_ml + first, rec_e + first, max((nc + per - 1) / per, 1), out + row * ldo + (int64_t)h * HD + d);
 }
 
+// The same for many parts: a workgroup a row and head.
+template <int HD, int K, int R>
+__global__ __launch_bounds__(64 * kJoin) void tree_join_wide_kernel(AttnKv c, float *out, int64_t ldo, const int *__restrict__ slot,
+                                                                    const int *__restrict__ base, int N, int parts,
+                                                                    const float *__restrict__ rec_o, const float2 *__restrict__ rec_ml,
+                                                                    const float *__restrict__ rec_e) {
+	const int h = blockIdx.x, row = blockIdx.y;
+	int sl, b, end;
+	tree_place(c, slot, base, row / N, N, sl, b, end);
+	const int nc = tile_steps<K>(end, c.prefix_len), per = tree_part<R>(nc, parts);
+	const size_t first = ((size_t)row * gridDim.x + h) * parts;
+	join<HD>(rec_o + first * HD, rec_ml + first, rec_e + first, max((nc + per - 1) / per, 1), out + row * ldo + h * HD);
+}
+
 // Trees of N nodes over parts of their keys, `slots` workgroups in all or fewer; launch(parts, blocks, records) of tiles
 // of `rows` rows.
 template <int HD, int K, int R, class Launch>
@@ -2237,7 +2251,8 @@ int tree_launch(const AttnKv &c, float *out, int64_t ldo, const int *slot, const
                 Launch launch) {
 	const int64_t tiles = ((int64_t)N * (H / c.kvh) + rows - 1) / rows, wgs = tiles * n_seq * c.kvh;
 	const int most = (tile_steps<K>(c.max_seq, c.prefix_len) + R - 1) / R;
-	const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(most, slots / wgs));
+	// (whole rounds of the eight dies: one tree of 448 rows at 8000, four heads, 41 us in 9 parts, 31 in 8)
+	const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(most, slots / (8 * tiles) * 8 / ((int64_t)n_seq * c.kvh)));
 	if ((wgs * parts + 8 * tiles) > kMaxThreads / 512 || (int64_t)n_seq * N * H * (HD / 4) > kMaxThreads)
 		return set_error(HAKO_GPU_EINVAL, "%lld workgroups in one call", (long long)(wgs * parts));
 	Records rec{};
@@ -2245,7 +2260,13 @@ int tree_launch(const AttnKv &c, float *out, int64_t ldo, const int *slot, const
 		if (int rc = records((size_t)n_seq * N * H * parts, HD, &rec)) return rc;
 	launch(parts, dim3(tree_blocks((int64_t)n_seq * c.kvh * parts, tiles)), rec);
 	HK_LAUNCHED("attention");
-	if (parts > 1) {
+	// many parts, or rows so few that the other join's would be alone with them (3B heads, us by the other / this: one tree of
+	// 4 nodes at 32000 in 64 parts 77 / 21, of 26 at 1025 in 9 12.9 / 12.0, but 8 of 64 at 4000 in 8 50 / 53)
+	if (parts > 16 || (parts > 6 && (int64_t)n_seq * N * H <= 1024)) {
+		hipLaunchKernelGGL((tree_join_wide_kernel<HD, K, R>), dim3(H, n_seq * N), dim3(64 * kJoin), 0, stream(), c, out, ldo, slot, base, N, parts,
+		                   rec.o, rec.ml, rec.e);
+		HK_LAUNCHED("attention join");
+	} else if (parts > 1) {
 		const int64_t blocks = ((int64_t)n_seq * N * H * (HD / 4) + 255) / 256;
 		hipLaunchKernelGGL((tree_join_kernel<HD, K, R>), dim3((unsigned)blocks), dim3(256), 0, stream(), c, out, ldo, slot, base, n_seq, N, H,
 		                   parts, rec.o, rec.ml, rec.e);

@@ -235,7 +235,14 @@ def test_verify(gpu, model, kind, cfg, n_nodes, prefix):
         for a, b in zip(other, (rows_of(gpu, dec, dec.cache(l), 0, 33) for l in range(cfg.n_layers))):
             for x, y in zip(a, b):
                 np.testing.assert_array_equal(x, y)
-        # the caches hold the text: its next step is that of the steps one at a time
+        # the caches hold the text's rows, turned by their places in it: layer 0's follow from tokens and places alone, so that
+        # they differ by a code at most, and seldom
+        step = 1 / 127 if kind == KV_Q8 else 2.0 ** -10
+        for a, b in zip(*(rows_of(gpu, d, d.cache(0), seq, pos[1]) for d in (dec, own))):
+            a, b = (x.reshape(-1, cfg.head_dim) for x in (a, b))
+            assert (np.abs(a - b) <= (step + 1e-5) * np.abs(b).max(1, keepdims=True)).all()
+            assert (np.abs(a - b) > 1e-5 * np.abs(b).max(1, keepdims=True)).mean() < 0.05
+        # ... and its next step is that of the steps one at a time
         for d in (dec, own):
             d.set_pos(pos)
         within("next step", dec.step([0, tok], logits=True)[1][1], own.step([0, tok], logits=True)[1][1], 5 * STEP_BAR[kind])
