@@ -1,5 +1,6 @@
 // attn.hip — attention over the quantised cache (include/hako_attn.h): single
-// tokens of many sequences, and whole packed prompts.
+// tokens of many sequences, whole packed prompts, both also under a window with
+// sinks, and trees of drafted tokens.
 //
 // One pass over the keys with a running maximum and sum (log2 units):
 //   u_p = scale log2(e) q.k_p,  M = max u_p,  l = sum 2^(u_p - M),
@@ -40,6 +41,7 @@ constexpr int kItems = 480;      // items of a launch whose order the host sets 
 constexpr int kWsAttn = 7;       // library workspace slot of the records
 constexpr int kKeys = 64;        // keys per chunk of the tiled kernel
 constexpr int kLongPart = 2048;  // keys of a part where sequences alone fill the chip
+constexpr int kLongWindow = 8192; // the same under a window
 constexpr int kWaves = 4;        // waves per workgroup of the direct and the single-token kernel
 // M is a whole number not below what it was taken from (the maximum of the
 // scores, in log2, plus the exponent of the value scales), so that what is
@@ -1836,7 +1838,7 @@ struct DecodePlan {
 	int64_t tiles;
 	int parts, least, pparts, unit, nrec;
 };
-DecodePlan decode_plan(int own, int prefix_len, int kvh, int n_seq, int H) {
+DecodePlan decode_plan(int own, int prefix_len, int kvh, int n_seq, int H, bool window) {
 	DecodePlan p{};
 	const int slots = 2 * cu_count();   // workgroups that run at once
 	// own keys: parts of 32 keys a wave or more, until the workgroups fill the chip (16 sequences of 4096, 64 pairs of
@@ -1845,7 +1847,9 @@ DecodePlan decode_plan(int own, int prefix_len, int kvh, int n_seq, int H) {
 	// part; all of 4096 56 to 58 us, 50 to 53 in one part). The lengths are not known here, so the parts are those of
 	// max_seq: 64 sequences of 1000 positions in slots of 2048 take 14.9 us, of 8192 17.4, of 32768 20.6
 	const int64_t pairs = (int64_t)n_seq * kvh;
-	p.least = pairs >= cu_count() ? kLongPart : 32 * kWaves;
+	// A window bounds how far lengths differ: longer parts then (64 sequences under 4096 49 us in parts of 2048, 44 in one,
+	// 128 under 2048 54 and 45)
+	p.least = pairs >= cu_count() ? (window ? kLongWindow : kLongPart) : 32 * kWaves;
 	p.parts = (own + p.least - 1) / p.least;
 	if (pairs < cu_count()) p.parts = std::min(p.parts, (int)(((prefix_len ? slots / 2 : slots) + pairs - 1) / pairs));
 	p.parts = std::max(1, p.parts);
@@ -1874,7 +1878,7 @@ template <int HD, bool Q8, bool WIN>
 int decode(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq, const int *slot, const int *len,
            int n_seq, int H, float scale) {
 	const int G = H / c.kvh;
-	const DecodePlan p = decode_plan(most_keys(c), c.prefix_len, c.kvh, n_seq, H);
+	const DecodePlan p = decode_plan(most_keys(c), c.prefix_len, c.kvh, n_seq, H, WIN);
 	const int parts = p.parts, least = p.least, pparts = p.pparts, unit = p.unit, nrec = p.nrec;
 	const int64_t tiles = p.tiles;
 	Records rec{};
@@ -2333,7 +2337,7 @@ int attn_decode_window(float *out, int64_t ldo, const float *q, int64_t ldq, con
 
 int attn_decode_reserve(const hako_gpu_kv *kv, int n_seq, int H, int prefix_len, int window, int sinks) {
 	const AttnKv c = window ? attn_kv_window(kv, 0, window, sinks) : attn_kv(kv, 0, prefix_len, 0);
-	const DecodePlan p = decode_plan(most_keys(c), prefix_len, kv->n_kv_heads, n_seq, H);
+	const DecodePlan p = decode_plan(most_keys(c), prefix_len, kv->n_kv_heads, n_seq, H, window > 0);
 	Records r;
 	return p.nrec ? records((size_t)n_seq * H * p.nrec, kv->head_dim, &r) : HAKO_GPU_OK;
 }

@@ -89,6 +89,21 @@ def test_decode_in_parts(gpu, kind, n, max_seq, window, sinks):
     c.free()
 
 
+def test_decode_of_many_in_parts(gpu):
+    """Sequences enough to fill the chip (they read two slots by turns) under a window of several long parts."""
+    H, KVH, hd, n, max_seq, W, S = 16, 16, 64, 17, 17000, 16500, 40
+    rng = np.random.default_rng(17)
+    c = ref.Cache(gpu, KV_Q8, 2, max_seq, KVH, hd, rng)
+    K, V = c.values()
+    lens = [17000, 3, 16541, 16540, 9000, 16999, 1, 0, 12345, 8192, 8193, 16384, 16500, 16501, 17000, 100, 16700]
+    q = rng.standard_normal((n, H, hd)).astype(np.float32)
+    slot = [i % 2 for i in range(n)]
+    got = run_decode(gpu, c, q, slot, lens, 0.125, W, S)
+    for i in range(n):
+        close(got[i], attend(q[i], K, V, slot[i], lens[i] - 1, 0.125, W, S))
+    c.free()
+
+
 def test_everything_in_sight_is_the_other_call(gpu):
     """A window that covers the text: the same numbers as without one, to the bound."""
     rng = np.random.default_rng(5)
