@@ -1121,16 +1121,14 @@ __device__ __forceinline__ void direct_rows(const AttnKv &c, DirectLds<HD> &s, c
 	const int tg = __shfl(tok_g, out);
 	if (tg < 0) return;
 	const bool blank = seen.kBlanks && tg & kBlank;
+	if (blank && !dest.o) return;   // (nobody reads a record of nothing)
 	const int tok = (seen.kBlanks ? tg & ~kBlank : tg) >> 4;
 	const size_t r = dest.first + tok * dest.rt + (tg & 15) * dest.rg;
 	float *to = dest.o ? dest.o + tok * dest.ot + (tg & 15) * dest.og : dest.rec.o + r * HD;
 	int x[kWaves];
 	float ls;
-	Base b = meet(s.ml, out, x, ls);
-	if (blank) {
-		b = {kNone, 0.0f};
-		ls = 0.0f;
-	}
+	const Base b = meet(s.ml, out, x, ls);
+	if (blank) ls = 0.0f;
 	const float z = !dest.o ? 1.0f : (ls == 0.0f ? 0.0f : 1.0f / ls);
 #pragma unroll
 	for (int d = 4 * (at & 7); d < HD; d += 32) {
@@ -2119,6 +2117,10 @@ __device__ __forceinline__ bool tree_place(const AttnKv &c, const int *slot, con
 	end = on ? min(b + N, c.max_seq) : 0;
 	return on;
 }
+// The nodes of a row that it sees, 0: it is not there.
+__device__ __forceinline__ uint64_t tree_bits(const uint64_t *seen, int64_t row, int N) {
+	return N < 64 ? seen[row] & ((1ull << N) - 1) : seen[row];
+}
 // Steps per part of a tile with nc steps, in whole rounds of R.
 template <int R>
 __device__ __forceinline__ int tree_part(int nc, int parts) {
@@ -2138,18 +2140,13 @@ __device__ __forceinline__ bool tree_item(int n_kvh, int n_seq, int parts, int t
 }
 unsigned tree_blocks(int64_t items, int64_t tiles) { return (unsigned)((items + 7) / 8 * 8 * tiles); }
 
-// Zeros, or records of nothing, for the 32 rows (node, g) that a wave's lanes hold (node -1: none), by a workgroup whose
-// waves hold the same.
+// Zeros for the 32 rows (node, g) that a wave's lanes hold (node -1: none), by a workgroup whose waves hold the same.
 template <int HD>
-__device__ __forceinline__ void tree_blank(int node, int g, int sq, int N, int head, float *out, int64_t ldo, int H, int parts, int part,
-                                           const Records &rec) {
-	const int row = threadIdx.x >> 3, n = __shfl(node, row), hd = head + __shfl(g, row);
+__device__ __forceinline__ void tree_blank(int node, int g, float *out, int64_t ldo) {
+	const int row = threadIdx.x >> 3, n = __shfl(node, row), hd = __shfl(g, row);
 	if (n < 0) return;
-	const size_t r = (((size_t)sq * N + n) * H + hd) * parts + part;
-	float *to = parts == 1 ? out + ((int64_t)sq * N + n) * ldo + (int64_t)hd * HD : rec.o + r * HD;
 #pragma unroll
-	for (int d = 4 * (threadIdx.x & 7); d < HD; d += 32) *(float4 *)(to + d) = make_float4(0, 0, 0, 0);
-	if (parts > 1 && (threadIdx.x & 7) == 0) rec.put(r, {kNone, 0.0f}, 0.0f);
+	for (int d = 4 * (threadIdx.x & 7); d < HD; d += 32) *(float4 *)(out + n * ldo + hd * HD + d) = make_float4(0, 0, 0, 0);
 }
 
 template <int HD, bool Q8>
@@ -2170,10 +2167,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(AttnKv c, float *o
 	const int per = tree_part<kWaves>(nc, parts), c0 = part * per;
 	if (c0 >= nc && part > 0) return;   // a record that the join does not read
 	const int64_t row = (int64_t)sq * N + node;
-	uint64_t bits = on && placed ? seen[row] : 0;
-	if (N < 64) bits &= (1ull << N) - 1;
+	const uint64_t bits = on && placed ? tree_bits(seen, row, N) : 0;
 	if (!__any(bits != 0)) {   // nodes that are not there, as in the last tiles of a padded tree
-		tree_blank<HD>(on ? node : -1, g, sq, N, head, out, ldo, H, parts, part, rec);
+		if (parts == 1) tree_blank<HD>(on ? node : -1, g, out + (int64_t)sq * N * ldo + head * HD, ldo);
 		return;
 	}
 	direct_rows<HD, Q8>(c, s, sp, c0, min(nc, c0 + per), on && bits ? q + row * ldq + (head + g) * HD : nullptr, scale, Nodes{b, bits, 0},
@@ -2200,26 +2196,25 @@ __global__ __launch_bounds__(64 * W, 2) void tree_tiled_kernel(AttnKv c, float *
 	const int per = tree_part<1>(nc, parts), c0 = part * per;
 	if (c0 >= nc && part > 0) return;   // a record that the join does not read
 	const int64_t row = (int64_t)sq * N + node;
-	uint64_t bits = on && placed ? seen[row] : 0;
-	if (N < 64) bits &= (1ull << N) - 1;
+	const uint64_t bits = on && placed ? tree_bits(seen, row, N) : 0;
 	// a wave without nodes sees nothing, a workgroup without any passes no chunk
 	const int hi = __any(bits != 0) ? end : 0, stop = __syncthreads_or(hi) ? min(nc, c0 + per) : c0;
 	Tile<HD, Q8, W> w;
 	w.chunks(c, sp, c0, stop, Nodes{b, bits, 0}, b, hi, s, tid,
 	         [&] { w.query(on ? q + row * ldq + head * HD : nullptr, scale, s, tid); });
-	if (!bits) w.clear();
 	if (parts == 1) {
+		if (!bits) w.clear();
 		w.put(on ? out + row * ldo + head * HD : nullptr, w.l == 0.0f ? 0.0f : 1.0f / w.l, s, tid);
 		return;
 	}
 	const size_t r0 = ((size_t)row * H + head) * parts + part;
-	w.put(on ? rec.o + r0 * HD : nullptr, 1.0f, s, tid);
-	if (on && lane < 32) rec.put(r0, {w.M, bits && w.big ? s.be[tid] : 0.0f}, w.l);
+	w.put(bits ? rec.o + r0 * HD : nullptr, 1.0f, s, tid);
+	if (bits && lane < 32) rec.put(r0, {w.M, w.big ? s.be[tid] : 0.0f}, w.l);
 }
 
 template <int HD, int K, int R>
 __global__ __launch_bounds__(256) void tree_join_kernel(AttnKv c, float *out, int64_t ldo, const int *__restrict__ slot,
-                                                        const int *__restrict__ base, int n_seq, int N, int H, int parts,
+                                                        const int *__restrict__ base, const uint64_t *__restrict__ seen, int n_seq, int N, int H, int parts,
                                                         const float *__restrict__ rec_o, const float2 *__restrict__ rec_ml,
                                                         const float *__restrict__ rec_e) {
 	constexpr int L = HD / 4;
@@ -2228,21 +2223,28 @@ __global__ __launch_bounds__(256) void tree_join_kernel(AttnKv c, float *out, in
 	const int h = (int)(i - row * H), d = threadIdx.x % L * 4, sq = (int)(row / N);
 	if (sq >= n_seq) return;
 	int sl, b, end;
-	tree_place(c, slot, base, sq, N, sl, b, end);
+	float *to = out + row * ldo + (int64_t)h * HD + d;
+	if (!tree_place(c, slot, base, sq, N, sl, b, end) || !tree_bits(seen, row, N)) {
+		*(float4 *)to = make_float4(0, 0, 0, 0);
+		return;
+	}
 	const int nc = tile_steps<K>(end, c.prefix_len), per = tree_part<R>(nc, parts);
 	const size_t first = (size_t)i * parts;
-	join_few(rec_o + first * HD + d, HD, rec_ml + first, rec_e + first, max((nc + per - 1) / per, 1), out + row * ldo + (int64_t)h * HD + d);
+	join_few(rec_o + first * HD + d, HD, rec_ml + first, rec_e + first, max((nc + per - 1) / per, 1), to);
 }
 
 // The same for many parts: a workgroup a row and head.
 template <int HD, int K, int R>
 __global__ __launch_bounds__(64 * kJoin) void tree_join_wide_kernel(AttnKv c, float *out, int64_t ldo, const int *__restrict__ slot,
-                                                                    const int *__restrict__ base, int N, int parts,
-                                                                    const float *__restrict__ rec_o, const float2 *__restrict__ rec_ml,
-                                                                    const float *__restrict__ rec_e) {
+                                                                    const int *__restrict__ base, const uint64_t *__restrict__ seen,
+                                                                    int N, int parts, const float *__restrict__ rec_o,
+                                                                    const float2 *__restrict__ rec_ml, const float *__restrict__ rec_e) {
 	const int h = blockIdx.x, row = blockIdx.y;
 	int sl, b, end;
-	tree_place(c, slot, base, row / N, N, sl, b, end);
+	if (!tree_place(c, slot, base, row / N, N, sl, b, end) || !tree_bits(seen, row, N)) {
+		if (threadIdx.x < HD) out[row * ldo + h * HD + threadIdx.x] = 0.0f;
+		return;
+	}
 	const int nc = tile_steps<K>(end, c.prefix_len), per = tree_part<R>(nc, parts);
 	const size_t first = ((size_t)row * gridDim.x + h) * parts;
 	join<HD>(rec_o + first * HD, rec_ml + first, rec_e + first, max((nc + per - 1) / per, 1), out + row * ldo + h * HD);
@@ -2251,7 +2253,7 @@ __global__ __launch_bounds__(64 * kJoin) void tree_join_wide_kernel(AttnKv c, fl
 // Trees of N nodes over parts of their keys, `slots` workgroups in all or fewer; launch(parts, blocks, records) of tiles
 // of `rows` rows.
 template <int HD, int K, int R, class Launch>
-int tree_launch(const AttnKv &c, float *out, int64_t ldo, const int *slot, const int *base, int n_seq, int N, int H, int rows, int64_t slots,
+int tree_launch(const AttnKv &c, float *out, int64_t ldo, const int *slot, const int *base, const uint64_t *seen, int n_seq, int N, int H, int rows, int64_t slots,
                 Launch launch) {
 	const int64_t tiles = ((int64_t)N * (H / c.kvh) + rows - 1) / rows, wgs = tiles * n_seq * c.kvh;
 	const int most = (tile_steps<K>(c.max_seq, c.prefix_len) + R - 1) / R;
@@ -2267,13 +2269,13 @@ int tree_launch(const AttnKv &c, float *out, int64_t ldo, const int *slot, const
 	// many parts, or rows so few that the other join's would be alone with them (3B heads, us by the other / this: one tree of
 	// 4 nodes at 32000 in 64 parts 77 / 21, of 26 at 1025 in 9 12.9 / 12.0, but 8 of 64 at 4000 in 8 50 / 53)
 	if (parts > 16 || (parts > 6 && (int64_t)n_seq * N * H <= 1024)) {
-		hipLaunchKernelGGL((tree_join_wide_kernel<HD, K, R>), dim3(H, n_seq * N), dim3(64 * kJoin), 0, stream(), c, out, ldo, slot, base, N, parts,
+		hipLaunchKernelGGL((tree_join_wide_kernel<HD, K, R>), dim3(H, n_seq * N), dim3(64 * kJoin), 0, stream(), c, out, ldo, slot, base, seen, N, parts,
 		                   rec.o, rec.ml, rec.e);
 		HK_LAUNCHED("attention join");
 	} else if (parts > 1) {
 		const int64_t blocks = ((int64_t)n_seq * N * H * (HD / 4) + 255) / 256;
-		hipLaunchKernelGGL((tree_join_kernel<HD, K, R>), dim3((unsigned)blocks), dim3(256), 0, stream(), c, out, ldo, slot, base, n_seq, N, H,
-		                   parts, rec.o, rec.ml, rec.e);
+		hipLaunchKernelGGL((tree_join_kernel<HD, K, R>), dim3((unsigned)blocks), dim3(256), 0, stream(), c, out, ldo, slot, base, seen, n_seq, N,
+		                   H, parts, rec.o, rec.ml, rec.e);
 		HK_LAUNCHED("attention join");
 	}
 	return HAKO_GPU_OK;
@@ -2302,16 +2304,16 @@ int tree(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq, 
 	const bool tiled = rows > 64 && steps >= 24 * 4 * (int64_t)cu_count();
 	const int kernel = g_attn_prompt ? g_attn_prompt : !tiled ? 1 : rows > 128 || 2 * (int64_t)n_seq * c.kvh > cu_count() ? 2 : 3;
 	if (kernel == 2)
-		return tree_launch<HD, kKeys, 1>(c, out, ldo, slot, base, n_seq, N, H, 256, cu_count(), [&](int parts, dim3 grid, const Records &rec) {
+		return tree_launch<HD, kKeys, 1>(c, out, ldo, slot, base, seen, n_seq, N, H, 256, cu_count(), [&](int parts, dim3 grid, const Records &rec) {
 			hipLaunchKernelGGL((tree_tiled_kernel<HD, Q8, 8>), grid, dim3(512), 0, stream(), c, out, ldo, q, ldq, slot, base, seen, n_seq, N, G,
 			                   scale * kLog2e, parts, rec);
 		});
 	if (kernel == 3)
-		return tree_launch<HD, kKeys, 1>(c, out, ldo, slot, base, n_seq, N, H, 128, 2 * cu_count(), [&](int parts, dim3 grid, const Records &rec) {
+		return tree_launch<HD, kKeys, 1>(c, out, ldo, slot, base, seen, n_seq, N, H, 128, 2 * cu_count(), [&](int parts, dim3 grid, const Records &rec) {
 			hipLaunchKernelGGL((tree_tiled_kernel<HD, Q8, 4>), grid, dim3(256), 0, stream(), c, out, ldo, q, ldq, slot, base, seen, n_seq, N, G,
 			                   scale * kLog2e, parts, rec);
 		});
-	return tree_launch<HD, 32, kWaves>(c, out, ldo, slot, base, n_seq, N, H, 32, 2 * cu_count(), [&](int parts, dim3 grid, const Records &rec) {
+	return tree_launch<HD, 32, kWaves>(c, out, ldo, slot, base, seen, n_seq, N, H, 32, 2 * cu_count(), [&](int parts, dim3 grid, const Records &rec) {
 		hipLaunchKernelGGL((tree_kernel<HD, Q8>), grid, dim3(64 * kWaves), 0, stream(), c, out, ldo, q, ldq, slot, base, seen, n_seq, N, G,
 		                   scale * kLog2e, parts, rec);
 	});
