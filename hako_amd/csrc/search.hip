@@ -486,8 +486,10 @@ __global__ __launch_bounds__(64 * kTreeWaves) void tree_plan_kernel(const int *_
 	if (lane >= n_tree) return;
 	if (seen) seen[at] = on ? m : 0;
 	if (node_slot) node_slot[at] = slot ? slot[sq] : sq;
-	if (row) row[at] = on ? b + lane : -1;
-	if (turn) turn[at] = on ? b + __popcll(m) - 1 : -1;
+	// (a place past what an int holds is outside every cache: none)
+	auto after = [&](int k) { return on ? max((int)((uint32_t)b + (uint32_t)k), -1) : -1; };
+	if (row) row[at] = after(lane);
+	if (turn) turn[at] = after(__popcll(m) - 1);
 }
 
 __global__ __launch_bounds__(64 * kTreeWaves) void tree_accept_kernel(const int *__restrict__ parent, const int *__restrict__ token,

@@ -35,8 +35,8 @@ extern "C" {
 /* ── beams ──
  * One step of n_req requests with n_beams beams each; beam b of request r is
  * row r*n_beams + b of logits (vocab floats, at most 2^24, rows ld floats
- * apart), score and done. score is the sum of the log probabilities of the beam's tokens (-inf:
- * no beam there). A continuation of beam b by token t is worth
+ * apart), score and done. score is the sum of the log probabilities of the
+ * beam's tokens (-inf: no beam there). A continuation of beam b by token t is worth
  *   score[b] + (logits[b][t] - log sum_j exp(logits[b][j])),
  * compared in 64 bits; done[b] != 0 marks a beam that has ended: its one
  * continuation is token eos at its own score. done may be NULL (none has).
@@ -63,7 +63,7 @@ int hako_gpu_beam_select(const float *logits, int64_t ld, int vocab, const float
 
 /* After it: beam p of request r takes the cache rows [since[r], len[r]) that
  * beam parent[r][p] of the request held, in all n_kv caches (of one shape, as
- * those of a model's layers; kv is a HOST array), as if all moved at once. A
+ * those of a model's layers, none twice; kv is a HOST array), as if all moved at once. A
  * parent outside 0..n_beams-1, or its own place, leaves a beam's rows as they
  * are. Beam b of request r is in slot slot[r*n_beams + b] (NULL: that number),
  * no two in one slot; a beam whose slot lies outside the cache neither takes
@@ -85,7 +85,7 @@ int hako_gpu_kv_reorder(const hako_gpu_kv *kv, int n_kv, const int *slot, const 
 
 /* A tree's plan: seen, for hako_gpu_attn_tree (bit i of node j: i is j or
  * leads to it; 0: not there), and for hako_gpu_kv_append_turned each node's
- * slot, row and turn (row and turn -1: not there). Any of the four may be
+ * slot, row and turn (row and turn -1: not there, or past 2^31 - 1). Any of the four may be
  * NULL. It follows base; the layers of a step share it. */
 int hako_gpu_tree_plan(const int *slot, const int *base, const int *parent, int n_seq, int n_tree, uint64_t *seen,
                        int *node_slot, int *row, int *turn);
@@ -100,8 +100,8 @@ int hako_gpu_tree_accept(const int *parent, const int *token, const int *pick, c
                          int *path, int *n_path, int *next, int *new_base);
 
 /* The path's rows together: row base[s] + path[s][d] to row base[s] + d for
- * d < n_path[s], as if all moved at once, in all n_kv caches (of one shape; kv
- * is a HOST array). Rows outside the cache, nodes outside the tree and a slot
+ * d < n_path[s], as if all moved at once, in all n_kv caches (of one shape,
+ * none twice; kv is a HOST array). Rows outside the cache, nodes outside the tree and a slot
  * outside the cache are left out, n_path past n_tree counts as n_tree. Then
  * positions below base[s] + n_path[s] are the text. No two sequences in one
  * slot. */
