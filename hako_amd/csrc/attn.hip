@@ -2160,14 +2160,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(AttnKv c, float *o
 	const int lane = threadIdx.x & 63, r = 32 * tile + (lane & 31), node = r / G, g = r - node * G;
 	const int head = kvh * G, H = c.kvh * G;
 	const bool on = node < N;
+	const int64_t row = (int64_t)sq * N + node;
+	uint64_t bits = on ? tree_bits(seen, row, N) : 0;   // (asked for together with the place)
 	int sl, b, end;
-	const bool placed = tree_place(c, slot, base, sq, N, sl, b, end);
+	if (!tree_place(c, slot, base, sq, N, sl, b, end)) bits = 0;
 	const Span sp = span_of<32, false>(c, kvh, sl, 0, 0, end);
 	const int nc = sp.n0 + (max(end - sp.b0, 0) + 31) / 32;
 	const int per = tree_part<kWaves>(nc, parts), c0 = part * per;
 	if (c0 >= nc && part > 0) return;   // a record that the join does not read
-	const int64_t row = (int64_t)sq * N + node;
-	const uint64_t bits = on && placed ? tree_bits(seen, row, N) : 0;
 	if (!__any(bits != 0)) {   // nodes that are not there, as in the last tiles of a padded tree
 		if (parts == 1) tree_blank<HD>(on ? node : -1, g, out + (int64_t)sq * N * ldo + head * HD, ldo);
 		return;
@@ -2189,14 +2189,15 @@ __global__ __launch_bounds__(64 * W, 2) void tree_tiled_kernel(AttnKv c, float *
 	if (!tree_item(c.kvh, n_seq, parts, (N * G + 32 * W - 1) / (32 * W), kvh, sq, part, tile)) return;
 	const int tid = threadIdx.x, lane = tid & 63, r = 32 * (W * tile + (tid >> 6)) + (lane & 31), node = r / G, g = r - node * G;
 	const int head = kvh * G + g, H = c.kvh * G;
+	const bool on = node < N;
+	const int64_t row = (int64_t)sq * N + node;
+	uint64_t bits = on ? tree_bits(seen, row, N) : 0;
 	int sl, b, end;
-	const bool on = node < N, placed = tree_place(c, slot, base, sq, N, sl, b, end);
+	if (!tree_place(c, slot, base, sq, N, sl, b, end)) bits = 0;
 	const Span sp = span_of<kKeys, false>(c, kvh, sl, 0, 0, end);
 	const int nc = sp.n0 + (max(end - sp.b0, 0) + kKeys - 1) / kKeys;
 	const int per = tree_part<1>(nc, parts), c0 = part * per;
 	if (c0 >= nc && part > 0) return;   // a record that the join does not read
-	const int64_t row = (int64_t)sq * N + node;
-	const uint64_t bits = on && placed ? tree_bits(seen, row, N) : 0;
 	// a wave without nodes sees nothing, a workgroup without any passes no chunk
 	const int hi = __any(bits != 0) ? end : 0, stop = __syncthreads_or(hi) ? min(nc, c0 + per) : c0;
 	Tile<HD, Q8, W> w;

@@ -25,7 +25,8 @@ __device__ __forceinline__ int lanes_below(uint64_t m) {
 // ── the n best of a stream of values, by one wave ──
 //
 // Values come in tiles of 64 E, position (i 64 + lane) 4 + c of a tile in
-// register 4 i + c; equal ones rank by position. Of a tile only what may still
+// register 4 i + c; equal ones rank by position, or by ids that rise with it
+// (register e's is id(e)). Of a tile only what may still
 // be among the n best is kept: values above the n-th best known so far, and
 // where more than n lanes have such values, above the n-th largest of the
 // lanes' own maxima, or what tells it from the next (found bit by bit, a
@@ -43,15 +44,15 @@ struct Best {
 	float least;    // a later value has to be larger
 
 	// (zeros of both signs are equal)
-	static __device__ __forceinline__ uint64_t key_of(float v, int pos) {
+	static __device__ __forceinline__ uint64_t key_of(float v, int id) {
 		const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.0f);
-		return (uint64_t)(b >> 31 ? ~b : b | 0x80000000u) << 32 | (uint32_t)~pos;
+		return (uint64_t)(b >> 31 ? ~b : b | 0x80000000u) << 32 | (uint32_t)~id;
 	}
 	static __device__ __forceinline__ float value(uint64_t key) {
 		const uint32_t k = (uint32_t)(key >> 32);
 		return __builtin_bit_cast(float, k >> 31 ? k & 0x7FFFFFFFu : ~k);
 	}
-	static __device__ __forceinline__ int place(uint64_t key) { return (int)~(uint32_t)key; }
+	static __device__ __forceinline__ int id_of(uint64_t key) { return (int)~(uint32_t)key; }
 
 	__device__ __forceinline__ void start(int want) {
 		n = want;
@@ -59,8 +60,12 @@ struct Best {
 		least = -kInf;
 	}
 
+	// A place of a tile from pos0.
+	static __device__ __forceinline__ int pos(int e, int pos0, int lane) { return pos0 + ((e >> 2) * 64 + lane) * 4 + (e & 3); }
+
 	// mx: the lane's largest value
-	__device__ __forceinline__ void tile(const float (&x)[E], float mx, int pos0, Lds &s, int lane) {
+	template <class Id>
+	__device__ __forceinline__ void tile(const float (&x)[E], float mx, const Id &id, Lds &s, int lane) {
 		const uint64_t hits = __ballot(mx > least);
 		if (!hits) return;
 		float t = least;
@@ -82,7 +87,7 @@ struct Best {
 		for (int e = 0; e < E; e++) {
 			const uint64_t m = __ballot(x[e] > t);
 			if (!m) continue;
-			if (x[e] > t) s.key[c + lanes_below(m)] = key_of(x[e], pos0 + ((e >> 2) * 64 + lane) * 4 + (e & 3));
+			if (x[e] > t) s.key[c + lanes_below(m)] = key_of(x[e], id(e));
 			c += __popcll(m);
 		}
 		if (ties) {
@@ -100,7 +105,7 @@ struct Best {
 #pragma unroll
 				for (int e = 0; e < 4; e++)
 					if (x[g + e] == t) {
-						if (before < ties) s.key[c + before] = key_of(t, pos0 + ((g >> 2) * 64 + lane) * 4 + e);
+						if (before < ties) s.key[c + before] = key_of(t, id(g + e));
 						before++;
 					}
 				c += min(all, ties);
@@ -188,7 +193,7 @@ __global__ __launch_bounds__(64 * kPickWaves) void beam_part_kernel(const float 
 	auto use = [&](float(&z)[kPickE], int t) {
 		if (t + kPickTile > n) {
 #pragma unroll
-			for (int e = 0; e < kPickE; e++) z[e] = t + ((e >> 2) * 64 + lane) * 4 + (e & 3) < n ? z[e] : -kInf;
+			for (int e = 0; e < kPickE; e++) z[e] = best.pos(e, t, lane) < n ? z[e] : -kInf;
 		}
 		float mx = z[0];
 #pragma unroll
@@ -207,7 +212,7 @@ __global__ __launch_bounds__(64 * kPickWaves) void beam_part_kernel(const float 
 			for (int e = 0; e < kPickE; e += 4)
 				sum += (double)((exp_(z[e] - top) + exp_(z[e + 1] - top)) + (exp_(z[e + 2] - top) + exp_(z[e + 3] - top)));
 		}
-		best.tile(z, mx, from + t, lds[wave], lane);
+		best.tile(z, mx, [&](int e) { return best.pos(e, from + t, lane); }, lds[wave], lane);
 	};
 	load(x, 0);
 	for (int t = 0; t < n; t += 2 * kPickTile) {
@@ -228,11 +233,12 @@ __global__ __launch_bounds__(64 * kPickWaves) void beam_part_kernel(const float 
 	if (lane < n_pick) {
 		const uint64_t key = lane < best.count ? lds[wave].list[lane] : 0;
 		out.v[rec * n_pick + lane] = lane < best.count ? best.value(key) : -kInf;
-		out.i[rec * n_pick + lane] = best.place(key);
+		out.i[rec * n_pick + lane] = best.id_of(key);
 	}
 }
 
-constexpr int kJoinE = 8;
+constexpr int kJoinE = 4;
+constexpr int kJoinR = 3;   // rounds of parts whose sums are asked for at once
 
 // A wave a beam: its sum and its n_pick best; then the request's best of those.
 __global__ __launch_bounds__(64 * HAKO_MAX_BEAMS) void beam_join_kernel(const float *__restrict__ score, const int *__restrict__ done,
@@ -241,45 +247,61 @@ __global__ __launch_bounds__(64 * HAKO_MAX_BEAMS) void beam_join_kernel(const fl
                                                                         float *__restrict__ score_out, int *__restrict__ done_out) {
 	__shared__ typename Best<kJoinE>::Lds lds[HAKO_MAX_BEAMS];
 	__shared__ double val[HAKO_MAX_BEAMS * HAKO_MAX_PICK];
-	__shared__ int tok[HAKO_MAX_BEAMS * HAKO_MAX_PICK], rank[HAKO_MAX_BEAMS * HAKO_MAX_PICK], pick[HAKO_MAX_PICK];
+	__shared__ int tok[HAKO_MAX_BEAMS * HAKO_MAX_PICK], rank[HAKO_MAX_BEAMS * HAKO_MAX_PICK], pick[HAKO_MAX_PICK], over[HAKO_MAX_BEAMS];
 	const int lane = threadIdx.x & 63, b = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	const int64_t req = blockIdx.x, row = req * n_beams + b;
 	const double old = (double)score[row];
 	const int ended = done ? done[row] : 0;
-	// the parts' lists in the order of their tokens; in a list equal values are in that order too
+	// the parts' lists in the order of their tokens; in a list equal values are in that order too (values and tokens come
+	// together, so that nothing is looked up for what was chosen)
 	const int64_t rec = row * parts;
 	const int n_list = parts * n_pick;
 	const __amdgpu_buffer_rsrc_t r = stream_rsrc(uniform_ptr(in.v + rec * n_pick), (uint32_t)n_list * 4u);
+	const __amdgpu_buffer_rsrc_t ri = stream_rsrc(uniform_ptr(in.i + rec * n_pick), (uint32_t)n_list * 4u);
 	float x[kJoinE];
+	int id[kJoinE];
 	auto load = [&](int t) {
 #pragma unroll
 		for (int g = 0; g < kJoinE / 4; g++) {
-			const uint4 w = ld_b128(r, 4u * (uint32_t)(t + (g * 64 + lane) * 4));
+			const uint32_t at = 4u * (uint32_t)(t + (g * 64 + lane) * 4);
+			const uint4 w = ld_b128(r, at), i = ld_b128(ri, at);
 			const float z[4] = {__builtin_bit_cast(float, w.x), __builtin_bit_cast(float, w.y), __builtin_bit_cast(float, w.z), __builtin_bit_cast(float, w.w)};
+			const uint32_t j[4] = {i.x, i.y, i.z, i.w};
 #pragma unroll
-			for (int e = 0; e < 4; e++) x[4 * g + e] = z[e];
+			for (int e = 0; e < 4; e++) {
+				x[4 * g + e] = z[e];
+				id[4 * g + e] = (int)j[e];
+			}
 		}
 	};
 	load(0);
 	// (an ended beam's are whatever was there)
-	const float top0 = lane < parts ? in.top[rec + lane] : -kInf;
-	const double sum0 = lane < parts ? in.sum[rec + lane] : 0.0;
+	float tops[kJoinR];
+	double sums[kJoinR];
+#pragma unroll
+	for (int k = 0; k < kJoinR; k++) {
+		const int p = k * 64 + lane;
+		tops[k] = p < parts ? in.top[rec + p] : -kInf;
+		sums[k] = p < parts ? in.sum[rec + p] : 0.0;
+	}
 	if (threadIdx.x < HAKO_MAX_PICK) pick[threadIdx.x] = -1;
+	if (lane == 0) over[b] = ended;
 	if (ended) {
 		if (lane < n_pick) {
 			val[b * n_pick + lane] = lane == 0 ? old : -(double)kInf;
 			tok[b * n_pick + lane] = eos;
 		}
 	} else {
-		float top = top0;
-		for (int p = lane + 64; p < parts; p += 64) top = __builtin_fmaxf(top, in.top[rec + p]);
+		float top = tops[0];
+#pragma unroll
+		for (int k = 1; k < kJoinR; k++) top = __builtin_fmaxf(top, tops[k]);
+		for (int p = kJoinR * 64 + lane; p < parts; p += 64) top = __builtin_fmaxf(top, in.top[rec + p]);
 		top = wave_max(top);
-		double sum = top0 == -kInf ? sum0 : sum0 * (double)exp_(top0 - top);
-		for (int p = lane + 64; p < parts; p += 64) {
-			const float t = in.top[rec + p];
-			const double w = in.sum[rec + p];
-			sum += t == -kInf ? w : w * (double)exp_(t - top);
-		}
+		double sum = 0.0;
+		auto add = [&](float t, double w) { sum += t == -kInf ? w : w * (double)exp_(t - top); };
+#pragma unroll
+		for (int k = 0; k < kJoinR; k++) add(tops[k], sums[k]);
+		for (int p = kJoinR * 64 + lane; p < parts; p += 64) add(in.top[rec + p], in.sum[rec + p]);
 #pragma unroll
 		for (int k = 1; k < 64; k <<= 1) sum += __shfl_xor(sum, k);
 		const double lse = (double)top + log(sum);
@@ -289,10 +311,10 @@ __global__ __launch_bounds__(64 * HAKO_MAX_BEAMS) void beam_join_kernel(const fl
 			float mx = -kInf;
 #pragma unroll
 			for (int e = 0; e < kJoinE; e++) {
-				x[e] = t + ((e >> 2) * 64 + lane) * 4 + (e & 3) < n_list ? x[e] : -kInf;
+				x[e] = best.pos(e, t, lane) < n_list ? x[e] : -kInf;
 				mx = __builtin_fmaxf(mx, x[e]);
 			}
-			best.tile(x, mx, t, lds[b], lane);
+			best.tile(x, mx, [&](int e) { return id[e]; }, lds[b], lane);
 			if (t + 64 * kJoinE < n_list) load(t + 64 * kJoinE);
 		}
 		best.settle(lds[b], lane);
@@ -300,7 +322,7 @@ __global__ __launch_bounds__(64 * HAKO_MAX_BEAMS) void beam_join_kernel(const fl
 			const bool on = lane < best.count;
 			const uint64_t key = on ? lds[b].list[lane] : 0;
 			val[b * n_pick + lane] = on ? old + ((double)best.value(key) - lse) : -(double)kInf;
-			tok[b * n_pick + lane] = on ? in.i[rec * n_pick + best.place(key)] : -1;
+			tok[b * n_pick + lane] = on ? best.id_of(key) : -1;
 		}
 	}
 	const int n = n_beams * n_pick;
@@ -345,7 +367,7 @@ __global__ __launch_bounds__(64 * HAKO_MAX_BEAMS) void beam_join_kernel(const fl
 	parent[o] = from;
 	token[o] = t;
 	score_out[o] = f < 0 ? -kInf : (float)val[f];
-	if (done_out) done_out[o] = f >= 0 && (t == eos || (done && done[req * n_beams + from]));
+	if (done_out) done_out[o] = f >= 0 && (t == eos || over[from]);
 }
 
 // ── cache rows that move ──
