@@ -279,6 +279,18 @@ __device__ __forceinline__ float scale_exp(float vmax) {
 // in the loop 0.90 (868 against 907 us on one box); staging at opposite ends
 // of a chunk by a SIMD's two waves 0.84. No difference: wave priorities around
 // either product, reads left to the compiler's own order (871 against 869).
+// Queries and outputs pass through LDS in whole lines, the first chunk's codes
+// on their way meanwhile: an item's start and end 13 us, 16 before (packed
+// prompts of 4097 tokens 92 us, 97; 8192 tokens under a window of 128 107, 123).
+//
+// Tiles of 128 rows and four waves, two workgroups a CU, stage each chunk for
+// half as many rows: for windows, whose tiles are short and much alike, where
+// half a round of items saves more (see window_kernel), and for small drafted
+// trees. Under a window a tile
+// passes the chunks of the sinks and those from its first token's window on,
+// and masks the chunks at either border alone: 16384 tokens under 4096 take
+// 1.45 ms on the fastest box seen, 1.16 PFLOP/s of matrix operations, matrix
+// pipes busy 63% of the cycles.
 
 // Rows in LDS are padded by 16 bytes, so that lanes on consecutive rows meet
 // different banks. A chunk's keys lie in the order of the score tiles' rows
@@ -1215,6 +1227,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_direct_kernel(AttnKv c,
 // 32768 and 20011 positions in 16 bits 20.8 us, then 17.9. The waves' number as
 // a scalar, so that the loop is one for the compiler too: 64 sequences of 1000
 // positions 15.1 us, now 14.8.
+//
+// Under a window the parts count the keys that are in sight, the sinks' in
+// whole steps, then the window's from wherever it starts; no step before it is
+// read, and its own start needs no mask. 64 sequences under 4096 keys, 236 MB:
+// 44 us, 5.3 TB/s; one of 9001 under 1024: 6.4, and the join 3.6.
 template <int HD, bool Q8>
 struct Row16 {
 	static constexpr int EB = Q8 ? 1 : 2;
@@ -2105,7 +2122,22 @@ int prompt(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, const float *q, 
 	                                      });
 }
 
-// ── drafted trees: 32 rows of (node, head of the group) of one sequence by the direct kernel ──
+// ── drafted trees ──
+//
+// Rows are (node, head of the group) of one sequence, node-major, against the
+// sequence's text and the tree's own rows behind it. A row sees all of the text
+// and of the 64 keys from base on its mask's bits: a step's 32 or 64 bits are
+// one shift of the mask (Nodes::at), so that masked steps cost what a causal
+// mask's do and the others nothing. Nodes that are not there have mask 0; their
+// waves pass no chunk and their rows have no records.
+//
+// Two kernels as for prompts. 32-row tiles straight from memory (direct): small
+// trees, latency. One tree of 26 nodes at 1025, 3B heads: 8.4 us, most
+// of it places, masks, first codes and queries one after the other; the join
+// 3.6. Tiles of 256 or 128 rows (tiled): 16 trees of 64 nodes at 4096, 7B
+// heads, 120 GFLOP with both halves: 119 to 130 us and the join 10; tiles of 448 rows
+// in 512, and parts of 33 chunks behind a start of 14 us, are what is lost. 32 trees of 1..16 nodes over a
+// prefix of 3001 in 16 bits: 61 us and 7, tiles 58% full.
 
 // Where a sequence's nodes go: rows [base, end), base 0 and no rows where it has no place.
 __device__ __forceinline__ bool tree_place(const AttnKv &c, const int *slot, const int *base, int sq, int N, int &sl, int &b, int &end) {
@@ -2213,10 +2245,11 @@ __global__ __launch_bounds__(64 * W, 2) void tree_tiled_kernel(AttnKv c, float *
 	if (bits && lane < 32) rec.put(r0, {w.M, w.big ? s.be[tid] : 0.0f}, w.l);
 }
 
+// A sequence's records, as many as its text has parts, joined; zeros for nodes that are not there.
 template <int HD, int K, int R>
 __global__ __launch_bounds__(256) void tree_join_kernel(AttnKv c, float *out, int64_t ldo, const int *__restrict__ slot,
-                                                        const int *__restrict__ base, const uint64_t *__restrict__ seen, int n_seq, int N, int H, int parts,
-                                                        const float *__restrict__ rec_o, const float2 *__restrict__ rec_ml,
+                                                        const int *__restrict__ base, const uint64_t *__restrict__ seen,
+                                                        int n_seq, int N, int H, int parts, const float *__restrict__ rec_o, const float2 *__restrict__ rec_ml,
                                                         const float *__restrict__ rec_e) {
 	constexpr int L = HD / 4;
 	const int64_t i = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
@@ -2254,8 +2287,8 @@ __global__ __launch_bounds__(64 * kJoin) void tree_join_wide_kernel(AttnKv c, fl
 // Trees of N nodes over parts of their keys, `slots` workgroups in all or fewer; launch(parts, blocks, records) of tiles
 // of `rows` rows.
 template <int HD, int K, int R, class Launch>
-int tree_launch(const AttnKv &c, float *out, int64_t ldo, const int *slot, const int *base, const uint64_t *seen, int n_seq, int N, int H, int rows, int64_t slots,
-                Launch launch) {
+int tree_launch(const AttnKv &c, float *out, int64_t ldo, const int *slot, const int *base, const uint64_t *seen, int n_seq, int N,
+                int H, int rows, int64_t slots, Launch launch) {
 	const int64_t tiles = ((int64_t)N * (H / c.kvh) + rows - 1) / rows, wgs = tiles * n_seq * c.kvh;
 	const int most = (tile_steps<K>(c.max_seq, c.prefix_len) + R - 1) / R;
 	// (whole rounds of the eight dies: one tree of 448 rows at 8000, four heads, 41 us in 9 parts, 31 in 8)

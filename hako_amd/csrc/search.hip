@@ -138,9 +138,21 @@ struct Best {
 
 // ── beam selection ──
 //
-// Two launches: waves over parts of the rows, then a workgroup a request.
+// value(b, t) = score_b + (x_bt - log sum_j exp x_bj). Within a beam the order
+// is that of the logits, so a pass over them keeps the n largest and the sum,
+// and values are formed for n_beams n_pick candidates alone. Two launches:
+// waves over parts of the rows (whole tiles, as many as fill the chip with 16
+// waves a CU), then a workgroup a request.
 // exp sums are taken against the part's maximum, in fp32 with the argument's
 // rounding put right, four at a time into 64 bits, and meet in 64 bits.
+//
+// Bound: HBM and the vector pipes. 32 requests of 8 beams over 152064 tokens
+// (156 MB, less the tenth of the beams that have ended) take 33.6 us and the
+// choice 6.7; where calls follow each other 66 MB of them come from HBM, the
+// rest from the memory-side cache. On the way, in all: every tile's candidates
+// ranked as they came 91 us; 64 at a time as 64-bit keys, 16 waves a CU in the
+// place of 8, 42. The bound found two bits at a time was slower, as was ranking
+// the lanes' maxima in LDS (36.5 us against 33.7).
 constexpr int kPickE = 16;                 // values of a lane's tile
 constexpr int kPickTile = 64 * kPickE;
 constexpr int kPickWaves = 4;
@@ -237,10 +249,15 @@ __global__ __launch_bounds__(64 * kPickWaves) void beam_part_kernel(const float 
 	}
 }
 
+// The join, a wave a beam: its sum and its n_pick best; then the request's best
+// of those. Bound by latency: all that it reads is asked for at once (one
+// request of 4 beams in 149 parts 6.1 us, 6.9 when sums of parts past the 64th
+// and the chosen ones' tokens were asked for later), and its code is short
+// where it may be (tiles of 512 values 7.0 us for 32 requests of 8 beams, of
+// 256 6.7).
 constexpr int kJoinE = 4;
 constexpr int kJoinR = 3;   // rounds of parts whose sums are asked for at once
 
-// A wave a beam: its sum and its n_pick best; then the request's best of those.
 __global__ __launch_bounds__(64 * HAKO_MAX_BEAMS) void beam_join_kernel(const float *__restrict__ score, const int *__restrict__ done,
                                                                         int eos, int n_beams, int n_pick, int parts, int arrange,
                                                                         Parts in, int *__restrict__ parent, int *__restrict__ token,
@@ -383,7 +400,13 @@ struct Shape {
 
 // A workgroup takes units of 16 bytes (and scales) of one head's rows in all
 // of a request's slots at once: every load comes before the first store, so any
-// map of places is good.
+// map of places is good, and a source that several places take is read once.
+//
+// Bound: HBM. 4 requests of 8 beams, 12 layers of 4 heads in 16 bits, half of
+// the places moved: 96 MB from memory and 192 MB to it in 68 us, 4.2 TB/s (a
+// copy of 1 GiB 5.0), waits three quarters of the waves' cycles. Units as vectors of the compiler (131
+// us as structs, whose copies became single words), stores past the caches (82
+// without).
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 template <int B>
 __global__ __launch_bounds__(256) void reorder_kernel(Layers layers, Shape c, const int *__restrict__ slot,
@@ -432,7 +455,10 @@ __global__ __launch_bounds__(256) void reorder_kernel(Layers layers, Shape c, co
 }
 
 // A wave takes a path's rows of one head, keys or values: all of its loads,
-// then its stores, so that a row may be another one's place.
+// then its stores, so that a row may be another one's place. Bound by latency:
+// a path is at most 16 KB a head, 28 layers of 32 paths of 1..9 rows (10.9 MB)
+// 7.4 us, 12 layers of one path 4.3: the path, its rows, their stores, one
+// after the other.
 constexpr int kKeepWaves = 4;
 __global__ __launch_bounds__(64 * kKeepWaves) void keep_kernel(Layers layers, Shape c, int n_layers, const int *__restrict__ slot,
                                                                const int *__restrict__ base, const int *__restrict__ path,
@@ -472,6 +498,9 @@ __global__ __launch_bounds__(64 * kKeepWaves) void keep_kernel(Layers layers, Sh
 }
 
 // ── drafted trees: a wave a tree, a lane a node ──
+//
+// A plan by pointer doubling, six rounds for 64 nodes, a path by a ballot a
+// step; 1.7 and 2.0 us for one tree, which is a launch.
 
 constexpr int kTreeWaves = 4;
 
