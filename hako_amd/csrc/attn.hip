@@ -1752,9 +1752,27 @@ __global__ __launch_bounds__(64 * kJoin) void decode_join_kernel(AttnKv c, float
 // n records, few, of one head joined for the four dims of ro.. (of each record HD floats).
 __device__ __forceinline__ void join_few(const float *__restrict__ ro, int HD, const float2 *__restrict__ ml, const float *__restrict__ re,
                                          int n, float *dst) {
+	// the first records and every maximum at once
+	constexpr int P = 4;
+	float4 y0[P];
+	float2 x0[P];
+#pragma unroll
+	for (int k = 0; k < P; k++) {
+		y0[k] = make_float4(0, 0, 0, 0);
+		x0[k] = make_float2(kNone, 0.0f);
+		if (k < n) {
+			y0[k] = *(const float4 *)(ro + (size_t)k * HD);
+			x0[k] = ml[k];
+		}
+	}
 	Base b = {kNone, 0.0f};
 	bool some = false;
-	for (int k = 0; k < n; k++) {
+#pragma unroll
+	for (int k = 0; k < P; k++) {
+		b.m = __builtin_fmaxf(b.m, x0[k].x);
+		some |= has_e(x0[k]);
+	}
+	for (int k = P; k < n; k++) {
 		const float2 x = ml[k];
 		b.m = __builtin_fmaxf(b.m, x.x);
 		some |= has_e(x);
@@ -1770,8 +1788,11 @@ __device__ __forceinline__ void join_few(const float *__restrict__ ro, int HD, c
 	if (__builtin_expect(big, 0)) {
 		for (int k = 0; k < n; k++) add_record(a, ls, *(const float4 *)(ro + (size_t)k * HD), ml[k].y, steps_down(base_of(ml[k], re + k), b));
 	} else {
+#pragma unroll
+		for (int k = 0; k < P; k++)
+			if (k < n) add_record(a, ls, y0[k], x0[k].y, steps_down({x0[k].x, 0.0f}, b));
 #pragma unroll 4
-		for (int k = 0; k < n; k++) {
+		for (int k = P; k < n; k++) {
 			const float4 y = *(const float4 *)(ro + (size_t)k * HD);
 			const float2 x = ml[k];
 			add_record(a, ls, y, x.y, steps_down({x.x, 0.0f}, b));
@@ -2135,9 +2156,11 @@ int prompt(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, const float *q, 
 // trees, latency. One tree of 26 nodes at 1025, 3B heads: 8.4 us, most
 // of it places, masks, first codes and queries one after the other; the join
 // 3.6. Tiles of 256 or 128 rows (tiled): 16 trees of 64 nodes at 4096, 7B
-// heads, 120 GFLOP with both halves: 119 to 130 us and the join 10; tiles of 448 rows
-// in 512, and parts of 33 chunks behind a start of 14 us, are what is lost. 32 trees of 1..16 nodes over a
-// prefix of 3001 in 16 bits: 61 us and 7, tiles 58% full.
+// heads, 120 GFLOP with both halves: 119 to 133 us by the chip, and the join
+// 9.4 (11 before it asked for its first records with their bases); tiles of 512
+// rows for 448, and parts of 33 chunks behind a start of 13 us, are what is
+// lost. 32 trees of 1..16 nodes over a prefix of 3001 in 16 bits: 62 us and 6,
+// tiles half full.
 
 // Where a sequence's nodes go: rows [base, end), base 0 and no rows where it has no place.
 __device__ __forceinline__ bool tree_place(const AttnKv &c, const int *slot, const int *base, int sq, int N, int &sl, int &b, int &end) {
@@ -2258,7 +2281,8 @@ __global__ __launch_bounds__(256) void tree_join_kernel(AttnKv c, float *out, in
 	if (sq >= n_seq) return;
 	int sl, b, end;
 	float *to = out + row * ldo + (int64_t)h * HD + d;
-	if (!tree_place(c, slot, base, sq, N, sl, b, end) || !tree_bits(seen, row, N)) {
+	const uint64_t bits = tree_bits(seen, row, N);
+	if (!tree_place(c, slot, base, sq, N, sl, b, end) || !bits) {
 		*(float4 *)to = make_float4(0, 0, 0, 0);
 		return;
 	}
@@ -2275,7 +2299,8 @@ __global__ __launch_bounds__(64 * kJoin) void tree_join_wide_kernel(AttnKv c, fl
                                                                     const float2 *__restrict__ rec_ml, const float *__restrict__ rec_e) {
 	const int h = blockIdx.x, row = blockIdx.y;
 	int sl, b, end;
-	if (!tree_place(c, slot, base, row / N, N, sl, b, end) || !tree_bits(seen, row, N)) {
+	const uint64_t bits = tree_bits(seen, row, N);
+	if (!tree_place(c, slot, base, row / N, N, sl, b, end) || !bits) {
 		if (threadIdx.x < HD) out[row * ldo + h * HD + threadIdx.x] = 0.0f;
 		return;
 	}
