@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 import attn_ref as ref
-from hako_amd.gpu import KV_F16, KV_Q8
+from hako_amd.gpu import KV_F16, KV_Q8, Kv
 from test_gpu_tree import ancestors, attend, close, i32, masks, random_tree
 
 pytestmark = pytest.mark.gpu
@@ -229,3 +229,65 @@ def test_calls_of_nothing(gpu):
     gpu.sync()
     one.free()
     c.free()
+
+
+def test_offsets_past_32_bits(gpu):
+    """A cache of 5 GiB an array: rows of its last slot appended, moved, reordered and attended to."""
+    slots, max_seq, KVH, hd, H, n, at = 80, 32768, 8, 128, 16, 24, 32700
+    rng = np.random.default_rng(11)
+    kv = Kv(KV_F16, slots, max_seq, KVH, hd)
+    codes, scales = gpu.kv_bytes(kv)
+    assert codes > 2 ** 32
+    arrays = [gpu.alloc(b) for b in (codes, codes, scales, scales)]
+    kv = Kv(KV_F16, slots, max_seq, KVH, hd, *(b.ptr for b in arrays))
+    W = KVH * hd
+
+    def write(slot, pos):
+        x = [gpu.upload(rng.standard_normal((n, W)).astype(np.float32)) for _ in range(2)]
+        ds, dp = i32(gpu, [slot] * n), i32(gpu, range(pos, pos + n))
+        gpu.kv_append(kv, ds, dp, n, *x, W)
+        for b in x + [ds, dp]:
+            b.free()
+
+    def read(slot, pos):
+        out = [gpu.alloc(4 * n * W) for _ in range(2)]
+        ds, dp = i32(gpu, [slot] * n), i32(gpu, range(pos, pos + n))
+        gpu.kv_read(kv, ds, dp, n, *out, W)
+        got = [gpu.download(b, np.float32, (n, KVH, hd)) for b in out]
+        for b in out + [ds, dp]:
+            b.free()
+        return got
+
+    for slot in (79, 78, 3):
+        write(slot, at)
+    write(79, 0)
+    layers = gpu.kv_layers([kv])
+    before = {s: read(s, at) for s in (79, 78, 3)}
+    # two requests: slots 79 and 3 change places, 78 takes nothing from a beam outside
+    ds, par, since, end = i32(gpu, [79, 3]), i32(gpu, [1, 0]), i32(gpu, [at]), i32(gpu, [at + n])
+    gpu.kv_reorder(layers, ds, par, 1, 2, since, end)
+    for a, b in ((79, 3), (3, 79), (78, 78)):
+        for x, y in zip(read(a, at), before[b]):
+            assert np.array_equal(x, y)
+    base, path, count = i32(gpu, [at]), i32(gpu, [0, 3, 7, 20] + [-1] * (n - 4)), i32(gpu, [4])
+    gpu.kv_keep(layers, ds, base, path, count, 1, n)
+    kept = read(79, at)
+    for x, y in zip(kept, before[3]):
+        assert np.array_equal(x[:4], y[[0, 3, 7, 20]]) and np.array_equal(x[4:], y[4:])
+    # the last positions under a window, and a tree near the slot's start
+    q = rng.standard_normal((n, H, hd)).astype(np.float32)
+    dq, out, scale = gpu.upload(q), gpu.alloc(q.nbytes), 1 / math.sqrt(hd)
+    gpu.attn_decode_window(out, H * hd, dq, H * hd, kv, ds, end, 1, H, scale, 15, 0)
+    K, V = (np.moveaxis(x.astype(np.float64), 0, 1)[None] for x in kept)
+    close(gpu.download(out, np.float32, (H, hd)), attend(q[0], K[:, :, n - 15:], V[:, :, n - 15:], 0, 15, {1}, 15, scale))
+    K, V = (np.moveaxis(x.astype(np.float64), 0, 1)[None] for x in read(79, 0))
+    sets = ancestors(random_tree(rng, 9, 9))
+    seen, first = gpu.upload(masks(sets)), i32(gpu, [15])
+    for knob in (1, 2, 3):
+        gpu.tune(TUNE_ATTN_PROMPT, knob)
+        gpu.attn_tree(out, H * hd, dq, H * hd, kv, ds, first, seen, 1, 9, H, scale)
+        got = gpu.download(out, np.float32, (9, H, hd))
+        close(got, np.array([attend(q[j], K, V, 0, 15, sets[j], n, scale) for j in range(9)]))
+    gpu.tune(TUNE_ATTN_PROMPT, 0)
+    for b in arrays + [ds, par, since, end, base, path, count, dq, out, seen, first]:
+        b.free()
