@@ -2353,8 +2353,8 @@ int tree_launch(const AttnKv &c, float *out, int64_t ldo, const int *slot, const
 //       64 of 8 at 2000         56          32                          49 / 72      62 / 72
 //   3B  8 of 64 at 4000        512          32                          52 / 50      58 / 50
 // So the tiled one from 24 on for more than 64 rows. Its tiles are of 128 rows where these hold them all and sequences and
-// heads do not give every other CU a tile (32 ragged trees of 16 over a prefix in 16 bits 66 us, 73 in tiles of 256, 8
-// bits 67 and 76; 64 of 16 at 2000 96 and 90, 87 and 83).
+// heads do not give every other CU a tile (32 ragged trees of 16 over a prefix in 16 bits 62 us, 72 in tiles of 256, 8
+// bits 65 and 74; 64 of 16 at 2000 96 and 89, 87 and 81).
 template <int HD, bool Q8>
 int tree(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq, const int *slot, const int *base, const uint64_t *seen,
          int n_seq, int N, int H, float scale) {
