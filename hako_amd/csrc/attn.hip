@@ -123,21 +123,30 @@ struct Within {
 		return k + K > min(lo, top) || (!first && k < hi - window);
 	}
 };
-// Those below lim, and of the 64 from there on those of its bits:
+// Those below lim, and of the 64 from there on those of its bits (any: all rows' bits, the same in every lane):
 struct Nodes {
 	static constexpr bool kHi = false, kBlanks = true;
 	int lim;
-	uint64_t bits, w;
+	uint64_t bits, any, w;
+	// the 64 keys from k on as bits: those below lim, then those of m
+	__device__ __forceinline__ uint64_t from(int k, uint64_t m) const {
+		const int s = k - lim;
+		if (s >= 0) return s < 64 ? m >> s : 0;
+		return s > -64 ? m << -s | ((1ull << -s) - 1) : ~0ull;
+	}
 	__device__ __forceinline__ void at(int k, int top, bool) {
-		const int s = k - lim, n = top - k;
-		if (s >= 0) w = s < 64 ? bits >> s : 0;
-		else w = s > -64 ? bits << -s | ((1ull << -s) - 1) : ~0ull;
+		const int n = top - k;
+		w = from(k, bits);
 		w = n >= 64 ? w : n > 0 ? w & ((1ull << n) - 1) : 0;
 	}
 	__device__ __forceinline__ bool sees(int i) const { return w >> i & 1; }
 	__device__ __forceinline__ bool reaches(int, bool, int) const { return true; }
 	template <int K>
 	__device__ __forceinline__ bool masks(int k, int top, bool, int lo, int) const { return k + K > min(lo, top); }
+	// whether a step of K keys at k may hold rows that nobody sees, which may never have been written; those that are not
+	template <int K>
+	__device__ __forceinline__ bool gaps(int k) const { return k + K > lim; }
+	__device__ __forceinline__ uint64_t written(int k) const { return from(k, any); }
 };
 
 // The same value, made anew where this stands: addresses and masks that
@@ -340,6 +349,19 @@ struct Stage {
 		if (tid < kKeys) {
 			ks = ld_f32(ksr, 4u * (uint32_t)(key0 + tid));
 			vs = ld_f32(vsr, 4u * (uint32_t)(key0 + tid));
+		}
+	}
+
+	// Values of rows that nobody sees become zeros: halves there may be infinite or NaN, which a weight of 0 does not take
+	// away. (Their scores are masked. Codes of 8 bits are finite whatever they are.)
+	__device__ __forceinline__ void keep(uint64_t written, int tid) {
+#pragma unroll
+		for (int i = 0; i < VL; i++) {
+			const uint32_t m = (uint32_t)(written >> (VK * ((tid + NT * i) / VQ) & 63));
+#pragma unroll
+			for (int j = 0; j < VK; j++)
+#pragma unroll
+				for (int w = 0; w < EB; w++) v[i][j][w] &= (uint32_t)__builtin_amdgcn_sbfe((int)m, j, 1);
 		}
 	}
 
@@ -610,6 +632,11 @@ struct Tile {
 			st.load(stream_rsrc(uniform_ptr(c.k + r * HD * EB), n * HD * EB), stream_rsrc(uniform_ptr(c.v + r * HD * EB), n * HD * EB),
 			        stream_rsrc(uniform_ptr(c.ks + r), n * 4), stream_rsrc(uniform_ptr(c.vs + r), n * 4), sp.key<kKeys>(ch), fresh(tid));
 		};
+		auto store = [&](int ch, int b) {
+			if constexpr (See::kBlanks && !Q8)
+				if (const int key0 = sp.key<kKeys>(ch); row.template gaps<kKeys>(key0)) st.keep(row.written(key0), fresh(tid));
+			st.store(s.k[b], s.v[b], s.ks[b], s.vs[b], &s.e[b], fresh(tid));
+		};
 		// A wave's registers hold the codes two chunks on from the buffer that is read. The waves of a SIMD (w, w + 4)
 		// put them into LDS at opposite ends of a chunk, so that one has vector work while the other has matrix work.
 		if (c0 < c1) load(c0);
@@ -617,7 +644,7 @@ struct Tile {
 		ask();
 		__syncthreads();
 		if (c0 < c1) {
-			st.store(s.k[0], s.v[0], s.ks[0], s.vs[0], &s.e[0], tid);
+			store(c0, 0);
 			if (c0 + 1 < c1) load(c0 + 1);
 		}
 		const bool early = __builtin_amdgcn_readfirstlane(tid >> 6) >= 4;
@@ -625,7 +652,7 @@ struct Tile {
 		for (int ch = c0; ch < c1; ch++) {
 			const int b = (ch - c0) & 1;
 			auto stage = [&] {
-				if (ch + 1 < c1) st.store(s.k[b ^ 1], s.v[b ^ 1], s.ks[b ^ 1], s.vs[b ^ 1], &s.e[b ^ 1], fresh(tid));
+				if (ch + 1 < c1) store(ch + 1, b ^ 1);
 				if (ch + 2 < c1) load(ch + 2);
 				__builtin_amdgcn_sched_barrier(0);
 			};
@@ -883,6 +910,15 @@ struct Direct {
 		}
 	}
 
+	// As Stage's.
+	__device__ __forceinline__ void keep(uint64_t written, int lane) {
+		const int m = (int)((uint32_t)written >> (lane >> 5) * 8);
+#pragma unroll
+		for (int n = 0; n < 16; n++)
+#pragma unroll
+			for (int w = 0; w < VW; w++) v[n][w] &= (uint32_t)__builtin_amdgcn_sbfe(m, 16 * (n >> 3) + (n & 7), 1);
+	}
+
 	// The step's 32 keys from key0; mask: some row does not see all of them. sx: 128 floats of the wave's own in LDS, the
 	// step's scales and every lane's base's e.
 	__device__ __forceinline__ void scores(f16v &sc, const uint8_t *keep, int lane) {
@@ -1107,6 +1143,8 @@ __device__ __forceinline__ void direct_rows(const AttnKv &c, DirectLds<HD> &s, c
 		f16v sc;
 		h8 ph[2], pl[2];
 		w.scores(sc, s.keep, fresh(lane));
+		if constexpr (See::kBlanks && !Q8)
+			if (seen.template gaps<32>(key0)) w.keep(seen.written(key0), fresh(lane));
 		const float e = w.scales(sx, lane);
 		if (ch + kWaves < c1) load_k(ch + kWaves);
 		__builtin_amdgcn_sched_barrier(0);
@@ -2150,7 +2188,9 @@ int prompt(const AttnKv &c, SeqTab &t, float *out, int64_t ldo, const float *q, 
 // and of the 64 keys from base on its mask's bits: a step's 32 or 64 bits are
 // one shift of the mask (Nodes::at), so that masked steps cost what a causal
 // mask's do and the others nothing. Nodes that are not there have mask 0; their
-// waves pass no chunk and their rows have no records.
+// waves pass no chunk and their rows have no records. Their cache rows may never
+// have been written: halves there are taken as zeros (Stage::keep; 0.2 us of one
+// tree of 26, 1.2 of 34 for 8 of 64 at 1000 in 16 bits).
 //
 // Two kernels as for prompts. 32-row tiles straight from memory (direct): small
 // trees, latency. One tree of 26 nodes at 1025, 3B heads: 8.4 us, most
@@ -2175,6 +2215,11 @@ __device__ __forceinline__ bool tree_place(const AttnKv &c, const int *slot, con
 // The nodes of a row that it sees, 0: it is not there.
 __device__ __forceinline__ uint64_t tree_bits(const uint64_t *seen, int64_t row, int N) {
 	return N < 64 ? seen[row] & ((1ull << N) - 1) : seen[row];
+}
+// The nodes that some row of the sequence sees. (Only halves need them: see Stage::keep.)
+template <bool Q8>
+__device__ __forceinline__ uint64_t tree_any(const uint64_t *seen, int sq, int N, int lane) {
+	return Q8 ? 0 : wave_or(lane < N ? seen[(int64_t)sq * N + lane] : 0);
 }
 // Steps per part of a tile with nc steps, in whole rounds of R.
 template <int R>
@@ -2217,6 +2262,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(AttnKv c, float *o
 	const bool on = node < N;
 	const int64_t row = (int64_t)sq * N + node;
 	uint64_t bits = on ? tree_bits(seen, row, N) : 0;   // (asked for together with the place)
+	const uint64_t any = tree_any<Q8>(seen, sq, N, lane);
 	int sl, b, end;
 	if (!tree_place(c, slot, base, sq, N, sl, b, end)) bits = 0;
 	const Span sp = span_of<32, false>(c, kvh, sl, 0, 0, end);
@@ -2227,7 +2273,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(AttnKv c, float *o
 		if (parts == 1) tree_blank<HD>(on ? node : -1, g, out + (int64_t)sq * N * ldo + head * HD, ldo);
 		return;
 	}
-	direct_rows<HD, Q8>(c, s, sp, c0, min(nc, c0 + per), on && bits ? q + row * ldq + (head + g) * HD : nullptr, scale, Nodes{b, bits, 0},
+	direct_rows<HD, Q8>(c, s, sp, c0, min(nc, c0 + per), on && bits ? q + row * ldq + (head + g) * HD : nullptr, scale, Nodes{b, bits, any, 0},
 	                    on ? node << 4 | g | (bits ? 0 : kBlank) : -1,
 	                    parts == 1 ? Dest(out + (int64_t)sq * N * ldo + head * HD, ldo, HD)
 	                               : Dest(rec, ((size_t)sq * N * H + head) * parts + part, H, parts));
@@ -2247,6 +2293,7 @@ __global__ __launch_bounds__(64 * W, 2) void tree_tiled_kernel(AttnKv c, float *
 	const bool on = node < N;
 	const int64_t row = (int64_t)sq * N + node;
 	uint64_t bits = on ? tree_bits(seen, row, N) : 0;
+	const uint64_t any = tree_any<Q8>(seen, sq, N, lane);
 	int sl, b, end;
 	if (!tree_place(c, slot, base, sq, N, sl, b, end)) bits = 0;
 	const Span sp = span_of<kKeys, false>(c, kvh, sl, 0, 0, end);
@@ -2256,7 +2303,7 @@ __global__ __launch_bounds__(64 * W, 2) void tree_tiled_kernel(AttnKv c, float *
 	// a wave without nodes sees nothing, a workgroup without any passes no chunk
 	const int hi = __any(bits != 0) ? end : 0, stop = __syncthreads_or(hi) ? min(nc, c0 + per) : c0;
 	Tile<HD, Q8, W> w;
-	w.chunks(c, sp, c0, stop, Nodes{b, bits, 0}, b, hi, s, tid,
+	w.chunks(c, sp, c0, stop, Nodes{b, bits, any, 0}, b, hi, s, tid,
 	         [&] { w.query(on ? q + row * ldq + head * HD : nullptr, scale, s, tid); });
 	if (parts == 1) {
 		if (!bits) w.clear();

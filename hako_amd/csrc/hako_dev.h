@@ -68,6 +68,19 @@ __device__ __forceinline__ float wave_max(float v) {
 	v = __builtin_fmaxf(v, __shfl_xor(v, 32));
 	return v;
 }
+// All lanes' bits, in scalar registers.
+__device__ __forceinline__ uint64_t wave_or(uint64_t v) {
+	int x[2] = {(int)(uint32_t)v, (int)(uint32_t)(v >> 32)};
+#pragma unroll
+	for (int &w : x) {
+		w |= dpp_i<kDppQuadSwap1>(w);
+		w |= dpp_i<kDppQuadSwap2>(w);
+		w |= dpp_i<kDppHalfMirror>(w);
+		w |= dpp_i<kDppMirror>(w);
+		w = __builtin_amdgcn_readlane(w, 0) | __builtin_amdgcn_readlane(w, 16) | __builtin_amdgcn_readlane(w, 32) | __builtin_amdgcn_readlane(w, 48);
+	}
+	return (uint64_t)(uint32_t)x[1] << 32 | (uint32_t)x[0];
+}
 
 // Sum over aligned segments of `seg` lanes (a power of two, 4..64); every
 // lane of a segment receives the segment's sum.

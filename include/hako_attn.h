@@ -171,6 +171,8 @@ int hako_gpu_attn_prompt_window(float *out, int64_t out_stride, const float *q, 
  * zeros. slot, base and seen are device arrays, read when the kernels run; a
  * base above max_seq counts as max_seq, and no row at max_seq or past it is
  * seen; a base below 0 or a slot outside the cache: the sequence gets zeros.
+ * Rows from base on that no node of a sequence sees, as those of the nodes that
+ * a padded tree lacks, need not have been written and may hold anything.
  * hako_gpu_tree_plan (hako_search.h) makes the masks of a tree from its
  * parents. A prefix in common as above. */
 int hako_gpu_attn_tree(float *out, int64_t out_stride, const float *q, int64_t q_stride, const hako_gpu_kv *kv,
