@@ -2753,8 +2753,9 @@ int hako_gpu_decoder_beam(hako_gpu_decoder *d, int n_beams, const int *tokens, i
 	const int S = d->n_seq, K = n_beams, R = S / K, V = d->m.vocab;
 	// arrays of S: tokens, positions, parents, since, rows, ends; scores
 	std::unique_ptr<int[]> host(new (std::nothrow) int[6 * S]);
+	std::unique_ptr<float[]> worth(new (std::nothrow) float[S]);
 	std::unique_ptr<int[]> hist(new (std::nothrow) int[(size_t)2 * n * S]);
-	if (!host || !hist) return set_error(HAKO_GPU_ENOMEM, "host memory for %d steps", n);
+	if (!host || !worth || !hist) return set_error(HAKO_GPU_ENOMEM, "host memory for %d steps", n);
 	int *tok = host.get(), *pos = tok + S, *parent = pos + S, *since = parent + S, *len = since + S, *done = len + S;
 	HK_HIP(hipMemcpyAsync(pos, d->pos, sizeof(int) * S, hipMemcpyDeviceToHost, stream()));
 	HK_HIP(hipStreamSynchronize(stream()));
@@ -2772,7 +2773,7 @@ int hako_gpu_decoder_beam(hako_gpu_decoder *d, int n_beams, const int *tokens, i
 			pos[r * K + b] = p;
 			parent[r * K + b] = 0;
 			done[r * K + b] = 0;
-			score[r * K + b] = b ? -__builtin_inff() : 0.0f;
+			worth[r * K + b] = b ? -__builtin_inff() : 0.0f;
 		}
 	}
 	if (int rc = beam_alloc(d)) return rc;
@@ -2804,7 +2805,7 @@ int hako_gpu_decoder_beam(hako_gpu_decoder *d, int n_beams, const int *tokens, i
 	}
 	HK_HIP(put(d->b_since, since, R));
 	HK_HIP(put(d->b_len, len, R));
-	HK_HIP(put(d->b_score, score, S));
+	HK_HIP(put(d->b_score, worth.get(), S));
 	HK_HIP(put(d->b_done, done, S));
 	HK_HIP(put(d->nout, done, S));
 	HK_HIP(put(d->tok, tok, S));
