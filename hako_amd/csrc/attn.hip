@@ -1921,8 +1921,10 @@ DecodePlan decode_plan(int own, int prefix_len, int kvh, int n_seq, int H, bool 
 	// part; all of 4096 56 to 58 us, 50 to 53 in one part). The lengths are not known here, so the parts are those of
 	// max_seq: 64 sequences of 1000 positions in slots of 2048 take 14.9 us, of 8192 17.4, of 32768 20.6
 	const int64_t pairs = (int64_t)n_seq * kvh;
-	// A window bounds how far lengths differ: longer parts then (64 sequences under 4096 49 us in parts of 2048, 44 in one,
-	// 128 under 2048 54 and 45)
+	// Windows of up to 8192 go undivided (64 sequences under 4096 49 us in parts of 2048, 44 in one; 128 under 2048 and some
+	// sinks, whose step more makes a second part, 54 and 45). That is for batches of like lengths: of 63 sequences of
+	// 100..400 positions and one of 8000 the long one is then a workgroup's alone (66.8 us under 8000, 38.3 under 4096, 22.2
+	// under 2000; without a window, in parts, 26)
 	p.least = pairs >= cu_count() ? (window ? kLongWindow : kLongPart) : 32 * kWaves;
 	p.parts = (own + p.least - 1) / p.least;
 	if (pairs < cu_count()) p.parts = std::min(p.parts, (int)(((prefix_len ? slots / 2 : slots) + pairs - 1) / pairs));
@@ -2363,7 +2365,9 @@ int tree_launch(const AttnKv &c, float *out, int64_t ldo, const int *slot, const
                 int H, int rows, int64_t slots, Launch launch) {
 	const int64_t tiles = ((int64_t)N * (H / c.kvh) + rows - 1) / rows, wgs = tiles * n_seq * c.kvh;
 	const int most = (tile_steps<K>(c.max_seq, c.prefix_len) + R - 1) / R;
-	// (whole rounds of the eight dies: one tree of 448 rows at 8000, four heads, 41 us in 9 parts, 31 in 8)
+	// (whole rounds of the eight dies: one tree of 448 rows at 8000, four heads, 41 us in 9 parts, 31 in 8. As many parts for
+	// all as fit at once: trees of 64 at 4096, four heads, fill the chip at 16, 126 us in two parts; 17 are one part, 136
+	// workgroups in 183 us, and 33 a second round, 395)
 	const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(most, slots / (8 * tiles) * 8 / ((int64_t)n_seq * c.kvh)));
 	if ((wgs * parts + 8 * tiles) > kMaxThreads / 512 || (int64_t)n_seq * N * H * (HD / 4) > kMaxThreads)
 		return set_error(HAKO_GPU_EINVAL, "%lld workgroups in one call", (long long)(wgs * parts));
@@ -2387,21 +2391,21 @@ int tree_launch(const AttnKv &c, float *out, int64_t ldo, const int *slot, const
 	return HAKO_GPU_OK;
 }
 
-// Which kernel (one MI355X, us by the direct / the tiled one; the texts fill their slots). Lengths are known on the device
+// Which kernel (one MI355X, us a call by the direct / the tiled one; the texts fill their slots). Lengths are known on the device
 // alone, so the work is taken as if slots were full: shorter texts may then take the tiled kernel, at up to 10 us more.
 //   rows of a sequence and head   wave-steps a SIMD (32 rows x 32 keys)   8 bits       16 bits
-//   7B  8 trees of 64 at 1000  448 rows     14                          29 / 38      32 / 37
-//       8 of 32 at 4000        224          28                          51 / 46      57 / 47
-//       16 of 64 at 4096       448         112                         166 / 125    190 / 126
-//       8 of 16 at 2000        112           8                          22 / 32      24 / 30
-//       16 of 12 at 4000        84          24                          50 / 46      56 / 48
-//       32 of 16 at 3400       112          54                          78 / 77      89 / 81
-//       64 of 16 at 2000       112          64                          93 / 83     118 / 92
-//       64 of 8 at 2000         56          32                          49 / 72      62 / 72
-//   3B  8 of 64 at 4000        512          32                          52 / 50      58 / 50
+//   7B  8 trees of 64 at 1000  448 rows     14                          33 / 39      36 / 39
+//       8 of 32 at 4000        224          28                          56 / 48      61 / 50
+//       16 of 64 at 4096       448         112                         168 / 124    189 / 134
+//       8 of 16 at 2000        112           8                          25 / 33      27 / 33
+//       16 of 12 at 4000        84          24                          54 / 51      59 / 51
+//       32 of 16 at 3400       112          54                          82 / 79      94 / 84
+//       64 of 16 at 2000       112          64                          98 / 91     120 / 96
+//       64 of 8 at 2000         56          32                          56 / 77      68 / 78
+//   3B  8 of 64 at 4000        512          32                          58 / 52      63 / 53
 // So the tiled one from 24 on for more than 64 rows. Its tiles are of 128 rows where these hold them all and sequences and
 // heads do not give every other CU a tile (32 ragged trees of 16 over a prefix in 16 bits 62 us, 72 in tiles of 256, 8
-// bits 65 and 74; 64 of 16 at 2000 96 and 89, 87 and 81).
+// bits 65 and 74; 64 of 16 at 2000 103 and 96, in 8 bits 89 and 91).
 template <int HD, bool Q8>
 int tree(const AttnKv &c, float *out, int64_t ldo, const float *q, int64_t ldq, const int *slot, const int *base, const uint64_t *seen,
          int n_seq, int N, int H, float scale) {

@@ -146,10 +146,11 @@ struct Best {
 // exp sums are taken against the part's maximum, in fp32 with the argument's
 // rounding put right, four at a time into 64 bits, and meet in 64 bits.
 //
-// Bound: HBM and the vector pipes. 32 requests of 8 beams over 152064 tokens
-// (156 MB, less the tenth of the beams that have ended) take 33.6 us and the
-// choice 6.7; where calls follow each other 66 MB of them come from HBM, the
-// rest from the memory-side cache. On the way, in all: every tile's candidates
+// Bound: no one thing. 32 requests of 8 beams over 152064 tokens (140 MB: the
+// tenth of the beams that have ended are not read) take 33.6 us, 4.2 TB/s (a copy
+// of 1 GiB 5.0), and the choice 6.7. Where calls follow each other 66 MB come
+// from HBM, the rest from the memory-side cache; of 48 wave cycles 23 are waits
+// and 11 vector instructions. On the way, in all: every tile's candidates
 // ranked as they came 91 us; 64 at a time as 64-bit keys, 16 waves a CU in the
 // place of 8, 42. The bound found two bits at a time was slower, as was ranking
 // the lanes' maxima in LDS (36.5 us against 33.7).

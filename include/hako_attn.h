@@ -20,7 +20,10 @@
  * sequences of single tokens up to n_seq * n_heads * (max_seq / 2048 + 1)
  * records of (head_dim + 3) * 4 bytes where n_seq * n_kv_heads fills the chip
  * (64 sequences of 28 heads of 128 in slots of 32768: 15 MB; 1024 in slots of
- * 131072: 1 GB), else a few MB. Calls are made from one thread at a time.
+ * 131072: 1 GB), else a few MB. Drafted trees take n_seq * n_tree * n_heads
+ * such records for each part of their keys, parts by the shape and max_seq (up
+ * to 65536 records, 34 MB with heads of 128), prompts by their lengths (up to
+ * 45 MB). Calls are made from one thread at a time.
  */
 #pragma once
 #include <stddef.h>

@@ -79,7 +79,7 @@ const char *hako_gpu_last_error(void);
 #define HAKO_TUNE_DEC_QKV_ITEMS  18  /* one-sequence decoder q/k/v launch: row items per wave, 2, 4 or 8, or 0 = by shape (default: 8 past d_model 2048, else 2); the same bits either way; read when a step is enqueued or captured */
 #define HAKO_TUNE_DEC_ATTN_PARTS 19  /* one-sequence decoder attention: workgroups that share a query-head group, 1..8, or 0 = by shape (default: 2 with 7 heads per group, else up to 4); the same bits either way; read when a step is enqueued or captured */
 #define HAKO_TUNE_Q6K_GEMM_TM   20   /* Q6_K multi-token matmul: 256-row tiles of 64 or 128 tokens (HAKO_TUNE_Q6K_GEMM_TN goes before it), or 0 = by shape (default); the same bits where K is not split */
-#define HAKO_TUNE_ATTN_PROMPT   21   /* hako_gpu_attn_prompt, _prompt_window and _tree: 1 = direct kernel (32 query rows, keys dealt to the waves), 2 = tiled kernel (256 rows), 3 = tiled kernel in 128 rows (windows and trees), 0 = by shape (default); it sets the order of the sums */
+#define HAKO_TUNE_ATTN_PROMPT   21   /* hako_gpu_attn_prompt, _prompt_window and _tree: 1 = direct kernel (32 query rows, keys dealt to the waves), 2 = tiled kernel (256 rows), 3 = tiled kernel in 128 rows (windows and trees; prompts without a window as 2), 0 = by shape (default); it sets the order of the sums */
 int hako_gpu_tune(int knob, int value);
 
 typedef struct {

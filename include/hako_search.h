@@ -38,7 +38,10 @@ extern "C" {
  * apart), score and done. score is the sum of the log probabilities of the
  * beam's tokens (-inf: no beam there). A continuation of beam b by token t is worth
  *   score[b] + (logits[b][t] - log sum_j exp(logits[b][j])),
- * compared in 64 bits; done[b] != 0 marks a beam that has ended: its one
+ * compared in 64 bits. The log is taken of 32-bit exponentials and good to
+ * 2^-19 (2^-25 as a rule), so continuations of different beams that lie closer
+ * than that may come in either order; those of one beam go by their logits
+ * alone. done[b] != 0 marks a beam that has ended: its one
  * continuation is token eos at its own score. done may be NULL (none has).
  *
  * The n_pick (1..HAKO_MAX_PICK) best continuations of a request, best first,
